@@ -161,6 +161,38 @@ SIGNATURES = {
         c_vp, c_i64, c_i64,            # out
         c_vp, c_sz, c_vp,              # workspace, bytes, stream
     ]),
+    # latent attention and the rotation (include/latent_attention.h)
+    "pa_rotary_embedding": (ctypes.c_int, [
+        c_i32, c_vp, c_i64, c_i64,     # dtype, x, strides
+        c_vp, c_vp, c_f32,             # positions, inv_freq, amplitude
+        c_i32, c_i32, c_i32, c_i32,    # tokens, heads, head_dim, start
+        c_i32, c_i32,                  # rotary_dim, interleaved
+        c_vp, c_i64, c_i64, c_vp,      # out, strides, stream
+    ]),
+    "pa_latent_store": (ctypes.c_int, [
+        c_vp, c_i64, c_vp, c_i64,      # latent, k_rope
+        c_vp, c_f32,                   # norm_weight, eps
+        c_vp, c_f32, c_i32,            # inv_freq, amplitude, interleaved
+        c_vp, c_vp, c_i32,             # positions, slot_mapping, num_tokens
+        c_i32, c_i32,                  # latent_dim, rope_dim
+        c_vp, c_i64, c_i64, c_i32,     # q_rope, strides, heads
+        c_vp, c_i64, c_i64,            # q_out
+        c_vp, c_i32, c_i32,            # cache, num_pages, page_size
+        c_i64, c_i64, c_vp,            # page/slot strides, stream
+    ]),
+    "pa_latent_decode_workspace_size": (c_sz, [c_i32] * 5),
+    "pa_latent_decode": (ctypes.c_int, [
+        c_vp, c_i64, c_i64,            # q_nope
+        c_vp, c_i64, c_i64,            # q_rope
+        c_vp, c_i32, c_i32,            # cache, num_pages, page_size
+        c_i64, c_i64,                  # page/slot strides
+        c_vp, c_i64, c_i32,            # block_tables, bt_stride, pages_per_seq
+        c_vp, c_i32, c_i32,            # lengths, batch, heads
+        c_i32, c_i32, c_i32, c_i32,    # latent, rope, nope, v dims
+        c_vp, c_vp, c_f32,             # w_uk_t, w_kv, scale
+        c_vp, c_i64, c_i64,            # out
+        c_vp, c_sz, c_vp,              # workspace, bytes, stream
+    ]),
 }
 # pa_decode_quant / pa_prefill_quant: a code_type (PA_CODE_*) before the
 # arguments of pa_decode_fp8 / pa_prefill_fp8

@@ -27,7 +27,8 @@ PHASES_LIB_PATH = os.path.join(os.path.dirname(PKG_DIR), "libpaged_attention_pha
 ARCH = "gfx950"
 
 SOURCES = ["pa_errors.cpp", "block_manager.cpp", "kv_store.hip", "decode.hip", "prefill.hip", "prefill_heads.hip",
-           "prefill_split.hip", "qk_norm_rope.hip", "mixed.hip", "any_head.hip"]
+           "prefill_split.hip", "qk_norm_rope.hip", "mixed.hip", "any_head.hip", "rotary.hip", "latent_store.hip",
+           "latent_product.hip", "latent_decode.hip"]
 PHASES_SOURCES = ["pa_errors.cpp", "prefill.hip", "any_head.hip"]  # any_head: the head-size check of the quantized entries
 
 # Packed-FP32 VALU forms are disabled for every device compile: the build
@@ -46,7 +47,7 @@ def _hipcc() -> str:
     raise RuntimeError("hipcc not found: cannot build the gfx950 paged-attention library")
 
 
-def build(verbose: bool = False, jobs: int = 4, phases: bool = False) -> str:
+def build(verbose: bool = False, jobs: int = 8, phases: bool = False) -> str:
     """Compile all sources and link ``libpaged_attention.so``; returns its
     path.  With ``phases`` build only the phase-timestamp prefill library."""
     hipcc = _hipcc()

@@ -1,0 +1,719 @@
+// Absorbed-form latent attention for gfx950: every cache row is key and value
+// of all heads at once.
+//
+//   s[n, j] = q_lat[n] . c_j + q_rope[n] . k_j,   o[n] = sum_j softmax_j(scale s) c_j
+//
+// for the rows n = (token, head) of a sequence.  Workgroup = kRows rows of one
+// sequence and a range of 32-token kv tiles; a tile (latent rows, then rotary
+// rows) sits in one stage of a four-stage LDS ring filled by direct loads
+// through the block table and serves both products.
+//
+// Eight waves in two roles, one of each on every SIMD:
+//   waves 0-3 (scores):  S^T[16 tokens][32 rows] per tile, v_mfma_f32_16x16x32
+//       with Q in registers (R = 512: 144), the running maximum and sum, P to LDS
+//   waves 4-7 (values):  O^T[R / 4][all rows] in registers, v_mfma_f32_32x32x16
+//       with V^T by transposing LDS reads and P^T from LDS
+// so that one wave's exponentials run under the other's matrix instructions:
+// the values' wave works on tile t - 1 while the scores' wave works on tile t,
+// half of it before and half behind the barrier at which the two score waves
+// of a row exchange their maxima.
+//
+// Work is cut on the device: the kv tiles of all (sequence, row tile) units,
+// laid end to end, are dealt to the workgroups in equal contiguous shares; a
+// workgroup that gets the whole of a unit writes its rows, one that gets a
+// part leaves O (float32), maximum and sum to latent_merge_kernel.
+#include <algorithm>
+
+#include "latent_attend.h"
+#include "pa_errors.h"
+#include "../../include/latent_attention.h"
+
+namespace pa {
+namespace {
+
+constexpr int kWgs = 256;      // one per CU
+constexpr int kTile = 32;      // kv tokens per tile
+constexpr int kLStages = 4;
+constexpr int kLThreads = 512;
+constexpr int kMaxBatch = 16384;  // their prefix sums fit the ring
+constexpr float kSlack = 8.f;  // log2 units the running maximum may lag
+constexpr float kNoMax = -1e30f;
+
+typedef s16x4 __attribute__((address_space(3))) * lds_tr_ptr;
+typedef void __attribute__((address_space(3))) * lds_void;
+typedef const char __attribute__((address_space(3))) * lds_bytes;
+
+__device__ __forceinline__ u32x4 lds_ld16(uint32_t a) {
+  return *reinterpret_cast<const u32x4 __attribute__((address_space(3)))*>((lds_bytes)(uintptr_t)a);
+}
+__device__ __forceinline__ u32x2 lds_tr8(uint32_t a) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(uintptr_t)a));
+}
+__device__ __forceinline__ void lds_dma16(const void* g, uint32_t block) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(block) : "memory", "m0");
+}
+// s_waitcnt vmcnt(N), other counters untouched
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  static_assert(N < 16);
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8));
+}
+__device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8)); }
+
+struct AttnParams {
+  LatentAttn a;
+  MagicDiv heads;
+  float scale_log2;
+  int32_t min_share, wgs, row_tiles;  // row_tiles: of max_q tokens
+  int32_t* prefix;  // [batch + 1] tiles before each sequence
+  float* parts;     // [2 wgs][rows * R]
+  float* stats;     // [2 wgs][rows][2]
+};
+
+template <int R, int DR, int ROWS>
+struct Dims {
+  static constexpr int kRowB = 2 * R;               // bytes of a latent row
+  static constexpr int kRopeB = 2 * DR;
+  static constexpr int kLatB = kTile * kRowB;
+  static constexpr int kStageB = kLatB + kTile * kRopeB;
+  static constexpr int kRing = kLStages * kStageB;
+  static constexpr int kPOff = kRing;                 // P: [ROWS][32] bf16
+  static constexpr int kMaxOff = kPOff + ROWS * 64;   // maxima [2][ROWS], then corrections [ROWS]
+  static constexpr int kCorrOff = kMaxOff + 2 * ROWS * 4;
+  static constexpr int kSumOff = kCorrOff + ROWS * 4;  // sums [2][ROWS], maxima [ROWS] at the end
+  static constexpr int kLds = kSumOff + 3 * ROWS * 4;
+  static constexpr int kKs = R / 32, kRs = DR / 32;   // 32-deep k-steps of the scores
+  static constexpr int kNr = ROWS / 32;               // 16-row blocks of a score wave
+  static constexpr int kDt = R / 128;                 // 32-row blocks of O^T of a value wave
+  static constexpr int kRb = ROWS / 32;               // its 32-row blocks of rows
+  static constexpr int kRowsPerDma = 1024 / kRowB;
+  static constexpr int kLatDma = 4 / kRowsPerDma;     // a wave loads four rows of a tile
+  static constexpr int kDma = kLatDma + 1;
+  static_assert(kLds <= 160 * 1024 && kRing >= 4 * kMaxBatch + 64, "LDS");
+};
+
+// 16-byte chunk swizzles (XOR on the chunk's low bits), so that 16 rows' reads
+// of one chunk and the transposing reads' four rows fall on distinct banks.
+__device__ __forceinline__ int lat_swz(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
+template <int DR>
+__device__ __forceinline__ int rope_swz(int r) {
+  return DR == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
+}
+
+struct Seq {
+  int q0, lq, lk, nt, nrt;
+};
+
+__device__ __forceinline__ Seq seq_of(const AttnParams& p, int b, int rows) {
+  Seq s;
+  s.q0 = b;
+  s.lq = 1;
+  if (p.a.cu_q) {
+    s.q0 = p.a.cu_q[b];
+    s.lq = min(p.a.cu_q[b + 1] - s.q0, p.a.max_q);
+    if (s.q0 < 0 || s.q0 >= p.a.num_tokens) s.lq = 0;
+    s.lq = max(0, min(s.lq, p.a.num_tokens - s.q0));
+  }
+  s.lk = latent_kv_len(p.a.pool, p.a.kv_lens ? p.a.kv_lens[b] : p.a.cu_k[b + 1] - p.a.cu_k[b]);
+  s.nt = (s.lk + kTile - 1) / kTile;
+  s.nrt = (s.lq * p.a.heads + rows - 1) / rows;
+  return s;
+}
+
+// Inclusive sum over the workgroup's threads (blockDim.x == kLThreads) below
+// and at this one; tmp: kLThreads / 64 ints.
+__device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int incl = (int)wave_scan((uint32_t)v);
+  __syncthreads();
+  if (lane == 63) tmp[wave] = incl;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kLThreads / 64; ++w) {
+    const int x = tmp[w];
+    before += w < wave ? x : 0;
+    total += x;
+  }
+  return incl + before;
+}
+
+template <int R, int DR, int ROWS>
+__global__ void __launch_bounds__(kLThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+latent_attn_kernel(AttnParams p) {
+  using D = Dims<R, DR, ROWS>;
+  __shared__ __attribute__((aligned(1024))) char smem[D::kLds];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void)smem;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const LatentPool& pool = p.a.pool;
+
+  // ---- this workgroup's share of the tiles.  Workgroups are dealt round-robin
+  // to the 8 XCDs: neighbours in the tile order go to one XCD, so that the row
+  // tiles of a sequence share its L2.
+  int g = blockIdx.x;
+  if (p.wgs % 8 == 0) g = (g & 7) * (p.wgs >> 3) + (g >> 3);
+  int* pref = reinterpret_cast<int*>(smem);
+  int* tmp = pref + kMaxBatch;
+  int total = 0;
+  for (int c = 0; c < p.a.batch; c += kLThreads) {
+    const int b = c + tid;
+    int v = 0;
+    if (b < p.a.batch) {
+      const Seq s = seq_of(p, b, ROWS);
+      v = s.nt * s.nrt;
+    }
+    int sum;
+    const int incl = block_scan(v, tmp, sum);
+    if (b < p.a.batch) pref[b] = total + incl - v;
+    total += sum;
+  }
+  __syncthreads();
+  if (g == 0) {
+    for (int b = tid; b < p.a.batch; b += kLThreads) p.prefix[b] = pref[b];
+    if (tid == 0) p.prefix[p.a.batch] = total;
+  }
+  const int share = max(p.min_share, (total + p.wgs - 1) / p.wgs);
+  int64_t at64 = (int64_t)g * share;
+  if (at64 >= total) return;  // uniform
+  int at = (int)at64;
+  const int end = (int)min((int64_t)total, at64 + share);
+  int b;
+  {
+    int lo = 0, hi = p.a.batch;  // last b with pref[b] <= at (sequences without tiles lie before it)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pref[mid] <= at) lo = mid;
+      else hi = mid;
+    }
+    b = __builtin_amdgcn_readfirstlane(lo);
+  }
+  int seq_at = __builtin_amdgcn_readfirstlane(pref[b]);
+  at = __builtin_amdgcn_readfirstlane(at);
+  __syncthreads();  // the ring is free from here on
+
+  while (at < end) {
+    const Seq sq = seq_of(p, b, ROWS);
+    const int seq_tiles = sq.nt * sq.nrt;
+    if (at >= seq_at + seq_tiles) {
+      seq_at += seq_tiles;
+      ++b;
+      continue;
+    }
+    const int rt = __builtin_amdgcn_readfirstlane((at - seq_at) / sq.nt);
+    const int t0 = at - seq_at - rt * sq.nt;
+    const int t1 = min(sq.nt, t0 + end - at);
+    at += t1 - t0;
+    const int n_rows = min(ROWS, sq.lq * p.a.heads - rt * ROWS);
+    const int lk = sq.lk;
+    const int32_t* bt = pool.tables + (int64_t)b * pool.bt_stride;
+
+    // ---- tile loads: this wave's rows are 4 wave .. 4 wave + 3 of every tile
+    auto row_ptr = [&](int t, int i) __attribute__((always_inline)) {
+      const int j = min(t * kTile + 4 * wave + i, lk - 1);
+      const int pg = (int)div_by((uint32_t)j, pool.page);
+      const int page = safe_page_scalar(bt, pg, pool.num_pages);
+      return pool.cache + page * pool.page_stride + (int64_t)(j - pg * (int)pool.page.d) * pool.slot_stride;
+    };
+    auto issue = [&](int t) __attribute__((always_inline)) {
+      const uint32_t st = lds0 + (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
+      const uint16_t* rp[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rp[i] = row_ptr(t, i);
+#pragma unroll
+      for (int i = 0; i < D::kLatDma; ++i) {
+        const int sub = D::kRowsPerDma == 1 ? 0 : lane >> 5;
+        const uint16_t* r = D::kRowsPerDma == 1 ? rp[i] : (sub ? rp[2 * i + 1] : rp[2 * i]);
+        const int row = 4 * wave + i * D::kRowsPerDma + sub;
+        const int c = lane & (D::kRowB / 16 - 1);
+        lds_dma16(r + 8 * (c ^ lat_swz(row)), st + (uint32_t)(4 * wave * D::kRowB + i * 1024));
+      }
+      constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
+      if (lane < 4 * kC) {
+        const int i = lane / kC;
+        const uint16_t* r = i < 2 ? (i == 0 ? rp[0] : rp[1]) : (i == 2 ? rp[2] : rp[3]);
+        const int c = (lane & (kC - 1)) ^ rope_swz<DR>(4 * wave + i);
+        lds_dma16(r + R + 8 * c, st + (uint32_t)(D::kLatB + 4 * wave * D::kRopeB));
+      }
+    };
+    issue(t0);
+    if (t0 + 1 < t1) issue(t0 + 1);
+
+    auto barrier = [&]() __attribute__((always_inline)) {
+      asm volatile("" ::: "memory");  // LDS accesses stay on their side
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");
+    };
+    // end of step t: this wave's share of tile t + 1 has landed
+    auto landed = [&](int t) __attribute__((always_inline)) {
+      if (t + 2 < t1) wait_vm<D::kDma>();
+      else wait_vm<0>();
+    };
+
+    if (wave < 4) {
+      // ================= scores
+      const int tb = wave & 1, rw = (wave >> 1) * 16 * D::kNr;
+      const int l16 = lane & 15, qd = lane >> 4;
+      bf16x8 q[D::kNr][D::kKs + D::kRs];
+      int lim[D::kNr];  // tokens a row sees
+#pragma unroll
+      for (int r = 0; r < D::kNr; ++r) {
+        const int row = rt * ROWS + min(rw + 16 * r + l16, n_rows - 1);
+        const int tok = (int)div_by((uint32_t)row, p.heads), hd = row - tok * p.a.heads;
+        lim[r] = min(lk, max(0, lk - sq.lq + tok + 1));
+        const uint16_t* ql = p.a.q_lat + (int64_t)(sq.q0 + tok) * p.a.ql_ts + hd * p.a.ql_hs + 8 * qd;
+        const uint16_t* qr = p.a.q_rope + (int64_t)(sq.q0 + tok) * p.a.qr_ts + hd * p.a.qr_hs + 8 * qd;
+#pragma unroll
+        for (int ks = 0; ks < D::kKs; ++ks) q[r][ks] = as_bf16x8(ld16(ql + 32 * ks));
+#pragma unroll
+        for (int ks = 0; ks < D::kRs; ++ks) q[r][D::kKs + ks] = as_bf16x8(ld16(qr + 32 * ks));
+      }
+      // first tile a row of this tile does not see in full
+      const int tok_first = (int)div_by((uint32_t)(rt * ROWS), p.heads);
+      const int free_tiles = max(0, min(lk, lk - sq.lq + tok_first + 1)) / kTile;
+      float m_ref[D::kNr], l_sum[D::kNr];
+#pragma unroll
+      for (int r = 0; r < D::kNr; ++r) {
+        m_ref[r] = kNoMax;
+        l_sum[r] = 0.f;
+      }
+      // reads of K: row 16 tb + l16, chunk 4 ks + qd
+      const int krow = 16 * tb + l16;
+      uint32_t koff[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) koff[i] = lds0 + krow * D::kRowB + 16 * ((4 * i + qd) ^ lat_swz(krow));
+      uint32_t roff[D::kRs];
+#pragma unroll
+      for (int i = 0; i < D::kRs; ++i)
+        roff[i] = lds0 + D::kLatB + krow * D::kRopeB + 16 * ((4 * i + qd) ^ rope_swz<DR>(krow));
+      float* maxes = reinterpret_cast<float*>(smem + D::kMaxOff);
+      float* corrs = reinterpret_cast<float*>(smem + D::kCorrOff);
+      wait_vm<0>();  // Q and both tiles
+      barrier();
+      for (int t = t0; t <= t1; ++t) {
+        if (t + 2 < t1) issue(t + 2);
+        f32x4 s[D::kNr];
+        float mx[D::kNr];
+        if (t < t1) {
+          const uint32_t st = (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
+          f32x4 s2[D::kNr];
+#pragma unroll
+          for (int r = 0; r < D::kNr; ++r) s[r] = s2[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < D::kKs; ++ks) {
+            const bf16x8 a = as_bf16x8(lds_ld16(koff[ks & 3] + st + (ks >> 2) * 256));
+#pragma unroll
+            for (int r = 0; r < D::kNr; ++r)
+              if (ks & 1) s2[r] = mfma16(a, q[r][ks], s2[r]);
+              else s[r] = mfma16(a, q[r][ks], s[r]);
+          }
+#pragma unroll
+          for (int ks = 0; ks < D::kRs; ++ks) {
+            const bf16x8 a = as_bf16x8(lds_ld16(roff[ks] + st));
+#pragma unroll
+            for (int r = 0; r < D::kNr; ++r)
+              if (ks & 1) s2[r] = mfma16(a, q[r][D::kKs + ks], s2[r]);
+              else s[r] = mfma16(a, q[r][D::kKs + ks], s[r]);
+          }
+          const int j0 = t * kTile + 16 * tb + 4 * qd;
+#pragma unroll
+          for (int r = 0; r < D::kNr; ++r) {
+            s[r] = (s[r] + s2[r]) * p.scale_log2;
+            if (t >= free_tiles) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[r][i] = j0 + i < lim[r] ? s[r][i] : -INFINITY;
+            }
+            mx[r] = __builtin_fmaxf(__builtin_fmaxf(s[r][0], s[r][1]), __builtin_fmaxf(s[r][2], s[r][3]));
+            mx[r] = max_xor32(max_xor16(mx[r]));
+            if (qd == 0) maxes[tb * ROWS + rw + 16 * r + l16] = mx[r];
+          }
+        }
+        wait_lgkm0();
+        barrier();
+        if (t < t1) {
+#pragma unroll
+          for (int r = 0; r < D::kNr; ++r) {
+            const int row = rw + 16 * r + l16;
+            const float m_t = __builtin_fmaxf(mx[r], maxes[(tb ^ 1) * ROWS + row]);
+            const float m_new = m_t > m_ref[r] + kSlack ? m_t : m_ref[r];
+            const float corr = fast_exp2(m_ref[r] - m_new);
+            m_ref[r] = m_new;
+            if (tb == 0 && qd == 0) corrs[row] = corr;
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = fast_exp2(s[r][i] - m_new);
+            l_sum[r] = l_sum[r] * corr + ((e[0] + e[1]) + (e[2] + e[3]));
+            // tokens 16 tb + 4 qd .. + 3 of the row: chunk 2 tb + (qd & 1), half
+            // qd >> 1 of it, the order in which the transposing reads take V
+            const int c = (2 * tb + (qd & 1)) ^ ((row >> 2) & 3);
+            *reinterpret_cast<u32x2*>(smem + D::kPOff + row * 64 + 16 * c + 8 * (qd >> 1)) =
+                u32x2{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3])};
+          }
+        }
+        landed(t);
+        wait_lgkm0();
+        barrier();
+      }
+      // ---- row sums and maxima
+      float* sums = reinterpret_cast<float*>(smem + D::kSumOff);
+#pragma unroll
+      for (int r = 0; r < D::kNr; ++r) {
+        const float l = sum_xor32(sum_xor16(l_sum[r]));
+        const int row = rw + 16 * r + l16;
+        if (qd == 0) {
+          sums[tb * ROWS + row] = l;
+          if (tb == 0) sums[2 * ROWS + row] = m_ref[r];
+        }
+      }
+      wait_lgkm0();
+      barrier();
+    } else {
+      // ================= values
+      const int pw = wave - 4;
+      const int n = lane & 31, h = lane >> 5;
+      f32x16 acc[D::kDt][D::kRb] = {};
+      // transposing reads of V^T: lane 16 gamma + s reads row 4 h + s / 4 (+ 8)
+      // of a 16-token step, columns 32 dt + 16 (gamma % 2) + 4 (s % 4)
+      const int ts = lane & 15, gamma = lane >> 4;
+      const int tr = 4 * h + (ts >> 2);
+      uint32_t voff0[D::kDt], voff1[D::kDt];
+#pragma unroll
+      for (int dt = 0; dt < D::kDt; ++dt) {
+        const int c = 4 * (pw * D::kDt + dt) + 2 * (gamma & 1) + ((ts & 3) >> 1);
+        voff0[dt] = lds0 + tr * D::kRowB + 16 * (c ^ lat_swz(tr)) + 8 * (ts & 1);
+        voff1[dt] = lds0 + (tr + 8) * D::kRowB + 16 * (c ^ lat_swz(tr + 8)) + 8 * (ts & 1);
+      }
+      uint32_t poff[D::kRb][2];
+#pragma unroll
+      for (int rb = 0; rb < D::kRb; ++rb)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          poff[rb][u] = lds0 + D::kPOff + (32 * rb + n) * 64 + 16 * ((2 * u + h) ^ ((n >> 2) & 3));
+      const float* corrs = reinterpret_cast<const float*>(smem + D::kCorrOff);
+      wait_vm<0>();
+      barrier();
+      bf16x8 pt[D::kRb][2];
+      auto product = [&](int u, uint32_t st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int dt = 0; dt < D::kDt; ++dt) {
+          const u32x2 lo = lds_tr8(voff0[dt] + st + 16 * u * D::kRowB);
+          const u32x2 hi = lds_tr8(voff1[dt] + st + 16 * u * D::kRowB);
+          const bf16x8 a = as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]});
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb) acc[dt][rb] = mfma32(a, pt[rb][u], acc[dt][rb]);
+        }
+      };
+      for (int t = t0; t <= t1; ++t) {
+        if (t + 2 < t1) issue(t + 2);
+        const uint32_t st = (uint32_t)((t - 1 - t0) & (kLStages - 1)) * D::kStageB;
+        if (t > t0) {
+          float corr[D::kRb];
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb) {
+            corr[rb] = corrs[32 * rb + n];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) pt[rb][u] = as_bf16x8(lds_ld16(poff[rb][u]));
+          }
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb)
+            if (__any(corr[rb] != 1.f)) {
+#pragma unroll
+              for (int dt = 0; dt < D::kDt; ++dt) acc[dt][rb] = acc[dt][rb] * corr[rb];
+            }
+          product(0, st);
+        }
+        wait_lgkm0();  // P is in registers: the score waves may overwrite it
+        barrier();
+        if (t > t0) product(1, st);
+        landed(t);
+        wait_lgkm0();
+        barrier();
+      }
+      barrier();  // sums are there
+      const float* sums = reinterpret_cast<const float*>(smem + D::kSumOff);
+      if (t0 == 0 && t1 == sq.nt) {
+#pragma unroll
+        for (int rb = 0; rb < D::kRb; ++rb) {
+          const int r = 32 * rb + n;
+          const float l = sums[r] + sums[ROWS + r];
+          const float inv = l > 0.f ? 1.f / l : 0.f;
+          if (r < n_rows) {
+            const int row = rt * ROWS + r;
+            const int tok = (int)div_by((uint32_t)row, p.heads), hd = row - tok * p.a.heads;
+            uint16_t* o = p.a.out + (int64_t)(sq.q0 + tok) * p.a.o_ts + hd * p.a.o_hs + pw * (R / 4) + 4 * h;
+#pragma unroll
+            for (int dt = 0; dt < D::kDt; ++dt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const f32x16& v = acc[dt][rb];
+                *reinterpret_cast<u32x2*>(o + 32 * dt + 8 * i) =
+                    u32x2{pack_bf16x2(v[4 * i] * inv, v[4 * i + 1] * inv),
+                          pack_bf16x2(v[4 * i + 2] * inv, v[4 * i + 3] * inv)};
+              }
+          }
+        }
+      } else {
+        const int slot = 2 * g + (t0 == 0 ? 1 : 0);
+        float* dst = p.parts + (int64_t)slot * (ROWS * R) + 4 * lane;
+#pragma unroll
+        for (int dt = 0; dt < D::kDt; ++dt)
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const f32x16& v = acc[dt][rb];
+              *reinterpret_cast<f32x4*>(dst + 256 * (((pw * D::kDt + dt) * D::kRb + rb) * 4 + i)) =
+                  f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+            }
+        if (pw == 0 && lane < ROWS) {
+          const float l = sums[lane] + sums[ROWS + lane];
+          *reinterpret_cast<f32x2*>(p.stats + ((int64_t)slot * ROWS + lane) * 2) = f32x2{sums[2 * ROWS + lane], l};
+        }
+      }
+    }
+    __syncthreads();  // LDS is free for the next segment
+  }
+}
+
+// Joins the parts of every (sequence, row tile) that more than one workgroup
+// worked on: o = sum_p w_p o_p / sum_p w_p l_p, w_p = 2^(m_p - max m).  A part's
+// O lies as the accumulators held it, 256 floats a (column block, row block,
+// quarter): a workgroup joins one such slice at a time, its waves taking the
+// parts in turn, and rows without any token to see come out zero.
+template <int R, int ROWS>
+__global__ void __launch_bounds__(256) latent_merge_kernel(AttnParams p) {
+  constexpr int kRb = ROWS / 32, kSlices = ROWS * R / 256;
+  __shared__ f32x4 s_acc[4][64];
+  __shared__ float s_m[4][32], s_l[4][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = lane & 31, h = lane >> 5;
+  const int b = blockIdx.x / p.row_tiles, rt = blockIdx.x - b * p.row_tiles;
+  const Seq sq = seq_of(p, b, ROWS);
+  if (rt >= sq.nrt) return;
+  const int total = p.prefix[p.a.batch];
+  const int share = max(p.min_share, (total + p.wgs - 1) / p.wgs);
+  const int64_t a = (int64_t)p.prefix[b] + (int64_t)rt * sq.nt;
+  const int g0 = (int)(a / share), g1 = sq.nt ? (int)((a + sq.nt - 1) / share) : g0 + 1;
+  if (g0 == g1) return;  // one workgroup had the whole unit
+  const int parts = sq.nt ? g1 - g0 + 1 : 0;
+  const int n_rows = min(ROWS, sq.lq * p.a.heads - rt * ROWS);
+  for (int sl = blockIdx.y; sl < kSlices; sl += gridDim.y) {
+    const int rb = (sl >> 2) % kRb;
+    const int r = 32 * rb + n;
+    float m = kNoMax, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i = wave; i < parts; i += 4) {
+      const int slot = 2 * (g0 + i) + (i == 0 ? 1 : 0);
+      const f32x2 ml = *reinterpret_cast<const f32x2*>(p.stats + ((int64_t)slot * ROWS + r) * 2);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(p.parts + (int64_t)slot * (ROWS * R) + 256 * sl + 4 * lane);
+      const float m_new = __builtin_fmaxf(m, ml[0]);
+      const float ca = fast_exp2(m - m_new), cb = fast_exp2(ml[0] - m_new);
+      acc = acc * ca + v * cb;
+      l = l * ca + ml[1] * cb;
+      m = m_new;
+    }
+    s_acc[wave][lane] = acc;
+    if (h == 0) {
+      s_m[wave][n] = m;
+      s_l[wave][n] = l;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      float mm = kNoMax;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = __builtin_fmaxf(mm, s_m[w][n]);
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      float ll = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float c = fast_exp2(s_m[w][n] - mm);
+        o = o + s_acc[w][lane] * c;
+        ll += s_l[w][n] * c;
+      }
+      const float inv = ll > 0.f ? 1.f / ll : 0.f;
+      if (r < n_rows) {
+        const int row = rt * ROWS + r;
+        const int tok = (int)div_by((uint32_t)row, p.heads), hd = row - tok * p.a.heads;
+        const int d = 32 * (sl / (4 * kRb)) + 8 * (sl & 3) + 4 * h;
+        *reinterpret_cast<u32x2*>(p.a.out + (int64_t)(sq.q0 + tok) * p.a.o_ts + hd * p.a.o_hs + d) =
+            u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Rows of a workgroup: 64, or 32 where a sequence has no more.
+int rows_of(int max_q, int heads) { return (int64_t)max_q * heads <= 32 ? 32 : 64; }
+
+constexpr int kMinShare = 4;  // tiles a workgroup takes at least
+
+int wgs_of(int64_t most_tiles) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(kWgs, (most_tiles + kMinShare - 1) / kMinShare));
+}
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+}  // namespace
+
+size_t latent_attn_workspace(int32_t batch, int32_t max_q, int32_t heads, int32_t latent, int64_t span,
+                             const char** why) {
+  const int rows = rows_of(max_q, heads);
+  const int64_t row_tiles = ((int64_t)max_q * heads + rows - 1) / rows;
+  const int64_t tiles = (span + kTile - 1) / kTile;
+  *why = nullptr;
+  if (batch > kMaxBatch) *why = "more than 16384 sequences";
+  else if (span > 0x7fffffff - kTile || (int64_t)max_q * heads > 0x7fffffff - 64 || tiles > 0x7fffffff / std::max<int64_t>(1, row_tiles * batch))
+    *why = "more than 2^31 tiles of work";
+  if (*why) return 0;
+  const int wgs = wgs_of(row_tiles * batch * tiles);
+  return align256(4 * ((size_t)batch + 1)) + align256((size_t)2 * wgs * rows * 8) + (size_t)2 * wgs * rows * latent * 4;
+}
+
+template <int R, int DR, int ROWS>
+static int attn_launch(const char* name, AttnParams p, void* workspace, hipStream_t s) {
+  char* ws = (char*)workspace;
+  p.prefix = (int32_t*)ws;
+  ws += align256(4 * ((size_t)p.a.batch + 1));
+  p.stats = (float*)ws;
+  ws += align256((size_t)2 * p.wgs * ROWS * 8);
+  p.parts = (float*)ws;
+  latent_attn_kernel<R, DR, ROWS><<<dim3((unsigned)p.wgs), dim3(kLThreads), 0, s>>>(p);
+  if (int rc = launch_status(name)) return rc;
+  const int64_t units = (int64_t)p.a.batch * p.row_tiles;
+  constexpr int kSlices = ROWS * R / 256;
+  const unsigned ny = (unsigned)std::max<int64_t>(1, std::min<int64_t>(kSlices, 1024 / units));
+  latent_merge_kernel<R, ROWS><<<dim3((unsigned)units, ny), dim3(256), 0, s>>>(p);
+  return launch_status(name);
+}
+
+int latent_attn_launch(const char* name, const LatentAttn& a, int latent, int rope, void* workspace, hipStream_t s) {
+  AttnParams p;
+  p.a = a;
+  p.heads = magic_div((uint32_t)a.heads);
+  p.scale_log2 = a.scale * kLog2e;
+  p.min_share = kMinShare;
+  const int rows = rows_of(a.max_q, a.heads);
+  p.row_tiles = (int)(((int64_t)a.max_q * a.heads + rows - 1) / rows);
+  const int64_t span = (int64_t)a.pool.pages_per_seq * a.pool.page.d;
+  p.wgs = wgs_of((int64_t)p.row_tiles * a.batch * ((span + kTile - 1) / kTile));
+  p.prefix = nullptr;
+  p.parts = p.stats = nullptr;
+#define PA_LATENT_CASE(R, DR)                                             \
+  if (latent == R && rope == DR)                                          \
+    return rows == 32 ? attn_launch<R, DR, 32>(name, p, workspace, s) : attn_launch<R, DR, 64>(name, p, workspace, s);
+  PA_LATENT_CASE(512, 64)
+  PA_LATENT_CASE(512, 32)
+  PA_LATENT_CASE(256, 64)
+  PA_LATENT_CASE(256, 32)
+#undef PA_LATENT_CASE
+  return fail(PA_ERR_UNSUPPORTED, "%s: latent_dim %d with rope_dim %d", name, latent, rope);
+}
+
+}  // namespace pa
+
+using namespace pa;
+
+static int latent_decode_need(const char* name, int32_t batch, int32_t num_heads, int32_t latent_dim,
+                              int32_t pages_per_seq, int32_t page_size, size_t& q_bytes, size_t& need) {
+  const char* why;
+  const size_t attn = latent_attn_workspace(batch, 1, num_heads, latent_dim, (int64_t)pages_per_seq * page_size, &why);
+  if (why) return fail(PA_ERR_UNSUPPORTED, "%s: %s", name, why);
+  q_bytes = ((size_t)batch * num_heads * latent_dim * 2 + 255) & ~(size_t)255;
+  need = 2 * q_bytes + attn;  // absorbed q, latent outputs, the attention's own
+  return PA_OK;
+}
+
+extern "C" size_t pa_latent_decode_workspace_size(int32_t batch, int32_t num_heads, int32_t latent_dim,
+                                                  int32_t pages_per_seq, int32_t page_size) {
+  if (batch <= 0 || num_heads <= 0 || latent_dim <= 0 || pages_per_seq < 0 || page_size <= 0) return 0;
+  size_t q, need;
+  return latent_decode_need("pa_latent_decode_workspace_size", batch, num_heads, latent_dim, pages_per_seq, page_size,
+                            q, need) == PA_OK
+             ? need
+             : 0;
+}
+
+extern "C" int pa_latent_decode(const uint16_t* q_nope, int64_t qn_tok_stride, int64_t qn_head_stride,
+                                const uint16_t* q_rope, int64_t qr_tok_stride, int64_t qr_head_stride,
+                                const uint16_t* cache, int32_t num_pages, int32_t page_size, int64_t page_stride,
+                                int64_t slot_stride, const int32_t* block_tables, int64_t bt_stride,
+                                int32_t pages_per_seq, const int32_t* lengths, int32_t batch, int32_t num_heads,
+                                int32_t latent_dim, int32_t rope_dim, int32_t nope_dim, int32_t v_dim,
+                                const uint16_t* w_uk_t, const uint16_t* w_kv, float scale, uint16_t* out,
+                                int64_t out_tok_stride, int64_t out_head_stride, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  const char* name = "pa_latent_decode";
+  if (batch < 0 || num_heads <= 0 || num_pages <= 0 || page_size <= 0 || pages_per_seq < 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: bad sizes (batch=%d, num_heads=%d, num_pages=%d, page_size=%d, "
+                "pages_per_seq=%d)", name, batch, num_heads, num_pages, page_size, pages_per_seq);
+  if (!latent_dims_ok(latent_dim, rope_dim) || !latent_head_ok(nope_dim, v_dim))
+    return fail(PA_ERR_UNSUPPORTED, "%s: latent_dim %d, rope_dim %d, nope_dim %d, v_dim %d not supported", name,
+                latent_dim, rope_dim, nope_dim, v_dim);
+  if (num_heads > 65535) return fail(PA_ERR_UNSUPPORTED, "%s: %d heads", name, num_heads);
+  if (batch == 0) return PA_OK;
+  if (!q_nope || !q_rope || !cache || !lengths || !w_uk_t || !w_kv || !out || (pages_per_seq && !block_tables))
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+  const uintptr_t align = (uintptr_t)q_nope | (uintptr_t)q_rope | (uintptr_t)cache | (uintptr_t)w_uk_t |
+                          (uintptr_t)w_kv | (uintptr_t)out | (uintptr_t)workspace;
+  if ((align & 15u) || (qn_tok_stride | qn_head_stride | qr_tok_stride | qr_head_stride | page_stride | slot_stride |
+                        out_tok_stride | out_head_stride) % 8)
+    return fail(PA_ERR_UNSUPPORTED, "%s: operands must be 16-byte aligned with strides multiple of 8", name);
+  size_t q_bytes, need;
+  if (int rc = latent_decode_need(name, batch, num_heads, latent_dim, pages_per_seq, page_size, q_bytes, need))
+    return rc;
+  if (!workspace || workspace_bytes < need)
+    return fail(PA_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", name, workspace_bytes, need);
+  hipStream_t s = (hipStream_t)stream;
+  uint16_t* q_lat = (uint16_t*)workspace;
+  uint16_t* o_lat = (uint16_t*)((char*)workspace + q_bytes);
+  HeadProduct hp;
+  hp.x = q_nope;
+  hp.x_ts = qn_tok_stride;
+  hp.x_hs = qn_head_stride;
+  hp.w = w_uk_t;
+  hp.w_hs = (int64_t)latent_dim * nope_dim;
+  hp.y = q_lat;
+  hp.y_ts = (int64_t)num_heads * latent_dim;
+  hp.y_hs = latent_dim;
+  hp.tokens = batch;
+  hp.heads = num_heads;
+  hp.n = latent_dim;
+  hp.k = nope_dim;
+  if (int rc = head_product_launch(name, hp, s)) return rc;
+  LatentAttn a;
+  a.q_lat = q_lat;
+  a.ql_ts = (int64_t)num_heads * latent_dim;
+  a.ql_hs = latent_dim;
+  a.q_rope = q_rope;
+  a.qr_ts = qr_tok_stride;
+  a.qr_hs = qr_head_stride;
+  a.pool = LatentPool{cache, num_pages, magic_div((uint32_t)page_size), page_stride, slot_stride,
+                      block_tables, bt_stride, pages_per_seq};
+  a.cu_q = nullptr;
+  a.cu_k = nullptr;
+  a.kv_lens = lengths;
+  a.batch = batch;
+  a.num_tokens = batch;
+  a.heads = num_heads;
+  a.max_q = 1;
+  a.scale = scale;
+  a.out = o_lat;
+  a.o_ts = (int64_t)num_heads * latent_dim;
+  a.o_hs = latent_dim;
+  if (int rc = latent_attn_launch(name, a, latent_dim, rope_dim, (char*)workspace + 2 * q_bytes, s)) return rc;
+  hp.x = o_lat;
+  hp.x_ts = (int64_t)num_heads * latent_dim;
+  hp.x_hs = latent_dim;
+  hp.w = w_kv + (int64_t)nope_dim * latent_dim;
+  hp.w_hs = (int64_t)(nope_dim + v_dim) * latent_dim;
+  hp.y = out;
+  hp.y_ts = out_tok_stride;
+  hp.y_hs = out_head_stride;
+  hp.n = v_dim;
+  hp.k = latent_dim;
+  return head_product_launch(name, hp, s);
+}

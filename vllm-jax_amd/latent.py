@@ -1,0 +1,226 @@
+"""Latent attention: one latent vector and one rotated key part a token in the
+cache, in place of K and V rows per head.
+
+A token's cache row is ``[c | k_r]``: the normalised latent ``c`` (``R``
+elements) and the rotary key part ``k_r`` (``Dr``), shared by all heads.  Head
+``h`` attends with ``K[h] = [W_uk[h] c | k_r]`` and ``V[h] = W_uv[h] c``.  The
+path mirrors ``attention()``'s: a store (:func:`latent_store`), a decode and a
+prefill entry, and the layer seam :func:`latent_attention` over the same
+metadata types.  The pool is ``[NB, BS, R + Dr]`` bf16, addressed by the same
+slot mappings and block tables as the engine's K/V pool.
+
+Decode runs in the absorbed form: q goes through ``W_uk[h]`` once, scores and
+values are taken against the cache rows themselves, and ``W_uv[h]`` maps the
+result back, so a cached token costs one row of ``R + Dr`` elements whatever
+the number of heads.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .attention import _checking_slots, check_slot_mapping
+from .kernels._common import require_bf16, require_device, stream_handle
+from .rotary import RotaryFrequencies, check_frequencies, check_tokens, on_device
+
+LATENT_DIMS, ROPE_DIMS, HEAD_DIMS = (256, 512), (32, 64), (64, 128)
+
+
+class LatentWeights:
+    """The up projection of a layer, laid out once for the kernels.
+
+    ``w_kv`` is ``[num_heads * (nope_dim + v_dim), R]`` bf16: the rows of
+    ``W_uk[h]``, then those of ``W_uv[h]``, head by head.  Kept as it is (a
+    contiguous copy if it is not) and with ``W_uk`` transposed, for the
+    absorbed form.  A changed ``w_kv`` needs a new object.
+    """
+
+    def __init__(self, w_kv: torch.Tensor, *, num_heads: int, nope_dim: int, v_dim: int):
+        require_device("w_kv", w_kv)
+        if w_kv.dtype != torch.bfloat16:
+            raise ValueError(f"w_kv must be bfloat16, got {w_kv.dtype}")
+        if num_heads <= 0 or nope_dim not in HEAD_DIMS or v_dim != nope_dim:
+            raise ValueError(f"num_heads {num_heads}, nope_dim {nope_dim}, v_dim {v_dim}: nope_dim and v_dim must be "
+                             f"equal and one of {HEAD_DIMS}")
+        if w_kv.dim() != 2 or w_kv.shape[0] != num_heads * (nope_dim + v_dim) or w_kv.shape[1] not in LATENT_DIMS:
+            raise ValueError(f"w_kv must be [{num_heads * (nope_dim + v_dim)}, R] with R one of {LATENT_DIMS}, got "
+                             f"{tuple(w_kv.shape)}")
+        self.num_heads, self.nope_dim, self.v_dim, self.latent_dim = num_heads, nope_dim, v_dim, w_kv.shape[1]
+        self.w_kv = w_kv.detach().contiguous().view(num_heads, nope_dim + v_dim, self.latent_dim)
+        if self.w_kv.data_ptr() % 16:
+            self.w_kv = self.w_kv.clone()
+        self.w_uk_t = self.w_kv[:, :nope_dim].transpose(1, 2).contiguous()  # [H, R, Dn]
+
+
+def _check_cache(latent_cache: torch.Tensor, latent_dim: Optional[int] = None) -> Tuple[int, int, int]:
+    """(pages, page size, row length) of a pool ``[NB, BS, R + Dr]``."""
+    require_device("latent_cache", latent_cache)
+    require_bf16("latent_cache", latent_cache)
+    if latent_cache.dim() != 3:
+        raise ValueError(f"latent_cache must be [NB, BS, R + Dr], got {tuple(latent_cache.shape)}")
+    if latent_dim is not None and latent_cache.shape[2] - latent_dim not in ROPE_DIMS:
+        raise ValueError(f"latent_cache rows of {latent_cache.shape[2]} do not fit latent_dim {latent_dim} (rope_dim "
+                         f"must be one of {ROPE_DIMS})")
+    return tuple(latent_cache.shape)
+
+
+def latent_store(latent: torch.Tensor, k_rope: torch.Tensor, norm_weight: Optional[torch.Tensor],
+                 positions: torch.Tensor, slot_mapping: torch.Tensor, latent_cache: torch.Tensor,
+                 freqs: RotaryFrequencies, *, eps: float = 1e-6, interleaved: bool = True,
+                 q_rope: Optional[torch.Tensor] = None,
+                 q_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The layer step between the down projections and attention, in one
+    kernel: ``cache[slot] = [rmsnorm(latent) | rope(k_rope)]`` in place, and
+    ``rope(q_rope)``.  Returns ``(latent_cache, q_out)``.
+
+    ``latent`` ``[T, R]`` and ``k_rope`` ``[T, Dr]`` may be slices of one
+    projection; ``norm_weight`` ``[R]``, or ``None`` for rows that come
+    normalised.  ``q_rope`` ``[T, H, Dr]`` (a slice of q's heads) is rotated
+    for every token, into ``q_out`` (``q_rope`` itself, or a new tensor).  Slots
+    outside the pool (padding tokens) are skipped.
+    """
+    for name, t in (("latent", latent), ("k_rope", k_rope)):
+        require_device(name, t)
+        require_bf16(name, t)
+        if t.dim() != 2:
+            raise ValueError(f"{name} must be [T, dim], got {tuple(t.shape)}")
+    t_count, r = latent.shape
+    nb, bs, row = _check_cache(latent_cache)
+    dr = k_rope.shape[1]
+    if r not in LATENT_DIMS or dr not in ROPE_DIMS or row != r + dr or k_rope.shape[0] != t_count:
+        raise ValueError(f"latent {tuple(latent.shape)} and k_rope {tuple(k_rope.shape)} do not fit a cache of rows of "
+                         f"{row} (R one of {LATENT_DIMS}, Dr one of {ROPE_DIMS})")
+    check_frequencies(freqs, latent)
+    if freqs.rotary_dim != dr:
+        raise ValueError(f"the frequencies are of rotary_dim {freqs.rotary_dim}, k_rope of {dr}")
+    if norm_weight is not None:
+        require_device("norm_weight", norm_weight)
+        require_bf16("norm_weight", norm_weight)
+        if tuple(norm_weight.shape) != (r,):
+            raise ValueError(f"norm_weight must be [{r}], got {tuple(norm_weight.shape)}")
+    pos = check_tokens("positions", positions, t_count, latent)
+    slots = check_tokens("slot_mapping", slot_mapping, t_count, latent)
+    heads, q_args = 0, (None, 0, 0, 0, None, 0, 0)
+    if q_rope is not None:
+        require_device("q_rope", q_rope)
+        require_bf16("q_rope", q_rope)
+        if q_rope.dim() != 3 or q_rope.shape[0] != t_count or q_rope.shape[2] != dr or q_rope.shape[1] == 0:
+            raise ValueError(f"q_rope must be [{t_count}, H, {dr}], got {tuple(q_rope.shape)}")
+        heads = q_rope.shape[1]
+        if q_out is None:
+            q_out = torch.empty_like(q_rope, memory_format=torch.contiguous_format)
+        else:
+            require_device("q_out", q_out)
+            require_bf16("q_out", q_out)
+            if tuple(q_out.shape) != tuple(q_rope.shape):
+                raise ValueError(f"q_out must have shape {tuple(q_rope.shape)}")
+        q_args = (q_rope.data_ptr(), q_rope.stride(0), q_rope.stride(1), heads, q_out.data_ptr(), q_out.stride(0),
+                  q_out.stride(1))
+    elif q_out is not None:
+        raise ValueError("q_out without q_rope")
+    same_device(latent, k_rope, norm_weight, latent_cache, q_rope, q_out)
+    if _checking_slots():
+        check_slot_mapping(slots, nb * bs)
+    if t_count == 0:
+        return latent_cache, q_out
+    with on_device(latent):
+        _lib.call("pa_latent_store", latent.data_ptr(), latent.stride(0), k_rope.data_ptr(), k_rope.stride(0),
+                  None if norm_weight is None else norm_weight.data_ptr(), float(eps), freqs.inv_freq.data_ptr(),
+                  float(freqs.amplitude), int(bool(interleaved)), pos.data_ptr(), slots.data_ptr(), t_count, r, dr,
+                  *q_args, latent_cache.data_ptr(), nb, bs, latent_cache.stride(0), latent_cache.stride(1),
+                  stream_handle(latent))
+    return latent_cache, q_out
+
+
+def same_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"operands live on {first.device} and {t.device}")
+
+
+def _check_q(q_nope, q_rope, latent_cache, weights):
+    """Checked shapes of an attention call: (tokens, rope_dim, pages, page size)."""
+    if not isinstance(weights, LatentWeights):
+        raise TypeError(f"weights must be LatentWeights, got {type(weights).__name__}")
+    nb, bs, row = _check_cache(latent_cache, weights.latent_dim)
+    dr = row - weights.latent_dim
+    for name, t, d in (("q_nope", q_nope, weights.nope_dim), ("q_rope", q_rope, dr)):
+        require_device(name, t)
+        require_bf16(name, t)
+        if t.dim() != 3 or t.shape[1] != weights.num_heads or t.shape[2] != d:
+            raise ValueError(f"{name} must be [T, {weights.num_heads}, {d}], got {tuple(t.shape)}")
+    if q_nope.shape[0] != q_rope.shape[0]:
+        raise ValueError(f"q_nope and q_rope have {q_nope.shape[0]} and {q_rope.shape[0]} tokens")
+    same_device(q_nope, q_rope, latent_cache, weights.w_kv)
+    return q_nope.shape[0], dr, nb, bs
+
+
+def _check_table(block_tables: torch.Tensor, batch: int, like: torch.Tensor) -> torch.Tensor:
+    require_device("block_tables", block_tables)
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != batch:
+        raise ValueError(f"block_tables must be int32 [{batch}, pages], got {block_tables.dtype} "
+                         f"{tuple(block_tables.shape)}")
+    same_device(like, block_tables)
+    return block_tables if block_tables.stride(-1) == 1 else block_tables.contiguous()
+
+
+def _output(out, shape, like):
+    if out is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=like.device)
+    require_device("out", out)
+    require_bf16("out", out)
+    if tuple(out.shape) != shape:
+        raise ValueError(f"out must have shape {shape}, got {tuple(out.shape)}")
+    same_device(like, out)
+    return out
+
+
+def _workspace(workspace, need, like):
+    if workspace is not None:
+        require_device("workspace", workspace)
+        same_device(like, workspace)
+        if workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= need:
+            return workspace
+    return torch.empty(max(need, 1), dtype=torch.uint8, device=like.device)
+
+
+def latent_decode_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_cache: torch.Tensor,
+                            weights: LatentWeights, block_tables: torch.Tensor, lengths: torch.Tensor, *,
+                            scale: float, workspace: Optional[torch.Tensor] = None,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One new token a sequence over the paged latent cache (absorbed form):
+    q_nope ``[B, H, Dn]`` and the rotated q_rope ``[B, H, Dr]`` against the
+    first ``lengths[b]`` rows of sequence ``b`` -> ``[B, H, Dv]`` bf16.
+
+    ``scale`` multiplies the scores (``(Dn + Dr) ** -0.5`` for an unscaled
+    model).  A length of zero gives a zero row; lengths past the block table's
+    span are clamped to it.  The absorbed q, the latent-wide result and the
+    split's partials go through ``workspace`` (``latent_decode_workspace_bytes``;
+    made here if it is not given or too small).  Scores, softmax statistics and
+    sums are float32; the absorbed q, the softmax weights and the latent-wide
+    result are rounded to bf16 for the matrix cores.
+    """
+    batch, dr, nb, bs = _check_q(q_nope, q_rope, latent_cache, weights)
+    bt = _check_table(block_tables, batch, q_nope)
+    lens = check_tokens("lengths", lengths, batch, q_nope)
+    out = _output(out, (batch, weights.num_heads, weights.v_dim), q_nope)
+    if batch == 0:
+        return out
+    need = latent_decode_workspace_bytes(batch, weights, bt.shape[1], bs)
+    ws = _workspace(workspace, need, q_nope)
+    with on_device(q_nope):
+        _lib.call("pa_latent_decode", q_nope.data_ptr(), q_nope.stride(0), q_nope.stride(1), q_rope.data_ptr(),
+                  q_rope.stride(0), q_rope.stride(1), latent_cache.data_ptr(), nb, bs, latent_cache.stride(0),
+                  latent_cache.stride(1), bt.data_ptr(), bt.stride(0), bt.shape[1], lens.data_ptr(), batch,
+                  weights.num_heads, weights.latent_dim, dr, weights.nope_dim, weights.v_dim,
+                  weights.w_uk_t.data_ptr(), weights.w_kv.data_ptr(), float(scale), out.data_ptr(), out.stride(0),
+                  out.stride(1), ws.data_ptr(), ws.numel() * ws.element_size(), stream_handle(q_nope))
+    return out
+
+
+def latent_decode_workspace_bytes(batch: int, weights: LatentWeights, pages_per_seq: int, page_size: int) -> int:
+    """Bytes of the workspace of a :func:`latent_decode_attention` call."""
+    return int(_lib.load().pa_latent_decode_workspace_size(batch, weights.num_heads, weights.latent_dim,
+                                                           pages_per_seq, page_size))
