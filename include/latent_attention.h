@@ -84,6 +84,39 @@ int pa_latent_decode(const uint16_t* q_nope, int64_t qn_tok_stride, int64_t qn_h
                      int64_t out_tok_stride, int64_t out_head_stride, void* workspace,
                      size_t workspace_bytes, void* stream);
 
+/*
+ * Ragged causal prefill: q_nope [num_tokens, num_heads, nope_dim], q_rope
+ * [num_tokens, num_heads, rope_dim] (rotated); sequence b has rows
+ * cu_seqlens_q[b] .. cu_seqlens_q[b + 1] (the first max_seqlen_q of them are
+ * computed) over lk cached ones, itself among them, given by cu_seqlens_k or by
+ * kv_lens (one of the two); row i sees the first lk - lq + i + 1.  A row that sees none is
+ * zero; rows outside the sequences are zeroed with zero_rest, else left alone.
+ * total_kv bounds the sum of the kv lengths (rows past it are dropped).
+ *
+ * pa_latent_prefill_route says which form a launch takes: K and V expanded for
+ * a group of heads at a time, or the absorbed form of pa_latent_decode for few
+ * new tokens behind long contexts; the workspace follows it.  1 .. 65535 heads.
+ */
+#define PA_LATENT_EXPANDED 0
+#define PA_LATENT_ABSORBED 1
+int pa_latent_prefill_route(int32_t batch, int32_t num_tokens, int32_t max_seqlen_q, int32_t total_kv,
+                            int32_t pages_per_seq, int32_t page_size, int32_t num_heads, int32_t latent_dim,
+                            int32_t rope_dim, int32_t nope_dim);
+size_t pa_latent_prefill_workspace_size(int32_t batch, int32_t num_tokens, int32_t max_seqlen_q,
+                                        int32_t total_kv, int32_t pages_per_seq, int32_t page_size,
+                                        int32_t num_heads, int32_t latent_dim, int32_t rope_dim,
+                                        int32_t nope_dim);
+int pa_latent_prefill(const uint16_t* q_nope, int64_t qn_tok_stride, int64_t qn_head_stride,
+                      const uint16_t* q_rope, int64_t qr_tok_stride, int64_t qr_head_stride,
+                      const uint16_t* cache, int32_t num_pages, int32_t page_size, int64_t page_stride,
+                      int64_t slot_stride, const int32_t* block_tables, int64_t bt_stride,
+                      int32_t pages_per_seq, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                      const int32_t* kv_lens, int32_t batch, int32_t num_tokens, int32_t max_seqlen_q,
+                      int32_t total_kv, int32_t num_heads, int32_t latent_dim, int32_t rope_dim,
+                      int32_t nope_dim, int32_t v_dim, const uint16_t* w_uk_t, const uint16_t* w_kv,
+                      float scale, int32_t zero_rest, uint16_t* out, int64_t out_tok_stride,
+                      int64_t out_head_stride, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

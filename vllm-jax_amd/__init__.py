@@ -13,8 +13,9 @@ Public surface (mirrors simpissa/vllm-jax):
   and prefill sequences in one unpadded launch;
 * ``rotary_embedding`` / ``rotary_frequencies`` -- the rotation in general:
   interleaved or half layout, part of the head, scaled for long contexts;
-* ``latent_store`` / ``latent_decode_attention`` with ``LatentWeights`` --
-  attention over a cache of one latent vector a token;
+* ``latent_attention`` with ``LatentWeights`` -- the layer seam for models
+  whose cache holds one latent vector a token, over ``latent_store``,
+  ``latent_decode_attention`` and ``latent_prefill_attention``;
 * ``KVCacheManager`` / ``copy_blocks`` -- the block manager of
   vllm/src/kv_cache_manager.py on a native allocator, with optional prefix
   caching and fork / copy-on-write.
@@ -34,7 +35,8 @@ from .attention import (DecodeAttentionMetadata, MixedAttentionMetadata, Prefill
 from .kernels.decode_paged_attention import decode_paged_attention  # noqa: F401
 from .kernels.mixed_paged_attention import mixed_paged_attention  # noqa: F401
 from .kernels.prefill_paged_attention import prefill_paged_attention  # noqa: F401
-from .latent import (LatentWeights, latent_decode_attention, latent_decode_workspace_bytes,  # noqa: F401
+from .latent import (LatentWeights, latent_attention, latent_decode_attention,  # noqa: F401
+                     latent_decode_workspace_bytes, latent_prefill_attention, latent_prefill_workspace_bytes,
                      latent_store)
 from .rotary import RotaryFrequencies, rotary_embedding, rotary_frequencies  # noqa: F401
 from .kv_cache_manager import Block, KVCacheManager, copy_blocks  # noqa: F401

@@ -193,11 +193,28 @@ SIGNATURES = {
         c_vp, c_i64, c_i64,            # out
         c_vp, c_sz, c_vp,              # workspace, bytes, stream
     ]),
+    "pa_latent_prefill_route": (ctypes.c_int, [c_i32] * 10),
+    "pa_latent_prefill_workspace_size": (c_sz, [c_i32] * 10),
+    "pa_latent_prefill": (ctypes.c_int, [
+        c_vp, c_i64, c_i64,            # q_nope
+        c_vp, c_i64, c_i64,            # q_rope
+        c_vp, c_i32, c_i32,            # cache, num_pages, page_size
+        c_i64, c_i64,                  # page/slot strides
+        c_vp, c_i64, c_i32,            # block_tables, bt_stride, pages_per_seq
+        c_vp, c_vp, c_vp,              # cu_seqlens_q, cu_seqlens_k, kv_lens
+        c_i32, c_i32, c_i32, c_i32,    # batch, num_tokens, max_seqlen_q, total_kv
+        c_i32,                         # heads
+        c_i32, c_i32, c_i32, c_i32,    # latent, rope, nope, v dims
+        c_vp, c_vp, c_f32, c_i32,      # w_uk_t, w_kv, scale, zero_rest
+        c_vp, c_i64, c_i64,            # out
+        c_vp, c_sz, c_vp,              # workspace, bytes, stream
+    ]),
 }
 # pa_decode_quant / pa_prefill_quant: a code_type (PA_CODE_*) before the
 # arguments of pa_decode_fp8 / pa_prefill_fp8
 SIGNATURES["pa_decode_quant"] = (ctypes.c_int, [c_i32] + SIGNATURES["pa_decode_fp8"][1])
 SIGNATURES["pa_prefill_quant"] = (ctypes.c_int, [c_i32] + SIGNATURES["pa_prefill_fp8"][1])
+PA_LATENT_EXPANDED, PA_LATENT_ABSORBED = 0, 1
 PA_CODE_E4M3, PA_CODE_INT8, PA_CODE_UINT8 = 0, 1, 2
 
 

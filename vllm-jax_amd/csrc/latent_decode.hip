@@ -23,8 +23,10 @@
 // workgroup that gets the whole of a unit writes its rows, one that gets a
 // part leaves O (float32), maximum and sum to latent_merge_kernel.
 #include <algorithm>
+#include <cmath>
 
 #include "latent_attend.h"
+#include "lds_tiles.h"
 #include "pa_errors.h"
 #include "../../include/latent_attention.h"
 
@@ -38,27 +40,6 @@ constexpr int kLThreads = 512;
 constexpr int kMaxBatch = 16384;  // their prefix sums fit the ring
 constexpr float kSlack = 8.f;  // log2 units the running maximum may lag
 constexpr float kNoMax = -1e30f;
-
-typedef s16x4 __attribute__((address_space(3))) * lds_tr_ptr;
-typedef void __attribute__((address_space(3))) * lds_void;
-typedef const char __attribute__((address_space(3))) * lds_bytes;
-
-__device__ __forceinline__ u32x4 lds_ld16(uint32_t a) {
-  return *reinterpret_cast<const u32x4 __attribute__((address_space(3)))*>((lds_bytes)(uintptr_t)a);
-}
-__device__ __forceinline__ u32x2 lds_tr8(uint32_t a) {
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(uintptr_t)a));
-}
-__device__ __forceinline__ void lds_dma16(const void* g, uint32_t block) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(block) : "memory", "m0");
-}
-// s_waitcnt vmcnt(N), other counters untouched
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  static_assert(N < 16);
-  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8));
-}
-__device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8)); }
 
 struct AttnParams {
   LatentAttn a;
@@ -92,29 +73,30 @@ struct Dims {
   static_assert(kLds <= 160 * 1024 && kRing >= 4 * kMaxBatch + 64, "LDS");
 };
 
-// 16-byte chunk swizzles (XOR on the chunk's low bits), so that 16 rows' reads
-// of one chunk and the transposing reads' four rows fall on distinct banks.
-__device__ __forceinline__ int lat_swz(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
 template <int DR>
 __device__ __forceinline__ int rope_swz(int r) {
-  return DR == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
+  return DR == 64 ? swz128(r) : swz64(r);
 }
 
 struct Seq {
   int q0, lq, lk, nt, nrt;
+  int first;  // token i sees first + i + 1 rows
 };
 
 __device__ __forceinline__ Seq seq_of(const AttnParams& p, int b, int rows) {
   Seq s;
   s.q0 = b;
   s.lq = 1;
+  int lq_all = 1;
   if (p.a.cu_q) {
     s.q0 = p.a.cu_q[b];
-    s.lq = min(p.a.cu_q[b + 1] - s.q0, p.a.max_q);
+    lq_all = p.a.cu_q[b + 1] - s.q0;
+    s.lq = min(lq_all, p.a.max_q);
     if (s.q0 < 0 || s.q0 >= p.a.num_tokens) s.lq = 0;
     s.lq = max(0, min(s.lq, p.a.num_tokens - s.q0));
   }
   s.lk = latent_kv_len(p.a.pool, p.a.kv_lens ? p.a.kv_lens[b] : p.a.cu_k[b + 1] - p.a.cu_k[b]);
+  s.first = s.lk - lq_all;
   s.nt = (s.lk + kTile - 1) / kTile;
   s.nrt = (s.lq * p.a.heads + rows - 1) / rows;
   return s;
@@ -227,7 +209,7 @@ latent_attn_kernel(AttnParams p) {
         const uint16_t* r = D::kRowsPerDma == 1 ? rp[i] : (sub ? rp[2 * i + 1] : rp[2 * i]);
         const int row = 4 * wave + i * D::kRowsPerDma + sub;
         const int c = lane & (D::kRowB / 16 - 1);
-        lds_dma16(r + 8 * (c ^ lat_swz(row)), st + (uint32_t)(4 * wave * D::kRowB + i * 1024));
+        lds_dma16(r + 8 * (c ^ swz256(row)), st + (uint32_t)(4 * wave * D::kRowB + i * 1024));
       }
       constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
       if (lane < 4 * kC) {
@@ -240,13 +222,6 @@ latent_attn_kernel(AttnParams p) {
     issue(t0);
     if (t0 + 1 < t1) issue(t0 + 1);
 
-    auto barrier = [&]() __attribute__((always_inline)) {
-      asm volatile("" ::: "memory");  // LDS accesses stay on their side
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("" ::: "memory");
-    };
     // end of step t: this wave's share of tile t + 1 has landed
     auto landed = [&](int t) __attribute__((always_inline)) {
       if (t + 2 < t1) wait_vm<D::kDma>();
@@ -263,7 +238,7 @@ latent_attn_kernel(AttnParams p) {
       for (int r = 0; r < D::kNr; ++r) {
         const int row = rt * ROWS + min(rw + 16 * r + l16, n_rows - 1);
         const int tok = (int)div_by((uint32_t)row, p.heads), hd = row - tok * p.a.heads;
-        lim[r] = min(lk, max(0, lk - sq.lq + tok + 1));
+        lim[r] = min(lk, max(0, sq.first + tok + 1));
         const uint16_t* ql = p.a.q_lat + (int64_t)(sq.q0 + tok) * p.a.ql_ts + hd * p.a.ql_hs + 8 * qd;
         const uint16_t* qr = p.a.q_rope + (int64_t)(sq.q0 + tok) * p.a.qr_ts + hd * p.a.qr_hs + 8 * qd;
 #pragma unroll
@@ -273,7 +248,7 @@ latent_attn_kernel(AttnParams p) {
       }
       // first tile a row of this tile does not see in full
       const int tok_first = (int)div_by((uint32_t)(rt * ROWS), p.heads);
-      const int free_tiles = max(0, min(lk, lk - sq.lq + tok_first + 1)) / kTile;
+      const int free_tiles = max(0, min(lk, sq.first + tok_first + 1)) / kTile;
       float m_ref[D::kNr], l_sum[D::kNr];
 #pragma unroll
       for (int r = 0; r < D::kNr; ++r) {
@@ -284,7 +259,7 @@ latent_attn_kernel(AttnParams p) {
       const int krow = 16 * tb + l16;
       uint32_t koff[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) koff[i] = lds0 + krow * D::kRowB + 16 * ((4 * i + qd) ^ lat_swz(krow));
+      for (int i = 0; i < 4; ++i) koff[i] = lds0 + krow * D::kRowB + 16 * ((4 * i + qd) ^ swz256(krow));
       uint32_t roff[D::kRs];
 #pragma unroll
       for (int i = 0; i < D::kRs; ++i)
@@ -292,7 +267,7 @@ latent_attn_kernel(AttnParams p) {
       float* maxes = reinterpret_cast<float*>(smem + D::kMaxOff);
       float* corrs = reinterpret_cast<float*>(smem + D::kCorrOff);
       wait_vm<0>();  // Q and both tiles
-      barrier();
+      lds_barrier();
       for (int t = t0; t <= t1; ++t) {
         if (t + 2 < t1) issue(t + 2);
         f32x4 s[D::kNr];
@@ -332,7 +307,7 @@ latent_attn_kernel(AttnParams p) {
           }
         }
         wait_lgkm0();
-        barrier();
+        lds_barrier();
         if (t < t1) {
 #pragma unroll
           for (int r = 0; r < D::kNr; ++r) {
@@ -355,7 +330,7 @@ latent_attn_kernel(AttnParams p) {
         }
         landed(t);
         wait_lgkm0();
-        barrier();
+        lds_barrier();
       }
       // ---- row sums and maxima
       float* sums = reinterpret_cast<float*>(smem + D::kSumOff);
@@ -369,7 +344,7 @@ latent_attn_kernel(AttnParams p) {
         }
       }
       wait_lgkm0();
-      barrier();
+      lds_barrier();
     } else {
       // ================= values
       const int pw = wave - 4;
@@ -383,8 +358,8 @@ latent_attn_kernel(AttnParams p) {
 #pragma unroll
       for (int dt = 0; dt < D::kDt; ++dt) {
         const int c = 4 * (pw * D::kDt + dt) + 2 * (gamma & 1) + ((ts & 3) >> 1);
-        voff0[dt] = lds0 + tr * D::kRowB + 16 * (c ^ lat_swz(tr)) + 8 * (ts & 1);
-        voff1[dt] = lds0 + (tr + 8) * D::kRowB + 16 * (c ^ lat_swz(tr + 8)) + 8 * (ts & 1);
+        voff0[dt] = lds0 + tr * D::kRowB + 16 * (c ^ swz256(tr)) + 8 * (ts & 1);
+        voff1[dt] = lds0 + (tr + 8) * D::kRowB + 16 * (c ^ swz256(tr + 8)) + 8 * (ts & 1);
       }
       uint32_t poff[D::kRb][2];
 #pragma unroll
@@ -394,7 +369,7 @@ latent_attn_kernel(AttnParams p) {
           poff[rb][u] = lds0 + D::kPOff + (32 * rb + n) * 64 + 16 * ((2 * u + h) ^ ((n >> 2) & 3));
       const float* corrs = reinterpret_cast<const float*>(smem + D::kCorrOff);
       wait_vm<0>();
-      barrier();
+      lds_barrier();
       bf16x8 pt[D::kRb][2];
       auto product = [&](int u, uint32_t st) __attribute__((always_inline)) {
 #pragma unroll
@@ -426,13 +401,13 @@ latent_attn_kernel(AttnParams p) {
           product(0, st);
         }
         wait_lgkm0();  // P is in registers: the score waves may overwrite it
-        barrier();
+        lds_barrier();
         if (t > t0) product(1, st);
         landed(t);
         wait_lgkm0();
-        barrier();
+        lds_barrier();
       }
-      barrier();  // sums are there
+      lds_barrier();  // sums are there
       const float* sums = reinterpret_cast<const float*>(smem + D::kSumOff);
       if (t0 == 0 && t1 == sq.nt) {
 #pragma unroll
@@ -654,6 +629,7 @@ extern "C" int pa_latent_decode(const uint16_t* q_nope, int64_t qn_tok_stride, i
     return fail(PA_ERR_UNSUPPORTED, "%s: latent_dim %d, rope_dim %d, nope_dim %d, v_dim %d not supported", name,
                 latent_dim, rope_dim, nope_dim, v_dim);
   if (num_heads > 65535) return fail(PA_ERR_UNSUPPORTED, "%s: %d heads", name, num_heads);
+  if (!(scale > 0.f) || !(scale < INFINITY)) return fail(PA_ERR_INVALID_ARGUMENT, "%s: scale must be positive", name);
   if (batch == 0) return PA_OK;
   if (!q_nope || !q_rope || !cache || !lengths || !w_uk_t || !w_kv || !out || (pages_per_seq && !block_tables))
     return fail(PA_ERR_INVALID_ARGUMENT, "%s: null pointer", name);

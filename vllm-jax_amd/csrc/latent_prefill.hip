@@ -1,0 +1,646 @@
+// Expanded-form latent attention for gfx950: ragged causal attention of new
+// tokens over expanded K and V rows, key size DN + DR (the rotary part shared by
+// all heads), value size DN.
+//
+// Workgroup = 256 query rows of one (sequence, head), eight waves of 32 rows.
+// kv tiles of 64 tokens come by direct loads into three-stage LDS rings, K's
+// unrotated part, K's rotary part and V apart, since K of a tile is read one
+// half step before its V:
+//   S^T[t][n] = K[t] . Q[n]     v_mfma_f32_32x32x16_bf16, K by 16-byte reads, Q^T
+//                               in registers
+//   O^T[d][n] += V^T P^T        V^T by transposing reads, P^T from the accumulators
+// Waves 0-3 and 4-7 share the SIMDs pairwise and run the same sequence half a
+// step apart, so that one wave's softmax runs under the other's products:
+//   segment 2t:   A: PV(t-1), QK(t)   B: softmax(t-1)
+//   segment 2t+1: A: softmax(t)       B: PV(t-1), QK(t)
+// with a barrier behind every segment.  Of tile T, A issues its share of K(T)
+// and V(T-1) behind its QK(T-2) and waits for it behind softmax(T-1); B issues
+// half a step earlier, behind QK(T-3), and waits behind softmax(T-2).  K(T)
+// overwrites K(T-3), last read by B in segment 2T-5; V(T-1) overwrites V(T-4),
+// last read by B in segment 2T-5 as well; both are issued in 2T-4 or later.
+//
+// Rows: the softmax reference of a row moves only when its maximum grows by
+// more than 2^8, so O is rarely rescaled; the exponent is one fused
+// multiply-add (scores are float32 sums of unscaled bf16 products).
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "latent_attend.h"
+#include "lds_tiles.h"
+#include "pa_errors.h"
+#include "../../include/latent_attention.h"
+
+namespace pa {
+namespace {
+
+constexpr int kRWaves = 8, kRThreads = 64 * kRWaves, kRRows = 32 * kRWaves;
+constexpr int kRTile = 64, kRStages = 3;
+constexpr float kRSlack = 8.f;
+
+struct RaggedParams {
+  LatentRagged r;
+  float scale_log2;
+  int32_t n_qtiles;
+};
+
+template <int DN, int DR>
+struct RDims {
+  static constexpr int kKB = 2 * DN, kRB = 2 * DR;  // bytes of a K, V and a rotary row
+  static constexpr int kKStage = kRTile * kKB, kRStage = kRTile * kRB;
+  static constexpr int kKOff = 0, kROff = kRStages * kKStage, kVOff = kROff + kRStages * kRStage;
+  static constexpr int kLds = kVOff + kRStages * kKStage;
+  static constexpr int kKDma = kKStage / (1024 * kRWaves);  // loads of a wave per tile of K and of V
+  static constexpr int kRowsK = 1024 / kKB;                 // rows of a load
+  static constexpr int kDma = 2 * kKDma + 1;
+  static constexpr int kKs = DN / 16, kRs = DR / 16;
+  static constexpr int kDt = DN / 32;
+};
+
+// s_waitcnt vmcnt(N) lgkmcnt(0)
+template <int N>
+__device__ __forceinline__ void wait_vm_lgkm() {
+  static_assert(N < 16);
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4));
+}
+
+template <int DN>
+__device__ __forceinline__ int k_swz(int r) {
+  return DN == 128 ? swz256(r) : swz128(r);
+}
+template <int DN>
+__device__ __forceinline__ int v_swz(int r) {
+  return DN == 128 ? swz256(r) : value_swz128(r);
+}
+template <int DR>
+__device__ __forceinline__ int r_swz(int r) {
+  return DR == 64 ? swz128(r) : swz64(r);
+}
+
+// Zeroes the rows of 512 tokens from t0 on that no sequence has.
+template <int DN>
+__device__ __forceinline__ void zero_rows(const LatentRagged& p, int64_t t0) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int i = wave; i < kRThreads; i += kRWaves) {
+    const int64_t t = t0 + i;
+    if (t >= p.num_tokens) return;
+    if (token_in_sequence(p.cu_q, p.batch, p.max_q, (int)t)) continue;
+    uint16_t* row = p.zero_out + t * p.o_ts;
+    for (int c = lane; c < p.zero_heads * (DN / 8); c += 64)
+      st16(row + (c / (DN / 8)) * p.o_hs + (c % (DN / 8)) * 8, u32x4{0, 0, 0, 0});
+  }
+}
+
+template <int DN, int DR>
+__global__ void __launch_bounds__(kRThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+latent_ragged_kernel(RaggedParams prm) {
+  using D = RDims<DN, DR>;
+  const LatentRagged& p = prm.r;
+  __shared__ __attribute__((aligned(1024))) char smem[D::kLds];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void)smem;
+  // Items from the last query tile down (the longest rows first); within a
+  // level (sequence, head) pairs in order, so that with a multiple of eight
+  // heads all query tiles of a pair run on one XCD and share its L2.
+  const int pairs = p.batch * p.heads;
+  const int level = blockIdx.x / pairs, pair = blockIdx.x - level * pairs;
+  if (level >= prm.n_qtiles) {
+    zero_rows<DN>(p, ((int64_t)blockIdx.x - (int64_t)prm.n_qtiles * pairs) * kRThreads);
+    return;
+  }
+  const int qt = prm.n_qtiles - 1 - level;
+  const int b = pair / p.heads, head = pair - b * p.heads;
+  const int q0 = p.cu_q[b];
+  const int lq_all = p.cu_q[b + 1] - q0;
+  const int lq = q0 < 0 || q0 >= p.num_tokens ? 0 : min(min(lq_all, p.max_q), p.num_tokens - q0);
+  if (qt * kRRows >= lq) return;
+  const int kbase = p.cu_k[b] - p.cu_k[0];
+  const int lk_all = max(0, min(p.cu_k[b + 1] - p.cu_k[b], p.span));
+  const int lk = kbase < 0 || kbase >= p.cap ? 0 : min(lk_all, p.cap - kbase);
+  const int first = lk_all - lq_all;  // row i sees first + i + 1 keys
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  const int row = qt * kRRows + 32 * wave + n;
+  const bool wave_live = qt * kRRows + 32 * wave < lq;
+  // tokens this row sees (rows past the sequence's end compute on its last row
+  // and store nothing)
+  const int seen = min(lk, max(0, first + min(row, lq - 1) + 1));
+  const int kv_hi = min(lk, max(0, first + min(lq, (qt + 1) * kRRows)));
+  const int n_tiles = (kv_hi + kRTile - 1) / kRTile;
+  const int n_free = min(lk, max(0, first + qt * kRRows + 1)) / kRTile;
+
+  const uint16_t* kv = p.kv + ((int64_t)head * p.cap + kbase) * (2 * DN);
+  const uint16_t* kr = p.k_rope + (int64_t)kbase * DR;
+
+  // ---- Q^T
+  bf16x8 q[D::kKs + D::kRs];
+  {
+    const int64_t t = q0 + min(row, lq - 1);
+    const uint16_t* qn = p.q_nope + t * p.qn_ts + head * p.qn_hs + 8 * h;
+    const uint16_t* qr = p.q_rope + t * p.qr_ts + head * p.qr_hs + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < D::kKs; ++ks) q[ks] = as_bf16x8(ld16(qn + 16 * ks));
+#pragma unroll
+    for (int ks = 0; ks < D::kRs; ++ks) q[D::kKs + ks] = as_bf16x8(ld16(qr + 16 * ks));
+  }
+
+  // ---- tile loads: this wave's rows of a tile are 8 wave .. 8 wave + 7
+  auto issue_k = [&](int t, int st) __attribute__((always_inline)) {
+    const int last = max(lk - 1 - t * kRTile, 0);  // rows past the end repeat the last one
+    const int64_t j0 = min(t * kRTile, max(lk - 1, 0));
+#pragma unroll
+    for (int i = 0; i < D::kKDma; ++i) {
+      const int r = 8 * wave + i * D::kRowsK + lane / (D::kKB / 16);
+      const int c = lane & (D::kKB / 16 - 1);
+      lds_dma16(kv + (j0 + min(r, last)) * (2 * DN) + 8 * (c ^ k_swz<DN>(r)),
+                lds0 + (uint32_t)(D::kKOff + st * D::kKStage + 8 * wave * D::kKB + 1024 * i));
+    }
+    constexpr int kC = D::kRB / 16;
+    if (lane < 8 * kC) {
+      const int r = 8 * wave + lane / kC, c = lane & (kC - 1);
+      lds_dma16(kr + (j0 + min(r, last)) * DR + 8 * (c ^ r_swz<DR>(r)),
+                lds0 + (uint32_t)(D::kROff + st * D::kRStage + 8 * wave * D::kRB));
+    }
+  };
+  auto issue_v = [&](int t, int st) __attribute__((always_inline)) {
+    const int last = max(lk - 1 - t * kRTile, 0);
+    const int64_t j0 = min(t * kRTile, max(lk - 1, 0));
+#pragma unroll
+    for (int i = 0; i < D::kKDma; ++i) {
+      const int r = 8 * wave + i * D::kRowsK + lane / (D::kKB / 16);
+      const int c = lane & (D::kKB / 16 - 1);
+      lds_dma16(kv + (j0 + min(r, last)) * (2 * DN) + DN + 8 * (c ^ v_swz<DN>(r)),
+                lds0 + (uint32_t)(D::kVOff + st * D::kKStage + 8 * wave * D::kKB + 1024 * i));
+    }
+  };
+
+  // ---- LDS read addresses
+  constexpr int kKAddr = D::kKs < 8 ? D::kKs : 8;
+  uint32_t koff[kKAddr], roff[D::kRs];
+#pragma unroll
+  for (int ks = 0; ks < kKAddr; ++ks)
+    koff[ks] = lds0 + D::kKOff + n * D::kKB + 16 * ((2 * ks + h) ^ k_swz<DN>(n));
+#pragma unroll
+  for (int ks = 0; ks < D::kRs; ++ks)
+    roff[ks] = lds0 + D::kROff + n * D::kRB + 16 * ((2 * ks + h) ^ r_swz<DR>(n));
+  const int ts = lane & 15, gamma = lane >> 4, tr = 4 * h + (ts >> 2);
+  uint32_t voff0[D::kDt], voff1[D::kDt];
+#pragma unroll
+  for (int dt = 0; dt < D::kDt; ++dt) {
+    const int c = 4 * dt + 2 * (gamma & 1) + ((ts & 3) >> 1);
+    voff0[dt] = lds0 + D::kVOff + tr * D::kKB + 16 * (c ^ v_swz<DN>(tr)) + 8 * (ts & 1);
+    voff1[dt] = lds0 + D::kVOff + (tr + 8) * D::kKB + 16 * (c ^ v_swz<DN>(tr + 8)) + 8 * (ts & 1);
+  }
+
+  f32x16 acc[D::kDt] = {};
+  float m_ref = 0.f;
+  float l_part[4] = {};
+  f32x16 s[2];
+  bf16x8 pt[4];
+
+  auto qk = [&](auto kst) __attribute__((always_inline)) {
+    constexpr int st = decltype(kst)::value;
+#pragma unroll
+    for (int ks = 0; ks < D::kKs + D::kRs; ++ks)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const uint32_t a = ks < D::kKs ? koff[ks % kKAddr] + st * D::kKStage + mt * (32 * D::kKB)
+                                       : roff[(ks - D::kKs) % D::kRs] + st * D::kRStage + mt * (32 * D::kRB);
+        s[mt] = mfma32(as_bf16x8(lds_ld16(a)), q[ks], ks == 0 ? f32x16{} : s[mt]);
+      }
+  };
+  auto pv = [&](int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int dt = 0; dt < D::kDt; ++dt) {
+        const u32x2 lo = lds_tr8(voff0[dt] + st * D::kKStage + 16 * u * D::kKB);
+        const u32x2 hi = lds_tr8(voff1[dt] + st * D::kKStage + 16 * u * D::kKB);
+        acc[dt] = mfma32(as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]}), pt[u], acc[dt]);
+      }
+  };
+  const float scale = prm.scale_log2;
+  auto softmax = [&](int t, auto&& between) __attribute__((always_inline)) {
+    // s[mt][i] is token 64 t + 32 mt + 8 (i / 4) + 4 h + i % 4
+    if (t >= n_free) {
+      int lim = min(max(seen - t * kRTile - 4 * h, 0), kRTile);
+      asm volatile("" : "+v"(lim));
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[mt][i] = 32 * mt + 8 * (i >> 2) + (i & 3) < lim ? s[mt][i] : -INFINITY;
+    }
+    float mq[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f32x16& v = s[k >> 1];
+      const int b0 = 8 * (k & 1);
+      float m = __builtin_fmaxf(__builtin_fmaxf(v[b0], v[b0 + 1]), v[b0 + 2]);
+      m = __builtin_fmaxf(__builtin_fmaxf(m, v[b0 + 3]), v[b0 + 4]);
+      m = __builtin_fmaxf(__builtin_fmaxf(m, v[b0 + 5]), v[b0 + 6]);
+      mq[k] = __builtin_fmaxf(m, v[b0 + 7]);
+    }
+    const float mx = max_xor32(__builtin_fmaxf(__builtin_fmaxf(mq[0], mq[1]), __builtin_fmaxf(mq[2], mq[3])));
+    const float up = mx * scale - m_ref;  // the scale is positive
+    if (t == 0 || __any(up > kRSlack)) {
+      // the first tile sets the reference to the row's maximum (a row that
+      // sees no key keeps 0)
+      const float d = t == 0 ? (mx == -INFINITY ? 0.f : up) : __builtin_fmaxf(up, 0.f);
+      if (t != 0) {
+        const float corr = fast_exp2(-d);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) l_part[u] *= corr;
+#pragma unroll
+        for (int dt = 0; dt < D::kDt; ++dt) acc[dt] = acc[dt] * corr;
+      }
+      m_ref += d;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      between(u);
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = fast_exp2(__builtin_fmaf(s[u >> 1][8 * (u & 1) + 2 * e], scale, -m_ref));
+        const float c = fast_exp2(__builtin_fmaf(s[u >> 1][8 * (u & 1) + 2 * e + 1], scale, -m_ref));
+        w[e] = pack_bf16x2(a, c);
+        l_part[u] += a + c;
+      }
+      pt[u] = as_bf16x8(w);
+      asm volatile("" : "+v"(pt[u]));  // made here, not in the next product segment
+    }
+    asm volatile("" : "+v"(l_part[0]), "+v"(l_part[1]), "+v"(l_part[2]), "+v"(l_part[3]));
+  };
+
+  const bool grp_b = wave >= kRWaves / 2;
+  using T_ = std::true_type;
+  using F_ = std::false_type;
+  auto iteration = [&](int t, auto stc, auto has_pv) __attribute__((always_inline)) {
+    constexpr int st = decltype(stc)::value;  // t % 3
+    constexpr bool kPv = decltype(has_pv)::value;
+    if (!kPv || wave_live) {
+      if constexpr (kPv) pv((st + 2) % 3);
+      qk(stc);
+    }
+    wait_lgkm0();
+    lds_barrier();
+    const int tk = t + (grp_b ? 3 : 2);  // K of tile tk, V of tile tk - 1
+    const int ks = grp_b ? st : (st + 2) % 3, vs = grp_b ? (st + 2) % 3 : (st + 1) % 3;
+    auto between = [&](int u) __attribute__((always_inline)) {
+      if (u == 0) issue_k(tk, ks);
+      if (u == 2) issue_v(tk - 1, vs);
+    };
+    if (!kPv || wave_live) {
+      softmax(t, between);
+    } else {
+      between(0);
+      between(2);
+    }
+    wait_vm_lgkm<D::kDma>();
+    lds_barrier();
+  };
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+  using S2 = std::integral_constant<int, 2>;
+
+  wait_vm<0>();  // Q is here; from now on vmcnt counts the tile loads
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int ks = 0; ks < D::kKs + D::kRs; ++ks) asm volatile("" : "+v"(q[ks]));
+  if (n_tiles > 0) {
+    issue_k(0, 0);
+    issue_k(1, 1);
+    issue_v(0, 0);
+    if (grp_b) {
+      issue_k(2, 2);
+      issue_v(1, 1);
+      wait_vm<2 * D::kDma>();
+    } else {
+      wait_vm<D::kDma>();
+    }
+    lds_barrier();
+    if (grp_b) {
+      wait_vm<D::kDma>();
+      lds_barrier();
+    }
+    iteration(0, S0{}, F_{});
+    int last = 0;  // stage of the last tile
+    for (int t = 1; t < n_tiles; ++t) {
+      iteration(t, S1{}, T_{});
+      last = 1;
+      if (++t == n_tiles) break;
+      iteration(t, S2{}, T_{});
+      last = 2;
+      if (++t == n_tiles) break;
+      iteration(t, S0{}, T_{});
+      last = 0;
+    }
+    // V of the last tile: A's share landed an iteration ago, B's before that
+    pv(last);
+    wait_vm_lgkm<0>();  // loads of tiles past the end may still be in flight
+    if (!grp_b) lds_barrier();
+  }
+
+  const float l = sum_xor32((l_part[0] + l_part[1]) + (l_part[2] + l_part[3]));
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (row < lq) {
+    uint16_t* o = p.out + (int64_t)(q0 + row) * p.o_ts + head * p.o_hs + 4 * h;
+#pragma unroll
+    for (int dt = 0; dt < D::kDt; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<u32x2*>(o + 32 * dt + 8 * i) =
+            u32x2{pack_bf16x2(acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv),
+                  pack_bf16x2(acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv)};
+  }
+}
+
+template <int DN, int DR>
+int ragged_launch(const char* name, const RaggedParams& p, hipStream_t s) {
+  const int64_t zero = p.r.zero_out ? ((int64_t)p.r.num_tokens + kRThreads - 1) / kRThreads : 0;
+  const int64_t blocks = (int64_t)p.n_qtiles * p.r.batch * p.r.heads + zero;
+  if (blocks > 0x7fffffff) return fail(PA_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)blocks);
+  if (blocks == 0) return PA_OK;
+  latent_ragged_kernel<DN, DR><<<dim3((unsigned)blocks), kRThreads, 0, s>>>(p);
+  return launch_status(name);
+}
+
+}  // namespace
+
+int latent_ragged_launch(const char* name, const LatentRagged& r, int nope, int rope, hipStream_t s) {
+  RaggedParams p;
+  p.r = r;
+  p.scale_log2 = r.scale * kLog2e;
+  p.n_qtiles = (r.max_q + kRRows - 1) / kRRows;
+  if (nope == 128) return rope == 64 ? ragged_launch<128, 64>(name, p, s) : ragged_launch<128, 32>(name, p, s);
+  return rope == 64 ? ragged_launch<64, 64>(name, p, s) : ragged_launch<64, 32>(name, p, s);
+}
+
+// Exclusive sums of the sequences' kv lengths, one workgroup.
+__global__ void __launch_bounds__(256) latent_sum_kernel(const int32_t* lens, int batch, int64_t span, int32_t* cu) {
+  __shared__ int tmp[256];
+  int base = 0;
+  for (int c = 0; c < batch; c += 256) {
+    const int b = c + threadIdx.x;
+    const int v = b < batch ? (int)max((int64_t)0, min((int64_t)lens[b], span)) : 0;
+    int total;
+    const int before = block_exclusive_scan<256>(v, tmp, total);
+    if (b < batch) cu[b] = base + before;
+    base += total;
+  }
+  if (threadIdx.x == 0) cu[batch] = base;
+}
+
+int latent_sum_launch(const char* name, const int32_t* lens, int batch, int64_t span, int32_t* cu, hipStream_t s) {
+  latent_sum_kernel<<<1, 256, 0, s>>>(lens, batch, span, cu);
+  return launch_status(name);
+}
+
+}  // namespace pa
+
+using namespace pa;
+
+namespace {
+
+constexpr size_t kGroupBytes = (size_t)2 << 30;  // K and V rows expanded at a time
+
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+struct PrefillPlan {
+  bool absorbed;
+  size_t cu, q_lat, attn;  // bytes: running kv lengths, absorbed q (and as much of results), the attention's own
+  size_t k_rope, kv;       // expanded rotary parts, K and V rows of `group` heads
+  int32_t group;
+  size_t need;
+};
+
+// Which form runs, by the operations of both with sequences of equal length:
+// the absorbed form multiplies each (query, key) pair R + Dr and R wide, the
+// expanded one Dn + Dr and Dn wide but expands every cached token first.
+bool absorbed_form(int32_t batch, int32_t num_tokens, int32_t max_q, int32_t total_kv, int32_t latent, int32_t rope,
+                   int32_t nope) {
+  const double tokens = std::min((double)num_tokens, (double)batch * max_q);
+  const double kv = (double)total_kv / batch, q = std::min(tokens / batch, kv);
+  const double pairs = tokens * (kv - q / 2);
+  const double product = 2. * nope * latent;
+  return pairs * (2 * latent + rope) + tokens * product < pairs * (2 * nope + rope) + total_kv * product;
+}
+
+int plan(const char* name, int32_t batch, int32_t num_tokens, int32_t max_q, int32_t total_kv, int32_t pages_per_seq,
+         int32_t page_size, int32_t heads, int32_t latent, int32_t rope, int32_t nope, PrefillPlan& p) {
+  p = PrefillPlan{};
+  p.absorbed = absorbed_form(batch, num_tokens, max_q, total_kv, latent, rope, nope);
+  p.cu = up256(4 * ((size_t)batch + 1));
+  if (p.absorbed) {
+    const char* why;
+    p.attn = latent_attn_workspace(batch, max_q, heads, latent, (int64_t)pages_per_seq * page_size, &why);
+    if (why) {
+      p.absorbed = false;  // sizes past the absorbed kernel's: the expanded form takes them
+    } else {
+      p.q_lat = up256((size_t)num_tokens * heads * latent * 2);
+      p.need = 2 * p.q_lat + p.attn;
+      return PA_OK;
+    }
+  }
+  const size_t head = (size_t)total_kv * 2 * nope * 2;
+  size_t g = head ? kGroupBytes / head : heads;
+  if (g >= 8) g &= ~(size_t)7;
+  p.group = (int32_t)std::max<size_t>(1, std::min<size_t>(g, heads));
+  p.k_rope = up256((size_t)total_kv * rope * 2);
+  p.kv = up256(head * p.group);
+  p.need = p.cu + p.k_rope + p.kv;
+  (void)name;
+  return PA_OK;
+}
+
+bool prefill_sizes_ok(int32_t batch, int32_t num_tokens, int32_t max_q, int32_t total_kv, int32_t pages_per_seq,
+                      int32_t page_size, int32_t heads, int32_t latent, int32_t rope, int32_t nope) {
+  return batch > 0 && num_tokens >= 0 && max_q >= 0 && total_kv >= 0 && pages_per_seq >= 0 && page_size > 0 &&
+         heads > 0 && latent_dims_ok(latent, rope) && latent_head_ok(nope, nope);
+}
+
+}  // namespace
+
+extern "C" int pa_latent_prefill_route(int32_t batch, int32_t num_tokens, int32_t max_seqlen_q, int32_t total_kv,
+                                       int32_t pages_per_seq, int32_t page_size, int32_t num_heads,
+                                       int32_t latent_dim, int32_t rope_dim, int32_t nope_dim) {
+  if (!prefill_sizes_ok(batch, num_tokens, max_seqlen_q, total_kv, pages_per_seq, page_size, num_heads, latent_dim,
+                        rope_dim, nope_dim))
+    return fail(PA_ERR_INVALID_ARGUMENT, "pa_latent_prefill_route: bad sizes");
+  PrefillPlan p;
+  plan("", batch, num_tokens, max_seqlen_q, total_kv, pages_per_seq, page_size, num_heads, latent_dim, rope_dim,
+       nope_dim, p);
+  return p.absorbed ? PA_LATENT_ABSORBED : PA_LATENT_EXPANDED;
+}
+
+extern "C" size_t pa_latent_prefill_workspace_size(int32_t batch, int32_t num_tokens, int32_t max_seqlen_q,
+                                                   int32_t total_kv, int32_t pages_per_seq, int32_t page_size,
+                                                   int32_t num_heads, int32_t latent_dim, int32_t rope_dim,
+                                                   int32_t nope_dim) {
+  if (!prefill_sizes_ok(batch, num_tokens, max_seqlen_q, total_kv, pages_per_seq, page_size, num_heads, latent_dim,
+                        rope_dim, nope_dim))
+    return 0;
+  PrefillPlan p;
+  plan("", batch, num_tokens, max_seqlen_q, total_kv, pages_per_seq, page_size, num_heads, latent_dim, rope_dim,
+       nope_dim, p);
+  return p.need;
+}
+
+extern "C" int pa_latent_prefill(const uint16_t* q_nope, int64_t qn_tok_stride, int64_t qn_head_stride,
+                                 const uint16_t* q_rope, int64_t qr_tok_stride, int64_t qr_head_stride,
+                                 const uint16_t* cache, int32_t num_pages, int32_t page_size, int64_t page_stride,
+                                 int64_t slot_stride, const int32_t* block_tables, int64_t bt_stride,
+                                 int32_t pages_per_seq, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                 const int32_t* kv_lens, int32_t batch, int32_t num_tokens, int32_t max_seqlen_q,
+                                 int32_t total_kv, int32_t num_heads, int32_t latent_dim, int32_t rope_dim,
+                                 int32_t nope_dim, int32_t v_dim, const uint16_t* w_uk_t, const uint16_t* w_kv,
+                                 float scale, int32_t zero_rest, uint16_t* out, int64_t out_tok_stride,
+                                 int64_t out_head_stride, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* name = "pa_latent_prefill";
+  if (batch < 0 || num_tokens < 0 || max_seqlen_q < 0 || total_kv < 0 || num_heads <= 0 || num_pages <= 0 ||
+      page_size <= 0 || pages_per_seq < 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: bad sizes (batch=%d, num_tokens=%d, max_seqlen_q=%d, total_kv=%d, "
+                "num_heads=%d, num_pages=%d, page_size=%d, pages_per_seq=%d)", name, batch, num_tokens, max_seqlen_q,
+                total_kv, num_heads, num_pages, page_size, pages_per_seq);
+  if (!latent_dims_ok(latent_dim, rope_dim) || !latent_head_ok(nope_dim, v_dim))
+    return fail(PA_ERR_UNSUPPORTED, "%s: latent_dim %d, rope_dim %d, nope_dim %d, v_dim %d not supported", name,
+                latent_dim, rope_dim, nope_dim, v_dim);
+  if (num_heads > 65535) return fail(PA_ERR_UNSUPPORTED, "%s: %d heads", name, num_heads);
+  if (!(scale > 0.f) || !(scale < INFINITY)) return fail(PA_ERR_INVALID_ARGUMENT, "%s: scale must be positive", name);
+  if (batch > 0 && !!cu_seqlens_k == !!kv_lens)
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: one of cu_seqlens_k and kv_lens", name);
+  if (num_tokens == 0 || (batch == 0 && !zero_rest)) return PA_OK;
+  if (!q_nope || !q_rope || !cache || !w_uk_t || !w_kv || !out ||
+      (batch > 0 && (!cu_seqlens_q || (pages_per_seq && !block_tables))))
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+  const uintptr_t align = (uintptr_t)q_nope | (uintptr_t)q_rope | (uintptr_t)cache | (uintptr_t)w_uk_t |
+                          (uintptr_t)w_kv | (uintptr_t)out | (uintptr_t)workspace;
+  if ((align & 15u) || (qn_tok_stride | qn_head_stride | qr_tok_stride | qr_head_stride | page_stride | slot_stride |
+                        out_tok_stride | out_head_stride) % 8)
+    return fail(PA_ERR_UNSUPPORTED, "%s: operands must be 16-byte aligned with strides multiple of 8", name);
+  hipStream_t s = (hipStream_t)stream;
+  LatentRagged r;
+  r.q_nope = q_nope;
+  r.qn_ts = qn_tok_stride;
+  r.qn_hs = qn_head_stride;
+  r.q_rope = q_rope;
+  r.qr_ts = qr_tok_stride;
+  r.qr_hs = qr_head_stride;
+  r.cu_q = cu_seqlens_q;
+  r.batch = batch;
+  r.num_tokens = num_tokens;
+  r.max_q = max_seqlen_q;
+  r.scale = scale;
+  r.o_ts = out_tok_stride;
+  r.o_hs = out_head_stride;
+  r.zero_out = zero_rest ? out : nullptr;
+  r.zero_heads = num_heads;
+  const int64_t span = std::min<int64_t>((int64_t)pages_per_seq * page_size, 0x7fffffff);
+  if (batch == 0 || max_seqlen_q == 0) {  // no rows but those to be zeroed
+    r.batch = 0;
+    r.heads = 1;
+    r.max_q = 0;
+    r.kv = r.k_rope = nullptr;
+    r.cu_k = nullptr;
+    r.cap = r.span = 0;
+    r.out = out;
+    return latent_ragged_launch(name, r, nope_dim, rope_dim, s);
+  }
+  PrefillPlan pl;
+  if (int rc = plan(name, batch, num_tokens, max_seqlen_q, total_kv, pages_per_seq, page_size, num_heads, latent_dim,
+                    rope_dim, nope_dim, pl))
+    return rc;
+  if (!workspace || workspace_bytes < pl.need)
+    return fail(PA_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", name, workspace_bytes, pl.need);
+  const LatentPool pool{cache, num_pages, magic_div((uint32_t)page_size), page_stride, slot_stride,
+                        block_tables, bt_stride, pages_per_seq};
+  char* ws = (char*)workspace;
+  const int64_t head_w = (int64_t)(nope_dim + v_dim) * latent_dim;
+  if (pl.absorbed) {
+    uint16_t* q_lat = (uint16_t*)ws;
+    uint16_t* o_lat = (uint16_t*)(ws + pl.q_lat);
+    HeadProduct hp;
+    hp.x = q_nope;
+    hp.x_ts = qn_tok_stride;
+    hp.x_hs = qn_head_stride;
+    hp.w = w_uk_t;
+    hp.w_hs = (int64_t)latent_dim * nope_dim;
+    hp.y = q_lat;
+    hp.y_ts = (int64_t)num_heads * latent_dim;
+    hp.y_hs = latent_dim;
+    hp.tokens = num_tokens;
+    hp.heads = num_heads;
+    hp.n = latent_dim;
+    hp.k = nope_dim;
+    if (int rc = head_product_launch(name, hp, s)) return rc;
+    LatentAttn a;
+    a.q_lat = q_lat;
+    a.ql_ts = hp.y_ts;
+    a.ql_hs = hp.y_hs;
+    a.q_rope = q_rope;
+    a.qr_ts = qr_tok_stride;
+    a.qr_hs = qr_head_stride;
+    a.pool = pool;
+    a.cu_q = cu_seqlens_q;
+    a.cu_k = cu_seqlens_k;
+    a.kv_lens = kv_lens;
+    a.batch = batch;
+    a.num_tokens = num_tokens;
+    a.heads = num_heads;
+    a.max_q = max_seqlen_q;
+    a.scale = scale;
+    a.out = o_lat;
+    a.o_ts = a.ql_ts;
+    a.o_hs = a.ql_hs;
+    if (int rc = latent_attn_launch(name, a, latent_dim, rope_dim, ws + 2 * pl.q_lat, s)) return rc;
+    hp.x = o_lat;
+    hp.x_ts = a.o_ts;
+    hp.x_hs = a.o_hs;
+    hp.w = w_kv + (int64_t)nope_dim * latent_dim;
+    hp.w_hs = head_w;
+    hp.y = out;
+    hp.y_ts = out_tok_stride;
+    hp.y_hs = out_head_stride;
+    hp.n = v_dim;
+    hp.k = latent_dim;
+    hp.cu_q = cu_seqlens_q;
+    hp.batch = batch;
+    hp.max_q = max_seqlen_q;
+    hp.zero_rest = zero_rest != 0;
+    return head_product_launch(name, hp, s);
+  }
+  const int32_t* cu_k = cu_seqlens_k;
+  if (!cu_k) {
+    int32_t* cu = (int32_t*)ws;
+    if (int rc = latent_sum_launch(name, kv_lens, batch, span, cu, s)) return rc;
+    cu_k = cu;
+  }
+  LatentExpand x;
+  x.pool = pool;
+  x.cu_k = cu_k;
+  x.batch = batch;
+  x.cap = total_kv;
+  x.w_kv = w_kv;
+  x.k_rope = (uint16_t*)(ws + pl.cu);
+  x.kv = (uint16_t*)(ws + pl.cu + pl.k_rope);
+  r.cu_k = cu_k;
+  r.cap = total_kv;
+  r.span = (int32_t)span;
+  r.kv = x.kv;
+  r.k_rope = x.k_rope;
+  for (int32_t h0 = 0; h0 < num_heads; h0 += pl.group) {
+    x.head0 = h0;
+    x.heads = r.heads = std::min(pl.group, num_heads - h0);
+    if (total_kv > 0 && pages_per_seq > 0)
+      if (int rc = latent_expand_launch(name, x, latent_dim, rope_dim, nope_dim, s)) return rc;
+    r.q_nope = q_nope + h0 * qn_head_stride;
+    r.q_rope = q_rope + h0 * qr_head_stride;
+    r.out = out + h0 * out_head_stride;
+    if (int rc = latent_ragged_launch(name, r, nope_dim, rope_dim, s)) return rc;
+    x.k_rope = nullptr;  // the rotary parts and the zeroed rows are done once
+    r.zero_out = nullptr;
+  }
+  return PA_OK;
+}

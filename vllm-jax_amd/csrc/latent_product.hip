@@ -48,6 +48,10 @@ __global__ void __launch_bounds__(256) head_product_kernel(HeadProduct p, int n_
   for (int m = 0; m < MB; ++m) {
     const int t = (mb * MB + m) * 32 + l;
     if (t >= p.tokens) continue;
+    if (p.cu_q && !token_in_sequence(p.cu_q, p.batch, p.max_q, t)) {
+      if (!p.zero_rest) continue;
+      acc[m] = f32x16{};
+    }
     uint16_t* y = p.y + t * p.y_ts + head * p.y_hs + 32 * nb + 4 * h2;
 #pragma unroll
     for (int q = 0; q < 4; ++q)

@@ -12,7 +12,8 @@ slot mappings and block tables as the engine's K/V pool.
 Decode runs in the absorbed form: q goes through ``W_uk[h]`` once, scores and
 values are taken against the cache rows themselves, and ``W_uv[h]`` maps the
 result back, so a cached token costs one row of ``R + Dr`` elements whatever
-the number of heads.
+the number of heads.  Prefill expands K and V of a group of heads at a time
+where many new tokens share the cost, and runs absorbed otherwise.
 """
 from __future__ import annotations
 
@@ -21,7 +22,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .attention import _checking_slots, check_slot_mapping
+from .attention import (AttentionMetadata, DecodeAttentionMetadata, MixedAttentionMetadata, PrefillAttentionMetadata,
+                        _checking_slots, _host_bound, check_slot_mapping)
 from .kernels._common import require_bf16, require_device, stream_handle
 from .rotary import RotaryFrequencies, check_frequencies, check_tokens, on_device
 
@@ -224,3 +226,134 @@ def latent_decode_workspace_bytes(batch: int, weights: LatentWeights, pages_per_
     """Bytes of the workspace of a :func:`latent_decode_attention` call."""
     return int(_lib.load().pa_latent_decode_workspace_size(batch, weights.num_heads, weights.latent_dim,
                                                            pages_per_seq, page_size))
+
+
+def latent_prefill_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_cache: torch.Tensor,
+                             weights: LatentWeights, block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                             cu_seqlens_k: Optional[torch.Tensor] = None, *, max_seqlen_q: int, scale: float,
+                             kv_lens: Optional[torch.Tensor] = None, max_seqlen_k: Optional[int] = None,
+                             total_kv_tokens: Optional[int] = None, workspace: Optional[torch.Tensor] = None,
+                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Ragged causal attention of new tokens over the paged latent cache:
+    q_nope ``[T, H, Dn]`` and the rotated q_rope ``[T, H, Dr]``, sequence ``b``
+    being rows ``cu_seqlens_q[b] .. cu_seqlens_q[b + 1]`` -> ``[T, H, Dv]`` bf16.
+
+    The kv lengths ``lk`` (cached rows, the new ones included; already stored) come as
+    ``cu_seqlens_k`` (differences), as ``kv_lens`` ``[B]``, or, with neither,
+    equal the new tokens'; row ``i`` of a sequence sees its first ``lk - lq +
+    i + 1`` rows, and is zero if that is none.  At most ``max_seqlen_q`` rows
+    of a sequence are computed.  Rows outside the sequences are zero in a new output and
+    left as they were in a given ``out``.
+
+    ``total_kv_tokens`` bounds the sum of the kv lengths on the host (rows
+    past it are dropped); without it ``max_seqlen_k``, or the block tables'
+    span, times the sequences.  Tight bounds keep the workspace
+    (``latent_prefill_workspace_bytes``) small and choose the form:
+    expanded K and V rows (bf16) for a group of heads at a time, or the absorbed
+    form where few new tokens stand behind long contexts.
+    """
+    tokens, dr, nb, bs = _check_q(q_nope, q_rope, latent_cache, weights)
+    require_device("cu_seqlens_q", cu_seqlens_q)
+    if cu_seqlens_q.dim() != 1 or cu_seqlens_q.numel() < 1:
+        raise ValueError(f"cu_seqlens_q must be int32 [B + 1], got {tuple(cu_seqlens_q.shape)}")
+    batch = cu_seqlens_q.numel() - 1
+    bt = _check_table(block_tables, batch, q_nope)
+    cu_q = check_tokens("cu_seqlens_q", cu_seqlens_q, batch + 1, q_nope)
+    if cu_seqlens_k is not None and kv_lens is not None:
+        raise ValueError("cu_seqlens_k and kv_lens are given both")
+    cu_k = lens = None
+    if kv_lens is not None:
+        lens = check_tokens("kv_lens", kv_lens, batch, q_nope)
+    elif cu_seqlens_k is not None:
+        cu_k = check_tokens("cu_seqlens_k", cu_seqlens_k, batch + 1, q_nope)
+    else:
+        cu_k = cu_q
+    if max_seqlen_q < 0 or max_seqlen_q > 0x7fffffff:
+        raise ValueError(f"max_seqlen_q {max_seqlen_q}")
+    total = _total_kv(batch, tokens, bt.shape[1] * bs, max_seqlen_k, total_kv_tokens, cu_k is cu_q)
+    zero_rest = out is None
+    out = _output(out, (tokens, weights.num_heads, weights.v_dim), q_nope)
+    if tokens == 0:
+        return out
+    need = 0
+    if batch:
+        need = _lib.load().pa_latent_prefill_workspace_size(batch, tokens, max_seqlen_q, total, bt.shape[1], bs,
+                                                            weights.num_heads, weights.latent_dim, dr,
+                                                            weights.nope_dim)
+    ws = _workspace(workspace, int(need), q_nope)
+    with on_device(q_nope):
+        _lib.call("pa_latent_prefill", q_nope.data_ptr(), q_nope.stride(0), q_nope.stride(1), q_rope.data_ptr(),
+                  q_rope.stride(0), q_rope.stride(1), latent_cache.data_ptr(), nb, bs, latent_cache.stride(0),
+                  latent_cache.stride(1), bt.data_ptr(), bt.stride(0), bt.shape[1], cu_q.data_ptr(),
+                  None if cu_k is None else cu_k.data_ptr(), None if lens is None else lens.data_ptr(), batch, tokens,
+                  max_seqlen_q, total, weights.num_heads, weights.latent_dim, dr, weights.nope_dim, weights.v_dim,
+                  weights.w_uk_t.data_ptr(), weights.w_kv.data_ptr(), float(scale), int(zero_rest), out.data_ptr(),
+                  out.stride(0), out.stride(1), ws.data_ptr(), ws.numel() * ws.element_size(), stream_handle(q_nope))
+    return out
+
+
+def _total_kv(batch, tokens, span, max_seqlen_k, total_kv_tokens, fresh) -> int:
+    """Bound of the kv lengths' sum, from what the host knows."""
+    if total_kv_tokens is not None:
+        total = int(total_kv_tokens)
+    elif fresh:
+        total = tokens
+    else:
+        total = batch * min(span, span if max_seqlen_k is None else int(max_seqlen_k))
+    if total < 0 or total > 0x7fffffff:
+        raise ValueError(f"the kv lengths' sum is bounded by {total}: give total_kv_tokens (at most 2^31 - 1)")
+    return total
+
+
+def latent_prefill_workspace_bytes(batch: int, num_tokens: int, max_seqlen_q: int, total_kv_tokens: int,
+                                   weights: LatentWeights, rope_dim: int, pages_per_seq: int, page_size: int) -> int:
+    """Bytes of the workspace of a :func:`latent_prefill_attention` call."""
+    return int(_lib.load().pa_latent_prefill_workspace_size(batch, num_tokens, max_seqlen_q, total_kv_tokens,
+                                                            pages_per_seq, page_size, weights.num_heads,
+                                                            weights.latent_dim, rope_dim, weights.nope_dim))
+
+
+def latent_attention(latent_cache: torch.Tensor, q: torch.Tensor, latent: torch.Tensor, k_rope: torch.Tensor,
+                     norm_weight: Optional[torch.Tensor], weights: LatentWeights, freqs: RotaryFrequencies,
+                     metadata: AttentionMetadata, *, scale: float, eps: float = 1e-6,
+                     interleaved: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """A layer's whole step between its projections, beside ``attention()``:
+    the latent store with both rotations (:func:`latent_store`), then decode,
+    prefill or a mixed step by ``metadata``, whose three types and fields are
+    ``attention()``'s.  q is ``[T, H, Dn + Dr]`` (not rotated; not changed).
+    Returns ``(latent_cache, out [T, H, Dv])``; rows outside the sequences are
+    zero.
+    """
+    if not isinstance(weights, LatentWeights):
+        raise TypeError(f"weights must be LatentWeights, got {type(weights).__name__}")
+    dn = weights.nope_dim
+    if q.dim() != 3 or q.shape[2] <= dn:
+        raise ValueError(f"q must be [T, {weights.num_heads}, {dn} + rope_dim], got {tuple(q.shape)}")
+    _, q_rope = latent_store(latent, k_rope, norm_weight, metadata.input_positions, metadata.slot_mapping,
+                             latent_cache, freqs, eps=eps, interleaved=interleaved, q_rope=q[..., dn:])
+    q_nope = q[..., :dn]
+    m = metadata
+    if isinstance(m, DecodeAttentionMetadata):
+        return latent_cache, latent_decode_attention(q_nope, q_rope, latent_cache, weights, m.block_tables,
+                                                     m.context_lens, scale=scale)
+    if isinstance(m, PrefillAttentionMetadata):
+        longest = _host_bound(m.max_seqlen_k) or None
+        out = latent_prefill_attention(q_nope, q_rope, latent_cache, weights, m.block_tables, m.cu_seqlens_q,
+                                       None if m.cu_seqlens_k is m.cu_seqlens_q else m.cu_seqlens_k,
+                                       max_seqlen_q=m.max_seqlen_bucket, max_seqlen_k=longest, scale=scale)
+        return latent_cache, out
+    if not isinstance(m, MixedAttentionMetadata):
+        raise TypeError(f"metadata of type {type(m).__name__}")
+    nd = m.num_decodes
+    if not 0 <= nd <= m.block_tables.shape[0] or nd > q.shape[0]:
+        raise ValueError(f"num_decodes {nd} of {m.block_tables.shape[0]} sequences and {q.shape[0]} tokens")
+    if nd == m.block_tables.shape[0]:
+        out = torch.zeros((q.shape[0], weights.num_heads, weights.v_dim), dtype=torch.bfloat16, device=q.device)
+    else:
+        out = latent_prefill_attention(q_nope, q_rope, latent_cache, weights, m.block_tables[nd:],
+                                       m.cu_seqlens_q[nd:], kv_lens=m.kv_lens[nd:], max_seqlen_q=m.max_seqlen_q,
+                                       scale=scale)
+    if nd:
+        latent_decode_attention(q_nope[:nd], q_rope[:nd], latent_cache, weights, m.block_tables[:nd], m.kv_lens[:nd],
+                                scale=scale, out=out[:nd])
+    return latent_cache, out
