@@ -9,7 +9,7 @@
 namespace pa {
 
 // Per-head products y[t, h, :] = W[h] x[t, h, :] (latent_product.hip): W[h] is
-// [n, k] with contiguous rows, k 64 .. 512 a multiple of 64, n a multiple of 32.
+// [n, k] contiguous, k 64, 128, 256 or 512, n a multiple of 32.
 struct HeadProduct {
   const uint16_t* x;
   int64_t x_ts, x_hs;

@@ -45,8 +45,13 @@ struct AttnParams {
   LatentAttn a;
   MagicDiv heads;
   float scale_log2;
-  int32_t min_share, wgs, row_tiles;  // row_tiles: of max_q tokens
-  int32_t* prefix;  // [batch + 1] tiles before each sequence
+  int32_t min_share, wgs;
+  bool pages8;      // the page size is a multiple of 8
+  // What latent_merge_kernel has to join, [4] each: sequence, row tile, parts (0: nothing), first
+  // workgroup; one entry a unit where there are no more units than workgroups
+  // (row_tiles > 0: those of a sequence), else one a workgroup.
+  int32_t* joins;
+  int32_t row_tiles;
   float* parts;     // [2 wgs][rows * R]
   float* stats;     // [2 wgs][rows][2]
 };
@@ -68,7 +73,7 @@ struct Dims {
   static constexpr int kDt = R / 128;                 // 32-row blocks of O^T of a value wave
   static constexpr int kRb = ROWS / 32;               // its 32-row blocks of rows
   static constexpr int kRowsPerDma = 1024 / kRowB;
-  static constexpr int kLatDma = 4 / kRowsPerDma;     // a wave loads four rows of a tile
+  static constexpr int kLatDma = 8 / kRowsPerDma;     // a value wave loads eight rows of a tile
   static constexpr int kDma = kLatDma + 1;
   static_assert(kLds <= 160 * 1024 && kRing >= 4 * kMaxBatch + 64, "LDS");
 };
@@ -76,6 +81,19 @@ struct Dims {
 template <int DR>
 __device__ __forceinline__ int rope_swz(int r) {
   return DR == 64 ? swz128(r) : swz64(r);
+}
+
+// The same value, as one that the compiler makes anew here: what hangs on it is
+// not carried in registers from outside the loops (the roles' 250 are full).
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// An address as the base of reads with constant offsets.
+__device__ __forceinline__ uint32_t fresh_addr(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 struct Seq {
@@ -152,13 +170,14 @@ latent_attn_kernel(AttnParams p) {
     total += sum;
   }
   __syncthreads();
-  if (g == 0) {
-    for (int b = tid; b < p.a.batch; b += kLThreads) p.prefix[b] = pref[b];
-    if (tid == 0) p.prefix[p.a.batch] = total;
-  }
   const int share = max(p.min_share, (total + p.wgs - 1) / p.wgs);
   int64_t at64 = (int64_t)g * share;
-  if (at64 >= total) return;  // uniform
+  int4* joins = reinterpret_cast<int4*>(p.joins);
+  int4 join = make_int4(0, 0, 0, g);
+  if (at64 >= total) {  // uniform
+    if (tid == 0 && p.row_tiles == 0) joins[g] = join;
+    return;
+  }
   int at = (int)at64;
   const int end = (int)min((int64_t)total, at64 + share);
   int b;
@@ -187,51 +206,19 @@ latent_attn_kernel(AttnParams p) {
     const int t0 = at - seq_at - rt * sq.nt;
     const int t1 = min(sq.nt, t0 + end - at);
     at += t1 - t0;
+    // a unit that starts here and goes on: its parts are this one and those of
+    // the workgroups behind
+    if (t0 == 0) {
+      if (t1 < sq.nt) join = make_int4(b, rt, 1 + (sq.nt - t1 + share - 1) / share, g);
+      if (tid == 0 && p.row_tiles > 0) joins[b * p.row_tiles + rt] = join;
+    }
     const int n_rows = min(ROWS, sq.lq * p.a.heads - rt * ROWS);
     const int lk = sq.lk;
-    const int32_t* bt = pool.tables + (int64_t)b * pool.bt_stride;
-
-    // ---- tile loads: this wave's rows are 4 wave .. 4 wave + 3 of every tile
-    auto row_ptr = [&](int t, int i) __attribute__((always_inline)) {
-      const int j = min(t * kTile + 4 * wave + i, lk - 1);
-      const int pg = (int)div_by((uint32_t)j, pool.page);
-      const int page = safe_page_scalar(bt, pg, pool.num_pages);
-      return pool.cache + page * pool.page_stride + (int64_t)(j - pg * (int)pool.page.d) * pool.slot_stride;
-    };
-    auto issue = [&](int t) __attribute__((always_inline)) {
-      const uint32_t st = lds0 + (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
-      const uint16_t* rp[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) rp[i] = row_ptr(t, i);
-#pragma unroll
-      for (int i = 0; i < D::kLatDma; ++i) {
-        const int sub = D::kRowsPerDma == 1 ? 0 : lane >> 5;
-        const uint16_t* r = D::kRowsPerDma == 1 ? rp[i] : (sub ? rp[2 * i + 1] : rp[2 * i]);
-        const int row = 4 * wave + i * D::kRowsPerDma + sub;
-        const int c = lane & (D::kRowB / 16 - 1);
-        lds_dma16(r + 8 * (c ^ swz256(row)), st + (uint32_t)(4 * wave * D::kRowB + i * 1024));
-      }
-      constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
-      if (lane < 4 * kC) {
-        const int i = lane / kC;
-        const uint16_t* r = i < 2 ? (i == 0 ? rp[0] : rp[1]) : (i == 2 ? rp[2] : rp[3]);
-        const int c = (lane & (kC - 1)) ^ rope_swz<DR>(4 * wave + i);
-        lds_dma16(r + R + 8 * c, st + (uint32_t)(D::kLatB + 4 * wave * D::kRopeB));
-      }
-    };
-    issue(t0);
-    if (t0 + 1 < t1) issue(t0 + 1);
-
-    // end of step t: this wave's share of tile t + 1 has landed
-    auto landed = [&](int t) __attribute__((always_inline)) {
-      if (t + 2 < t1) wait_vm<D::kDma>();
-      else wait_vm<0>();
-    };
 
     if (wave < 4) {
       // ================= scores
       const int tb = wave & 1, rw = (wave >> 1) * 16 * D::kNr;
-      const int l16 = lane & 15, qd = lane >> 4;
+      const int ln = fresh(lane), l16 = ln & 15, qd = ln >> 4;
       bf16x8 q[D::kNr][D::kKs + D::kRs];
       int lim[D::kNr];  // tokens a row sees
 #pragma unroll
@@ -266,10 +253,8 @@ latent_attn_kernel(AttnParams p) {
         roff[i] = lds0 + D::kLatB + krow * D::kRopeB + 16 * ((4 * i + qd) ^ rope_swz<DR>(krow));
       float* maxes = reinterpret_cast<float*>(smem + D::kMaxOff);
       float* corrs = reinterpret_cast<float*>(smem + D::kCorrOff);
-      wait_vm<0>();  // Q and both tiles
-      lds_barrier();
+      lds_barrier();  // the first tile is there
       for (int t = t0; t <= t1; ++t) {
-        if (t + 2 < t1) issue(t + 2);
         f32x4 s[D::kNr];
         float mx[D::kNr];
         if (t < t1) {
@@ -277,21 +262,29 @@ latent_attn_kernel(AttnParams p) {
           f32x4 s2[D::kNr];
 #pragma unroll
           for (int r = 0; r < D::kNr; ++r) s[r] = s2[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+          uint32_t ka[4], ra[D::kRs];
 #pragma unroll
-          for (int ks = 0; ks < D::kKs; ++ks) {
-            const bf16x8 a = as_bf16x8(lds_ld16(koff[ks & 3] + st + (ks >> 2) * 256));
+          for (int i = 0; i < 4; ++i) ka[i] = fresh_addr(koff[i] + st);
+#pragma unroll
+          for (int i = 0; i < D::kRs; ++i) ra[i] = fresh_addr(roff[i] + st);
+          // every read is issued kAhead k-steps before the products it feeds
+          constexpr int kAll = D::kKs + D::kRs, kAhead = 6;
+          bf16x8 a[kAll];
+          auto read_k = [&](int ks) __attribute__((always_inline)) {
+            a[ks] = as_bf16x8(ks < D::kKs ? lds_ld16(ka[ks & 3] + (ks >> 2) * 256)
+                                          : lds_ld16(ra[(ks - D::kKs) % D::kRs]));
+          };
+#pragma unroll
+          for (int ks = 0; ks < kAhead; ++ks) read_k(ks);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int ks = 0; ks < kAll; ++ks) {
 #pragma unroll
             for (int r = 0; r < D::kNr; ++r)
-              if (ks & 1) s2[r] = mfma16(a, q[r][ks], s2[r]);
-              else s[r] = mfma16(a, q[r][ks], s[r]);
-          }
-#pragma unroll
-          for (int ks = 0; ks < D::kRs; ++ks) {
-            const bf16x8 a = as_bf16x8(lds_ld16(roff[ks] + st));
-#pragma unroll
-            for (int r = 0; r < D::kNr; ++r)
-              if (ks & 1) s2[r] = mfma16(a, q[r][D::kKs + ks], s2[r]);
-              else s[r] = mfma16(a, q[r][D::kKs + ks], s[r]);
+              if (ks & 1) s2[r] = mfma16(a[ks], q[r][ks], s2[r]);
+              else s[r] = mfma16(a[ks], q[r][ks], s[r]);
+            if (ks + kAhead < kAll) read_k(ks + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
           }
           const int j0 = t * kTile + 16 * tb + 4 * qd;
 #pragma unroll
@@ -328,7 +321,6 @@ latent_attn_kernel(AttnParams p) {
                 u32x2{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3])};
           }
         }
-        landed(t);
         wait_lgkm0();
         lds_barrier();
       }
@@ -348,11 +340,74 @@ latent_attn_kernel(AttnParams p) {
     } else {
       // ================= values
       const int pw = wave - 4;
-      const int n = lane & 31, h = lane >> 5;
+      const int lv = fresh(lane), n = lv & 31, h = lv >> 5;
+
+      // ---- tile loads: this wave's rows are 8 pw .. 8 pw + 7 of every tile.
+      // Page ids of 64 pages from p0 on sit in the lanes of one register.
+      int p0 = 0x40000000, page_ids = 0;
+      const int32_t* bt = pool.tables + (int64_t)b * pool.bt_stride;
+      auto row_at = [&](int j) __attribute__((always_inline)) {  // uniform j
+        const int pg = (int)div_by((uint32_t)j, pool.page);
+        const int page = __builtin_amdgcn_readlane(page_ids, pg - p0);
+        return pool.cache + (page * pool.page_stride + (int64_t)(j - pg * (int)pool.page.d) * pool.slot_stride);
+      };
+      auto issue = [&](int t) __attribute__((always_inline)) {
+        const uint32_t st = lds0 + (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
+        const uint32_t lat = st + (uint32_t)(8 * pw * D::kRowB), rope = st + (uint32_t)(D::kLatB + 8 * pw * D::kRopeB);
+        const int j = t * kTile + 8 * pw;
+        const int ln = fresh(lane);
+        {
+          const int lo = (int)div_by((uint32_t)min(j, lk - 1), pool.page);
+          const int hi = (int)div_by((uint32_t)min(j + 7, lk - 1), pool.page);
+          if (lo < p0 || hi - p0 >= 64) {  // uniform
+            p0 = lo;
+            page_ids = safe_page(bt, min(p0 + lane, pool.pages_per_seq - 1), pool.num_pages);
+            asm volatile("" : "+v"(page_ids));
+          }
+        }
+        constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
+        const int rr = ln / kC;           // (lns below 8 kC) row of the rotary load
+        const int rc = 8 * ((ln & (kC - 1)) ^ rope_swz<DR>(8 * pw + rr));
+        if (p.pages8) {
+          // eight aligned rows lie in one page; rows past the end repeat the last
+          const int j8 = min(j, (lk - 1) & ~7), last = lk - 1 - j8;
+          const uint16_t* base = row_at(j8);
+#pragma unroll
+          for (int i = 0; i < D::kLatDma; ++i) {
+            if constexpr (D::kRowsPerDma == 1) {
+              lds_dma16s((uint32_t)(16 * (ln ^ swz256(8 * pw + i))), base + min(i, last) * pool.slot_stride,
+                         lat + 1024 * i);
+            } else {
+              const int r = 2 * i + (ln >> 5);
+              lds_dma16(base + min(r, last) * pool.slot_stride + 8 * ((ln & 31) ^ swz256(8 * pw + r)),
+                        lat + 1024 * i);
+            }
+          }
+          if (ln < 8 * kC) lds_dma16(base + min(rr, last) * pool.slot_stride + R + rc, rope);
+        } else {
+          const uint16_t* mine = nullptr;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint16_t* r = row_at(min(j + i, lk - 1));
+            if (D::kRowsPerDma == 1) {
+              lds_dma16s((uint32_t)(16 * (ln ^ swz256(8 * pw + i))), r, lat + 1024 * i);
+            } else {
+              if (i & 1) {
+                const uint16_t* own = ln >> 5 ? r : row_at(min(j + i - 1, lk - 1));
+                lds_dma16(own + 8 * ((ln & 31) ^ swz256(8 * pw + i - 1 + (ln >> 5))), lat + 1024 * (i >> 1));
+              }
+            }
+            if (rr == i) mine = r;
+          }
+          if (ln < 8 * kC) lds_dma16(mine + R + rc, rope);
+        }
+      };
+      issue(t0);
+      if (t0 + 1 < t1) issue(t0 + 1);
       f32x16 acc[D::kDt][D::kRb] = {};
       // transposing reads of V^T: lane 16 gamma + s reads row 4 h + s / 4 (+ 8)
       // of a 16-token step, columns 32 dt + 16 (gamma % 2) + 4 (s % 4)
-      const int ts = lane & 15, gamma = lane >> 4;
+      const int ts = lv & 15, gamma = lv >> 4;
       const int tr = 4 * h + (ts >> 2);
       uint32_t voff0[D::kDt], voff1[D::kDt];
 #pragma unroll
@@ -368,22 +423,31 @@ latent_attn_kernel(AttnParams p) {
         for (int u = 0; u < 2; ++u)
           poff[rb][u] = lds0 + D::kPOff + (32 * rb + n) * 64 + 16 * ((2 * u + h) ^ ((n >> 2) & 3));
       const float* corrs = reinterpret_cast<const float*>(smem + D::kCorrOff);
-      wait_vm<0>();
-      lds_barrier();
-      bf16x8 pt[D::kRb][2];
-      auto product = [&](int u, uint32_t st) __attribute__((always_inline)) {
+      // (set here, or the compiler carries them through the segments)
+      bf16x8 pt[D::kRb][2] = {};
+      bf16x8 v0[D::kDt] = {}, v1[D::kDt] = {};  // V^T of the first and second 16 tokens of a tile
+      auto read_v = [&](bf16x8(&v)[D::kDt], int u, int t) __attribute__((always_inline)) {
+        const uint32_t st = (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
 #pragma unroll
         for (int dt = 0; dt < D::kDt; ++dt) {
-          const u32x2 lo = lds_tr8(voff0[dt] + st + 16 * u * D::kRowB);
-          const u32x2 hi = lds_tr8(voff1[dt] + st + 16 * u * D::kRowB);
-          const bf16x8 a = as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]});
-#pragma unroll
-          for (int rb = 0; rb < D::kRb; ++rb) acc[dt][rb] = mfma32(a, pt[rb][u], acc[dt][rb]);
+          const u32x2 lo = lds_tr8(fresh_addr(voff0[dt] + st) + 16 * u * D::kRowB);
+          const u32x2 hi = lds_tr8(fresh_addr(voff1[dt] + st) + 16 * u * D::kRowB);
+          v[dt] = as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]});
         }
       };
+      auto product = [&](const bf16x8(&v)[D::kDt], int u) __attribute__((always_inline)) {
+#pragma unroll
+        for (int dt = 0; dt < D::kDt; ++dt)
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb) acc[dt][rb] = mfma32(v[dt], pt[rb][u], acc[dt][rb]);
+      };
+      // Tile t + 1 has landed when at most tile t + 2's loads are outstanding.
+      if (t0 + 1 < t1) wait_vm<D::kDma>();
+      else wait_vm<0>();
+      lds_barrier();
+      // Step t: the first half of tile t - 1 before the barrier at which the score
+      // waves exchange maxima, the second behind it; V is read half a step ahead.
       for (int t = t0; t <= t1; ++t) {
-        if (t + 2 < t1) issue(t + 2);
-        const uint32_t st = (uint32_t)((t - 1 - t0) & (kLStages - 1)) * D::kStageB;
         if (t > t0) {
           float corr[D::kRb];
 #pragma unroll
@@ -392,33 +456,39 @@ latent_attn_kernel(AttnParams p) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) pt[rb][u] = as_bf16x8(lds_ld16(poff[rb][u]));
           }
+          read_v(v1, 1, t - 1);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int rb = 0; rb < D::kRb; ++rb)
             if (__any(corr[rb] != 1.f)) {
 #pragma unroll
               for (int dt = 0; dt < D::kDt; ++dt) acc[dt][rb] = acc[dt][rb] * corr[rb];
             }
-          product(0, st);
+          product(v0, 0);
         }
+        if (t + 2 < t1) issue(t + 2);  // under the products; into the stage of tile t - 2
         wait_lgkm0();  // P is in registers: the score waves may overwrite it
         lds_barrier();
-        if (t > t0) product(1, st);
-        landed(t);
+        if (t > t0) product(v1, 1);
+        if (t < t1) read_v(v0, 0, t);
+        if (t + 2 < t1) wait_vm<D::kDma>();
+        else wait_vm<0>();
         wait_lgkm0();
         lds_barrier();
       }
       lds_barrier();  // sums are there
+      const int le = fresh(lane), ne = le & 31, he = le >> 5;
       const float* sums = reinterpret_cast<const float*>(smem + D::kSumOff);
       if (t0 == 0 && t1 == sq.nt) {
 #pragma unroll
         for (int rb = 0; rb < D::kRb; ++rb) {
-          const int r = 32 * rb + n;
+          const int r = 32 * rb + ne;
           const float l = sums[r] + sums[ROWS + r];
           const float inv = l > 0.f ? 1.f / l : 0.f;
           if (r < n_rows) {
             const int row = rt * ROWS + r;
             const int tok = (int)div_by((uint32_t)row, p.heads), hd = row - tok * p.a.heads;
-            uint16_t* o = p.a.out + (int64_t)(sq.q0 + tok) * p.a.o_ts + hd * p.a.o_hs + pw * (R / 4) + 4 * h;
+            uint16_t* o = p.a.out + (int64_t)(sq.q0 + tok) * p.a.o_ts + hd * p.a.o_hs + pw * (R / 4) + 4 * he;
 #pragma unroll
             for (int dt = 0; dt < D::kDt; ++dt)
 #pragma unroll
@@ -432,7 +502,7 @@ latent_attn_kernel(AttnParams p) {
         }
       } else {
         const int slot = 2 * g + (t0 == 0 ? 1 : 0);
-        float* dst = p.parts + (int64_t)slot * (ROWS * R) + 4 * lane;
+        float* dst = p.parts + (int64_t)slot * (ROWS * R) + 4 * le;
 #pragma unroll
         for (int dt = 0; dt < D::kDt; ++dt)
 #pragma unroll
@@ -443,79 +513,126 @@ latent_attn_kernel(AttnParams p) {
               *reinterpret_cast<f32x4*>(dst + 256 * (((pw * D::kDt + dt) * D::kRb + rb) * 4 + i)) =
                   f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
             }
-        if (pw == 0 && lane < ROWS) {
-          const float l = sums[lane] + sums[ROWS + lane];
-          *reinterpret_cast<f32x2*>(p.stats + ((int64_t)slot * ROWS + lane) * 2) = f32x2{sums[2 * ROWS + lane], l};
+        if (pw == 0 && le < ROWS) {
+          const float l = sums[le] + sums[ROWS + le];
+          *reinterpret_cast<f32x2*>(p.stats + ((int64_t)slot * ROWS + le) * 2) = f32x2{sums[2 * ROWS + le], l};
         }
       }
     }
     __syncthreads();  // LDS is free for the next segment
   }
+  if (tid == 0 && p.row_tiles == 0) joins[g] = join;
 }
 
 // Joins the parts of every (sequence, row tile) that more than one workgroup
-// worked on: o = sum_p w_p o_p / sum_p w_p l_p, w_p = 2^(m_p - max m).  A part's
-// O lies as the accumulators held it, 256 floats a (column block, row block,
-// quarter): a workgroup joins one such slice at a time, its waves taking the
-// parts in turn, and rows without any token to see come out zero.
+// worked on: o = sum_p w_p o_p / sum_p w_p l_p, w_p = 2^(m_p - max m), and gives
+// sequences without any cached token zero rows.  A part's O lies as the
+// accumulators held it, 256 floats a slice (column block, row block, quarter).
+// Few parts: each wave joins slices of its own.  Many: the waves of a workgroup
+// share a slice's parts and add up through LDS.
+constexpr int kJoinWaves = 8, kJoinFly = 4;  // parts in flight a wave
+
+struct Joined {
+  float m, l;
+  f32x4 acc;
+};
+
 template <int R, int ROWS>
-__global__ void __launch_bounds__(256) latent_merge_kernel(AttnParams p) {
+__device__ __forceinline__ Joined join_parts(const AttnParams& p, int g, int parts, int first, int step, int sl, int r,
+                                             int lane) {
+  Joined j = {kNoMax, 0.f, {0.f, 0.f, 0.f, 0.f}};
+  for (int i0 = first; i0 < parts; i0 += step * kJoinFly) {
+    f32x2 ml[kJoinFly];
+    f32x4 v[kJoinFly];
+#pragma unroll
+    for (int k = 0; k < kJoinFly; ++k) {
+      const int i = min(i0 + step * k, parts - 1);  // past the last: that one again, without weight
+      const int64_t slot = 2 * (g + i) + (i == 0 ? 1 : 0);
+      ml[k] = *reinterpret_cast<const f32x2*>(p.stats + (slot * ROWS + r) * 2);
+      v[k] = *reinterpret_cast<const f32x4*>(p.parts + slot * (ROWS * R) + 256 * sl + 4 * lane);
+    }
+    float m_new = j.m;
+#pragma unroll
+    for (int k = 0; k < kJoinFly; ++k) m_new = __builtin_fmaxf(m_new, ml[k][0]);
+    const float ca = fast_exp2(j.m - m_new);
+    j.acc = j.acc * ca;
+    j.l *= ca;
+#pragma unroll
+    for (int k = 0; k < kJoinFly; ++k) {
+      // (a part whose rows saw nothing has l = 0 and O = 0)
+      const float c = i0 + step * k < parts ? fast_exp2(ml[k][0] - m_new) : 0.f;
+      j.acc = j.acc + v[k] * c;
+      j.l += ml[k][1] * c;
+    }
+    j.m = m_new;
+  }
+  return j;
+}
+
+template <int R, int ROWS>
+__global__ void __launch_bounds__(64 * kJoinWaves) latent_merge_kernel(AttnParams p) {
   constexpr int kRb = ROWS / 32, kSlices = ROWS * R / 256;
-  __shared__ f32x4 s_acc[4][64];
-  __shared__ float s_m[4][32], s_l[4][32];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ f32x4 s_acc[kJoinWaves][64];
+  __shared__ f32x2 s_ml[kJoinWaves][32];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
-  const int b = blockIdx.x / p.row_tiles, rt = blockIdx.x - b * p.row_tiles;
+  const int4 join = reinterpret_cast<const int4*>(p.joins)[blockIdx.x];
+  for (int b = blockIdx.x * gridDim.y + blockIdx.y; b < p.a.batch; b += gridDim.x * gridDim.y) {
+    const Seq sq = seq_of(p, b, ROWS);
+    if (sq.nt > 0) continue;
+    for (int i = wave; i < sq.lq * p.a.heads; i += kJoinWaves) {
+      const int tok = (int)div_by((uint32_t)i, p.heads), hd = i - tok * p.a.heads;
+      uint16_t* o = p.a.out + (int64_t)(sq.q0 + tok) * p.a.o_ts + hd * p.a.o_hs;
+      if (8 * lane < R) st16(o + 8 * lane, u32x4{0, 0, 0, 0});
+    }
+  }
+  if (p.row_tiles > 0) {
+    // an entry is written by the workgroup that starts the unit: there is none
+    // for a unit without tiles or without rows
+    const int ub = blockIdx.x / p.row_tiles;
+    const Seq us = seq_of(p, ub, ROWS);
+    if (us.nt == 0 || (int)blockIdx.x - ub * p.row_tiles >= us.nrt) return;
+  }
+  const int b = join.x, rt = join.y, parts = join.z, g = join.w;
+  if (parts == 0) return;
   const Seq sq = seq_of(p, b, ROWS);
-  if (rt >= sq.nrt) return;
-  const int total = p.prefix[p.a.batch];
-  const int share = max(p.min_share, (total + p.wgs - 1) / p.wgs);
-  const int64_t a = (int64_t)p.prefix[b] + (int64_t)rt * sq.nt;
-  const int g0 = (int)(a / share), g1 = sq.nt ? (int)((a + sq.nt - 1) / share) : g0 + 1;
-  if (g0 == g1) return;  // one workgroup had the whole unit
-  const int parts = sq.nt ? g1 - g0 + 1 : 0;
   const int n_rows = min(ROWS, sq.lq * p.a.heads - rt * ROWS);
+  auto store = [&](int sl, int r, const f32x4& o, float l) __attribute__((always_inline)) {
+    if (r >= n_rows) return;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int row = rt * ROWS + r;
+    const int tok = (int)div_by((uint32_t)row, p.heads), hd = row - tok * p.a.heads;
+    const int d = 32 * (sl / (4 * kRb)) + 8 * (sl & 3) + 4 * h;
+    *reinterpret_cast<u32x2*>(p.a.out + (int64_t)(sq.q0 + tok) * p.a.o_ts + hd * p.a.o_hs + d) =
+        u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+  };
+  if (parts <= 2 * kJoinFly) {
+    for (int sl = blockIdx.y * kJoinWaves + wave; sl < kSlices; sl += gridDim.y * kJoinWaves) {
+      const int r = 32 * ((sl >> 2) % kRb) + n;
+      const Joined j = join_parts<R, ROWS>(p, g, parts, 0, 1, sl, r, lane);
+      store(sl, r, j.acc, j.l);
+    }
+    return;
+  }
   for (int sl = blockIdx.y; sl < kSlices; sl += gridDim.y) {
-    const int rb = (sl >> 2) % kRb;
-    const int r = 32 * rb + n;
-    float m = kNoMax, l = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int i = wave; i < parts; i += 4) {
-      const int slot = 2 * (g0 + i) + (i == 0 ? 1 : 0);
-      const f32x2 ml = *reinterpret_cast<const f32x2*>(p.stats + ((int64_t)slot * ROWS + r) * 2);
-      const f32x4 v = *reinterpret_cast<const f32x4*>(p.parts + (int64_t)slot * (ROWS * R) + 256 * sl + 4 * lane);
-      const float m_new = __builtin_fmaxf(m, ml[0]);
-      const float ca = fast_exp2(m - m_new), cb = fast_exp2(ml[0] - m_new);
-      acc = acc * ca + v * cb;
-      l = l * ca + ml[1] * cb;
-      m = m_new;
-    }
-    s_acc[wave][lane] = acc;
-    if (h == 0) {
-      s_m[wave][n] = m;
-      s_l[wave][n] = l;
-    }
+    const int r = 32 * ((sl >> 2) % kRb) + n;
+    const Joined j = join_parts<R, ROWS>(p, g, parts, wave, kJoinWaves, sl, r, lane);
+    s_acc[wave][lane] = j.acc;
+    if (h == 0) s_ml[wave][n] = f32x2{j.m, j.l};
     __syncthreads();
     if (wave == 0) {
       float mm = kNoMax;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) mm = __builtin_fmaxf(mm, s_m[w][n]);
+      for (int w = 0; w < kJoinWaves; ++w) mm = __builtin_fmaxf(mm, s_ml[w][n][0]);
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
-      float ll = 0.f;
+      float l = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float c = fast_exp2(s_m[w][n] - mm);
+      for (int w = 0; w < kJoinWaves; ++w) {
+        const float c = fast_exp2(s_ml[w][n][0] - mm);
         o = o + s_acc[w][lane] * c;
-        ll += s_l[w][n] * c;
+        l += s_ml[w][n][1] * c;
       }
-      const float inv = ll > 0.f ? 1.f / ll : 0.f;
-      if (r < n_rows) {
-        const int row = rt * ROWS + r;
-        const int tok = (int)div_by((uint32_t)row, p.heads), hd = row - tok * p.a.heads;
-        const int d = 32 * (sl / (4 * kRb)) + 8 * (sl & 3) + 4 * h;
-        *reinterpret_cast<u32x2*>(p.a.out + (int64_t)(sq.q0 + tok) * p.a.o_ts + hd * p.a.o_hs + d) =
-            u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
-      }
+      store(sl, r, o, l);
     }
     __syncthreads();
   }
@@ -545,23 +662,24 @@ size_t latent_attn_workspace(int32_t batch, int32_t max_q, int32_t heads, int32_
     *why = "more than 2^31 tiles of work";
   if (*why) return 0;
   const int wgs = wgs_of(row_tiles * batch * tiles);
-  return align256(4 * ((size_t)batch + 1)) + align256((size_t)2 * wgs * rows * 8) + (size_t)2 * wgs * rows * latent * 4;
+  return align256((size_t)16 * wgs) + align256((size_t)2 * wgs * rows * 8) + (size_t)2 * wgs * rows * latent * 4;
 }
 
 template <int R, int DR, int ROWS>
-static int attn_launch(const char* name, AttnParams p, void* workspace, hipStream_t s) {
+static int attn_launch(const char* name, AttnParams p, int64_t units, void* workspace, hipStream_t s) {
   char* ws = (char*)workspace;
-  p.prefix = (int32_t*)ws;
-  ws += align256(4 * ((size_t)p.a.batch + 1));
+  p.joins = (int32_t*)ws;
+  ws += align256((size_t)16 * p.wgs);
   p.stats = (float*)ws;
   ws += align256((size_t)2 * p.wgs * ROWS * 8);
   p.parts = (float*)ws;
   latent_attn_kernel<R, DR, ROWS><<<dim3((unsigned)p.wgs), dim3(kLThreads), 0, s>>>(p);
   if (int rc = launch_status(name)) return rc;
-  const int64_t units = (int64_t)p.a.batch * p.row_tiles;
+  // at least eight workgroups a join, as many as there are slices for few joins
+  const int64_t joins = p.row_tiles > 0 ? units : p.wgs;
   constexpr int kSlices = ROWS * R / 256;
-  const unsigned ny = (unsigned)std::max<int64_t>(1, std::min<int64_t>(kSlices, 1024 / units));
-  latent_merge_kernel<R, ROWS><<<dim3((unsigned)units, ny), dim3(256), 0, s>>>(p);
+  const unsigned ny = (unsigned)std::max<int64_t>(8, std::min<int64_t>(kSlices, 1024 / joins));
+  latent_merge_kernel<R, ROWS><<<dim3((unsigned)joins, ny), dim3(64 * kJoinWaves), 0, s>>>(p);
   return launch_status(name);
 }
 
@@ -571,15 +689,19 @@ int latent_attn_launch(const char* name, const LatentAttn& a, int latent, int ro
   p.heads = magic_div((uint32_t)a.heads);
   p.scale_log2 = a.scale * kLog2e;
   p.min_share = kMinShare;
+  p.pages8 = a.pool.page.d % 8 == 0;
   const int rows = rows_of(a.max_q, a.heads);
-  p.row_tiles = (int)(((int64_t)a.max_q * a.heads + rows - 1) / rows);
+  const int64_t row_tiles = ((int64_t)a.max_q * a.heads + rows - 1) / rows;
   const int64_t span = (int64_t)a.pool.pages_per_seq * a.pool.page.d;
-  p.wgs = wgs_of((int64_t)p.row_tiles * a.batch * ((span + kTile - 1) / kTile));
-  p.prefix = nullptr;
+  const int64_t units = row_tiles * a.batch;
+  p.wgs = wgs_of(units * ((span + kTile - 1) / kTile));
+  p.row_tiles = units <= p.wgs ? (int)row_tiles : 0;
+  p.joins = nullptr;
   p.parts = p.stats = nullptr;
 #define PA_LATENT_CASE(R, DR)                                             \
   if (latent == R && rope == DR)                                          \
-    return rows == 32 ? attn_launch<R, DR, 32>(name, p, workspace, s) : attn_launch<R, DR, 64>(name, p, workspace, s);
+    return rows == 32 ? attn_launch<R, DR, 32>(name, p, units, workspace, s)  \
+                      : attn_launch<R, DR, 64>(name, p, units, workspace, s);
   PA_LATENT_CASE(512, 64)
   PA_LATENT_CASE(512, 32)
   PA_LATENT_CASE(256, 64)

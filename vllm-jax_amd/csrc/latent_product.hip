@@ -12,64 +12,89 @@
 namespace pa {
 namespace {
 
-constexpr int kStep = 64;  // k values in flight
-
-template <int MB>
-__global__ void __launch_bounds__(256) head_product_kernel(HeadProduct p, int n_blocks, int m_blocks) {
+// A workgroup's four waves share 32 outputs and split the depth (kSplit = 4), or
+// take 32 outputs each with the whole of it (kSplit = 1); a wave's part, kDepth
+// deep, is all in flight before the first product.
+template <int MB, int kDepth, int kSplit>
+__global__ void __launch_bounds__(256) head_product_kernel(HeadProduct p, int n_groups) {
+  constexpr int kSteps = kDepth / 16;
+  __shared__ f32x4 part[kSplit == 1 ? 1 : 4][MB][4][64];
   const int lane = threadIdx.x & 63;
   const int h2 = lane >> 5, l = lane & 31;
-  const int gw = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int head = blockIdx.y;
-  const int mb = gw / n_blocks, nb = gw - mb * n_blocks;
-  if (mb >= m_blocks) return;
-  const uint16_t* w = p.w + head * p.w_hs + (int64_t)(32 * nb + l) * p.k + 8 * h2;
-  const uint16_t* x[MB];
+  const int mb = blockIdx.x / n_groups, ng = blockIdx.x - mb * n_groups;
+  const int nb = kSplit == 1 ? 4 * ng + wave : ng;
+  if (32 * nb >= p.n) return;  // (kSplit == 1) no barrier below
+  const int k0 = kSplit == 1 ? 0 : wave * kDepth;
+  const uint16_t* w = p.w + head * p.w_hs + (int64_t)(32 * nb + l) * (kDepth * kSplit) + k0 + 8 * h2;
+  bf16x8 a[kSteps], b[MB][kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) a[s] = as_bf16x8(ld16(w + 16 * s));
 #pragma unroll
   for (int m = 0; m < MB; ++m) {
     const int t = min((mb * MB + m) * 32 + l, p.tokens - 1);
-    x[m] = p.x + t * p.x_ts + head * p.x_hs + 8 * h2;
+    const uint16_t* x = p.x + t * p.x_ts + head * p.x_hs + k0 + 8 * h2;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) b[m][s] = as_bf16x8(ld16(x + 16 * s));
   }
   f32x16 acc[MB] = {};
-  for (int k0 = 0; k0 < p.k; k0 += kStep) {
-    bf16x8 a[kStep / 16], b[MB][kStep / 16];
 #pragma unroll
-    for (int s = 0; s < kStep / 16; ++s) {
-      a[s] = as_bf16x8(ld16(w + k0 + 16 * s));
+  for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int m = 0; m < MB; ++m) b[m][s] = as_bf16x8(ld16(x[m] + k0 + 16 * s));
-    }
-#pragma unroll
-    for (int s = 0; s < kStep / 16; ++s)
-#pragma unroll
-      for (int m = 0; m < MB; ++m) acc[m] = mfma32(a[s], b[m][s], acc[m]);
-  }
+    for (int m = 0; m < MB; ++m) acc[m] = mfma32(a[s], b[m][s], acc[m]);
   // lane (l, h2) holds token l, outputs 8 (i / 4) + 4 h2 + i % 4
-#pragma unroll
-  for (int m = 0; m < MB; ++m) {
+  auto store = [&](int m, int q, const f32x4& v) __attribute__((always_inline)) {
     const int t = (mb * MB + m) * 32 + l;
-    if (t >= p.tokens) continue;
+    if (t >= p.tokens) return;
+    u32x2 o = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
     if (p.cu_q && !token_in_sequence(p.cu_q, p.batch, p.max_q, t)) {
-      if (!p.zero_rest) continue;
-      acc[m] = f32x16{};
+      if (!p.zero_rest) return;
+      o = u32x2{0, 0};
     }
-    uint16_t* y = p.y + t * p.y_ts + head * p.y_hs + 32 * nb + 4 * h2;
+    *reinterpret_cast<u32x2*>(p.y + t * p.y_ts + head * p.y_hs + 32 * nb + 8 * q + 4 * h2) = o;
+  };
+  if constexpr (kSplit == 1) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<u32x2*>(y + 8 * q) =
-          u32x2{pack_bf16x2(acc[m][4 * q], acc[m][4 * q + 1]), pack_bf16x2(acc[m][4 * q + 2], acc[m][4 * q + 3])};
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        store(m, q, f32x4{acc[m][4 * q], acc[m][4 * q + 1], acc[m][4 * q + 2], acc[m][4 * q + 3]});
+  } else {
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        part[wave][m][q][lane] = f32x4{acc[m][4 * q], acc[m][4 * q + 1], acc[m][4 * q + 2], acc[m][4 * q + 3]};
+    __syncthreads();
+    // wave q writes quarter q
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+      store(m, wave, (part[0][m][wave][lane] + part[1][m][wave][lane]) +
+                         (part[2][m][wave][lane] + part[3][m][wave][lane]));
   }
+}
+
+template <int kDepth, int kSplit>
+void launch(const HeadProduct& p, hipStream_t s) {
+  const int n_groups = kSplit == 1 ? (p.n + 127) / 128 : p.n / 32;
+  const bool two = p.tokens > 32;
+  const int m_blocks = (p.tokens + (two ? 63 : 31)) / (two ? 64 : 32);
+  const dim3 g((unsigned)(n_groups * m_blocks), (unsigned)p.heads);
+  if (two) head_product_kernel<2, kDepth, kSplit><<<g, 256, 0, s>>>(p, n_groups);
+  else head_product_kernel<1, kDepth, kSplit><<<g, 256, 0, s>>>(p, n_groups);
 }
 
 }  // namespace
 
 int head_product_launch(const char* name, const HeadProduct& p, hipStream_t s) {
-  const int n_blocks = p.n / 32;
-  const bool two = p.tokens > 32;
-  const int m_blocks = (p.tokens + (two ? 63 : 31)) / (two ? 64 : 32);
-  const int64_t waves = (int64_t)n_blocks * m_blocks;
-  const dim3 g((unsigned)((waves + 3) / 4), (unsigned)p.heads);
-  if (two) head_product_kernel<2><<<g, 256, 0, s>>>(p, n_blocks, m_blocks);
-  else head_product_kernel<1><<<g, 256, 0, s>>>(p, n_blocks, m_blocks);
+  switch (p.k) {
+    case 64: launch<64, 1>(p, s); break;
+    case 128: launch<128, 1>(p, s); break;
+    case 256: launch<64, 4>(p, s); break;
+    case 512: launch<128, 4>(p, s); break;
+    default: return fail(PA_ERR_UNSUPPORTED, "%s: depth %d", name, p.k);
+  }
   return launch_status(name);
 }
 

@@ -23,6 +23,11 @@ __device__ __forceinline__ u32x2 lds_tr8(uint32_t a) {
 __device__ __forceinline__ void lds_dma16(const void* g, uint32_t block) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(block) : "memory", "m0");
 }
+// The same from a scalar base: lane l loads the 16 bytes at base + voff.
+__device__ __forceinline__ void lds_dma16s(uint32_t voff, const void* base, uint32_t block) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(block)
+               : "memory", "m0");
+}
 // s_waitcnt vmcnt(N), other counters untouched
 template <int N>
 __device__ __forceinline__ void wait_vm() {
