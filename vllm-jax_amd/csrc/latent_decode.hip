@@ -14,9 +14,10 @@
 //   waves 4-7 (values):  O^T[R / 4][all rows] in registers, v_mfma_f32_32x32x16
 //       with V^T by transposing LDS reads and P^T from LDS
 // so that one wave's exponentials run under the other's matrix instructions:
-// the values' wave works on tile t - 1 while the scores' wave works on tile t,
+// the values' wave multiplies tile t - 1 while the scores' wave works on tile t,
 // half of it before and half behind the barrier at which the two score waves
-// of a row exchange their maxima.
+// of a row exchange their maxima.  The value waves issue all loads, three tiles
+// ahead.
 //
 // Work is cut on the device: the kv tiles of all (sequence, row tile) units,
 // laid end to end, are dealt to the workgroups in equal contiguous shares; a
@@ -46,7 +47,7 @@ struct AttnParams {
   MagicDiv heads;
   float scale_log2;
   int32_t min_share, wgs;
-  bool pages8;      // the page size is a multiple of 8
+  bool pages8;      // eight aligned rows lie in one page, within 32-bit byte offsets
   // What latent_merge_kernel has to join, [4] each: sequence, row tile, parts (0: nothing), first
   // workgroup; one entry a unit where there are no more units than workgroups
   // (row_tiles > 0: those of a sequence), else one a workgroup.
@@ -88,6 +89,13 @@ __device__ __forceinline__ int rope_swz(int r) {
 __device__ __forceinline__ int fresh(int x) {
   asm volatile("" : "+v"(x));
   return x;
+}
+
+// A wave-uniform pointer, in scalar registers.
+__device__ __forceinline__ const uint16_t* uniform_ptr(const uint16_t* p) {
+  const uint64_t x = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+  return (const uint16_t*)(uintptr_t)((uint64_t)hi << 32 | lo);
 }
 
 // An address as the base of reads with constant offsets.
@@ -288,37 +296,48 @@ latent_attn_kernel(AttnParams p) {
           }
           const int j0 = t * kTile + 16 * tb + 4 * qd;
 #pragma unroll
-          for (int r = 0; r < D::kNr; ++r) {
-            s[r] = (s[r] + s2[r]) * p.scale_log2;
-            if (t >= free_tiles) {
+          for (int r = 0; r < D::kNr; ++r) s[r] = (s[r] + s2[r]) * p.scale_log2;
+          if (t >= free_tiles) {
+#pragma unroll
+            for (int r = 0; r < D::kNr; ++r)
 #pragma unroll
               for (int i = 0; i < 4; ++i) s[r][i] = j0 + i < lim[r] ? s[r][i] : -INFINITY;
-            }
-            mx[r] = __builtin_fmaxf(__builtin_fmaxf(s[r][0], s[r][1]), __builtin_fmaxf(s[r][2], s[r][3]));
-            mx[r] = max_xor32(max_xor16(mx[r]));
-            if (qd == 0) maxes[tb * ROWS + rw + 16 * r + l16] = mx[r];
           }
+#pragma unroll
+          for (int r = 0; r < D::kNr; ++r)
+            mx[r] = __builtin_fmaxf(__builtin_fmaxf(s[r][0], s[r][1]), __builtin_fmaxf(s[r][2], s[r][3]));
+#pragma unroll
+          for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor16(mx[r]);
+#pragma unroll
+          for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor32(mx[r]);
+          // lanes 16 r + l16 write row block r
+          if (qd < D::kNr) maxes[tb * ROWS + rw + ln] = qd == 0 ? mx[0] : mx[D::kNr - 1];
         }
         wait_lgkm0();
         lds_barrier();
         if (t < t1) {
+          float corr[D::kNr];
+#pragma unroll
+          for (int r = 0; r < D::kNr; ++r)
+            mx[r] = __builtin_fmaxf(mx[r], maxes[(tb ^ 1) * ROWS + rw + 16 * r + l16]);
 #pragma unroll
           for (int r = 0; r < D::kNr; ++r) {
-            const int row = rw + 16 * r + l16;
-            const float m_t = __builtin_fmaxf(mx[r], maxes[(tb ^ 1) * ROWS + row]);
-            const float m_new = m_t > m_ref[r] + kSlack ? m_t : m_ref[r];
-            const float corr = fast_exp2(m_ref[r] - m_new);
+            const float m_new = mx[r] > m_ref[r] + kSlack ? mx[r] : m_ref[r];
+            corr[r] = fast_exp2(m_ref[r] - m_new);
             m_ref[r] = m_new;
-            if (tb == 0 && qd == 0) corrs[row] = corr;
-            float e[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = fast_exp2(s[r][i] - m_new);
-            l_sum[r] = l_sum[r] * corr + ((e[0] + e[1]) + (e[2] + e[3]));
+            for (int i = 0; i < 4; ++i) s[r][i] = fast_exp2(s[r][i] - m_new);
+          }
+          if (tb == 0 && qd < D::kNr) corrs[rw + ln] = qd == 0 ? corr[0] : corr[D::kNr - 1];
+#pragma unroll
+          for (int r = 0; r < D::kNr; ++r) {
             // tokens 16 tb + 4 qd .. + 3 of the row: chunk 2 tb + (qd & 1), half
             // qd >> 1 of it, the order in which the transposing reads take V
+            const int row = rw + 16 * r + l16;
             const int c = (2 * tb + (qd & 1)) ^ ((row >> 2) & 3);
             *reinterpret_cast<u32x2*>(smem + D::kPOff + row * 64 + 16 * c + 8 * (qd >> 1)) =
-                u32x2{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3])};
+                u32x2{pack_bf16x2(s[r][0], s[r][1]), pack_bf16x2(s[r][2], s[r][3])};
+            l_sum[r] = l_sum[r] * corr[r] + ((s[r][0] + s[r][1]) + (s[r][2] + s[r][3]));
           }
         }
         wait_lgkm0();
@@ -351,59 +370,77 @@ latent_attn_kernel(AttnParams p) {
         const int page = __builtin_amdgcn_readlane(page_ids, pg - p0);
         return pool.cache + (page * pool.page_stride + (int64_t)(j - pg * (int)pool.page.d) * pool.slot_stride);
       };
-      auto issue = [&](int t) __attribute__((always_inline)) {
-        const uint32_t st = lds0 + (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
-        const uint32_t lat = st + (uint32_t)(8 * pw * D::kRowB), rope = st + (uint32_t)(D::kLatB + 8 * pw * D::kRopeB);
+      // A tile's loads: prepare() finds its rows, load(i) issues piece i of kDma,
+      // so that they can be spread through other work.  Where pages hold eight
+      // aligned rows and all of them are there, a piece is one scalar base and a
+      // lane offset kept in a register; other tiles are looked up row by row, all
+      // of it in load(0).
+      constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
+      uint32_t voff[D::kDma];
+      {
+        const uint32_t sb = 2u * (uint32_t)pool.slot_stride;
+#pragma unroll
+        for (int i = 0; i < D::kLatDma; ++i) {
+          const int r = i * D::kRowsPerDma + (D::kRowsPerDma == 1 ? 0 : lv >> 5);
+          voff[i] = (uint32_t)r * sb + 16 * ((lv & (D::kRowB / 16 - 1)) ^ swz256(8 * pw + r));
+        }
+        const int rr = lv / kC;
+        voff[D::kLatDma] = (uint32_t)rr * sb + 2 * R + 16 * ((lv & (kC - 1)) ^ rope_swz<DR>(8 * pw + rr));
+      }
+      const uint16_t* base = nullptr;
+      int first_row = 0;
+      uint32_t stage = 0;
+      bool rows8 = false;
+      auto prepare = [&](int t) __attribute__((always_inline)) {
+        stage = lds0 + (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
         const int j = t * kTile + 8 * pw;
-        const int ln = fresh(lane);
-        {
-          const int lo = (int)div_by((uint32_t)min(j, lk - 1), pool.page);
-          const int hi = (int)div_by((uint32_t)min(j + 7, lk - 1), pool.page);
-          if (lo < p0 || hi - p0 >= 64) {  // uniform
-            p0 = lo;
-            page_ids = safe_page(bt, min(p0 + lane, pool.pages_per_seq - 1), pool.num_pages);
-            asm volatile("" : "+v"(page_ids));
-          }
+        const int lo = (int)div_by((uint32_t)min(j, lk - 1), pool.page);
+        const int hi = (int)div_by((uint32_t)min(j + 7, lk - 1), pool.page);
+        if (lo < p0 || hi - p0 >= 64) {  // uniform
+          p0 = lo;
+          page_ids = safe_page(bt, min(p0 + lane, pool.pages_per_seq - 1), pool.num_pages);
+          asm volatile("" : "+v"(page_ids));
         }
-        constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
-        const int rr = ln / kC;           // (lns below 8 kC) row of the rotary load
-        const int rc = 8 * ((ln & (kC - 1)) ^ rope_swz<DR>(8 * pw + rr));
-        if (p.pages8) {
-          // eight aligned rows lie in one page; rows past the end repeat the last
-          const int j8 = min(j, (lk - 1) & ~7), last = lk - 1 - j8;
-          const uint16_t* base = row_at(j8);
-#pragma unroll
-          for (int i = 0; i < D::kLatDma; ++i) {
-            if constexpr (D::kRowsPerDma == 1) {
-              lds_dma16s((uint32_t)(16 * (ln ^ swz256(8 * pw + i))), base + min(i, last) * pool.slot_stride,
-                         lat + 1024 * i);
-            } else {
-              const int r = 2 * i + (ln >> 5);
-              lds_dma16(base + min(r, last) * pool.slot_stride + 8 * ((ln & 31) ^ swz256(8 * pw + r)),
-                        lat + 1024 * i);
-            }
+        first_row = j;
+        rows8 = p.pages8 && j + 8 <= lk;
+        if (rows8) base = row_at(j);
+      };
+      auto load_rows = [&]() __attribute__((always_inline)) {
+        const int ln = fresh(lane), rr = ln / kC, j = first_row;
+        const uint16_t* mine = nullptr;
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          const uint16_t* r = row_at(min(j + i, lk - 1));  // rows past the end repeat the last
+          const uint32_t lat = stage + (uint32_t)(8 * pw * D::kRowB);
+          if constexpr (D::kRowsPerDma == 1) {
+            lds_dma16(r + 8 * (ln ^ swz256(8 * pw + i)), lat + 1024 * i);
+          } else if (i & 1) {
+            const uint16_t* own = ln >> 5 ? r : row_at(min(j + i - 1, lk - 1));
+            lds_dma16(own + 8 * ((ln & 31) ^ swz256(8 * pw + i - 1 + (ln >> 5))), lat + 512 * (i - 1));
           }
-          if (ln < 8 * kC) lds_dma16(base + min(rr, last) * pool.slot_stride + R + rc, rope);
-        } else {
-          const uint16_t* mine = nullptr;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint16_t* r = row_at(min(j + i, lk - 1));
-            if (D::kRowsPerDma == 1) {
-              lds_dma16s((uint32_t)(16 * (ln ^ swz256(8 * pw + i))), r, lat + 1024 * i);
-            } else {
-              if (i & 1) {
-                const uint16_t* own = ln >> 5 ? r : row_at(min(j + i - 1, lk - 1));
-                lds_dma16(own + 8 * ((ln & 31) ^ swz256(8 * pw + i - 1 + (ln >> 5))), lat + 1024 * (i >> 1));
-              }
-            }
-            if (rr == i) mine = r;
-          }
-          if (ln < 8 * kC) lds_dma16(mine + R + rc, rope);
+          if (rr == i) mine = r;
         }
+        if (ln < 8 * kC)
+          lds_dma16(mine + R + 8 * ((ln & (kC - 1)) ^ rope_swz<DR>(8 * pw + rr)),
+                    stage + (uint32_t)(D::kLatB + 8 * pw * D::kRopeB));
+      };
+      auto load = [&](int i) __attribute__((always_inline)) {
+        if (!rows8) {
+          if (i == 0) load_rows();
+        } else if (i < D::kLatDma) {
+          lds_dma16s(voff[i], uniform_ptr(base), stage + (uint32_t)(8 * pw * D::kRowB + 1024 * i));
+        } else if (8 * kC == 64 || fresh(lane) < 8 * kC) {
+          lds_dma16s(voff[i], uniform_ptr(base), stage + (uint32_t)(D::kLatB + 8 * pw * D::kRopeB));
+        }
+      };
+      auto issue = [&](int t) __attribute__((always_inline)) {
+        prepare(t);
+#pragma unroll
+        for (int i = 0; i < D::kDma; ++i) load(i);
       };
       issue(t0);
       if (t0 + 1 < t1) issue(t0 + 1);
+      if (t0 + 2 < t1) issue(t0 + 2);
       f32x16 acc[D::kDt][D::kRb] = {};
       // transposing reads of V^T: lane 16 gamma + s reads row 4 h + s / 4 (+ 8)
       // of a 16-token step, columns 32 dt + 16 (gamma % 2) + 4 (s % 4)
@@ -435,19 +472,31 @@ latent_attn_kernel(AttnParams p) {
           v[dt] = as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]});
         }
       };
-      auto product = [&](const bf16x8(&v)[D::kDt], int u) __attribute__((always_inline)) {
+      // The products of 16 tokens; between(i) runs behind the i-th.
+      auto product = [&](const bf16x8(&v)[D::kDt], int u, auto&& between) __attribute__((always_inline)) {
 #pragma unroll
         for (int dt = 0; dt < D::kDt; ++dt)
 #pragma unroll
-          for (int rb = 0; rb < D::kRb; ++rb) acc[dt][rb] = mfma32(v[dt], pt[rb][u], acc[dt][rb]);
+          for (int rb = 0; rb < D::kRb; ++rb) {
+            acc[dt][rb] = mfma32(v[dt], pt[rb][u], acc[dt][rb]);
+            between(dt * D::kRb + rb);
+          }
       };
-      // Tile t + 1 has landed when at most tile t + 2's loads are outstanding.
-      if (t0 + 1 < t1) wait_vm<D::kDma>();
-      else wait_vm<0>();
+      // Tile t has landed when at most the loads of those behind it are outstanding.
+      auto landed = [&](int t, int newest) __attribute__((always_inline)) {
+        if (newest - t >= 2) wait_vm<2 * D::kDma>();
+        else if (newest - t == 1) wait_vm<D::kDma>();
+        else wait_vm<0>();
+      };
+      landed(t0, min(t0 + 2, t1 - 1));
       lds_barrier();
       // Step t: the first half of tile t - 1 before the barrier at which the score
-      // waves exchange maxima, the second behind it; V is read half a step ahead.
+      // waves exchange maxima, the second behind it.  V of tile t is read behind that
+      // barrier too, so that a stage is in use for one step, and tile t + 3's loads
+      // (into the stage of tile t - 1) run between the products.
       for (int t = t0; t <= t1; ++t) {
+        const bool more = t + 3 < t1;
+        constexpr int kProducts = D::kDt * D::kRb, kHalf = (D::kDma + 1) / 2;
         if (t > t0) {
           float corr[D::kRb];
 #pragma unroll
@@ -456,23 +505,46 @@ latent_attn_kernel(AttnParams p) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) pt[rb][u] = as_bf16x8(lds_ld16(poff[rb][u]));
           }
-          read_v(v1, 1, t - 1);
           __builtin_amdgcn_sched_barrier(0);
+          if (more) {
+            prepare(t + 3);
+            load(0);
+          }
 #pragma unroll
           for (int rb = 0; rb < D::kRb; ++rb)
             if (__any(corr[rb] != 1.f)) {
 #pragma unroll
               for (int dt = 0; dt < D::kDt; ++dt) acc[dt][rb] = acc[dt][rb] * corr[rb];
             }
-          product(v0, 0);
+          product(v0, 0, [&](int i) __attribute__((always_inline)) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) {
+#pragma unroll
+              for (int k = 1 + i * (kHalf - 1) / kProducts; k < 1 + (i + 1) * (kHalf - 1) / kProducts; ++k) load(k);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          });
+        } else if (more) {
+          issue(t + 3);
         }
-        if (t + 2 < t1) issue(t + 2);  // under the products; into the stage of tile t - 2
         wait_lgkm0();  // P is in registers: the score waves may overwrite it
         lds_barrier();
-        if (t > t0) product(v1, 1);
         if (t < t1) read_v(v0, 0, t);
-        if (t + 2 < t1) wait_vm<D::kDma>();
-        else wait_vm<0>();
+        __builtin_amdgcn_sched_barrier(0);
+        if (t > t0)
+          product(v1, 1, [&](int i) __attribute__((always_inline)) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) {
+#pragma unroll
+              for (int k = kHalf + i * (D::kDma - kHalf) / kProducts; k < kHalf + (i + 1) * (D::kDma - kHalf) / kProducts;
+                   ++k)
+                load(k);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          });
+        __builtin_amdgcn_sched_barrier(0);
+        if (t < t1) read_v(v1, 1, t);
+        landed(t + 1, min(t + 3, t1 - 1));
         wait_lgkm0();
         lds_barrier();
       }
@@ -689,7 +761,8 @@ int latent_attn_launch(const char* name, const LatentAttn& a, int latent, int ro
   p.heads = magic_div((uint32_t)a.heads);
   p.scale_log2 = a.scale * kLog2e;
   p.min_share = kMinShare;
-  p.pages8 = a.pool.page.d % 8 == 0;
+  // eight rows' byte offsets from the first fit 32 bits
+  p.pages8 = a.pool.page.d % 8 == 0 && a.pool.slot_stride >= 0 && a.pool.slot_stride < (1 << 27);
   const int rows = rows_of(a.max_q, a.heads);
   const int64_t row_tiles = ((int64_t)a.max_q * a.heads + rows - 1) / rows;
   const int64_t span = (int64_t)a.pool.pages_per_seq * a.pool.page.d;

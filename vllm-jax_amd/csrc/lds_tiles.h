@@ -31,8 +31,8 @@ __device__ __forceinline__ void lds_dma16s(uint32_t voff, const void* base, uint
 // s_waitcnt vmcnt(N), other counters untouched
 template <int N>
 __device__ __forceinline__ void wait_vm() {
-  static_assert(N < 16);
-  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8));
+  static_assert(N < 64);
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
 }
 __device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8)); }
 
