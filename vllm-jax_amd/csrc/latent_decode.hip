@@ -15,9 +15,7 @@
 //       with V^T by transposing LDS reads and P^T from LDS
 // so that one wave's exponentials run under the other's matrix instructions:
 // the values' wave multiplies tile t - 1 while the scores' wave works on tile t,
-// half of it before and half behind the barrier at which the two score waves
-// of a row exchange their maxima.  The value waves issue all loads, three tiles
-// ahead.
+// with one barrier a tile.  The value waves issue all loads, three tiles ahead.
 //
 // Work is cut on the device: the kv tiles of all (sequence, row tile) units,
 // laid end to end, are dealt to the workgroups in equal contiguous shares; a
@@ -39,7 +37,8 @@ constexpr int kTile = 32;      // kv tokens per tile
 constexpr int kLStages = 4;
 constexpr int kLThreads = 512;
 constexpr int kMaxBatch = 16384;  // their prefix sums fit the ring
-constexpr float kSlack = 8.f;  // log2 units the running maximum may lag
+constexpr float kSlack = 8.f;  // log2 units a tile's reference may lag behind the maximum of those before it
+constexpr float kJump = 64.f;  // and a half tile's behind its own
 constexpr float kNoMax = -1e30f;
 
 struct AttnParams {
@@ -64,11 +63,14 @@ struct Dims {
   static constexpr int kLatB = kTile * kRowB;
   static constexpr int kStageB = kLatB + kTile * kRopeB;
   static constexpr int kRing = kLStages * kStageB;
-  static constexpr int kPOff = kRing;                 // P: [ROWS][32] bf16
-  static constexpr int kMaxOff = kPOff + ROWS * 64;   // maxima [2][ROWS], then corrections [ROWS]
-  static constexpr int kCorrOff = kMaxOff + 2 * ROWS * 4;
-  static constexpr int kSumOff = kCorrOff + ROWS * 4;  // sums [2][ROWS], maxima [ROWS] at the end
-  static constexpr int kLds = kSumOff + 3 * ROWS * 4;
+  // Of even and odd tiles: P [ROWS][32] bf16, and for each half tile and row its
+  // maximum and the reference of its P.  Sums [2][ROWS] at the end.
+  static constexpr int kPB = ROWS * 64, kRefB = 2 * ROWS * 4;
+  static constexpr int kPOff = kRing;
+  static constexpr int kMaxOff = kPOff + 2 * kPB;
+  static constexpr int kRefOff = kMaxOff + 2 * kRefB;
+  static constexpr int kSumOff = kRefOff + 2 * kRefB;
+  static constexpr int kLds = kSumOff + 2 * ROWS * 4;
   static constexpr int kKs = R / 32, kRs = DR / 32;   // 32-deep k-steps of the scores
   static constexpr int kNr = ROWS / 32;               // 16-row blocks of a score wave
   static constexpr int kDt = R / 128;                 // 32-row blocks of O^T of a value wave
@@ -244,10 +246,15 @@ latent_attn_kernel(AttnParams p) {
       // first tile a row of this tile does not see in full
       const int tok_first = (int)div_by((uint32_t)(rt * ROWS), p.heads);
       const int free_tiles = max(0, min(lk, sq.first + tok_first + 1)) / kTile;
-      float m_ref[D::kNr], l_sum[D::kNr];
+      // The reference of a tile's P is common to both half tiles: that of O, or the
+      // previous tile's maximum where that passes it by the slack.  The waves of a
+      // row see each other's maxima a tile late; a half tile whose own maximum
+      // passes the common reference by kJump takes its maximum, and the value
+      // waves bring the halves together.
+      float common[D::kNr], own_ref[D::kNr], own_max[D::kNr], l_sum[D::kNr];
 #pragma unroll
       for (int r = 0; r < D::kNr; ++r) {
-        m_ref[r] = kNoMax;
+        common[r] = own_ref[r] = own_max[r] = kNoMax;
         l_sum[r] = 0.f;
       }
       // reads of K: row 16 tb + l16, chunk 4 ks + qd
@@ -259,100 +266,96 @@ latent_attn_kernel(AttnParams p) {
 #pragma unroll
       for (int i = 0; i < D::kRs; ++i)
         roff[i] = lds0 + D::kLatB + krow * D::kRopeB + 16 * ((4 * i + qd) ^ rope_swz<DR>(krow));
-      float* maxes = reinterpret_cast<float*>(smem + D::kMaxOff);
-      float* corrs = reinterpret_cast<float*>(smem + D::kCorrOff);
       lds_barrier();  // the first tile is there
-      for (int t = t0; t <= t1; ++t) {
-        f32x4 s[D::kNr];
-        float mx[D::kNr];
-        if (t < t1) {
-          const uint32_t st = (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
-          f32x4 s2[D::kNr];
+      for (int t = t0; t < t1; ++t) {
+        const uint32_t st = (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
+        float other[D::kNr];  // (first tile: not used)
+        {
+          const float* maxes = reinterpret_cast<const float*>(smem + D::kMaxOff + ((t - 1) & 1) * D::kRefB);
 #pragma unroll
-          for (int r = 0; r < D::kNr; ++r) s[r] = s2[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-          uint32_t ka[4], ra[D::kRs];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) ka[i] = fresh_addr(koff[i] + st);
-#pragma unroll
-          for (int i = 0; i < D::kRs; ++i) ra[i] = fresh_addr(roff[i] + st);
-          // every read is issued kAhead k-steps before the products it feeds
-          constexpr int kAll = D::kKs + D::kRs, kAhead = 6;
-          bf16x8 a[kAll];
-          auto read_k = [&](int ks) __attribute__((always_inline)) {
-            a[ks] = as_bf16x8(ks < D::kKs ? lds_ld16(ka[ks & 3] + (ks >> 2) * 256)
-                                          : lds_ld16(ra[(ks - D::kKs) % D::kRs]));
-          };
-#pragma unroll
-          for (int ks = 0; ks < kAhead; ++ks) read_k(ks);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int ks = 0; ks < kAll; ++ks) {
-#pragma unroll
-            for (int r = 0; r < D::kNr; ++r)
-              if (ks & 1) s2[r] = mfma16(a[ks], q[r][ks], s2[r]);
-              else s[r] = mfma16(a[ks], q[r][ks], s[r]);
-            if (ks + kAhead < kAll) read_k(ks + kAhead);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-          const int j0 = t * kTile + 16 * tb + 4 * qd;
-#pragma unroll
-          for (int r = 0; r < D::kNr; ++r) s[r] = (s[r] + s2[r]) * p.scale_log2;
-          if (t >= free_tiles) {
-#pragma unroll
-            for (int r = 0; r < D::kNr; ++r)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) s[r][i] = j0 + i < lim[r] ? s[r][i] : -INFINITY;
-          }
-#pragma unroll
-          for (int r = 0; r < D::kNr; ++r)
-            mx[r] = __builtin_fmaxf(__builtin_fmaxf(s[r][0], s[r][1]), __builtin_fmaxf(s[r][2], s[r][3]));
-#pragma unroll
-          for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor16(mx[r]);
-#pragma unroll
-          for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor32(mx[r]);
-          // lanes 16 r + l16 write row block r
-          if (qd < D::kNr) maxes[tb * ROWS + rw + ln] = qd == 0 ? mx[0] : mx[D::kNr - 1];
+          for (int r = 0; r < D::kNr; ++r) other[r] = maxes[(tb ^ 1) * ROWS + rw + 16 * r + l16];
         }
-        wait_lgkm0();
-        lds_barrier();
-        if (t < t1) {
-          float corr[D::kNr];
+        f32x4 s[D::kNr], s2[D::kNr];
+        float mx[D::kNr];
+#pragma unroll
+        for (int r = 0; r < D::kNr; ++r) s[r] = s2[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+        uint32_t ka[4], ra[D::kRs];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ka[i] = fresh_addr(koff[i] + st);
+#pragma unroll
+        for (int i = 0; i < D::kRs; ++i) ra[i] = fresh_addr(roff[i] + st);
+        // every read is issued kAhead k-steps before the products it feeds
+        constexpr int kAll = D::kKs + D::kRs, kAhead = 6;
+        bf16x8 a[kAll];
+        auto read_k = [&](int ks) __attribute__((always_inline)) {
+          a[ks] = as_bf16x8(ks < D::kKs ? lds_ld16(ka[ks & 3] + (ks >> 2) * 256)
+                                        : lds_ld16(ra[(ks - D::kKs) % D::kRs]));
+        };
+#pragma unroll
+        for (int ks = 0; ks < kAhead; ++ks) read_k(ks);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < kAll; ++ks) {
 #pragma unroll
           for (int r = 0; r < D::kNr; ++r)
-            mx[r] = __builtin_fmaxf(mx[r], maxes[(tb ^ 1) * ROWS + rw + 16 * r + l16]);
+            if (ks & 1) s2[r] = mfma16(a[ks], q[r][ks], s2[r]);
+            else s[r] = mfma16(a[ks], q[r][ks], s[r]);
+          if (ks + kAhead < kAll) read_k(ks + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const int j0 = t * kTile + 16 * tb + 4 * qd;
 #pragma unroll
-          for (int r = 0; r < D::kNr; ++r) {
-            const float m_new = mx[r] > m_ref[r] + kSlack ? mx[r] : m_ref[r];
-            corr[r] = fast_exp2(m_ref[r] - m_new);
-            m_ref[r] = m_new;
+        for (int r = 0; r < D::kNr; ++r) s[r] = (s[r] + s2[r]) * p.scale_log2;
+        if (t >= free_tiles) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[r][i] = fast_exp2(s[r][i] - m_new);
+          for (int r = 0; r < D::kNr; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[r][i] = j0 + i < lim[r] ? s[r][i] : -INFINITY;
+        }
+#pragma unroll
+        for (int r = 0; r < D::kNr; ++r)
+          mx[r] = __builtin_fmaxf(__builtin_fmaxf(s[r][0], s[r][1]), __builtin_fmaxf(s[r][2], s[r][3]));
+#pragma unroll
+        for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor16(mx[r]);
+#pragma unroll
+        for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor32(mx[r]);
+#pragma unroll
+        for (int r = 0; r < D::kNr; ++r) {
+          if (t > t0) {
+            const float other_ref = other[r] > common[r] + kJump ? other[r] : common[r];
+            const float ref = __builtin_fmaxf(own_ref[r], other_ref), m = __builtin_fmaxf(own_max[r], other[r]);
+            common[r] = m > ref + kSlack ? m : ref;
           }
-          if (tb == 0 && qd < D::kNr) corrs[rw + ln] = qd == 0 ? corr[0] : corr[D::kNr - 1];
+          const float ref = mx[r] > common[r] + kJump ? mx[r] : common[r];
+          own_max[r] = mx[r];
 #pragma unroll
-          for (int r = 0; r < D::kNr; ++r) {
-            // tokens 16 tb + 4 qd .. + 3 of the row: chunk 2 tb + (qd & 1), half
-            // qd >> 1 of it, the order in which the transposing reads take V
-            const int row = rw + 16 * r + l16;
-            const int c = (2 * tb + (qd & 1)) ^ ((row >> 2) & 3);
-            *reinterpret_cast<u32x2*>(smem + D::kPOff + row * 64 + 16 * c + 8 * (qd >> 1)) =
-                u32x2{pack_bf16x2(s[r][0], s[r][1]), pack_bf16x2(s[r][2], s[r][3])};
-            l_sum[r] = l_sum[r] * corr[r] + ((s[r][0] + s[r][1]) + (s[r][2] + s[r][3]));
-          }
+          for (int i = 0; i < 4; ++i) s[r][i] = fast_exp2(s[r][i] - ref);
+          l_sum[r] = l_sum[r] * fast_exp2(own_ref[r] - ref) + ((s[r][0] + s[r][1]) + (s[r][2] + s[r][3]));
+          own_ref[r] = ref;
+          // tokens 16 tb + 4 qd .. + 3 of the row: chunk 2 tb + (qd & 1), half
+          // qd >> 1 of it, the order in which the transposing reads take V
+          const int row = rw + 16 * r + l16;
+          const int c = (2 * tb + (qd & 1)) ^ ((row >> 2) & 3);
+          *reinterpret_cast<u32x2*>(smem + D::kPOff + (t & 1) * D::kPB + row * 64 + 16 * c + 8 * (qd >> 1)) =
+              u32x2{pack_bf16x2(s[r][0], s[r][1]), pack_bf16x2(s[r][2], s[r][3])};
+        }
+        // lanes 16 r + l16 write row block r
+        if (qd < D::kNr) {
+          const int at = (t & 1) * D::kRefB + (tb * ROWS + rw + ln) * 4;
+          *reinterpret_cast<float*>(smem + D::kMaxOff + at) = qd == 0 ? mx[0] : mx[D::kNr - 1];
+          *reinterpret_cast<float*>(smem + D::kRefOff + at) = qd == 0 ? own_ref[0] : own_ref[D::kNr - 1];
         }
         wait_lgkm0();
         lds_barrier();
       }
-      // ---- row sums and maxima
+      lds_barrier();  // the value waves' last step
+      // ---- row sums, relative to the last tile's references
       float* sums = reinterpret_cast<float*>(smem + D::kSumOff);
 #pragma unroll
       for (int r = 0; r < D::kNr; ++r) {
         const float l = sum_xor32(sum_xor16(l_sum[r]));
         const int row = rw + 16 * r + l16;
-        if (qd == 0) {
-          sums[tb * ROWS + row] = l;
-          if (tb == 0) sums[2 * ROWS + row] = m_ref[r];
-        }
+        if (qd == 0) sums[tb * ROWS + row] = l;
       }
       wait_lgkm0();
       lds_barrier();
@@ -373,8 +376,8 @@ latent_attn_kernel(AttnParams p) {
       // A tile's loads: prepare() finds its rows, load(i) issues piece i of kDma,
       // so that they can be spread through other work.  Where pages hold eight
       // aligned rows and all of them are there, a piece is one scalar base and a
-      // lane offset kept in a register; other tiles are looked up row by row, all
-      // of it in load(0).
+      // lane offset kept in a register; other tiles are looked up row by row
+      // (load_rows).
       constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
       uint32_t voff[D::kDma];
       {
@@ -425,9 +428,7 @@ latent_attn_kernel(AttnParams p) {
                     stage + (uint32_t)(D::kLatB + 8 * pw * D::kRopeB));
       };
       auto load = [&](int i) __attribute__((always_inline)) {
-        if (!rows8) {
-          if (i == 0) load_rows();
-        } else if (i < D::kLatDma) {
+        if (i < D::kLatDma) {
           lds_dma16s(voff[i], uniform_ptr(base), stage + (uint32_t)(8 * pw * D::kRowB + 1024 * i));
         } else if (8 * kC == 64 || fresh(lane) < 8 * kC) {
           lds_dma16s(voff[i], uniform_ptr(base), stage + (uint32_t)(D::kLatB + 8 * pw * D::kRopeB));
@@ -435,8 +436,12 @@ latent_attn_kernel(AttnParams p) {
       };
       auto issue = [&](int t) __attribute__((always_inline)) {
         prepare(t);
+        if (rows8) {
 #pragma unroll
-        for (int i = 0; i < D::kDma; ++i) load(i);
+          for (int i = 0; i < D::kDma; ++i) load(i);
+        } else {
+          load_rows();
+        }
       };
       issue(t0);
       if (t0 + 1 < t1) issue(t0 + 1);
@@ -459,7 +464,9 @@ latent_attn_kernel(AttnParams p) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
           poff[rb][u] = lds0 + D::kPOff + (32 * rb + n) * 64 + 16 * ((2 * u + h) ^ ((n >> 2) & 3));
-      const float* corrs = reinterpret_cast<const float*>(smem + D::kCorrOff);
+      float m_ref[D::kRb];  // reference of O
+#pragma unroll
+      for (int rb = 0; rb < D::kRb; ++rb) m_ref[rb] = kNoMax;
       // (set here, or the compiler carries them through the segments)
       bf16x8 pt[D::kRb][2] = {};
       bf16x8 v0[D::kDt] = {}, v1[D::kDt] = {};  // V^T of the first and second 16 tokens of a tile
@@ -490,72 +497,93 @@ latent_attn_kernel(AttnParams p) {
       };
       landed(t0, min(t0 + 2, t1 - 1));
       lds_barrier();
-      // Step t: the first half of tile t - 1 before the barrier at which the score
-      // waves exchange maxima, the second behind it.  V of tile t is read behind that
-      // barrier too, so that a stage is in use for one step, and tile t + 3's loads
-      // (into the stage of tile t - 1) run between the products.
-      for (int t = t0; t <= t1; ++t) {
+      // Step t: the products of tile t - 1; V of tile t is read behind them, so that
+      // a stage is in use for one step only (behind the last tile: stale rows, not
+      // used), and tile t + 3's loads (into the stage of tile t - 1) run between them.
+      read_v(v0, 0, t0);
+      read_v(v1, 1, t0);
+      if (t0 + 3 < t1) issue(t0 + 3);
+      landed(t0 + 1, min(t0 + 3, t1 - 1));
+      wait_lgkm0();
+      lds_barrier();
+      for (int t = t0 + 1; t <= t1; ++t) {
         const bool more = t + 3 < t1;
-        constexpr int kProducts = D::kDt * D::kRb, kHalf = (D::kDma + 1) / 2;
-        if (t > t0) {
-          float corr[D::kRb];
+        constexpr int kProducts = 2 * D::kDt * D::kRb;
+        const uint32_t odd = (uint32_t)((t - 1) & 1);
+        const float* refs = reinterpret_cast<const float*>(smem + D::kRefOff + odd * D::kRefB);
+        float a0[D::kRb], a1[D::kRb];
 #pragma unroll
-          for (int rb = 0; rb < D::kRb; ++rb) {
-            corr[rb] = corrs[32 * rb + n];
+        for (int rb = 0; rb < D::kRb; ++rb) {
+          a0[rb] = refs[32 * rb + n];
+          a1[rb] = refs[ROWS + 32 * rb + n];
+        }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) pt[rb][u] = as_bf16x8(lds_ld16(poff[rb][u]));
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb) pt[rb][u] = as_bf16x8(lds_ld16(poff[rb][u] + odd * D::kPB));
+        __builtin_amdgcn_sched_barrier(0);
+        bool spread = false;
+        if (more) {
+          prepare(t + 3);
+          spread = rows8;
+          if (!spread) load_rows();
+        }
+        // A tile whose halves do not share O's reference: the larger of theirs is the
+        // new one; O and the other half's P are brought to it.
+        float up[D::kRb];
+#pragma unroll
+        for (int rb = 0; rb < D::kRb; ++rb) {
+          const float m_new = __builtin_fmaxf(a0[rb], a1[rb]);
+          up[rb] = fast_exp2(m_ref[rb] - m_new);
+          m_ref[rb] = m_new;
+        }
+#pragma unroll
+        for (int rb = 0; rb < D::kRb; ++rb)
+          if (__any(up[rb] != 1.f)) {
+#pragma unroll
+            for (int dt = 0; dt < D::kDt; ++dt) acc[dt][rb] = acc[dt][rb] * up[rb];
+          }
+#pragma unroll
+        for (int rb = 0; rb < D::kRb; ++rb)
+          if (__any(a0[rb] != a1[rb])) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float f = fast_exp2((u ? a1[rb] : a0[rb]) - m_ref[rb]);
+              u32x4 w = as_u32x4(pt[rb][u]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(bf16_lo(w[e]) * f, bf16_hi(w[e]) * f);
+              pt[rb][u] = as_bf16x8(w);
+            }
+          }
+        auto loads = [&](int i) __attribute__((always_inline)) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (spread) {
+#pragma unroll
+            for (int k = i * D::kDma / kProducts; k < (i + 1) * D::kDma / kProducts; ++k) load(k);
           }
           __builtin_amdgcn_sched_barrier(0);
-          if (more) {
-            prepare(t + 3);
-            load(0);
-          }
-#pragma unroll
-          for (int rb = 0; rb < D::kRb; ++rb)
-            if (__any(corr[rb] != 1.f)) {
-#pragma unroll
-              for (int dt = 0; dt < D::kDt; ++dt) acc[dt][rb] = acc[dt][rb] * corr[rb];
-            }
-          product(v0, 0, [&](int i) __attribute__((always_inline)) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (more) {
-#pragma unroll
-              for (int k = 1 + i * (kHalf - 1) / kProducts; k < 1 + (i + 1) * (kHalf - 1) / kProducts; ++k) load(k);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-          });
-        } else if (more) {
-          issue(t + 3);
-        }
-        wait_lgkm0();  // P is in registers: the score waves may overwrite it
-        lds_barrier();
-        if (t < t1) read_v(v0, 0, t);
-        __builtin_amdgcn_sched_barrier(0);
-        if (t > t0)
-          product(v1, 1, [&](int i) __attribute__((always_inline)) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (more) {
-#pragma unroll
-              for (int k = kHalf + i * (D::kDma - kHalf) / kProducts; k < kHalf + (i + 1) * (D::kDma - kHalf) / kProducts;
-                   ++k)
-                load(k);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-          });
-        __builtin_amdgcn_sched_barrier(0);
-        if (t < t1) read_v(v1, 1, t);
+        };
+        product(v0, 0, loads);
+        read_v(v0, 0, t);
+        product(v1, 1, [&](int i) __attribute__((always_inline)) { loads(kProducts / 2 + i); });
+        read_v(v1, 1, t);
         landed(t + 1, min(t + 3, t1 - 1));
         wait_lgkm0();
         lds_barrier();
       }
       lds_barrier();  // sums are there
       const int le = fresh(lane), ne = le & 31, he = le >> 5;
+      // a row's sum: those of its half tiles, brought to O's reference
       const float* sums = reinterpret_cast<const float*>(smem + D::kSumOff);
+      const float* refs = reinterpret_cast<const float*>(smem + D::kRefOff + ((t1 - 1) & 1) * D::kRefB);
+      auto row_sum = [&](int r, float m) __attribute__((always_inline)) {
+        return sums[r] * fast_exp2(refs[r] - m) + sums[ROWS + r] * fast_exp2(refs[ROWS + r] - m);
+      };
       if (t0 == 0 && t1 == sq.nt) {
 #pragma unroll
         for (int rb = 0; rb < D::kRb; ++rb) {
           const int r = 32 * rb + ne;
-          const float l = sums[r] + sums[ROWS + r];
+          const float l = row_sum(r, m_ref[rb]);
           const float inv = l > 0.f ? 1.f / l : 0.f;
           if (r < n_rows) {
             const int row = rt * ROWS + r;
@@ -585,9 +613,11 @@ latent_attn_kernel(AttnParams p) {
               *reinterpret_cast<f32x4*>(dst + 256 * (((pw * D::kDt + dt) * D::kRb + rb) * 4 + i)) =
                   f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
             }
-        if (pw == 0 && le < ROWS) {
-          const float l = sums[le] + sums[ROWS + le];
-          *reinterpret_cast<f32x2*>(p.stats + ((int64_t)slot * ROWS + le) * 2) = f32x2{sums[2 * ROWS + le], l};
+        if (pw == 0 && he == 0) {
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb)
+            *reinterpret_cast<f32x2*>(p.stats + ((int64_t)slot * ROWS + 32 * rb + ne) * 2) =
+                f32x2{m_ref[rb], row_sum(32 * rb + ne, m_ref[rb])};
         }
       }
     }

@@ -21,11 +21,11 @@ __device__ __forceinline__ u32x2 lds_tr8(uint32_t a) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(uintptr_t)a));
 }
 __device__ __forceinline__ void lds_dma16(const void* g, uint32_t block) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(block) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(__builtin_amdgcn_readfirstlane(block)) : "memory", "m0");
 }
 // The same from a scalar base: lane l loads the 16 bytes at base + voff.
 __device__ __forceinline__ void lds_dma16s(uint32_t voff, const void* base, uint32_t block) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(block)
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(__builtin_amdgcn_readfirstlane(block))
                : "memory", "m0");
 }
 // s_waitcnt vmcnt(N), other counters untouched
