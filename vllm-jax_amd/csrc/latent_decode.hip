@@ -14,8 +14,8 @@
 //   waves 4-7 (values):  O^T[R / 4][all rows] in registers, v_mfma_f32_32x32x16
 //       with V^T by transposing LDS reads and P^T from LDS
 // so that one wave's exponentials run under the other's matrix instructions:
-// the values' wave multiplies tile t - 1 while the scores' wave works on tile t,
-// with one barrier a tile.  The value waves issue all loads, three tiles ahead.
+// the values' wave multiplies tile t - 2 while the scores' wave works on tile t,
+// with one barrier a tile.  The value waves issue all loads, two tiles ahead.
 //
 // Work is cut on the device: the kv tiles of all (sequence, row tile) units,
 // laid end to end, are dealt to the workgroups in equal contiguous shares; a
@@ -63,13 +63,15 @@ struct Dims {
   static constexpr int kLatB = kTile * kRowB;
   static constexpr int kStageB = kLatB + kTile * kRopeB;
   static constexpr int kRing = kLStages * kStageB;
-  // Of even and odd tiles: P [ROWS][32] bf16, and for each half tile and row its
-  // maximum and the reference of its P.  Sums [2][ROWS] at the end.
+  // Of even and odd tiles: P [ROWS][32] bf16, for each half tile and row its
+  // maximum and the reference of its P, and for each row the reference that the
+  // value waves ask for.  Sums [2][ROWS] at the end.
   static constexpr int kPB = ROWS * 64, kRefB = 2 * ROWS * 4;
   static constexpr int kPOff = kRing;
   static constexpr int kMaxOff = kPOff + 2 * kPB;
   static constexpr int kRefOff = kMaxOff + 2 * kRefB;
-  static constexpr int kSumOff = kRefOff + 2 * kRefB;
+  static constexpr int kAskOff = kRefOff + 2 * kRefB;
+  static constexpr int kSumOff = kAskOff + kRefB;
   static constexpr int kLds = kSumOff + 2 * ROWS * 4;
   static constexpr int kKs = R / 32, kRs = DR / 32;   // 32-deep k-steps of the scores
   static constexpr int kNr = ROWS / 32;               // 16-row blocks of a score wave
@@ -246,15 +248,14 @@ latent_attn_kernel(AttnParams p) {
       // first tile a row of this tile does not see in full
       const int tok_first = (int)div_by((uint32_t)(rt * ROWS), p.heads);
       const int free_tiles = max(0, min(lk, sq.first + tok_first + 1)) / kTile;
-      // The reference of a tile's P is common to both half tiles: that of O, or the
-      // previous tile's maximum where that passes it by the slack.  The waves of a
-      // row see each other's maxima a tile late; a half tile whose own maximum
-      // passes the common reference by kJump takes its maximum, and the value
-      // waves bring the halves together.
-      float common[D::kNr], own_ref[D::kNr], own_max[D::kNr], l_sum[D::kNr];
+      // The reference of a half tile's P: the one the value waves ask for (the
+      // maximum two tiles ago, where that passes O's reference by the slack) or
+      // this wave's own last one; a half tile whose maximum passes that by kJump
+      // takes its maximum.  The value waves bring the halves together.
+      float own_ref[D::kNr], l_sum[D::kNr];
 #pragma unroll
       for (int r = 0; r < D::kNr; ++r) {
-        common[r] = own_ref[r] = own_max[r] = kNoMax;
+        own_ref[r] = kNoMax;
         l_sum[r] = 0.f;
       }
       // reads of K: row 16 tb + l16, chunk 4 ks + qd
@@ -269,16 +270,16 @@ latent_attn_kernel(AttnParams p) {
       lds_barrier();  // the first tile is there
       for (int t = t0; t < t1; ++t) {
         const uint32_t st = (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
-        float other[D::kNr];  // (first tile: not used)
+        float ask[D::kNr];  // (first two tiles: not written yet)
         {
-          const float* maxes = reinterpret_cast<const float*>(smem + D::kMaxOff + ((t - 1) & 1) * D::kRefB);
+          const float* asks = reinterpret_cast<const float*>(smem + D::kAskOff + ((t - 1) & 1) * (ROWS * 4));
 #pragma unroll
-          for (int r = 0; r < D::kNr; ++r) other[r] = maxes[(tb ^ 1) * ROWS + rw + 16 * r + l16];
+          for (int r = 0; r < D::kNr; ++r) ask[r] = asks[rw + 16 * r + l16];
         }
-        f32x4 s[D::kNr], s2[D::kNr];
+        f32x4 s[D::kNr];
         float mx[D::kNr];
 #pragma unroll
-        for (int r = 0; r < D::kNr; ++r) s[r] = s2[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < D::kNr; ++r) s[r] = f32x4{0.f, 0.f, 0.f, 0.f};
         uint32_t ka[4], ra[D::kRs];
 #pragma unroll
         for (int i = 0; i < 4; ++i) ka[i] = fresh_addr(koff[i] + st);
@@ -298,14 +299,11 @@ latent_attn_kernel(AttnParams p) {
         for (int ks = 0; ks < kAll; ++ks) {
 #pragma unroll
           for (int r = 0; r < D::kNr; ++r)
-            if (ks & 1) s2[r] = mfma16(a[ks], q[r][ks], s2[r]);
-            else s[r] = mfma16(a[ks], q[r][ks], s[r]);
+            s[r] = mfma16(a[ks], q[r][ks], s[r]);
           if (ks + kAhead < kAll) read_k(ks + kAhead);
           __builtin_amdgcn_sched_barrier(0);
         }
         const int j0 = t * kTile + 16 * tb + 4 * qd;
-#pragma unroll
-        for (int r = 0; r < D::kNr; ++r) s[r] = (s[r] + s2[r]) * p.scale_log2;
         if (t >= free_tiles) {
 #pragma unroll
           for (int r = 0; r < D::kNr; ++r)
@@ -319,19 +317,21 @@ latent_attn_kernel(AttnParams p) {
         for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor16(mx[r]);
 #pragma unroll
         for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor32(mx[r]);
+        float corr[D::kNr];
 #pragma unroll
         for (int r = 0; r < D::kNr; ++r) {
-          if (t > t0) {
-            const float other_ref = other[r] > common[r] + kJump ? other[r] : common[r];
-            const float ref = __builtin_fmaxf(own_ref[r], other_ref), m = __builtin_fmaxf(own_max[r], other[r]);
-            common[r] = m > ref + kSlack ? m : ref;
-          }
-          const float ref = mx[r] > common[r] + kJump ? mx[r] : common[r];
-          own_max[r] = mx[r];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[r][i] = fast_exp2(s[r][i] - ref);
-          l_sum[r] = l_sum[r] * fast_exp2(own_ref[r] - ref) + ((s[r][0] + s[r][1]) + (s[r][2] + s[r][3]));
+          mx[r] *= p.scale_log2;  // positive
+          const float base = t > t0 + 1 ? __builtin_fmaxf(own_ref[r], ask[r]) : own_ref[r];
+          const float ref = mx[r] > base + kJump ? mx[r] : base;
+          corr[r] = fast_exp2(own_ref[r] - ref);
           own_ref[r] = ref;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int r = 0; r < D::kNr; ++r) s[r][i] = fast_exp2(__builtin_fmaf(s[r][i], p.scale_log2, -own_ref[r]));
+#pragma unroll
+        for (int r = 0; r < D::kNr; ++r) {
           // tokens 16 tb + 4 qd .. + 3 of the row: chunk 2 tb + (qd & 1), half
           // qd >> 1 of it, the order in which the transposing reads take V
           const int row = rw + 16 * r + l16;
@@ -345,6 +345,8 @@ latent_attn_kernel(AttnParams p) {
           *reinterpret_cast<float*>(smem + D::kMaxOff + at) = qd == 0 ? mx[0] : mx[D::kNr - 1];
           *reinterpret_cast<float*>(smem + D::kRefOff + at) = qd == 0 ? own_ref[0] : own_ref[D::kNr - 1];
         }
+#pragma unroll
+        for (int r = 0; r < D::kNr; ++r) l_sum[r] = l_sum[r] * corr[r] + ((s[r][0] + s[r][1]) + (s[r][2] + s[r][3]));
         wait_lgkm0();
         lds_barrier();
       }
@@ -365,19 +367,12 @@ latent_attn_kernel(AttnParams p) {
       const int lv = fresh(lane), n = lv & 31, h = lv >> 5;
 
       // ---- tile loads: this wave's rows are 8 pw .. 8 pw + 7 of every tile.
-      // Page ids of 64 pages from p0 on sit in the lanes of one register.
-      int p0 = 0x40000000, page_ids = 0;
       const int32_t* bt = pool.tables + (int64_t)b * pool.bt_stride;
-      auto row_at = [&](int j) __attribute__((always_inline)) {  // uniform j
-        const int pg = (int)div_by((uint32_t)j, pool.page);
-        const int page = __builtin_amdgcn_readlane(page_ids, pg - p0);
-        return pool.cache + (page * pool.page_stride + (int64_t)(j - pg * (int)pool.page.d) * pool.slot_stride);
-      };
       // A tile's loads: prepare() finds its rows, load(i) issues piece i of kDma,
       // so that they can be spread through other work.  Where pages hold eight
-      // aligned rows and all of them are there, a piece is one scalar base and a
-      // lane offset kept in a register; other tiles are looked up row by row
-      // (load_rows).
+      // aligned rows and all of them are there, a piece is one scalar base (made
+      // for 64 tiles at a time, one a lane) and a lane offset kept in a register;
+      // other tiles are looked up row by row (load_rows).
       constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
       uint32_t voff[D::kDma];
       {
@@ -391,37 +386,50 @@ latent_attn_kernel(AttnParams p) {
         voff[D::kLatDma] = (uint32_t)rr * sb + 2 * R + 16 * ((lv & (kC - 1)) ^ rope_swz<DR>(8 * pw + rr));
       }
       const uint16_t* base = nullptr;
-      int first_row = 0;
-      uint32_t stage = 0;
+      uint32_t stage = 0, base_lo = 0, base_hi = 0;
+      int bases_at = t0 - 64;  // tile of lane 0
       bool rows8 = false;
+      int first_row = 0;
       auto prepare = [&](int t) __attribute__((always_inline)) {
         stage = lds0 + (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
-        const int j = t * kTile + 8 * pw;
-        const int lo = (int)div_by((uint32_t)min(j, lk - 1), pool.page);
-        const int hi = (int)div_by((uint32_t)min(j + 7, lk - 1), pool.page);
-        if (lo < p0 || hi - p0 >= 64) {  // uniform
-          p0 = lo;
-          page_ids = safe_page(bt, min(p0 + lane, pool.pages_per_seq - 1), pool.num_pages);
-          asm volatile("" : "+v"(page_ids));
+        first_row = t * kTile + 8 * pw;
+        rows8 = p.pages8 && first_row + 8 <= lk;
+        if (t - bases_at >= 64) {
+          bases_at = t;
+          const int j = min(first_row + kTile * lane, (lk - 1) & ~7);
+          const int pg = (int)div_by((uint32_t)j, pool.page);
+          const int page = safe_page(bt, pg, pool.num_pages);
+          const uint64_t at = (uint64_t)(uintptr_t)(pool.cache + page * pool.page_stride +
+                                                    (int64_t)(j - pg * (int)pool.page.d) * pool.slot_stride);
+          base_lo = (uint32_t)at;
+          base_hi = (uint32_t)(at >> 32);
+          asm volatile("" : "+v"(base_lo), "+v"(base_hi));
         }
-        first_row = j;
-        rows8 = p.pages8 && j + 8 <= lk;
-        if (rows8) base = row_at(j);
+        const uint32_t lo = __builtin_amdgcn_readlane(base_lo, t - bases_at);
+        const uint32_t hi = __builtin_amdgcn_readlane(base_hi, t - bases_at);
+        base = (const uint16_t*)(uintptr_t)((uint64_t)hi << 32 | lo);
       };
       auto load_rows = [&]() __attribute__((always_inline)) {
-        const int ln = fresh(lane), rr = ln / kC, j = first_row;
-        const uint16_t* mine = nullptr;
-#pragma unroll 1
+        const int ln = fresh(lane), rr = ln / kC;
+        const uint16_t* rows[8];
+#pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint16_t* r = row_at(min(j + i, lk - 1));  // rows past the end repeat the last
+          const int j = min(first_row + i, lk - 1);  // rows past the end repeat the last
+          const int pg = (int)div_by((uint32_t)j, pool.page);
+          const int page = safe_page_scalar(bt, pg, pool.num_pages);
+          rows[i] = pool.cache + page * pool.page_stride + (int64_t)(j - pg * (int)pool.page.d) * pool.slot_stride;
+        }
+        const uint16_t* mine = rows[0];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
           const uint32_t lat = stage + (uint32_t)(8 * pw * D::kRowB);
           if constexpr (D::kRowsPerDma == 1) {
-            lds_dma16(r + 8 * (ln ^ swz256(8 * pw + i)), lat + 1024 * i);
+            lds_dma16(rows[i] + 8 * (ln ^ swz256(8 * pw + i)), lat + 1024 * i);
           } else if (i & 1) {
-            const uint16_t* own = ln >> 5 ? r : row_at(min(j + i - 1, lk - 1));
+            const uint16_t* own = ln >> 5 ? rows[i] : rows[i - 1];
             lds_dma16(own + 8 * ((ln & 31) ^ swz256(8 * pw + i - 1 + (ln >> 5))), lat + 512 * (i - 1));
           }
-          if (rr == i) mine = r;
+          if (rr == i) mine = rows[i];
         }
         if (ln < 8 * kC)
           lds_dma16(mine + R + 8 * ((ln & (kC - 1)) ^ rope_swz<DR>(8 * pw + rr)),
@@ -443,9 +451,6 @@ latent_attn_kernel(AttnParams p) {
           load_rows();
         }
       };
-      issue(t0);
-      if (t0 + 1 < t1) issue(t0 + 1);
-      if (t0 + 2 < t1) issue(t0 + 2);
       f32x16 acc[D::kDt][D::kRb] = {};
       // transposing reads of V^T: lane 16 gamma + s reads row 4 h + s / 4 (+ 8)
       // of a 16-token step, columns 32 dt + 16 (gamma % 2) + 4 (s % 4)
@@ -489,72 +494,30 @@ latent_attn_kernel(AttnParams p) {
             between(dt * D::kRb + rb);
           }
       };
-      // Tile t has landed when at most the loads of those behind it are outstanding.
-      auto landed = [&](int t, int newest) __attribute__((always_inline)) {
-        if (newest - t >= 2) wait_vm<2 * D::kDma>();
-        else if (newest - t == 1) wait_vm<D::kDma>();
+      // Of the tiles up to `newest`, all but that one have landed.
+      auto landed = [&](int newest) __attribute__((always_inline)) {
+        if (newest < t1) wait_vm<D::kDma>();
         else wait_vm<0>();
       };
-      landed(t0, min(t0 + 2, t1 - 1));
-      lds_barrier();
-      // Step t: the products of tile t - 1; V of tile t is read behind them, so that
-      // a stage is in use for one step only (behind the last tile: stale rows, not
-      // used), and tile t + 3's loads (into the stage of tile t - 1) run between them.
-      read_v(v0, 0, t0);
-      read_v(v1, 1, t0);
-      if (t0 + 3 < t1) issue(t0 + 3);
-      landed(t0 + 1, min(t0 + 3, t1 - 1));
-      wait_lgkm0();
-      lds_barrier();
+#pragma unroll 1
+      for (int t = t0; t < t0 + 3; ++t) {
+        if (t < t1) issue(t);
+        if (t == t0) continue;
+        landed(t);  // tile t - 1
+        lds_barrier();  // the first tile is there; the score waves' first step is done
+      }
+      bool spread = false;  // the next tile's loads go between the products
+      auto plan = [&](int t) __attribute__((always_inline)) {
+        if (t < t1) prepare(t);
+        spread = t < t1 && rows8;
+      };
+      plan(t0 + 3);
+      // Step t: the products of tile t - 2 (zeros at first), whose operands were read
+      // a step before, with tile t + 2's loads (into the stage of tile t - 2) between
+      // them; then tile t - 1's operands.
       for (int t = t0 + 1; t <= t1; ++t) {
-        const bool more = t + 3 < t1;
         constexpr int kProducts = 2 * D::kDt * D::kRb;
-        const uint32_t odd = (uint32_t)((t - 1) & 1);
-        const float* refs = reinterpret_cast<const float*>(smem + D::kRefOff + odd * D::kRefB);
-        float a0[D::kRb], a1[D::kRb];
-#pragma unroll
-        for (int rb = 0; rb < D::kRb; ++rb) {
-          a0[rb] = refs[32 * rb + n];
-          a1[rb] = refs[ROWS + 32 * rb + n];
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int rb = 0; rb < D::kRb; ++rb) pt[rb][u] = as_bf16x8(lds_ld16(poff[rb][u] + odd * D::kPB));
-        __builtin_amdgcn_sched_barrier(0);
-        bool spread = false;
-        if (more) {
-          prepare(t + 3);
-          spread = rows8;
-          if (!spread) load_rows();
-        }
-        // A tile whose halves do not share O's reference: the larger of theirs is the
-        // new one; O and the other half's P are brought to it.
-        float up[D::kRb];
-#pragma unroll
-        for (int rb = 0; rb < D::kRb; ++rb) {
-          const float m_new = __builtin_fmaxf(a0[rb], a1[rb]);
-          up[rb] = fast_exp2(m_ref[rb] - m_new);
-          m_ref[rb] = m_new;
-        }
-#pragma unroll
-        for (int rb = 0; rb < D::kRb; ++rb)
-          if (__any(up[rb] != 1.f)) {
-#pragma unroll
-            for (int dt = 0; dt < D::kDt; ++dt) acc[dt][rb] = acc[dt][rb] * up[rb];
-          }
-#pragma unroll
-        for (int rb = 0; rb < D::kRb; ++rb)
-          if (__any(a0[rb] != a1[rb])) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const float f = fast_exp2((u ? a1[rb] : a0[rb]) - m_ref[rb]);
-              u32x4 w = as_u32x4(pt[rb][u]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(bf16_lo(w[e]) * f, bf16_hi(w[e]) * f);
-              pt[rb][u] = as_bf16x8(w);
-            }
-          }
+        if (t + 2 < t1 && !spread) load_rows();
         auto loads = [&](int i) __attribute__((always_inline)) {
           __builtin_amdgcn_sched_barrier(0);
           if (spread) {
@@ -563,14 +526,65 @@ latent_attn_kernel(AttnParams p) {
           }
           __builtin_amdgcn_sched_barrier(0);
         };
+        const uint32_t odd = (uint32_t)((t - 1) & 1);
+        auto read_p = [&](int u) __attribute__((always_inline)) {
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb) pt[rb][u] = as_bf16x8(lds_ld16(poff[rb][u] + odd * D::kPB));
+        };
         product(v0, 0, loads);
-        read_v(v0, 0, t);
+        read_p(0);
+        read_v(v0, 0, t - 1);
+        __builtin_amdgcn_sched_barrier(0);
         product(v1, 1, [&](int i) __attribute__((always_inline)) { loads(kProducts / 2 + i); });
-        read_v(v1, 1, t);
-        landed(t + 1, min(t + 3, t1 - 1));
+        const float* refs = reinterpret_cast<const float*>(smem + D::kRefOff + odd * D::kRefB);
+        float a0[D::kRb], a1[D::kRb];
+#pragma unroll
+        for (int rb = 0; rb < D::kRb; ++rb) {
+          a0[rb] = refs[32 * rb + n];
+          a1[rb] = refs[ROWS + 32 * rb + n];
+        }
+        read_p(1);
+        read_v(v1, 1, t - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        plan(t + 3);
+        // O's reference is the largest of those of its parts: where a half tile's
+        // is another (seldom), O or that half's P is brought to it.
+        bool differ = false;
+#pragma unroll
+        for (int rb = 0; rb < D::kRb; ++rb) differ |= (a0[rb] != m_ref[rb]) | (a1[rb] != m_ref[rb]);
+        if (__builtin_amdgcn_ballot_w64(differ) != 0) {
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb) {
+            const float m_new = __builtin_fmaxf(m_ref[rb], __builtin_fmaxf(a0[rb], a1[rb]));
+            const float up = fast_exp2(m_ref[rb] - m_new);
+            m_ref[rb] = m_new;
+#pragma unroll
+            for (int dt = 0; dt < D::kDt; ++dt) acc[dt][rb] = acc[dt][rb] * up;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float f = fast_exp2((u ? a1[rb] : a0[rb]) - m_new);
+              u32x4 w = as_u32x4(pt[rb][u]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(bf16_lo(w[e]) * f, bf16_hi(w[e]) * f);
+              pt[rb][u] = as_bf16x8(w);
+            }
+          }
+        }
+        if (pw == 0) {
+          const float* maxes = reinterpret_cast<const float*>(smem + D::kMaxOff + odd * D::kRefB);
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb) {
+            const float mx = __builtin_fmaxf(maxes[32 * rb + n], maxes[ROWS + 32 * rb + n]);
+            *reinterpret_cast<float*>(smem + D::kAskOff + (t & 1) * (ROWS * 4) + (32 * rb + n) * 4) =
+                mx > m_ref[rb] + kSlack ? mx : m_ref[rb];
+          }
+        }
+        landed(t + 2);
         wait_lgkm0();
         lds_barrier();
       }
+      product(v0, 0, [](int) {});
+      product(v1, 1, [](int) {});
       lds_barrier();  // sums are there
       const int le = fresh(lane), ne = le & 31, he = le >> 5;
       // a row's sum: those of its half tiles, brought to O's reference
