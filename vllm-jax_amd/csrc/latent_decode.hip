@@ -15,7 +15,7 @@
 //       with V^T by transposing LDS reads and P^T from LDS
 // so that one wave's exponentials run under the other's matrix instructions:
 // the values' wave multiplies tile t - 2 while the scores' wave works on tile t,
-// with one barrier a tile.  The value waves issue all loads, two tiles ahead.
+// with one barrier a tile.  Both issue loads, two tiles ahead.
 //
 // Work is cut on the device: the kv tiles of all (sequence, row tile) units,
 // laid end to end, are dealt to the workgroups in equal contiguous shares; a
@@ -79,7 +79,8 @@ struct Dims {
   static constexpr int kRb = ROWS / 32;               // its 32-row blocks of rows
   static constexpr int kRowsPerDma = 1024 / kRowB;
   static constexpr int kLatDma = 8 / kRowsPerDma;     // a value wave loads eight rows of a tile
-  static constexpr int kDma = kLatDma + 1;
+  // loads of a tile: a value wave's, a score wave's (the rotary parts among them)
+  static constexpr int kVDma = kLatDma / 2, kSDma = kLatDma + 1 - kVDma;
   static_assert(kLds <= 160 * 1024 && kRing >= 4 * kMaxBatch + 64, "LDS");
 };
 
@@ -106,6 +107,125 @@ __device__ __forceinline__ const uint16_t* uniform_ptr(const uint16_t* p) {
 __device__ __forceinline__ uint32_t fresh_addr(uint32_t x) {
   asm volatile("" : "+v"(x));
   return x;
+}
+
+// Direct loads of kCount of a tile's pieces from piece kFirst on, into the ring:
+// the pieces of waves w and w + 4 are the eight rows 8 w .. 8 w + 7, 1 KiB of
+// latent rows each and the rotary parts last.  prepare() finds a tile's rows,
+// load(i) issues a piece, so that they can be spread through other work (the CU
+// takes one in 20 to 30 cycles).  Where pages hold eight aligned rows and all of
+// them are there, a piece is one scalar base (made for 64 tiles at a time, one
+// a lane) and a lane offset kept in a register; other tiles are looked up row
+// by row (load_rows).
+template <typename D, int R, int DR, int kFirst, int kCount>
+struct TileLoader {
+  static constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
+  const LatentPool& pool;
+  const int32_t* bt;
+  uint32_t lds0;
+  int w, lane, t0, lk;
+  bool pages8;
+  uint32_t voff[kCount];
+  const uint16_t* base;
+  uint32_t stage, base_lo, base_hi;
+  int bases_at, first_row;  // bases_at: tile of lane 0
+  bool rows8;
+
+  __device__ __forceinline__ TileLoader(const LatentPool& pool_, const int32_t* bt_, uint32_t lds0_, int w_, int lane_,
+                                        int t0_, int lk_, bool pages8_)
+      : pool(pool_), bt(bt_), lds0(lds0_), w(w_), lane(lane_), t0(t0_), lk(lk_), pages8(pages8_) {
+    base = nullptr;
+    stage = base_lo = base_hi = 0;
+    bases_at = t0 - 64;
+    first_row = 0;
+    rows8 = false;
+    const uint32_t sb = 2u * (uint32_t)pool.slot_stride;
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+      const int i = kFirst + k;
+      if (i < D::kLatDma) {
+        const int r = i * D::kRowsPerDma + (D::kRowsPerDma == 1 ? 0 : lane >> 5);
+        voff[k] = (uint32_t)r * sb + 16 * ((lane & (D::kRowB / 16 - 1)) ^ swz256(8 * w + r));
+      } else {
+        const int rr = lane / kC;
+        voff[k] = (uint32_t)rr * sb + 2 * R + 16 * ((lane & (kC - 1)) ^ rope_swz<DR>(8 * w + rr));
+      }
+    }
+  }
+  __device__ __forceinline__ uint32_t piece(int i) const {
+    return stage + (i < D::kLatDma ? (uint32_t)(8 * w * D::kRowB + 1024 * i)
+                                   : (uint32_t)(D::kLatB + 8 * w * D::kRopeB));
+  }
+  __device__ __forceinline__ void prepare(int t) {
+    stage = lds0 + (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
+    first_row = t * kTile + 8 * w;
+    rows8 = pages8 && first_row + 8 <= lk;
+    if (t - bases_at >= 64) {
+      bases_at = t;
+      const int j = min(first_row + kTile * lane, (lk - 1) & ~7);
+      const int pg = (int)div_by((uint32_t)j, pool.page);
+      const int page = safe_page(bt, pg, pool.num_pages);
+      const uint64_t at = (uint64_t)(uintptr_t)(pool.cache + page * pool.page_stride +
+                                                (int64_t)(j - pg * (int)pool.page.d) * pool.slot_stride);
+      base_lo = (uint32_t)at;
+      base_hi = (uint32_t)(at >> 32);
+      asm volatile("" : "+v"(base_lo), "+v"(base_hi));
+    }
+    const uint32_t lo = __builtin_amdgcn_readlane(base_lo, t - bases_at);
+    const uint32_t hi = __builtin_amdgcn_readlane(base_hi, t - bases_at);
+    base = (const uint16_t*)(uintptr_t)((uint64_t)hi << 32 | lo);
+  }
+  // Piece k of this wave's (rows8).
+  __device__ __forceinline__ void load(int k) {
+    if (kFirst + k < D::kLatDma || 8 * kC == 64 || fresh(lane) < 8 * kC)
+      lds_dma16s(voff[k], uniform_ptr(base), piece(kFirst + k));
+  }
+  __device__ __forceinline__ void load_rows() {
+    const int ln = fresh(lane), rr = ln / kC;
+    const uint16_t* rows[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int j = min(first_row + i, lk - 1);  // rows past the end repeat the last
+      const int pg = (int)div_by((uint32_t)j, pool.page);
+      const int page = safe_page_scalar(bt, pg, pool.num_pages);
+      rows[i] = pool.cache + page * pool.page_stride + (int64_t)(j - pg * (int)pool.page.d) * pool.slot_stride;
+    }
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+      const int i = kFirst + k;
+      if (i < D::kLatDma) {
+        if constexpr (D::kRowsPerDma == 1) {
+          lds_dma16(rows[i & 7] + 8 * (ln ^ swz256(8 * w + i)), piece(i));
+        } else {
+          const uint16_t* own = ln >> 5 ? rows[(2 * i + 1) & 7] : rows[(2 * i) & 7];
+          lds_dma16(own + 8 * ((ln & 31) ^ swz256(8 * w + 2 * i + (ln >> 5))), piece(i));
+        }
+      } else {
+        const uint16_t* mine = rows[0];
+#pragma unroll
+        for (int r = 1; r < 8; ++r) mine = rr == r ? rows[r] : mine;
+        if (ln < 8 * kC) lds_dma16(mine + R + 8 * ((ln & (kC - 1)) ^ rope_swz<DR>(8 * w + rr)), piece(i));
+      }
+    }
+  }
+  // All of tile t's pieces at once.
+  __device__ __forceinline__ void issue(int t) {
+    prepare(t);
+    if (rows8) {
+#pragma unroll
+      for (int k = 0; k < kCount; ++k) load(k);
+    } else {
+      load_rows();
+    }
+  }
+};
+
+// Waits until all tiles but the newest one issued have landed (`open`: there is
+// a newer one), for a wave with kCount loads a tile.
+template <int kCount>
+__device__ __forceinline__ void landed(bool open) {
+  if (open) wait_vm<kCount>();
+  else wait_vm<0>();
 }
 
 struct Seq {
@@ -227,10 +347,15 @@ latent_attn_kernel(AttnParams p) {
     const int n_rows = min(ROWS, sq.lq * p.a.heads - rt * ROWS);
     const int lk = sq.lk;
 
+    const int32_t* bt = pool.tables + (int64_t)b * pool.bt_stride;
+
     if (wave < 4) {
       // ================= scores
       const int tb = wave & 1, rw = (wave >> 1) * 16 * D::kNr;
       const int ln = fresh(lane), l16 = ln & 15, qd = ln >> 4;
+      TileLoader<D, R, DR, D::kVDma, D::kSDma> loader(pool, bt, lds0, wave, ln, t0, lk, p.pages8);
+#pragma unroll 1
+      for (int t = t0; t < min(t0 + 2, t1); ++t) loader.issue(t);
       bf16x8 q[D::kNr][D::kKs + D::kRs];
       int lim[D::kNr];  // tokens a row sees
 #pragma unroll
@@ -267,7 +392,14 @@ latent_attn_kernel(AttnParams p) {
 #pragma unroll
       for (int i = 0; i < D::kRs; ++i)
         roff[i] = lds0 + D::kLatB + krow * D::kRopeB + 16 * ((4 * i + qd) ^ rope_swz<DR>(krow));
-      lds_barrier();  // the first tile is there
+      // Q and the first two tiles (here, or the compiler would wait for every load
+      // at Q's uses in the loop)
+#pragma unroll
+      for (int r = 0; r < D::kNr; ++r)
+#pragma unroll
+        for (int ks = 0; ks < D::kKs + D::kRs; ++ks) asm volatile("" : "+v"(q[r][ks]));
+      wait_vm<0>();
+      lds_barrier();
       for (int t = t0; t < t1; ++t) {
         const uint32_t st = (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
         float ask[D::kNr];  // (first two tiles: not written yet)
@@ -304,6 +436,23 @@ latent_attn_kernel(AttnParams p) {
           __builtin_amdgcn_sched_barrier(0);
         }
         const int j0 = t * kTile + 16 * tb + 4 * qd;
+        // tile t + 2's loads go into the stage of tile t - 2
+        const bool more = t + 2 < t1;
+        bool spread = false;
+        if (more) {
+          loader.prepare(t + 2);
+          spread = loader.rows8;
+          if (!spread) loader.load_rows();
+        }
+        auto loads = [&](int from, int to) __attribute__((always_inline)) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (spread) {
+#pragma unroll
+            for (int k = from; k < to; ++k) loader.load(k);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        loads(0, 1);
         if (t >= free_tiles) {
 #pragma unroll
           for (int r = 0; r < D::kNr; ++r)
@@ -317,6 +466,7 @@ latent_attn_kernel(AttnParams p) {
         for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor16(mx[r]);
 #pragma unroll
         for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor32(mx[r]);
+        loads(1, 2);
         float corr[D::kNr];
 #pragma unroll
         for (int r = 0; r < D::kNr; ++r) {
@@ -326,6 +476,7 @@ latent_attn_kernel(AttnParams p) {
           corr[r] = fast_exp2(own_ref[r] - ref);
           own_ref[r] = ref;
         }
+        loads(2, 3);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -347,6 +498,8 @@ latent_attn_kernel(AttnParams p) {
         }
 #pragma unroll
         for (int r = 0; r < D::kNr; ++r) l_sum[r] = l_sum[r] * corr[r] + ((s[r][0] + s[r][1]) + (s[r][2] + s[r][3]));
+        loads(3, D::kSDma);
+        landed<D::kSDma>(more);
         wait_lgkm0();
         lds_barrier();
       }
@@ -365,92 +518,7 @@ latent_attn_kernel(AttnParams p) {
       // ================= values
       const int pw = wave - 4;
       const int lv = fresh(lane), n = lv & 31, h = lv >> 5;
-
-      // ---- tile loads: this wave's rows are 8 pw .. 8 pw + 7 of every tile.
-      const int32_t* bt = pool.tables + (int64_t)b * pool.bt_stride;
-      // A tile's loads: prepare() finds its rows, load(i) issues piece i of kDma,
-      // so that they can be spread through other work.  Where pages hold eight
-      // aligned rows and all of them are there, a piece is one scalar base (made
-      // for 64 tiles at a time, one a lane) and a lane offset kept in a register;
-      // other tiles are looked up row by row (load_rows).
-      constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
-      uint32_t voff[D::kDma];
-      {
-        const uint32_t sb = 2u * (uint32_t)pool.slot_stride;
-#pragma unroll
-        for (int i = 0; i < D::kLatDma; ++i) {
-          const int r = i * D::kRowsPerDma + (D::kRowsPerDma == 1 ? 0 : lv >> 5);
-          voff[i] = (uint32_t)r * sb + 16 * ((lv & (D::kRowB / 16 - 1)) ^ swz256(8 * pw + r));
-        }
-        const int rr = lv / kC;
-        voff[D::kLatDma] = (uint32_t)rr * sb + 2 * R + 16 * ((lv & (kC - 1)) ^ rope_swz<DR>(8 * pw + rr));
-      }
-      const uint16_t* base = nullptr;
-      uint32_t stage = 0, base_lo = 0, base_hi = 0;
-      int bases_at = t0 - 64;  // tile of lane 0
-      bool rows8 = false;
-      int first_row = 0;
-      auto prepare = [&](int t) __attribute__((always_inline)) {
-        stage = lds0 + (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
-        first_row = t * kTile + 8 * pw;
-        rows8 = p.pages8 && first_row + 8 <= lk;
-        if (t - bases_at >= 64) {
-          bases_at = t;
-          const int j = min(first_row + kTile * lane, (lk - 1) & ~7);
-          const int pg = (int)div_by((uint32_t)j, pool.page);
-          const int page = safe_page(bt, pg, pool.num_pages);
-          const uint64_t at = (uint64_t)(uintptr_t)(pool.cache + page * pool.page_stride +
-                                                    (int64_t)(j - pg * (int)pool.page.d) * pool.slot_stride);
-          base_lo = (uint32_t)at;
-          base_hi = (uint32_t)(at >> 32);
-          asm volatile("" : "+v"(base_lo), "+v"(base_hi));
-        }
-        const uint32_t lo = __builtin_amdgcn_readlane(base_lo, t - bases_at);
-        const uint32_t hi = __builtin_amdgcn_readlane(base_hi, t - bases_at);
-        base = (const uint16_t*)(uintptr_t)((uint64_t)hi << 32 | lo);
-      };
-      auto load_rows = [&]() __attribute__((always_inline)) {
-        const int ln = fresh(lane), rr = ln / kC;
-        const uint16_t* rows[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = min(first_row + i, lk - 1);  // rows past the end repeat the last
-          const int pg = (int)div_by((uint32_t)j, pool.page);
-          const int page = safe_page_scalar(bt, pg, pool.num_pages);
-          rows[i] = pool.cache + page * pool.page_stride + (int64_t)(j - pg * (int)pool.page.d) * pool.slot_stride;
-        }
-        const uint16_t* mine = rows[0];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t lat = stage + (uint32_t)(8 * pw * D::kRowB);
-          if constexpr (D::kRowsPerDma == 1) {
-            lds_dma16(rows[i] + 8 * (ln ^ swz256(8 * pw + i)), lat + 1024 * i);
-          } else if (i & 1) {
-            const uint16_t* own = ln >> 5 ? rows[i] : rows[i - 1];
-            lds_dma16(own + 8 * ((ln & 31) ^ swz256(8 * pw + i - 1 + (ln >> 5))), lat + 512 * (i - 1));
-          }
-          if (rr == i) mine = rows[i];
-        }
-        if (ln < 8 * kC)
-          lds_dma16(mine + R + 8 * ((ln & (kC - 1)) ^ rope_swz<DR>(8 * pw + rr)),
-                    stage + (uint32_t)(D::kLatB + 8 * pw * D::kRopeB));
-      };
-      auto load = [&](int i) __attribute__((always_inline)) {
-        if (i < D::kLatDma) {
-          lds_dma16s(voff[i], uniform_ptr(base), stage + (uint32_t)(8 * pw * D::kRowB + 1024 * i));
-        } else if (8 * kC == 64 || fresh(lane) < 8 * kC) {
-          lds_dma16s(voff[i], uniform_ptr(base), stage + (uint32_t)(D::kLatB + 8 * pw * D::kRopeB));
-        }
-      };
-      auto issue = [&](int t) __attribute__((always_inline)) {
-        prepare(t);
-        if (rows8) {
-#pragma unroll
-          for (int i = 0; i < D::kDma; ++i) load(i);
-        } else {
-          load_rows();
-        }
-      };
+      TileLoader<D, R, DR, 0, D::kVDma> loader(pool, bt, lds0, pw, lv, t0, lk, p.pages8);
       f32x16 acc[D::kDt][D::kRb] = {};
       // transposing reads of V^T: lane 16 gamma + s reads row 4 h + s / 4 (+ 8)
       // of a 16-token step, columns 32 dt + 16 (gamma % 2) + 4 (s % 4)
@@ -494,22 +562,17 @@ latent_attn_kernel(AttnParams p) {
             between(dt * D::kRb + rb);
           }
       };
-      // Of the tiles up to `newest`, all but that one have landed.
-      auto landed = [&](int newest) __attribute__((always_inline)) {
-        if (newest < t1) wait_vm<D::kDma>();
-        else wait_vm<0>();
-      };
 #pragma unroll 1
       for (int t = t0; t < t0 + 3; ++t) {
-        if (t < t1) issue(t);
+        if (t < t1) loader.issue(t);
         if (t == t0) continue;
-        landed(t);  // tile t - 1
+        landed<D::kVDma>(t < t1);  // tile t - 1
         lds_barrier();  // the first tile is there; the score waves' first step is done
       }
       bool spread = false;  // the next tile's loads go between the products
       auto plan = [&](int t) __attribute__((always_inline)) {
-        if (t < t1) prepare(t);
-        spread = t < t1 && rows8;
+        if (t < t1) loader.prepare(t);
+        spread = t < t1 && loader.rows8;
       };
       plan(t0 + 3);
       // Step t: the products of tile t - 2 (zeros at first), whose operands were read
@@ -517,12 +580,12 @@ latent_attn_kernel(AttnParams p) {
       // them; then tile t - 1's operands.
       for (int t = t0 + 1; t <= t1; ++t) {
         constexpr int kProducts = 2 * D::kDt * D::kRb;
-        if (t + 2 < t1 && !spread) load_rows();
+        if (t + 2 < t1 && !spread) loader.load_rows();
         auto loads = [&](int i) __attribute__((always_inline)) {
           __builtin_amdgcn_sched_barrier(0);
           if (spread) {
 #pragma unroll
-            for (int k = i * D::kDma / kProducts; k < (i + 1) * D::kDma / kProducts; ++k) load(k);
+            for (int k = i * D::kVDma / kProducts; k < (i + 1) * D::kVDma / kProducts; ++k) loader.load(k);
           }
           __builtin_amdgcn_sched_barrier(0);
         };
@@ -579,7 +642,7 @@ latent_attn_kernel(AttnParams p) {
                 mx > m_ref[rb] + kSlack ? mx : m_ref[rb];
           }
         }
-        landed(t + 2);
+        landed<D::kVDma>(t + 2 < t1);
         wait_lgkm0();
         lds_barrier();
       }
