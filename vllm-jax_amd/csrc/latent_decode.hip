@@ -14,8 +14,9 @@
 //   waves 4-7 (values):  O^T[R / 4][all rows] in registers, v_mfma_f32_32x32x16
 //       with V^T by transposing LDS reads and P^T from LDS
 // so that one wave's exponentials run under the other's matrix instructions:
-// the values' wave multiplies tile t - 2 while the scores' wave works on tile t,
-// with one barrier a tile.  Both issue loads, two tiles ahead.
+// the values' wave reads tile t - 1's operands while the scores' wave multiplies
+// tile t, and multiplies while that takes its exponentials, with one barrier a
+// tile.  Both issue loads, two tiles ahead.
 //
 // Work is cut on the device: the kv tiles of all (sequence, row tile) units,
 // laid end to end, are dealt to the workgroups in equal contiguous shares; a
@@ -540,9 +541,8 @@ latent_attn_kernel(AttnParams p) {
       float m_ref[D::kRb];  // reference of O
 #pragma unroll
       for (int rb = 0; rb < D::kRb; ++rb) m_ref[rb] = kNoMax;
-      // (set here, or the compiler carries them through the segments)
-      bf16x8 pt[D::kRb][2] = {};
-      bf16x8 v0[D::kDt] = {}, v1[D::kDt] = {};  // V^T of the first and second 16 tokens of a tile
+      bf16x8 pt[D::kRb][2];
+      bf16x8 v0[D::kDt], v1[D::kDt];  // V^T of the first and second 16 tokens of a tile
       auto read_v = [&](bf16x8(&v)[D::kDt], int u, int t) __attribute__((always_inline)) {
         const uint32_t st = (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
 #pragma unroll
@@ -574,31 +574,12 @@ latent_attn_kernel(AttnParams p) {
         if (t < t1) loader.prepare(t);
         spread = t < t1 && loader.rows8;
       };
-      plan(t0 + 3);
-      // Step t: the products of tile t - 2 (zeros at first), whose operands were read
-      // a step before, with tile t + 2's loads (into the stage of tile t - 2) between
-      // them; then tile t - 1's operands.
+      // Step t: tile t - 1's operands while the score waves multiply tile t, then its
+      // products while they take the exponentials, with tile t + 2's loads (into the
+      // stage of tile t - 2) between them.
       for (int t = t0 + 1; t <= t1; ++t) {
         constexpr int kProducts = 2 * D::kDt * D::kRb;
-        if (t + 2 < t1 && !spread) loader.load_rows();
-        auto loads = [&](int i) __attribute__((always_inline)) {
-          __builtin_amdgcn_sched_barrier(0);
-          if (spread) {
-#pragma unroll
-            for (int k = i * D::kVDma / kProducts; k < (i + 1) * D::kVDma / kProducts; ++k) loader.load(k);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        };
         const uint32_t odd = (uint32_t)((t - 1) & 1);
-        auto read_p = [&](int u) __attribute__((always_inline)) {
-#pragma unroll
-          for (int rb = 0; rb < D::kRb; ++rb) pt[rb][u] = as_bf16x8(lds_ld16(poff[rb][u] + odd * D::kPB));
-        };
-        product(v0, 0, loads);
-        read_p(0);
-        read_v(v0, 0, t - 1);
-        __builtin_amdgcn_sched_barrier(0);
-        product(v1, 1, [&](int i) __attribute__((always_inline)) { loads(kProducts / 2 + i); });
         const float* refs = reinterpret_cast<const float*>(smem + D::kRefOff + odd * D::kRefB);
         float a0[D::kRb], a1[D::kRb];
 #pragma unroll
@@ -606,16 +587,22 @@ latent_attn_kernel(AttnParams p) {
           a0[rb] = refs[32 * rb + n];
           a1[rb] = refs[ROWS + 32 * rb + n];
         }
-        read_p(1);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb) pt[rb][u] = as_bf16x8(lds_ld16(poff[rb][u] + odd * D::kPB));
+        read_v(v0, 0, t - 1);
         read_v(v1, 1, t - 1);
         __builtin_amdgcn_sched_barrier(0);
-        plan(t + 3);
+        plan(t + 2);
+        if (t + 2 < t1 && !spread) loader.load_rows();
         // O's reference is the largest of those of its parts: where a half tile's
         // is another (seldom), O or that half's P is brought to it.
-        bool differ = false;
+        // (two branches: with one the compiler keeps two copies of O)
+        bool moved = false, differ = false;
 #pragma unroll
-        for (int rb = 0; rb < D::kRb; ++rb) differ |= (a0[rb] != m_ref[rb]) | (a1[rb] != m_ref[rb]);
-        if (__builtin_amdgcn_ballot_w64(differ) != 0) {
+        for (int rb = 0; rb < D::kRb; ++rb) moved |= __builtin_fmaxf(a0[rb], a1[rb]) > m_ref[rb];
+        if (__builtin_amdgcn_ballot_w64(moved) != 0) {
 #pragma unroll
           for (int rb = 0; rb < D::kRb; ++rb) {
             const float m_new = __builtin_fmaxf(m_ref[rb], __builtin_fmaxf(a0[rb], a1[rb]));
@@ -623,15 +610,21 @@ latent_attn_kernel(AttnParams p) {
             m_ref[rb] = m_new;
 #pragma unroll
             for (int dt = 0; dt < D::kDt; ++dt) acc[dt][rb] = acc[dt][rb] * up;
+          }
+        }
+#pragma unroll
+        for (int rb = 0; rb < D::kRb; ++rb) differ |= (a0[rb] != m_ref[rb]) | (a1[rb] != m_ref[rb]);
+        if (__builtin_amdgcn_ballot_w64(differ) != 0) {
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              const float f = fast_exp2((u ? a1[rb] : a0[rb]) - m_new);
+              const float f = fast_exp2((u ? a1[rb] : a0[rb]) - m_ref[rb]);
               u32x4 w = as_u32x4(pt[rb][u]);
 #pragma unroll
               for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(bf16_lo(w[e]) * f, bf16_hi(w[e]) * f);
               pt[rb][u] = as_bf16x8(w);
             }
-          }
         }
         if (pw == 0) {
           const float* maxes = reinterpret_cast<const float*>(smem + D::kMaxOff + odd * D::kRefB);
@@ -642,12 +635,20 @@ latent_attn_kernel(AttnParams p) {
                 mx > m_ref[rb] + kSlack ? mx : m_ref[rb];
           }
         }
+        auto loads = [&](int i) __attribute__((always_inline)) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (spread) {
+#pragma unroll
+            for (int k = i * D::kVDma / kProducts; k < (i + 1) * D::kVDma / kProducts; ++k) loader.load(k);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        product(v0, 0, loads);
+        product(v1, 1, [&](int i) __attribute__((always_inline)) { loads(kProducts / 2 + i); });
         landed<D::kVDma>(t + 2 < t1);
         wait_lgkm0();
         lds_barrier();
       }
-      product(v0, 0, [](int) {});
-      product(v1, 1, [](int) {});
       lds_barrier();  // sums are there
       const int le = fresh(lane), ne = le & 31, he = le >> 5;
       // a row's sum: those of its half tiles, brought to O's reference
