@@ -418,8 +418,16 @@ latent_attn_kernel(AttnParams p) {
         for (int i = 0; i < 4; ++i) ka[i] = fresh_addr(koff[i] + st);
 #pragma unroll
         for (int i = 0; i < D::kRs; ++i) ra[i] = fresh_addr(roff[i] + st);
+        // tile t + 2's loads (into the stage of tile t - 2) go between the products
+        const bool more = t + 2 < t1;
+        bool spread = false;
+        if (more) {
+          loader.prepare(t + 2);
+          spread = loader.rows8;
+          if (!spread) loader.load_rows();
+        }
         // every read is issued kAhead k-steps before the products it feeds
-        constexpr int kAll = D::kKs + D::kRs, kAhead = 6;
+        constexpr int kAll = D::kKs + D::kRs, kAhead = 6, kEach = kAll / D::kSDma;
         bf16x8 a[kAll];
         auto read_k = [&](int ks) __attribute__((always_inline)) {
           a[ks] = as_bf16x8(ks < D::kKs ? lds_ld16(ka[ks & 3] + (ks >> 2) * 256)
@@ -435,25 +443,12 @@ latent_attn_kernel(AttnParams p) {
             s[r] = mfma16(a[ks], q[r][ks], s[r]);
           if (ks + kAhead < kAll) read_k(ks + kAhead);
           __builtin_amdgcn_sched_barrier(0);
+          if (ks % kEach == kEach - 1 && ks / kEach < D::kSDma) {
+            if (spread) loader.load(ks / kEach);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
         const int j0 = t * kTile + 16 * tb + 4 * qd;
-        // tile t + 2's loads go into the stage of tile t - 2
-        const bool more = t + 2 < t1;
-        bool spread = false;
-        if (more) {
-          loader.prepare(t + 2);
-          spread = loader.rows8;
-          if (!spread) loader.load_rows();
-        }
-        auto loads = [&](int from, int to) __attribute__((always_inline)) {
-          __builtin_amdgcn_sched_barrier(0);
-          if (spread) {
-#pragma unroll
-            for (int k = from; k < to; ++k) loader.load(k);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        };
-        loads(0, 1);
         if (t >= free_tiles) {
 #pragma unroll
           for (int r = 0; r < D::kNr; ++r)
@@ -467,7 +462,6 @@ latent_attn_kernel(AttnParams p) {
         for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor16(mx[r]);
 #pragma unroll
         for (int r = 0; r < D::kNr; ++r) mx[r] = max_xor32(mx[r]);
-        loads(1, 2);
         float corr[D::kNr];
 #pragma unroll
         for (int r = 0; r < D::kNr; ++r) {
@@ -477,7 +471,6 @@ latent_attn_kernel(AttnParams p) {
           corr[r] = fast_exp2(own_ref[r] - ref);
           own_ref[r] = ref;
         }
-        loads(2, 3);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -499,7 +492,6 @@ latent_attn_kernel(AttnParams p) {
         }
 #pragma unroll
         for (int r = 0; r < D::kNr; ++r) l_sum[r] = l_sum[r] * corr[r] + ((s[r][0] + s[r][1]) + (s[r][2] + s[r][3]));
-        loads(3, D::kSDma);
         landed<D::kSDma>(more);
         wait_lgkm0();
         lds_barrier();
@@ -581,11 +573,14 @@ latent_attn_kernel(AttnParams p) {
         constexpr int kProducts = 2 * D::kDt * D::kRb;
         const uint32_t odd = (uint32_t)((t - 1) & 1);
         const float* refs = reinterpret_cast<const float*>(smem + D::kRefOff + odd * D::kRefB);
-        float a0[D::kRb], a1[D::kRb];
+        const float* maxes = reinterpret_cast<const float*>(smem + D::kMaxOff + odd * D::kRefB);
+        float a0[D::kRb], a1[D::kRb], m0[D::kRb], m1[D::kRb];
 #pragma unroll
         for (int rb = 0; rb < D::kRb; ++rb) {
           a0[rb] = refs[32 * rb + n];
           a1[rb] = refs[ROWS + 32 * rb + n];
+          m0[rb] = maxes[32 * rb + n];
+          m1[rb] = maxes[ROWS + 32 * rb + n];
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -626,15 +621,6 @@ latent_attn_kernel(AttnParams p) {
               pt[rb][u] = as_bf16x8(w);
             }
         }
-        if (pw == 0) {
-          const float* maxes = reinterpret_cast<const float*>(smem + D::kMaxOff + odd * D::kRefB);
-#pragma unroll
-          for (int rb = 0; rb < D::kRb; ++rb) {
-            const float mx = __builtin_fmaxf(maxes[32 * rb + n], maxes[ROWS + 32 * rb + n]);
-            *reinterpret_cast<float*>(smem + D::kAskOff + (t & 1) * (ROWS * 4) + (32 * rb + n) * 4) =
-                mx > m_ref[rb] + kSlack ? mx : m_ref[rb];
-          }
-        }
         auto loads = [&](int i) __attribute__((always_inline)) {
           __builtin_amdgcn_sched_barrier(0);
           if (spread) {
@@ -645,6 +631,14 @@ latent_attn_kernel(AttnParams p) {
         };
         product(v0, 0, loads);
         product(v1, 1, [&](int i) __attribute__((always_inline)) { loads(kProducts / 2 + i); });
+        if (pw == 0) {
+#pragma unroll
+          for (int rb = 0; rb < D::kRb; ++rb) {
+            const float mx = __builtin_fmaxf(m0[rb], m1[rb]);
+            *reinterpret_cast<float*>(smem + D::kAskOff + (t & 1) * (ROWS * 4) + (32 * rb + n) * 4) =
+                mx > m_ref[rb] + kSlack ? mx : m_ref[rb];
+          }
+        }
         landed<D::kVDma>(t + 2 < t1);
         wait_lgkm0();
         lds_barrier();
