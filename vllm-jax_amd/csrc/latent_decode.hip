@@ -82,6 +82,7 @@ struct Dims {
   static constexpr int kLatDma = 8 / kRowsPerDma;     // a value wave loads eight rows of a tile
   // loads of a tile: a value wave's, a score wave's (the rotary parts among them)
   static constexpr int kVDma = kLatDma / 2, kSDma = kLatDma + 1 - kVDma;
+  static_assert(ROWS * (kRowB + kRopeB) <= 2 * kStageB, "Q in two stages");
   static_assert(kLds <= 160 * 1024 && kRing >= 4 * kMaxBatch + 64, "LDS");
 };
 
@@ -350,6 +351,37 @@ latent_attn_kernel(AttnParams p) {
 
     const int32_t* bt = pool.tables + (int64_t)b * pool.bt_stride;
 
+    // ---- Q's rows, whole lines at a time, into the last two stages (rows past the
+    // end repeat the last): those of a wave are an eighth
+    {
+      constexpr int kMine = ROWS / 8;
+      const int ln = fresh(lane);
+      const uint32_t qa = lds0 + 2 * D::kStageB;
+      auto row_of = [&](int r, int& tok, int& hd) __attribute__((always_inline)) {
+        const int row = rt * ROWS + min(r, n_rows - 1);
+        tok = (int)div_by((uint32_t)row, p.heads);
+        hd = row - tok * p.a.heads;
+      };
+#pragma unroll
+      for (int i = 0; i < kMine / D::kRowsPerDma; ++i) {
+        const int r = kMine * wave + i * D::kRowsPerDma + (D::kRowsPerDma == 1 ? 0 : ln >> 5);
+        int tok, hd;
+        row_of(r, tok, hd);
+        lds_dma16(p.a.q_lat + (int64_t)(sq.q0 + tok) * p.a.ql_ts + hd * p.a.ql_hs +
+                      8 * ((ln & (D::kRowB / 16 - 1)) ^ swz256(r)),
+                  qa + (uint32_t)(kMine * wave * D::kRowB + 1024 * i));
+      }
+      constexpr int kC = D::kRopeB / 16;
+      if (ln < kMine * kC) {
+        const int r = kMine * wave + ln / kC;
+        int tok, hd;
+        row_of(r, tok, hd);
+        lds_dma16(p.a.q_rope + (int64_t)(sq.q0 + tok) * p.a.qr_ts + hd * p.a.qr_hs +
+                      8 * ((ln & (kC - 1)) ^ rope_swz<DR>(r)),
+                  qa + (uint32_t)(ROWS * D::kRowB + kMine * wave * D::kRopeB));
+      }
+    }
+
     if (wave < 4) {
       // ================= scores
       const int tb = wave & 1, rw = (wave >> 1) * 16 * D::kNr;
@@ -362,14 +394,7 @@ latent_attn_kernel(AttnParams p) {
 #pragma unroll
       for (int r = 0; r < D::kNr; ++r) {
         const int row = rt * ROWS + min(rw + 16 * r + l16, n_rows - 1);
-        const int tok = (int)div_by((uint32_t)row, p.heads), hd = row - tok * p.a.heads;
-        lim[r] = min(lk, max(0, sq.first + tok + 1));
-        const uint16_t* ql = p.a.q_lat + (int64_t)(sq.q0 + tok) * p.a.ql_ts + hd * p.a.ql_hs + 8 * qd;
-        const uint16_t* qr = p.a.q_rope + (int64_t)(sq.q0 + tok) * p.a.qr_ts + hd * p.a.qr_hs + 8 * qd;
-#pragma unroll
-        for (int ks = 0; ks < D::kKs; ++ks) q[r][ks] = as_bf16x8(ld16(ql + 32 * ks));
-#pragma unroll
-        for (int ks = 0; ks < D::kRs; ++ks) q[r][D::kKs + ks] = as_bf16x8(ld16(qr + 32 * ks));
+        lim[r] = min(lk, max(0, sq.first + (int)div_by((uint32_t)row, p.heads) + 1));
       }
       // first tile a row of this tile does not see in full
       const int tok_first = (int)div_by((uint32_t)(rt * ROWS), p.heads);
@@ -393,14 +418,22 @@ latent_attn_kernel(AttnParams p) {
 #pragma unroll
       for (int i = 0; i < D::kRs; ++i)
         roff[i] = lds0 + D::kLatB + krow * D::kRopeB + 16 * ((4 * i + qd) ^ rope_swz<DR>(krow));
-      // Q and the first two tiles (here, or the compiler would wait for every load
-      // at Q's uses in the loop)
-#pragma unroll
-      for (int r = 0; r < D::kNr; ++r)
-#pragma unroll
-        for (int ks = 0; ks < D::kKs + D::kRs; ++ks) asm volatile("" : "+v"(q[r][ks]));
       wait_vm<0>();
-      lds_barrier();
+      lds_barrier();  // Q and the first two tiles are there
+#pragma unroll
+      for (int r = 0; r < D::kNr; ++r) {
+        const int row = rw + 16 * r + l16;
+        const uint32_t qa = lds0 + 2 * D::kStageB;
+#pragma unroll
+        for (int ks = 0; ks < D::kKs; ++ks)
+          q[r][ks] = as_bf16x8(lds_ld16(qa + row * D::kRowB + 16 * ((4 * ks + qd) ^ swz256(row))));
+#pragma unroll
+        for (int ks = 0; ks < D::kRs; ++ks)
+          q[r][D::kKs + ks] = as_bf16x8(
+              lds_ld16(qa + ROWS * D::kRowB + row * D::kRopeB + 16 * ((4 * ks + qd) ^ rope_swz<DR>(row))));
+      }
+      wait_lgkm0();
+      lds_barrier();  // the stages that held Q are free
       for (int t = t0; t < t1; ++t) {
         const uint32_t st = (uint32_t)((t - t0) & (kLStages - 1)) * D::kStageB;
         float ask[D::kNr];  // (first two tiles: not written yet)
@@ -556,11 +589,15 @@ latent_attn_kernel(AttnParams p) {
       };
 #pragma unroll 1
       for (int t = t0; t < t0 + 3; ++t) {
+        if (t == t0 + 2) {
+          wait_vm<0>();
+          lds_barrier();  // Q and the first two tiles are there
+          lds_barrier();  // Q is in the score waves' registers
+        }
         if (t < t1) loader.issue(t);
-        if (t == t0) continue;
-        landed<D::kVDma>(t < t1);  // tile t - 1
-        lds_barrier();  // the first tile is there; the score waves' first step is done
       }
+      landed<D::kVDma>(t0 + 2 < t1);
+      lds_barrier();  // the score waves' first step is done
       bool spread = false;  // the next tile's loads go between the products
       auto plan = [&](int t) __attribute__((always_inline)) {
         if (t < t1) loader.prepare(t);
