@@ -145,34 +145,46 @@ latent_ragged_kernel(RaggedParams prm) {
     for (int ks = 0; ks < D::kRs; ++ks) q[D::kKs + ks] = as_bf16x8(ld16(qr + 16 * ks));
   }
 
-  // ---- tile loads: this wave's rows of a tile are 8 wave .. 8 wave + 7
-  auto issue_k = [&](int t, int st) __attribute__((always_inline)) {
-    const int last = max(lk - 1 - t * kRTile, 0);  // rows past the end repeat the last one
-    const int64_t j0 = min(t * kRTile, max(lk - 1, 0));
+  // ---- tile loads: this wave's rows of a tile are 8 wave .. 8 wave + 7, each load
+  // a scalar tile base and a lane offset kept in a register.  Piece i of kDma:
+  // K's, the rotary parts', V's.  Rows past the kv length repeat the last one.
+  constexpr int kRowChunks = D::kKB / 16, kRopeChunks = D::kRB / 16;
+  uint32_t off_k[D::kKDma], off_v[D::kKDma], off_r;
 #pragma unroll
-    for (int i = 0; i < D::kKDma; ++i) {
-      const int r = 8 * wave + i * D::kRowsK + lane / (D::kKB / 16);
-      const int c = lane & (D::kKB / 16 - 1);
-      lds_dma16(kv + (j0 + min(r, last)) * (2 * DN) + 8 * (c ^ k_swz<DN>(r)),
-                lds0 + (uint32_t)(D::kKOff + st * D::kKStage + 8 * wave * D::kKB + 1024 * i));
-    }
-    constexpr int kC = D::kRB / 16;
-    if (lane < 8 * kC) {
-      const int r = 8 * wave + lane / kC, c = lane & (kC - 1);
-      lds_dma16(kr + (j0 + min(r, last)) * DR + 8 * (c ^ r_swz<DR>(r)),
-                lds0 + (uint32_t)(D::kROff + st * D::kRStage + 8 * wave * D::kRB));
+  for (int i = 0; i < D::kKDma; ++i) {
+    const int r = 8 * wave + i * D::kRowsK + lane / kRowChunks, c = lane & (kRowChunks - 1);
+    off_k[i] = 2 * D::kKB * r + 16 * (c ^ k_swz<DN>(r));
+    off_v[i] = 2 * D::kKB * r + D::kKB + 16 * (c ^ v_swz<DN>(r));
+  }
+  {
+    const int r = 8 * wave + (lane / kRopeChunks & 7), c = lane & (kRopeChunks - 1);
+    off_r = D::kRB * r + 16 * (c ^ r_swz<DR>(r));
+  }
+  auto issue = [&](int i, int tk, int ks, int tv, int vs) __attribute__((always_inline)) {
+    const int t = i <= D::kKDma ? tk : tv;
+    const int j0 = min(t * kRTile, max(lk - 1, 0)), last = max(lk - 1 - t * kRTile, 0);
+    const int lrow = i == D::kKDma ? lane / kRopeChunks & 7
+                                   : (i < D::kKDma ? i : i - D::kKDma - 1) * D::kRowsK + lane / kRowChunks;
+    // rows of the tile past the last valid one
+    const int past = last < kRTile - 1 ? max(8 * wave + lrow - last, 0) : 0;
+    if (i < D::kKDma) {
+      lds_dma16s(off_k[i] - 2 * D::kKB * past, kv + (int64_t)j0 * (2 * DN),
+                 lds0 + (uint32_t)(D::kKOff + ks * D::kKStage + 8 * wave * D::kKB + 1024 * i));
+    } else if (i > D::kKDma) {
+      lds_dma16s(off_v[i - D::kKDma - 1] - 2 * D::kKB * past, kv + (int64_t)j0 * (2 * DN),
+                 lds0 + (uint32_t)(D::kVOff + vs * D::kKStage + 8 * wave * D::kKB + 1024 * (i - D::kKDma - 1)));
+    } else if (kRopeChunks == 8 || lane < 8 * kRopeChunks) {
+      lds_dma16s(off_r - D::kRB * past, kr + (int64_t)j0 * DR,
+                 lds0 + (uint32_t)(D::kROff + ks * D::kRStage + 8 * wave * D::kRB));
     }
   };
-  auto issue_v = [&](int t, int st) __attribute__((always_inline)) {
-    const int last = max(lk - 1 - t * kRTile, 0);
-    const int64_t j0 = min(t * kRTile, max(lk - 1, 0));
+  auto issue_k = [&](int t, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < D::kKDma; ++i) {
-      const int r = 8 * wave + i * D::kRowsK + lane / (D::kKB / 16);
-      const int c = lane & (D::kKB / 16 - 1);
-      lds_dma16(kv + (j0 + min(r, last)) * (2 * DN) + DN + 8 * (c ^ v_swz<DN>(r)),
-                lds0 + (uint32_t)(D::kVOff + st * D::kKStage + 8 * wave * D::kKB + 1024 * i));
-    }
+    for (int i = 0; i <= D::kKDma; ++i) issue(i, t, st, 0, 0);
+  };
+  auto issue_v = [&](int t, int st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = D::kKDma + 1; i < D::kDma; ++i) issue(i, 0, 0, t, st);
   };
 
   // ---- LDS read addresses
@@ -199,27 +211,52 @@ latent_ragged_kernel(RaggedParams prm) {
   f32x16 s[2];
   bf16x8 pt[4];
 
-  auto qk = [&](auto kst) __attribute__((always_inline)) {
-    constexpr int st = decltype(kst)::value;
+  // Product i of a segment: those of O^T += V^T P^T of the previous tile (stage
+  // `vst`), then those of S^T = K Q^T (stage `kst`).  Every operand is read
+  // kAhead products before the one it feeds.
+  constexpr int kPvN = 4 * D::kDt, kQkN = 2 * (D::kKs + D::kRs), kAhead = 6;
+  auto products = [&](auto from_c, auto to_c, int vst, int kst) __attribute__((always_inline)) {
+    constexpr int from = decltype(from_c)::value, to = decltype(to_c)::value;
+    bf16x8 a[to];
+    uint32_t ka[kKAddr], ra[D::kRs], va0[D::kDt], va1[D::kDt];
 #pragma unroll
-    for (int ks = 0; ks < D::kKs + D::kRs; ++ks)
+    for (int i = 0; i < kKAddr; ++i) ka[i] = koff[i] + kst * D::kKStage;
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const uint32_t a = ks < D::kKs ? koff[ks % kKAddr] + st * D::kKStage + mt * (32 * D::kKB)
-                                       : roff[(ks - D::kKs) % D::kRs] + st * D::kRStage + mt * (32 * D::kRB);
-        s[mt] = mfma32(as_bf16x8(lds_ld16(a)), q[ks], ks == 0 ? f32x16{} : s[mt]);
+    for (int i = 0; i < D::kRs; ++i) ra[i] = roff[i] + kst * D::kRStage;
+#pragma unroll
+    for (int i = 0; i < D::kDt; ++i) {
+      va0[i] = voff0[i] + vst * D::kKStage;
+      va1[i] = voff1[i] + vst * D::kKStage;
+    }
+    auto fetch = [&](int i) __attribute__((always_inline)) {
+      if (i < kPvN) {
+        const int u = i / D::kDt, dt = i % D::kDt;
+        const u32x2 lo = lds_tr8(va0[dt] + 16 * u * D::kKB), hi = lds_tr8(va1[dt] + 16 * u * D::kKB);
+        a[i] = as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]});
+      } else {
+        const int ks = (i - kPvN) / 2, mt = (i - kPvN) % 2;
+        a[i] = as_bf16x8(lds_ld16(ks < D::kKs ? ka[ks % kKAddr] + mt * (32 * D::kKB)
+                                              : ra[(ks - D::kKs) % D::kRs] + mt * (32 * D::kRB)));
       }
-  };
-  auto pv = [&](int st) __attribute__((always_inline)) {
+    };
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int i = from; i < from + kAhead; ++i) fetch(i);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int dt = 0; dt < D::kDt; ++dt) {
-        const u32x2 lo = lds_tr8(voff0[dt] + st * D::kKStage + 16 * u * D::kKB);
-        const u32x2 hi = lds_tr8(voff1[dt] + st * D::kKStage + 16 * u * D::kKB);
-        acc[dt] = mfma32(as_bf16x8(u32x4{lo[0], lo[1], hi[0], hi[1]}), pt[u], acc[dt]);
+    for (int i = from; i < to; ++i) {
+      if (i < kPvN) {
+        acc[i % D::kDt] = mfma32(a[i], pt[i / D::kDt], acc[i % D::kDt]);
+      } else {
+        const int ks = (i - kPvN) / 2, mt = (i - kPvN) % 2;
+        s[mt] = mfma32(a[i], q[ks], ks == 0 ? f32x16{} : s[mt]);
       }
+      if (i + kAhead < to) fetch(i + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
+  using PvBegin = std::integral_constant<int, 0>;
+  using QkBegin = std::integral_constant<int, kPvN>;
+  using QkEnd = std::integral_constant<int, kPvN + kQkN>;
   const float scale = prm.scale_log2;
   auto softmax = [&](int t, auto&& between) __attribute__((always_inline)) {
     // s[mt][i] is token 64 t + 32 mt + 8 (i / 4) + 4 h + i % 4
@@ -281,22 +318,22 @@ latent_ragged_kernel(RaggedParams prm) {
     constexpr int st = decltype(stc)::value;  // t % 3
     constexpr bool kPv = decltype(has_pv)::value;
     if (!kPv || wave_live) {
-      if constexpr (kPv) pv((st + 2) % 3);
-      qk(stc);
+      if constexpr (kPv) products(PvBegin{}, QkEnd{}, (st + 2) % 3, st);
+      else products(QkBegin{}, QkEnd{}, 0, st);
     }
     wait_lgkm0();
     lds_barrier();
     const int tk = t + (grp_b ? 3 : 2);  // K of tile tk, V of tile tk - 1
     const int ks = grp_b ? st : (st + 2) % 3, vs = grp_b ? (st + 2) % 3 : (st + 1) % 3;
     auto between = [&](int u) __attribute__((always_inline)) {
-      if (u == 0) issue_k(tk, ks);
-      if (u == 2) issue_v(tk - 1, vs);
+#pragma unroll
+      for (int i = u * D::kDma / 4; i < (u + 1) * D::kDma / 4; ++i) issue(i, tk, ks, tk - 1, vs);
     };
     if (!kPv || wave_live) {
       softmax(t, between);
     } else {
-      between(0);
-      between(2);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) between(u);
     }
     wait_vm_lgkm<D::kDma>();
     lds_barrier();
@@ -338,7 +375,7 @@ latent_ragged_kernel(RaggedParams prm) {
       last = 0;
     }
     // V of the last tile: A's share landed an iteration ago, B's before that
-    pv(last);
+    products(PvBegin{}, QkBegin{}, last, 0);
     wait_vm_lgkm<0>();  // loads of tiles past the end may still be in flight
     if (!grp_b) lds_barrier();
   }
