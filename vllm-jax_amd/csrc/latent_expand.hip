@@ -3,10 +3,17 @@
 //
 //   kv[h][t] = [ W_uk[h] c_t | W_uv[h] c_t ],   k_rope[t] = the row's rotary part
 //
-// A matrix product of 256 tokens by one head's outputs per workgroup, depth R,
-// v_mfma_f32_32x32x16_bf16 with A = weight rows and B = token rows.  Both come
-// 64 deep at a time into a two-stage LDS ring by direct loads, the token rows
-// through the block tables.
+// A matrix product of all tokens by all heads' outputs, depth R.  A workgroup
+// keeps 256 token rows in registers, 32 a wave (R = 512: 128 of them), gathered
+// once through the block tables, and streams its share of the weight rows
+// through a four-stage LDS ring, 32 rows a step: v_mfma_f32_32x32x16_bf16 with A
+// = weight rows (16-byte LDS reads, shared by the eight waves) and B = token
+// rows.  Token rows are read once per share, weights once per 256 tokens; the
+// LDS reads of the weights (32 KiB per wave and step) are as long as the
+// products.  Results go out through a wave's own 2 KiB of LDS, 64 bytes of a
+// token at a time.
+#include <algorithm>
+
 #include "latent_attend.h"
 #include "lds_tiles.h"
 #include "pa_errors.h"
@@ -17,7 +24,7 @@ namespace {
 
 constexpr int kXTokens = 256;
 constexpr int kXThreads = 512;
-constexpr int kXDepth = 64;  // elements of a k-step: rows of 128 bytes
+constexpr int kXStages = 4;
 
 // Cache row of flat token t (of the sequences laid end to end by cu_k).
 __device__ __forceinline__ const uint16_t* flat_row(const LatentExpand& p, int t) {
@@ -35,111 +42,123 @@ __device__ __forceinline__ const uint16_t* flat_row(const LatentExpand& p, int t
   return p.pool.cache + page * p.pool.page_stride + (int64_t)(j - pg * (int)p.pool.page.d) * p.pool.slot_stride;
 }
 
-// N: outputs of a head (nope + v).
-template <int N>
-__global__ void __launch_bounds__(kXThreads) latent_expand_kernel(LatentExpand p, int latent, int rope) {
-  constexpr int kWn = N / 64;                // waves along the outputs, 64 each
-  constexpr int kWt = 8 / kWn;               // waves along the tokens
-  constexpr int kTb = kXTokens / kWt / 32;   // 32-token blocks of a wave
-  constexpr int kXb = kXTokens * 128, kWb = N * 128;  // bytes of a stage
-  constexpr int kXDma = kXb / (1024 * 8), kWDma = kWb / (1024 * 8);
-  __shared__ __attribute__((aligned(1024))) char smem[2 * (kXb + kWb)];
+// blocks: 32-output blocks of all heads; share: those of a workgroup.
+template <int R>
+__global__ void __launch_bounds__(kXThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+latent_expand_kernel(LatentExpand p, int rope, int n, int blocks, int share, int tiles) {
+  constexpr int kRowB = 2 * R, kStageB = 32 * kRowB, kKs = R / 16;
+  constexpr int kDma = kStageB / (1024 * 8), kRowsPerDma = 1024 / kRowB;
+  __shared__ __attribute__((aligned(1024))) char smem[kXStages * kStageB + 8 * 2048];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void)smem;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int head = blockIdx.x % p.heads, t0 = (blockIdx.x / p.heads) * kXTokens;
+  // workgroups that run together work on all tokens and few weight rows
+  const int part = blockIdx.x / tiles, t0 = (blockIdx.x - part * tiles) * kXTokens;
   const int total = min(p.cap, p.cu_k[p.batch] - p.cu_k[0]);
   if (t0 >= total) return;
+  const int first = part * share, last = min(blocks, first + share);
+  const int l = lane & 31, h = lane >> 5;
+  const int t = t0 + 32 * wave + l;
+  const bool live = t < total;
 
-  // This wave's pieces of a stage: 1 KiB blocks of eight rows, lane l row l / 8,
-  // chunk l % 8 of it (the logical one is that XOR the row's swizzle).
-  const int r8 = lane >> 3, c8 = lane & 7;
-  const uint16_t* xr[kXDma];
-  const uint16_t* wr[kWDma];
+  // ---- this wave's token rows: lane (l, h) holds chunks 2 ks + h of token l
+  const uint16_t* row = flat_row(p, min(t, total - 1));
+  bf16x8 x[kKs];
 #pragma unroll
-  for (int i = 0; i < kXDma; ++i) {
-    const int row = 8 * (kXDma * wave + i) + r8;
-    xr[i] = flat_row(p, min(t0 + row, total - 1));
-    if (p.k_rope && head == 0) {
-      // the rotary parts ride along: chunks c8 .. of the same rows
-      const uint16_t* src = xr[i] + latent;
-      if (8 * c8 < rope && t0 + row < total) st16(p.k_rope + (int64_t)(t0 + row) * rope + 8 * c8, ld16(src + 8 * c8));
-    }
-    xr[i] += 8 * (c8 ^ swz128(row));
+  for (int ks = 0; ks < kKs; ++ks) x[ks] = as_bf16x8(ld16(row + 16 * ks + 8 * h));
+  if (p.k_rope && part == 0 && live) {
+    for (int c = h; c < rope / 8; c += 2) st16(p.k_rope + (int64_t)t * rope + 8 * c, ld16(row + R + 8 * c));
   }
+
+  // ---- weight rows: block b's 32 rows are contiguous; a wave loads kDma KiB
+  const uint16_t* w = p.w_kv + (int64_t)p.head0 * n * R;
+  uint32_t woff[kDma];
 #pragma unroll
-  for (int i = 0; i < kWDma; ++i) {
-    const int row = 8 * (kWDma * wave + i) + r8;
-    wr[i] = p.w_kv + ((int64_t)(p.head0 + head) * N + row) * latent + 8 * (c8 ^ swz128(row));
+  for (int i = 0; i < kDma; ++i) {
+    const int r = (kDma * wave + i) * kRowsPerDma + lane / (kRowB / 16), c = lane & (kRowB / 16 - 1);
+    woff[i] = (uint32_t)(r * kRowB + 16 * (c ^ swz256(r)));
   }
-  auto issue = [&](int k, int st) __attribute__((always_inline)) {
-    const uint32_t base = lds0 + (uint32_t)(st * (kXb + kWb));
+  auto issue = [&](int b) __attribute__((always_inline)) {
+    const char* src = (const char*)(w + (int64_t)min(b, last - 1) * 32 * R);  // past the end: the last block again
+    const uint32_t st = lds0 + (uint32_t)((b - first) & (kXStages - 1)) * kStageB;
 #pragma unroll
-    for (int i = 0; i < kXDma; ++i) lds_dma16(xr[i] + k, base + (uint32_t)(1024 * (kXDma * wave + i)));
-#pragma unroll
-    for (int i = 0; i < kWDma; ++i) lds_dma16(wr[i] + k, base + (uint32_t)(kXb + 1024 * (kWDma * wave + i)));
+    for (int i = 0; i < kDma; ++i) lds_dma16s(woff[i], src, st + (uint32_t)(1024 * (kDma * wave + i)));
   };
-  const int wn = wave % kWn, wt = wave / kWn;
-  const int n = lane & 31, h = lane >> 5;
-  f32x16 acc[2][kTb] = {};
-  asm volatile("" ::: "memory");
-  wait_vm<0>();  // the waits below count the direct loads alone
-  issue(0, 0);
-  const int steps = latent / kXDepth;
-  for (int ks = 0; ks < steps; ++ks) {
-    // the other stage's readers are done (barrier at the end of the last step)
-    if (ks + 1 < steps) {
-      issue((ks + 1) * kXDepth, (ks + 1) & 1);
-      wait_vm<kXDma + kWDma>();
-    } else {
-      wait_vm<0>();
-    }
+  uint32_t aoff[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) aoff[i] = lds0 + l * kRowB + 16 * ((2 * i + h) ^ swz256(l));
+  const uint32_t own = lds0 + kXStages * kStageB + 2048 * wave;
+
+#pragma unroll
+  for (int ks = 0; ks < kKs; ++ks) asm volatile("" : "+v"(x[ks]));  // here, not waited for in the loop
+  issue(first);
+  issue(first + 1);
+  issue(first + 2);
+  for (int b = first; b < last; ++b) {
+    // block b has landed (loads complete in order, so at most those of the two
+    // blocks behind it may be outstanding); everybody is done with block b - 1
+    wait_vm<2 * kDma>();
     lds_barrier();
-    const uint32_t base = lds0 + (uint32_t)((ks & 1) * (kXb + kWb));
+    issue(b + 3);
+    const uint32_t st = (uint32_t)((b - first) & (kXStages - 1)) * kStageB;
+    uint32_t ao[8];
 #pragma unroll
-    for (int u = 0; u < kXDepth / 16; ++u) {
-      bf16x8 a[2], b[kTb];
+    for (int i = 0; i < 8; ++i) {
+      ao[i] = aoff[i] + st;
+      asm volatile("" : "+v"(ao[i]));
+    }
+    constexpr int kAhead = 6;
+    f32x16 acc[2] = {};
+    bf16x8 a[kKs];
+    auto fetch = [&](int ks) __attribute__((always_inline)) {
+      a[ks] = as_bf16x8(lds_ld16(ao[ks % 8] + (ks / 8) * 256));
+    };
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = 64 * wn + 32 * i + n;
-        a[i] = as_bf16x8(lds_ld16(base + kXb + row * 128 + 16 * ((2 * u + h) ^ swz128(row))));
-      }
+    for (int ks = 0; ks < kAhead; ++ks) fetch(ks);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < kTb; ++i) {
-        const int row = 32 * (wt * kTb + i) + n;
-        b[i] = as_bf16x8(lds_ld16(base + row * 128 + 16 * ((2 * u + h) ^ swz128(row))));
-      }
+    for (int ks = 0; ks < kKs; ++ks) {
+      acc[ks & 1] = mfma32(a[ks], x[ks], acc[ks & 1]);
+      if (ks + kAhead < kKs) fetch(ks + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // lane (l, h) holds token l, outputs 8 q + 4 h + i: to the wave's own rows of
+    // 64 bytes (16-byte chunk q of token l at q ^ (l / 4 % 4)), then out 16 bytes a lane
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < kTb; ++j) acc[i][j] = mfma32(a[i], b[j], acc[i][j]);
+    for (int q = 0; q < 4; ++q) {
+      const f32x16 s = acc[0] + acc[1];
+      const u32x2 v = {pack_bf16x2(s[4 * q], s[4 * q + 1]), pack_bf16x2(s[4 * q + 2], s[4 * q + 3])};
+      *reinterpret_cast<u32x2 __attribute__((address_space(3)))*>(
+          (uintptr_t)(own + 64 * l + 16 * (q ^ (l >> 2 & 3)) + 8 * h)) = v;
     }
     wait_lgkm0();
-    lds_barrier();
+    asm volatile("" ::: "memory");
+    const int head = 32 * b / n, col = 32 * b - head * n;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 16 * i + (lane >> 2), c = lane & 3;
+      const u32x4 v = lds_ld16(own + 64 * r + 16 * (c ^ (r >> 2 & 3)));
+      const int tr = t0 + 32 * wave + r;
+      if (tr < total) st16(p.kv + ((int64_t)head * p.cap + tr) * n + col + 8 * c, v);
+    }
   }
-  // lane (n, h) holds token n, outputs 8 (i / 4) + 4 h + i % 4 of its block
-#pragma unroll
-  for (int j = 0; j < kTb; ++j) {
-    const int t = t0 + 32 * (wt * kTb + j) + n;
-    if (t >= total) continue;
-    uint16_t* dst = p.kv + ((int64_t)head * p.cap + t) * N + 64 * wn + 4 * h;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<u32x2*>(dst + 32 * i + 8 * q) =
-            u32x2{pack_bf16x2(acc[i][j][4 * q], acc[i][j][4 * q + 1]),
-                  pack_bf16x2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
-  }
+  wait_vm<0>();  // loads past the end are still in flight
 }
 
 }  // namespace
 
 int latent_expand_launch(const char* name, const LatentExpand& p, int latent, int rope, int nope, hipStream_t s) {
-  const int64_t blocks = ((int64_t)p.cap + kXTokens - 1) / kXTokens * p.heads;
-  if (blocks > 0x7fffffff) return fail(PA_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)blocks);
-  if (nope == 128) latent_expand_kernel<256><<<dim3((unsigned)blocks), kXThreads, 0, s>>>(p, latent, rope);
-  else latent_expand_kernel<128><<<dim3((unsigned)blocks), kXThreads, 0, s>>>(p, latent, rope);
+  const int n = 2 * nope, blocks = p.heads * n / 32;
+  const int64_t tiles = ((int64_t)p.cap + kXTokens - 1) / kXTokens;
+  // three rounds of workgroups where there are tokens enough, at least two
+  // blocks each (the gathered rows cost about two steps)
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(blocks / 2, (3 * 256 + tiles - 1) / tiles));
+  const int share = (int)((blocks + parts - 1) / parts);
+  const int64_t grid = tiles * ((blocks + share - 1) / share);
+  if (grid > 0x7fffffff) return fail(PA_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)grid);
+  const dim3 g((unsigned)grid), b(kXThreads);
+  if (latent == 512) latent_expand_kernel<512><<<g, b, 0, s>>>(p, rope, n, blocks, share, (int)tiles);
+  else latent_expand_kernel<256><<<g, b, 0, s>>>(p, rope, n, blocks, share, (int)tiles);
   return launch_status(name);
 }
 
