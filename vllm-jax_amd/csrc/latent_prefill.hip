@@ -133,18 +133,6 @@ latent_ragged_kernel(RaggedParams prm) {
   const uint16_t* kv = p.kv + ((int64_t)head * p.cap + kbase) * (2 * DN);
   const uint16_t* kr = p.k_rope + (int64_t)kbase * DR;
 
-  // ---- Q^T
-  bf16x8 q[D::kKs + D::kRs];
-  {
-    const int64_t t = q0 + min(row, lq - 1);
-    const uint16_t* qn = p.q_nope + t * p.qn_ts + head * p.qn_hs + 8 * h;
-    const uint16_t* qr = p.q_rope + t * p.qr_ts + head * p.qr_hs + 8 * h;
-#pragma unroll
-    for (int ks = 0; ks < D::kKs; ++ks) q[ks] = as_bf16x8(ld16(qn + 16 * ks));
-#pragma unroll
-    for (int ks = 0; ks < D::kRs; ++ks) q[D::kKs + ks] = as_bf16x8(ld16(qr + 16 * ks));
-  }
-
   // ---- tile loads: this wave's rows of a tile are 8 wave .. 8 wave + 7, each load
   // a scalar tile base and a lane offset kept in a register.  Piece i of kDma:
   // K's, the rotary parts', V's.  Rows past the kv length repeat the last one.
@@ -205,6 +193,7 @@ latent_ragged_kernel(RaggedParams prm) {
     voff1[dt] = lds0 + D::kVOff + (tr + 8) * D::kKB + 16 * (c ^ v_swz<DN>(tr + 8)) + 8 * (ts & 1);
   }
 
+  bf16x8 q[D::kKs + D::kRs];
   f32x16 acc[D::kDt] = {};
   float m_ref = 0.f;
   float l_part[4] = {};
@@ -342,10 +331,7 @@ latent_ragged_kernel(RaggedParams prm) {
   using S1 = std::integral_constant<int, 1>;
   using S2 = std::integral_constant<int, 2>;
 
-  wait_vm<0>();  // Q is here; from now on vmcnt counts the tile loads
-  asm volatile("" ::: "memory");
-#pragma unroll
-  for (int ks = 0; ks < D::kKs + D::kRs; ++ks) asm volatile("" : "+v"(q[ks]));
+  // The first tiles' loads, then Q's, so that their latencies overlap.
   if (n_tiles > 0) {
     issue_k(0, 0);
     issue_k(1, 1);
@@ -353,15 +339,25 @@ latent_ragged_kernel(RaggedParams prm) {
     if (grp_b) {
       issue_k(2, 2);
       issue_v(1, 1);
-      wait_vm<2 * D::kDma>();
-    } else {
-      wait_vm<D::kDma>();
     }
+  }
+  // ---- Q^T (waited for here, and with it all loads above: from now on vmcnt
+  // counts the loop's tile loads)
+  {
+    const int64_t t = q0 + min(row, lq - 1);
+    const uint16_t* qn = p.q_nope + t * p.qn_ts + head * p.qn_hs + 8 * h;
+    const uint16_t* qr = p.q_rope + t * p.qr_ts + head * p.qr_hs + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < D::kKs; ++ks) q[ks] = as_bf16x8(ld16(qn + 16 * ks));
+#pragma unroll
+    for (int ks = 0; ks < D::kRs; ++ks) q[D::kKs + ks] = as_bf16x8(ld16(qr + 16 * ks));
+  }
+#pragma unroll
+  for (int ks = 0; ks < D::kKs + D::kRs; ++ks) asm volatile("" : "+v"(q[ks]));
+  wait_vm<0>();
+  if (n_tiles > 0) {
     lds_barrier();
-    if (grp_b) {
-      wait_vm<D::kDma>();
-      lds_barrier();
-    }
+    if (grp_b) lds_barrier();
     iteration(0, S0{}, F_{});
     int last = 0;  // stage of the last tile
     for (int t = 1; t < n_tiles; ++t) {
