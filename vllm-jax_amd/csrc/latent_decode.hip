@@ -53,6 +53,7 @@ struct AttnParams {
   // (row_tiles > 0: those of a sequence), else one a workgroup.
   int32_t* joins;
   int32_t row_tiles;
+  int32_t unit_tiles;  // not 0: a workgroup a unit, this many row tiles a sequence, no cut and nothing to join
   float* parts;     // [2 wgs][rows * R]
   float* stats;     // [2 wgs][rows][2]
 };
@@ -273,6 +274,17 @@ __device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
   return incl + before;
 }
 
+// Zero rows for row tile rt of a sequence without any cached token.
+template <int R, int ROWS>
+__device__ __forceinline__ void zero_unit(const AttnParams& p, const Seq& sq, int rt, int wave, int waves, int lane) {
+  const int rows = min((rt + 1) * ROWS, sq.lq * p.a.heads);
+  for (int i = rt * ROWS + wave; i < rows; i += waves) {
+    const int tok = (int)div_by((uint32_t)i, p.heads), hd = i - tok * p.a.heads;
+    uint16_t* o = p.a.out + (int64_t)(sq.q0 + tok) * p.a.o_ts + hd * p.a.o_hs;
+    if (8 * lane < R) st16(o + 8 * lane, u32x4{0, 0, 0, 0});
+  }
+}
+
 template <int R, int DR, int ROWS>
 __global__ void __launch_bounds__(kLThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 latent_attn_kernel(AttnParams p) {
@@ -288,45 +300,59 @@ latent_attn_kernel(AttnParams p) {
   // tiles of a sequence share its L2.
   int g = blockIdx.x;
   if (p.wgs % 8 == 0) g = (g & 7) * (p.wgs >> 3) + (g >> 3);
-  int* pref = reinterpret_cast<int*>(smem);
-  int* tmp = pref + kMaxBatch;
-  int total = 0;
-  for (int c = 0; c < p.a.batch; c += kLThreads) {
-    const int b = c + tid;
-    int v = 0;
-    if (b < p.a.batch) {
-      const Seq s = seq_of(p, b, ROWS);
-      v = s.nt * s.nrt;
-    }
-    int sum;
-    const int incl = block_scan(v, tmp, sum);
-    if (b < p.a.batch) pref[b] = total + incl - v;
-    total += sum;
-  }
-  __syncthreads();
-  const int share = max(p.min_share, (total + p.wgs - 1) / p.wgs);
-  int64_t at64 = (int64_t)g * share;
   int4* joins = reinterpret_cast<int4*>(p.joins);
   int4 join = make_int4(0, 0, 0, g);
-  if (at64 >= total) {  // uniform
-    if (tid == 0 && p.row_tiles == 0) joins[g] = join;
-    return;
-  }
-  int at = (int)at64;
-  const int end = (int)min((int64_t)total, at64 + share);
-  int b;
-  {
-    int lo = 0, hi = p.a.batch;  // last b with pref[b] <= at (sequences without tiles lie before it)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (pref[mid] <= at) lo = mid;
-      else hi = mid;
+  int at, end, b, seq_at, share = 1;
+  if (p.unit_tiles > 0) {
+    b = g / p.unit_tiles;
+    const int rt = g - b * p.unit_tiles;
+    const Seq sq = seq_of(p, b, ROWS);
+    if (rt >= sq.nrt) return;
+    if (sq.nt == 0) {
+      zero_unit<R, ROWS>(p, sq, rt, tid >> 6, kLThreads / 64, lane);
+      return;
     }
-    b = __builtin_amdgcn_readfirstlane(lo);
+    seq_at = 0;
+    at = rt * sq.nt;
+    end = at + sq.nt;
+  } else {
+    int* pref = reinterpret_cast<int*>(smem);
+    int* tmp = pref + kMaxBatch;
+    int total = 0;
+    for (int c = 0; c < p.a.batch; c += kLThreads) {
+      const int b = c + tid;
+      int v = 0;
+      if (b < p.a.batch) {
+        const Seq s = seq_of(p, b, ROWS);
+        v = s.nt * s.nrt;
+      }
+      int sum;
+      const int incl = block_scan(v, tmp, sum);
+      if (b < p.a.batch) pref[b] = total + incl - v;
+      total += sum;
+    }
+    __syncthreads();
+    share = max(p.min_share, (total + p.wgs - 1) / p.wgs);
+    int64_t at64 = (int64_t)g * share;
+    if (at64 >= total) {  // uniform
+      if (tid == 0 && p.row_tiles == 0) joins[g] = join;
+      return;
+    }
+    at = (int)at64;
+    end = (int)min((int64_t)total, at64 + share);
+    {
+      int lo = 0, hi = p.a.batch;  // last b with pref[b] <= at (sequences without tiles lie before it)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pref[mid] <= at) lo = mid;
+        else hi = mid;
+      }
+      b = __builtin_amdgcn_readfirstlane(lo);
+    }
+    seq_at = __builtin_amdgcn_readfirstlane(pref[b]);
+    at = __builtin_amdgcn_readfirstlane(at);
+    __syncthreads();  // the ring is free from here on
   }
-  int seq_at = __builtin_amdgcn_readfirstlane(pref[b]);
-  at = __builtin_amdgcn_readfirstlane(at);
-  __syncthreads();  // the ring is free from here on
 
   while (at < end) {
     const Seq sq = seq_of(p, b, ROWS);
@@ -342,7 +368,7 @@ latent_attn_kernel(AttnParams p) {
     at += t1 - t0;
     // a unit that starts here and goes on: its parts are this one and those of
     // the workgroups behind
-    if (t0 == 0) {
+    if (t0 == 0 && p.unit_tiles == 0) {
       if (t1 < sq.nt) join = make_int4(b, rt, 1 + (sq.nt - t1 + share - 1) / share, g);
       if (tid == 0 && p.row_tiles > 0) joins[b * p.row_tiles + rt] = join;
     }
@@ -732,7 +758,7 @@ latent_attn_kernel(AttnParams p) {
     }
     __syncthreads();  // LDS is free for the next segment
   }
-  if (tid == 0 && p.row_tiles == 0) joins[g] = join;
+  if (tid == 0 && p.row_tiles == 0 && p.unit_tiles == 0) joins[g] = join;
 }
 
 // Joins the parts of every (sequence, row tile) that more than one workgroup
@@ -791,11 +817,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) latent_merge_kernel(AttnParam
   for (int b = blockIdx.x * gridDim.y + blockIdx.y; b < p.a.batch; b += gridDim.x * gridDim.y) {
     const Seq sq = seq_of(p, b, ROWS);
     if (sq.nt > 0) continue;
-    for (int i = wave; i < sq.lq * p.a.heads; i += kJoinWaves) {
-      const int tok = (int)div_by((uint32_t)i, p.heads), hd = i - tok * p.a.heads;
-      uint16_t* o = p.a.out + (int64_t)(sq.q0 + tok) * p.a.o_ts + hd * p.a.o_hs;
-      if (8 * lane < R) st16(o + 8 * lane, u32x4{0, 0, 0, 0});
-    }
+    for (int rt = 0; rt < sq.nrt; ++rt) zero_unit<R, ROWS>(p, sq, rt, wave, kJoinWaves, lane);
   }
   if (p.row_tiles > 0) {
     // an entry is written by the workgroup that starts the unit: there is none
@@ -853,6 +875,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) latent_merge_kernel(AttnParam
 int rows_of(int max_q, int heads) { return (int64_t)max_q * heads <= 32 ? 32 : 64; }
 
 constexpr int kMinShare = 4;  // tiles a workgroup takes at least
+constexpr int kDirect = 8;    // tiles of a sequence up to which it is not cut
 
 int wgs_of(int64_t most_tiles) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(kWgs, (most_tiles + kMinShare - 1) / kMinShare));
@@ -886,6 +909,7 @@ static int attn_launch(const char* name, AttnParams p, int64_t units, void* work
   p.parts = (float*)ws;
   latent_attn_kernel<R, DR, ROWS><<<dim3((unsigned)p.wgs), dim3(kLThreads), 0, s>>>(p);
   if (int rc = launch_status(name)) return rc;
+  if (p.unit_tiles > 0) return PA_OK;
   // at least eight workgroups a join, as many as there are slices for few joins
   const int64_t joins = p.row_tiles > 0 ? units : p.wgs;
   constexpr int kSlices = ROWS * R / 256;
@@ -908,6 +932,10 @@ int latent_attn_launch(const char* name, const LatentAttn& a, int latent, int ro
   const int64_t units = row_tiles * a.batch;
   p.wgs = wgs_of(units * ((span + kTile - 1) / kTile));
   p.row_tiles = units <= p.wgs ? (int)row_tiles : 0;
+  // Sequences of at most kDirect tiles: a workgroup each, which saves the cut's
+  // scan and the merge's launch.
+  p.unit_tiles = (span + kTile - 1) / kTile <= kDirect && units <= 0x7fffffff ? (int)row_tiles : 0;
+  if (p.unit_tiles > 0) p.wgs = (int)units;
   p.joins = nullptr;
   p.parts = p.stats = nullptr;
 #define PA_LATENT_CASE(R, DR)                                             \

@@ -54,6 +54,7 @@ class LatentWeights:
         if self.w_kv.data_ptr() % 16:
             self.w_kv = self.w_kv.clone()
         self.w_uk_t = self.w_kv[:, :nope_dim].transpose(1, 2).contiguous()  # [H, R, Dn]
+        self.pointers = (self.w_uk_t.data_ptr(), self.w_kv.data_ptr())
 
 
 def _check_cache(latent_cache: torch.Tensor, latent_dim: Optional[int] = None) -> Tuple[int, int, int]:
@@ -137,8 +138,9 @@ def latent_store(latent: torch.Tensor, k_rope: torch.Tensor, norm_weight: Option
 
 
 def same_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    at = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != at:
             raise ValueError(f"operands live on {first.device} and {t.device}")
 
 
@@ -217,7 +219,7 @@ def latent_decode_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_c
                   q_rope.stride(0), q_rope.stride(1), latent_cache.data_ptr(), nb, bs, latent_cache.stride(0),
                   latent_cache.stride(1), bt.data_ptr(), bt.stride(0), bt.shape[1], lens.data_ptr(), batch,
                   weights.num_heads, weights.latent_dim, dr, weights.nope_dim, weights.v_dim,
-                  weights.w_uk_t.data_ptr(), weights.w_kv.data_ptr(), float(scale), out.data_ptr(), out.stride(0),
+                  *weights.pointers, float(scale), out.data_ptr(), out.stride(0),
                   out.stride(1), ws.data_ptr(), ws.numel() * ws.element_size(), stream_handle(q_nope))
     return out
 
@@ -287,7 +289,7 @@ def latent_prefill_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_
                   latent_cache.stride(1), bt.data_ptr(), bt.stride(0), bt.shape[1], cu_q.data_ptr(),
                   None if cu_k is None else cu_k.data_ptr(), None if lens is None else lens.data_ptr(), batch, tokens,
                   max_seqlen_q, total, weights.num_heads, weights.latent_dim, dr, weights.nope_dim, weights.v_dim,
-                  weights.w_uk_t.data_ptr(), weights.w_kv.data_ptr(), float(scale), int(zero_rest), out.data_ptr(),
+                  *weights.pointers, float(scale), int(zero_rest), out.data_ptr(),
                   out.stride(0), out.stride(1), ws.data_ptr(), ws.numel() * ws.element_size(), stream_handle(q_nope))
     return out
 

@@ -114,24 +114,24 @@ _NOTHING = _Nothing()
 def on_device(t: torch.Tensor):
     """Context in which launches go to ``t``'s device (nothing to do, and
     nothing spent, where that is the current one)."""
-    return _NOTHING if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _NOTHING if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def check_frequencies(freqs: RotaryFrequencies, like: torch.Tensor) -> None:
     if not isinstance(freqs, RotaryFrequencies):
         raise TypeError(f"freqs must be RotaryFrequencies, got {type(freqs).__name__}")
-    if freqs.inv_freq.device != like.device:
+    if freqs.inv_freq.get_device() != like.get_device():
         raise ValueError(f"the frequencies live on {freqs.inv_freq.device}, the rows on {like.device}")
 
 
 def check_tokens(name: str, t: torch.Tensor, count: int, like: torch.Tensor) -> torch.Tensor:
     """int32 ``[T]`` metadata on the rows' device, contiguous."""
     require_device(name, t)
-    if t.dtype != torch.int32 or tuple(t.shape) != (count,):
+    if t.dtype != torch.int32 or t.shape != (count,):
         raise ValueError(f"{name} must be int32 of shape [{count}], got {t.dtype} {tuple(t.shape)}")
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise ValueError(f"{name} lives on {t.device}, the rows on {like.device}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, freqs: RotaryFrequencies, *, start: int = 0,
