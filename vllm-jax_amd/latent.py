@@ -57,16 +57,23 @@ class LatentWeights:
         self.pointers = (self.w_uk_t.data_ptr(), self.w_kv.data_ptr())
 
 
-def _check_cache(latent_cache: torch.Tensor, latent_dim: Optional[int] = None) -> Tuple[int, int, int]:
-    """(pages, page size, row length) of a pool ``[NB, BS, R + Dr]``."""
-    require_device("latent_cache", latent_cache)
-    require_bf16("latent_cache", latent_cache)
-    if latent_cache.dim() != 3:
-        raise ValueError(f"latent_cache must be [NB, BS, R + Dr], got {tuple(latent_cache.shape)}")
-    if latent_dim is not None and latent_cache.shape[2] - latent_dim not in ROPE_DIMS:
-        raise ValueError(f"latent_cache rows of {latent_cache.shape[2]} do not fit latent_dim {latent_dim} (rope_dim "
-                         f"must be one of {ROPE_DIMS})")
-    return tuple(latent_cache.shape)
+def _bf16(name: str, t: torch.Tensor, dims: int, like: Optional[torch.Tensor] = None) -> Tuple[int, ...]:
+    """Strides of a bf16 device operand of ``dims`` dimensions, contiguous in
+    the last, on ``like``'s device (one call each: this runs on every call)."""
+    require_device(name, t)
+    stride = t.stride()
+    if t.dtype is not torch.bfloat16 or len(stride) != dims or stride[-1] != 1:
+        require_bf16(name, t)
+        raise ValueError(f"{name} must have {dims} dimensions, got {tuple(t.shape)}")
+    if like is not None and t.get_device() != like.get_device():
+        raise ValueError(f"{name} lives on {t.device}, the other operands on {like.device}")
+    return stride
+
+
+def _check_cache(latent_cache: torch.Tensor, like: torch.Tensor):
+    """(pages, page size, row length), (page, slot) strides of a pool ``[NB, BS, R + Dr]``."""
+    stride = _bf16("latent_cache", latent_cache, 3, like)
+    return latent_cache.shape, stride[:2]
 
 
 def latent_store(latent: torch.Tensor, k_rope: torch.Tensor, norm_weight: Optional[torch.Tensor],
@@ -84,110 +91,112 @@ def latent_store(latent: torch.Tensor, k_rope: torch.Tensor, norm_weight: Option
     for every token, into ``q_out`` (``q_rope`` itself, or a new tensor).  Slots
     outside the pool (padding tokens) are skipped.
     """
-    for name, t in (("latent", latent), ("k_rope", k_rope)):
-        require_device(name, t)
-        require_bf16(name, t)
-        if t.dim() != 2:
-            raise ValueError(f"{name} must be [T, dim], got {tuple(t.shape)}")
+    latent_stride = _bf16("latent", latent, 2)
+    k_stride = _bf16("k_rope", k_rope, 2, latent)
     t_count, r = latent.shape
-    nb, bs, row = _check_cache(latent_cache)
-    dr = k_rope.shape[1]
-    if r not in LATENT_DIMS or dr not in ROPE_DIMS or row != r + dr or k_rope.shape[0] != t_count:
+    (nb, bs, row), cache_stride = _check_cache(latent_cache, latent)
+    k_count, dr = k_rope.shape
+    if r not in LATENT_DIMS or dr not in ROPE_DIMS or row != r + dr or k_count != t_count:
         raise ValueError(f"latent {tuple(latent.shape)} and k_rope {tuple(k_rope.shape)} do not fit a cache of rows of "
                          f"{row} (R one of {LATENT_DIMS}, Dr one of {ROPE_DIMS})")
     check_frequencies(freqs, latent)
     if freqs.rotary_dim != dr:
         raise ValueError(f"the frequencies are of rotary_dim {freqs.rotary_dim}, k_rope of {dr}")
+    norm = None
     if norm_weight is not None:
-        require_device("norm_weight", norm_weight)
-        require_bf16("norm_weight", norm_weight)
-        if tuple(norm_weight.shape) != (r,):
+        _bf16("norm_weight", norm_weight, 1, latent)
+        if norm_weight.shape != (r,):
             raise ValueError(f"norm_weight must be [{r}], got {tuple(norm_weight.shape)}")
+        norm = norm_weight.data_ptr()
     pos = check_tokens("positions", positions, t_count, latent)
     slots = check_tokens("slot_mapping", slot_mapping, t_count, latent)
-    heads, q_args = 0, (None, 0, 0, 0, None, 0, 0)
+    q_args = (None, 0, 0, 0, None, 0, 0)
     if q_rope is not None:
-        require_device("q_rope", q_rope)
-        require_bf16("q_rope", q_rope)
-        if q_rope.dim() != 3 or q_rope.shape[0] != t_count or q_rope.shape[2] != dr or q_rope.shape[1] == 0:
-            raise ValueError(f"q_rope must be [{t_count}, H, {dr}], got {tuple(q_rope.shape)}")
+        q_stride = _bf16("q_rope", q_rope, 3, latent)
         heads = q_rope.shape[1]
+        if q_rope.shape != (t_count, heads, dr) or heads == 0:
+            raise ValueError(f"q_rope must be [{t_count}, H, {dr}], got {tuple(q_rope.shape)}")
         if q_out is None:
             q_out = torch.empty_like(q_rope, memory_format=torch.contiguous_format)
+            out_stride = (heads * dr, dr)
         else:
-            require_device("q_out", q_out)
-            require_bf16("q_out", q_out)
-            if tuple(q_out.shape) != tuple(q_rope.shape):
+            out_stride = _bf16("q_out", q_out, 3, latent)
+            if q_out.shape != q_rope.shape:
                 raise ValueError(f"q_out must have shape {tuple(q_rope.shape)}")
-        q_args = (q_rope.data_ptr(), q_rope.stride(0), q_rope.stride(1), heads, q_out.data_ptr(), q_out.stride(0),
-                  q_out.stride(1))
+        q_args = (q_rope.data_ptr(), q_stride[0], q_stride[1], heads, q_out.data_ptr(), out_stride[0], out_stride[1])
     elif q_out is not None:
         raise ValueError("q_out without q_rope")
-    same_device(latent, k_rope, norm_weight, latent_cache, q_rope, q_out)
     if _checking_slots():
         check_slot_mapping(slots, nb * bs)
     if t_count == 0:
         return latent_cache, q_out
     with on_device(latent):
-        _lib.call("pa_latent_store", latent.data_ptr(), latent.stride(0), k_rope.data_ptr(), k_rope.stride(0),
-                  None if norm_weight is None else norm_weight.data_ptr(), float(eps), freqs.inv_freq.data_ptr(),
-                  float(freqs.amplitude), int(bool(interleaved)), pos.data_ptr(), slots.data_ptr(), t_count, r, dr,
-                  *q_args, latent_cache.data_ptr(), nb, bs, latent_cache.stride(0), latent_cache.stride(1),
+        _lib.call("pa_latent_store", latent.data_ptr(), latent_stride[0], k_rope.data_ptr(), k_stride[0], norm,
+                  float(eps), freqs.pointer, freqs.amplitude, int(bool(interleaved)), pos.data_ptr(),
+                  slots.data_ptr(), t_count, r, dr, *q_args, latent_cache.data_ptr(), nb, bs, *cache_stride,
                   stream_handle(latent))
     return latent_cache, q_out
 
 
-def same_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    at = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != at:
-            raise ValueError(f"operands live on {first.device} and {t.device}")
-
-
 def _check_q(q_nope, q_rope, latent_cache, weights):
-    """Checked shapes of an attention call: (tokens, rope_dim, pages, page size)."""
+    """Checked shapes of an attention call: tokens, (nope, v, rope) sizes, pages, page size, and the leading arguments
+    of the C entries (q and cache pointers and strides)."""
     if not isinstance(weights, LatentWeights):
         raise TypeError(f"weights must be LatentWeights, got {type(weights).__name__}")
-    nb, bs, row = _check_cache(latent_cache, weights.latent_dim)
+    heads, dn = weights.num_heads, weights.nope_dim
+    qn = _bf16("q_nope", q_nope, 3)
+    (nb, bs, row), cache_stride = _check_cache(latent_cache, q_nope)
     dr = row - weights.latent_dim
-    for name, t, d in (("q_nope", q_nope, weights.nope_dim), ("q_rope", q_rope, dr)):
-        require_device(name, t)
-        require_bf16(name, t)
-        if t.dim() != 3 or t.shape[1] != weights.num_heads or t.shape[2] != d:
-            raise ValueError(f"{name} must be [T, {weights.num_heads}, {d}], got {tuple(t.shape)}")
-    if q_nope.shape[0] != q_rope.shape[0]:
-        raise ValueError(f"q_nope and q_rope have {q_nope.shape[0]} and {q_rope.shape[0]} tokens")
-    same_device(q_nope, q_rope, latent_cache, weights.w_kv)
-    return q_nope.shape[0], dr, nb, bs
+    if dr not in ROPE_DIMS:
+        raise ValueError(f"latent_cache rows of {row} do not fit latent_dim {weights.latent_dim} (rope_dim must be one "
+                         f"of {ROPE_DIMS})")
+    qr = _bf16("q_rope", q_rope, 3, q_nope)
+    tokens = q_nope.shape[0]
+    for name, t, d in (("q_nope", q_nope, dn), ("q_rope", q_rope, dr)):
+        if t.shape != (tokens, heads, d):
+            raise ValueError(f"{name} must be [{tokens}, {heads}, {d}], got {tuple(t.shape)}")
+    if weights.w_kv.get_device() != q_nope.get_device():
+        raise ValueError(f"the weights live on {weights.w_kv.device}, q on {q_nope.device}")
+    return tokens, dr, nb, bs, (q_nope.data_ptr(), qn[0], qn[1], q_rope.data_ptr(), qr[0], qr[1],
+                                latent_cache.data_ptr(), nb, bs, *cache_stride)
 
 
-def _check_table(block_tables: torch.Tensor, batch: int, like: torch.Tensor) -> torch.Tensor:
+def _check_table(block_tables: torch.Tensor, batch: int, like: torch.Tensor):
+    """(pointer, row stride, pages) of int32 ``[batch, pages]`` block tables, and the tensor they are in."""
     require_device("block_tables", block_tables)
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != batch:
+    if block_tables.dtype is not torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != batch:
         raise ValueError(f"block_tables must be int32 [{batch}, pages], got {block_tables.dtype} "
                          f"{tuple(block_tables.shape)}")
-    same_device(like, block_tables)
-    return block_tables if block_tables.stride(-1) == 1 else block_tables.contiguous()
+    if block_tables.get_device() != like.get_device():
+        raise ValueError(f"block_tables lives on {block_tables.device}, q on {like.device}")
+    stride = block_tables.stride()
+    if stride[1] != 1 and block_tables.shape[1] > 1:
+        block_tables = block_tables.contiguous()
+        stride = block_tables.stride()
+    return (block_tables.data_ptr(), stride[0], block_tables.shape[1]), block_tables
 
 
 def _output(out, shape, like):
+    """The output tensor and its (token, head) strides."""
     if out is None:
-        return torch.empty(shape, dtype=torch.bfloat16, device=like.device)
-    require_device("out", out)
-    require_bf16("out", out)
-    if tuple(out.shape) != shape:
+        return torch.empty(shape, dtype=torch.bfloat16, device=like.device), (shape[1] * shape[2], shape[2])
+    stride = _bf16("out", out, 3, like)
+    if out.shape != shape:
         raise ValueError(f"out must have shape {shape}, got {tuple(out.shape)}")
-    same_device(like, out)
-    return out
+    return out, stride[:2]
 
 
 def _workspace(workspace, need, like):
+    """The caller's workspace where it is large enough, else a new one; and its bytes."""
     if workspace is not None:
         require_device("workspace", workspace)
-        same_device(like, workspace)
-        if workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= need:
-            return workspace
-    return torch.empty(max(need, 1), dtype=torch.uint8, device=like.device)
+        if workspace.get_device() != like.get_device():
+            raise ValueError(f"workspace lives on {workspace.device}, q on {like.device}")
+        given = workspace.numel() * workspace.element_size()
+        if workspace.is_contiguous() and given >= need and workspace.data_ptr() % 16 == 0:
+            return workspace, given
+    need = max(need, 1)
+    return torch.empty(need, dtype=torch.uint8, device=like.device), need
 
 
 def latent_decode_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_cache: torch.Tensor,
@@ -206,21 +215,19 @@ def latent_decode_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_c
     sums are float32; the absorbed q, the softmax weights and the latent-wide
     result are rounded to bf16 for the matrix cores.
     """
-    batch, dr, nb, bs = _check_q(q_nope, q_rope, latent_cache, weights)
-    bt = _check_table(block_tables, batch, q_nope)
+    batch, dr, nb, bs, rows = _check_q(q_nope, q_rope, latent_cache, weights)
+    table, _keep = _check_table(block_tables, batch, q_nope)
     lens = check_tokens("lengths", lengths, batch, q_nope)
-    out = _output(out, (batch, weights.num_heads, weights.v_dim), q_nope)
+    w = weights
+    out, out_stride = _output(out, (batch, w.num_heads, w.v_dim), q_nope)
     if batch == 0:
         return out
-    need = latent_decode_workspace_bytes(batch, weights, bt.shape[1], bs)
-    ws = _workspace(workspace, need, q_nope)
+    need = latent_decode_workspace_bytes(batch, w, table[2], bs)
+    ws, ws_bytes = _workspace(workspace, need, q_nope)
     with on_device(q_nope):
-        _lib.call("pa_latent_decode", q_nope.data_ptr(), q_nope.stride(0), q_nope.stride(1), q_rope.data_ptr(),
-                  q_rope.stride(0), q_rope.stride(1), latent_cache.data_ptr(), nb, bs, latent_cache.stride(0),
-                  latent_cache.stride(1), bt.data_ptr(), bt.stride(0), bt.shape[1], lens.data_ptr(), batch,
-                  weights.num_heads, weights.latent_dim, dr, weights.nope_dim, weights.v_dim,
-                  *weights.pointers, float(scale), out.data_ptr(), out.stride(0),
-                  out.stride(1), ws.data_ptr(), ws.numel() * ws.element_size(), stream_handle(q_nope))
+        _lib.call("pa_latent_decode", *rows, *table, lens.data_ptr(), batch, w.num_heads, w.latent_dim, dr, w.nope_dim,
+                  w.v_dim, *w.pointers, float(scale), out.data_ptr(), *out_stride, ws.data_ptr(), ws_bytes,
+                  stream_handle(q_nope))
     return out
 
 
@@ -254,12 +261,13 @@ def latent_prefill_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_
     expanded K and V rows (bf16) for a group of heads at a time, or the absorbed
     form where few new tokens stand behind long contexts.
     """
-    tokens, dr, nb, bs = _check_q(q_nope, q_rope, latent_cache, weights)
+    tokens, dr, nb, bs, rows = _check_q(q_nope, q_rope, latent_cache, weights)
+    w = weights
     require_device("cu_seqlens_q", cu_seqlens_q)
     if cu_seqlens_q.dim() != 1 or cu_seqlens_q.numel() < 1:
         raise ValueError(f"cu_seqlens_q must be int32 [B + 1], got {tuple(cu_seqlens_q.shape)}")
     batch = cu_seqlens_q.numel() - 1
-    bt = _check_table(block_tables, batch, q_nope)
+    table, _keep = _check_table(block_tables, batch, q_nope)
     cu_q = check_tokens("cu_seqlens_q", cu_seqlens_q, batch + 1, q_nope)
     if cu_seqlens_k is not None and kv_lens is not None:
         raise ValueError("cu_seqlens_k and kv_lens are given both")
@@ -272,25 +280,18 @@ def latent_prefill_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_
         cu_k = cu_q
     if max_seqlen_q < 0 or max_seqlen_q > 0x7fffffff:
         raise ValueError(f"max_seqlen_q {max_seqlen_q}")
-    total = _total_kv(batch, tokens, bt.shape[1] * bs, max_seqlen_k, total_kv_tokens, cu_k is cu_q)
+    total = _total_kv(batch, tokens, table[2] * bs, max_seqlen_k, total_kv_tokens, cu_k is cu_q)
     zero_rest = out is None
-    out = _output(out, (tokens, weights.num_heads, weights.v_dim), q_nope)
+    out, out_stride = _output(out, (tokens, w.num_heads, w.v_dim), q_nope)
     if tokens == 0:
         return out
-    need = 0
-    if batch:
-        need = _lib.load().pa_latent_prefill_workspace_size(batch, tokens, max_seqlen_q, total, bt.shape[1], bs,
-                                                            weights.num_heads, weights.latent_dim, dr,
-                                                            weights.nope_dim)
-    ws = _workspace(workspace, int(need), q_nope)
+    need = latent_prefill_workspace_bytes(batch, tokens, max_seqlen_q, total, w, dr, table[2], bs) if batch else 0
+    ws, ws_bytes = _workspace(workspace, need, q_nope)
     with on_device(q_nope):
-        _lib.call("pa_latent_prefill", q_nope.data_ptr(), q_nope.stride(0), q_nope.stride(1), q_rope.data_ptr(),
-                  q_rope.stride(0), q_rope.stride(1), latent_cache.data_ptr(), nb, bs, latent_cache.stride(0),
-                  latent_cache.stride(1), bt.data_ptr(), bt.stride(0), bt.shape[1], cu_q.data_ptr(),
-                  None if cu_k is None else cu_k.data_ptr(), None if lens is None else lens.data_ptr(), batch, tokens,
-                  max_seqlen_q, total, weights.num_heads, weights.latent_dim, dr, weights.nope_dim, weights.v_dim,
-                  *weights.pointers, float(scale), int(zero_rest), out.data_ptr(),
-                  out.stride(0), out.stride(1), ws.data_ptr(), ws.numel() * ws.element_size(), stream_handle(q_nope))
+        _lib.call("pa_latent_prefill", *rows, *table, cu_q.data_ptr(), None if cu_k is None else cu_k.data_ptr(),
+                  None if lens is None else lens.data_ptr(), batch, tokens, max_seqlen_q, total, w.num_heads,
+                  w.latent_dim, dr, w.nope_dim, w.v_dim, *w.pointers, float(scale), int(zero_rest), out.data_ptr(),
+                  *out_stride, ws.data_ptr(), ws_bytes, stream_handle(q_nope))
     return out
 
 

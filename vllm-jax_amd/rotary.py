@@ -39,9 +39,10 @@ class RotaryFrequencies:
         if not f.is_contiguous():
             raise ValueError("inv_freq must be contiguous")
 
-    @property
-    def rotary_dim(self) -> int:
-        return 2 * self.inv_freq.numel()
+        # (frozen: set once, read on every call)
+        object.__setattr__(self, "rotary_dim", 2 * f.numel())
+        object.__setattr__(self, "pointer", f.data_ptr())
+        object.__setattr__(self, "amplitude", float(self.amplitude))
 
 
 def rotary_frequencies(rotary_dim: int, base: float, *, scaling: Optional[dict] = None,
@@ -148,26 +149,31 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, freqs: RotaryFreq
     require_device("x", x)
     if x.dim() != 3:
         raise ValueError(f"x must be [T, H, d], got {tuple(x.shape)}")
-    if x.dtype not in _DTYPES:
+    code = _DTYPES.get(x.dtype)
+    if code is None:
         raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
-    if x.stride(-1) != 1:
+    stride = x.stride()
+    if stride[2] != 1:
         raise ValueError("x must be contiguous in its last dimension")
     check_frequencies(freqs, x)
     t, h, d = x.shape
-    if start < 0 or start + freqs.rotary_dim > d:
-        raise ValueError(f"the rotated part [{start}, {start + freqs.rotary_dim}) lies outside a head of {d}")
+    r = freqs.rotary_dim
+    if start < 0 or start + r > d:
+        raise ValueError(f"the rotated part [{start}, {start + r}) lies outside a head of {d}")
     pos = check_tokens("positions", positions, t, x)
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        out_stride = (h * d, d, 1)
     else:
         require_device("out", out)
-        if tuple(out.shape) != (t, h, d) or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
+        out_stride = out.stride()
+        if out.shape != x.shape or out.dtype != x.dtype or out.get_device() != x.get_device() or out_stride[2] != 1:
             raise ValueError(f"out must be {x.dtype} of shape {(t, h, d)} on {x.device}, contiguous in its last "
                              "dimension")
     if t == 0 or h == 0:
         return out
     with on_device(x):
-        _lib.call("pa_rotary_embedding", _DTYPES[x.dtype], x.data_ptr(), x.stride(0), x.stride(1), pos.data_ptr(),
-                  freqs.inv_freq.data_ptr(), float(freqs.amplitude), t, h, d, start, freqs.rotary_dim,
-                  int(bool(interleaved)), out.data_ptr(), out.stride(0), out.stride(1), stream_handle(x))
+        _lib.call("pa_rotary_embedding", code, x.data_ptr(), stride[0], stride[1], pos.data_ptr(), freqs.pointer,
+                  freqs.amplitude, t, h, d, start, r, int(bool(interleaved)), out.data_ptr(), out_stride[0],
+                  out_stride[1], stream_handle(x))
     return out
