@@ -128,6 +128,7 @@ struct TileLoader {
   uint32_t lds0;
   int w, lane, t0, lk;
   bool pages8;
+  bool once;  // (32 rows: one row tile a sequence) every cached row is read by one workgroup
   uint32_t voff[kCount];
   const uint16_t* base;
   uint32_t stage, base_lo, base_hi;
@@ -135,8 +136,8 @@ struct TileLoader {
   bool rows8;
 
   __device__ __forceinline__ TileLoader(const LatentPool& pool_, const int32_t* bt_, uint32_t lds0_, int w_, int lane_,
-                                        int t0_, int lk_, bool pages8_)
-      : pool(pool_), bt(bt_), lds0(lds0_), w(w_), lane(lane_), t0(t0_), lk(lk_), pages8(pages8_) {
+                                        int t0_, int lk_, bool pages8_, bool once_)
+      : pool(pool_), bt(bt_), lds0(lds0_), w(w_), lane(lane_), t0(t0_), lk(lk_), pages8(pages8_), once(once_) {
     base = nullptr;
     stage = base_lo = base_hi = 0;
     bases_at = t0 - 64;
@@ -180,8 +181,10 @@ struct TileLoader {
   }
   // Piece k of this wave's (rows8).
   __device__ __forceinline__ void load(int k) {
-    if (kFirst + k < D::kLatDma || 8 * kC == 64 || fresh(lane) < 8 * kC)
-      lds_dma16s(voff[k], uniform_ptr(base), piece(kFirst + k));
+    if (kFirst + k < D::kLatDma || 8 * kC == 64 || fresh(lane) < 8 * kC) {
+      if (once) lds_dma16s_once(voff[k], uniform_ptr(base), piece(kFirst + k));
+      else lds_dma16s(voff[k], uniform_ptr(base), piece(kFirst + k));
+    }
   }
   __device__ __forceinline__ void load_rows() {
     const int ln = fresh(lane), rr = ln / kC;
@@ -412,7 +415,7 @@ latent_attn_kernel(AttnParams p) {
       // ================= scores
       const int tb = wave & 1, rw = (wave >> 1) * 16 * D::kNr;
       const int ln = fresh(lane), l16 = ln & 15, qd = ln >> 4;
-      TileLoader<D, R, DR, D::kVDma, D::kSDma> loader(pool, bt, lds0, wave, ln, t0, lk, p.pages8);
+      TileLoader<D, R, DR, D::kVDma, D::kSDma> loader(pool, bt, lds0, wave, ln, t0, lk, p.pages8, ROWS == 32);
 #pragma unroll 1
       for (int t = t0; t < min(t0 + 2, t1); ++t) loader.issue(t);
       bf16x8 q[D::kNr][D::kKs + D::kRs];
@@ -570,7 +573,7 @@ latent_attn_kernel(AttnParams p) {
       // ================= values
       const int pw = wave - 4;
       const int lv = fresh(lane), n = lv & 31, h = lv >> 5;
-      TileLoader<D, R, DR, 0, D::kVDma> loader(pool, bt, lds0, pw, lv, t0, lk, p.pages8);
+      TileLoader<D, R, DR, 0, D::kVDma> loader(pool, bt, lds0, pw, lv, t0, lk, p.pages8, ROWS == 32);
       f32x16 acc[D::kDt][D::kRb] = {};
       // transposing reads of V^T: lane 16 gamma + s reads row 4 h + s / 4 (+ 8)
       // of a 16-token step, columns 32 dt + 16 (gamma % 2) + 4 (s % 4)
@@ -874,7 +877,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) latent_merge_kernel(AttnParam
 // Rows of a workgroup: 64, or 32 where a sequence has no more.
 int rows_of(int max_q, int heads) { return (int64_t)max_q * heads <= 32 ? 32 : 64; }
 
-constexpr int kMinShare = 4;  // tiles a workgroup takes at least
+constexpr int kMinShare = 8;  // tiles a workgroup takes at least
 constexpr int kDirect = 8;    // tiles of a sequence up to which it is not cut
 
 int wgs_of(int64_t most_tiles) {

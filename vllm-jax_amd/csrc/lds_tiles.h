@@ -28,6 +28,12 @@ __device__ __forceinline__ void lds_dma16s(uint32_t voff, const void* base, uint
   asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(__builtin_amdgcn_readfirstlane(block))
                : "memory", "m0");
 }
+// The same for data that is read once: it does not displace other lines of L2.
+__device__ __forceinline__ void lds_dma16s_once(uint32_t voff, const void* base, uint32_t block) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voff), "s"(base),
+               "s"(__builtin_amdgcn_readfirstlane(block))
+               : "memory", "m0");
+}
 // s_waitcnt vmcnt(N), other counters untouched
 template <int N>
 __device__ __forceinline__ void wait_vm() {
