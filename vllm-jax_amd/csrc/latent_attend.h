@@ -9,7 +9,8 @@
 namespace pa {
 
 // Per-head products y[t, h, :] = W[h] x[t, h, :] (latent_product.hip): W[h] is
-// [n, k] contiguous, k 64, 128, 256 or 512, n a multiple of 32.
+// [n, k] contiguous; k 64 or 128 with n a multiple of 128, or k 256 or 512 with n
+// a multiple of 64.
 struct HeadProduct {
   const uint16_t* x;
   int64_t x_ts, x_hs;

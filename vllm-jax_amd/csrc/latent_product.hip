@@ -1,10 +1,11 @@
 // Per-head products of the absorbed form: y[t, h, :] = W[h] x[t, h, :].
 //
 // q_lat[h] = W_uk[h]^T q_nope[h] before the attention, out[h] = W_uv[h] o_lat[h]
-// behind it.  A wave computes 32 outputs for 32 or 64 tokens of one head with
+// behind it.  Blocks of 32 outputs by 32 or 64 tokens of one head with
 // v_mfma_f32_32x32x16_bf16: A = weight rows, B = token rows, both 16 bytes a
 // lane straight from memory (each weight is used once per wave, so LDS would
-// only add a hop).  With few tokens the weights' read bounds it.
+// only add a hop).  With few tokens the weights' read bounds it, with many the
+// latent-wide rows'.
 #include "latent_attend.h"
 #include "pa_errors.h"
 #include "../../include/latent_attention.h"
@@ -12,23 +13,25 @@
 namespace pa {
 namespace {
 
-// A workgroup's four waves share 32 outputs and split the depth (kSplit = 4), or
-// take 32 outputs each with the whole of it (kSplit = 1); a wave's part, kDepth
-// deep, is all in flight before the first product.
+// kSplit = 1: a workgroup's four waves take 32 outputs each with the whole
+// depth; kSplit = 4: they split the depth and share 64 outputs, whose sums go
+// through LDS.  A wave's part, kDepth deep, is all in flight before the first
+// product.  Results go out through LDS, 256 (128) contiguous bytes of a token.
 template <int MB, int kDepth, int kSplit>
 __global__ void __launch_bounds__(256) head_product_kernel(HeadProduct p, int n_groups) {
-  constexpr int kSteps = kDepth / 16;
-  __shared__ f32x4 part[kSplit == 1 ? 1 : 4][MB][4][64];
+  constexpr int kSteps = kDepth / 16, kNb = kSplit == 1 ? 1 : 2;
+  constexpr int kOuts = kSplit == 1 ? 128 : 64, kChunks = kOuts / 8;  // of the workgroup
+  __shared__ f32x4 part[kSplit == 1 ? 1 : 4][kSplit == 1 ? 1 : MB][4][64];
+  __shared__ u32x4 tile[32 * MB][kChunks];
   const int lane = threadIdx.x & 63;
   const int h2 = lane >> 5, l = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int head = blockIdx.y;
   const int mb = blockIdx.x / n_groups, ng = blockIdx.x - mb * n_groups;
-  const int nb = kSplit == 1 ? 4 * ng + wave : ng;
-  if (32 * nb >= p.n) return;  // (kSplit == 1) no barrier below
+  const int nb0 = kSplit == 1 ? 4 * ng + wave : 2 * ng;  // first 32-output block
   const int k0 = kSplit == 1 ? 0 : wave * kDepth;
-  const uint16_t* w = p.w + head * p.w_hs + (int64_t)(32 * nb + l) * (kDepth * kSplit) + k0 + 8 * h2;
   bf16x8 a[kSteps], b[MB][kSteps];
+  const uint16_t* w = p.w + head * p.w_hs + (int64_t)(32 * nb0 + l) * (kDepth * kSplit) + k0 + 8 * h2;
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) a[s] = as_bf16x8(ld16(w + 16 * s));
 #pragma unroll
@@ -38,46 +41,65 @@ __global__ void __launch_bounds__(256) head_product_kernel(HeadProduct p, int n_
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) b[m][s] = as_bf16x8(ld16(x + 16 * s));
   }
-  f32x16 acc[MB] = {};
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-    for (int m = 0; m < MB; ++m) acc[m] = mfma32(a[s], b[m][s], acc[m]);
-  // lane (l, h2) holds token l, outputs 8 (i / 4) + 4 h2 + i % 4
-  auto store = [&](int m, int q, const f32x4& v) __attribute__((always_inline)) {
-    const int t = (mb * MB + m) * 32 + l;
-    if (t >= p.tokens) return;
-    u32x2 o = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-    if (p.cu_q && !token_in_sequence(p.cu_q, p.batch, p.max_q, t)) {
-      if (!p.zero_rest) return;
-      o = u32x2{0, 0};
-    }
-    *reinterpret_cast<u32x2*>(p.y + t * p.y_ts + head * p.y_hs + 32 * nb + 8 * q + 4 * h2) = o;
+  __builtin_amdgcn_sched_barrier(0);  // all of them in flight
+  // outputs 8 q + 4 h2 .. + 3 of a block for token 32 m + l: half h2 of chunk 4 block + q
+  auto put = [&](int m, int block, int q, const f32x4& v) __attribute__((always_inline)) {
+    const int r = 32 * m + l, c = (4 * block + q) ^ (r & (kChunks - 1));
+    reinterpret_cast<u32x2*>(&tile[r][c])[h2] = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
   };
-  if constexpr (kSplit == 1) {
 #pragma unroll
-    for (int m = 0; m < MB; ++m)
+  for (int nb = 0; nb < kNb; ++nb) {
+    f32x16 acc[MB] = {};
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        store(m, q, f32x4{acc[m][4 * q], acc[m][4 * q + 1], acc[m][4 * q + 2], acc[m][4 * q + 3]});
-  } else {
+    for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-    for (int m = 0; m < MB; ++m)
+      for (int m = 0; m < MB; ++m) acc[m] = mfma32(a[s], b[m][s], acc[m]);
+    if (nb + 1 < kNb) {
+      w += (int64_t)32 * (kDepth * kSplit);
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        part[wave][m][q][lane] = f32x4{acc[m][4 * q], acc[m][4 * q + 1], acc[m][4 * q + 2], acc[m][4 * q + 3]};
-    __syncthreads();
-    // wave q writes quarter q
+      for (int s = 0; s < kSteps; ++s) a[s] = as_bf16x8(ld16(w + 16 * s));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // lane (l, h2) holds token l, outputs 8 q + 4 h2 + i
+    if constexpr (kSplit == 1) {
 #pragma unroll
-    for (int m = 0; m < MB; ++m)
-      store(m, wave, (part[0][m][wave][lane] + part[1][m][wave][lane]) +
-                         (part[2][m][wave][lane] + part[3][m][wave][lane]));
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          put(m, wave, q, f32x4{acc[m][4 * q], acc[m][4 * q + 1], acc[m][4 * q + 2], acc[m][4 * q + 3]});
+    } else {
+      if (nb > 0) __syncthreads();  // the sums of the block before are taken
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          part[wave][m][q][lane] = f32x4{acc[m][4 * q], acc[m][4 * q + 1], acc[m][4 * q + 2], acc[m][4 * q + 3]};
+      __syncthreads();
+      // wave q sums quarter q
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+        put(m, nb, wave, (part[0][m][wave][lane] + part[1][m][wave][lane]) +
+                             (part[2][m][wave][lane] + part[3][m][wave][lane]));
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32 * MB * kChunks / 256; ++i) {
+    const int e = i * 256 + threadIdx.x, r = e / kChunks, c = e & (kChunks - 1);
+    const int t = mb * MB * 32 + r;
+    if (t >= p.tokens) continue;
+    u32x4 v = tile[r][c ^ (r & (kChunks - 1))];
+    if (p.cu_q && !token_in_sequence(p.cu_q, p.batch, p.max_q, t)) {
+      if (!p.zero_rest) continue;
+      v = u32x4{0, 0, 0, 0};
+    }
+    st16(p.y + t * p.y_ts + head * p.y_hs + kOuts * ng + 8 * c, v);
   }
 }
 
 template <int kDepth, int kSplit>
 void launch(const HeadProduct& p, hipStream_t s) {
-  const int n_groups = kSplit == 1 ? (p.n + 127) / 128 : p.n / 32;
+  const int n_groups = p.n / (kSplit == 1 ? 128 : 64);
   const bool two = p.tokens > 32;
   const int m_blocks = (p.tokens + (two ? 63 : 31)) / (two ? 64 : 32);
   const dim3 g((unsigned)(n_groups * m_blocks), (unsigned)p.heads);
@@ -88,6 +110,7 @@ void launch(const HeadProduct& p, hipStream_t s) {
 }  // namespace
 
 int head_product_launch(const char* name, const HeadProduct& p, hipStream_t s) {
+  // (absorbing: depth 64 or 128 to a latent size; projecting: a latent size to 64 or 128)
   switch (p.k) {
     case 64: launch<64, 1>(p, s); break;
     case 128: launch<128, 1>(p, s); break;
