@@ -822,16 +822,17 @@ __global__ void __launch_bounds__(64 * kJoinWaves) latent_merge_kernel(AttnParam
     if (sq.nt > 0) continue;
     for (int rt = 0; rt < sq.nrt; ++rt) zero_unit<R, ROWS>(p, sq, rt, wave, kJoinWaves, lane);
   }
+  // Where the entries are the units', one is written by the workgroup that starts
+  // its unit: there is none for a unit without tiles or without rows.
+  int b = join.x, rt = join.y;
   if (p.row_tiles > 0) {
-    // an entry is written by the workgroup that starts the unit: there is none
-    // for a unit without tiles or without rows
-    const int ub = blockIdx.x / p.row_tiles;
-    const Seq us = seq_of(p, ub, ROWS);
-    if (us.nt == 0 || (int)blockIdx.x - ub * p.row_tiles >= us.nrt) return;
+    b = blockIdx.x / p.row_tiles;
+    rt = blockIdx.x - b * p.row_tiles;
   }
-  const int b = join.x, rt = join.y, parts = join.z, g = join.w;
-  if (parts == 0) return;
+  if (p.row_tiles == 0 && join.z == 0) return;
   const Seq sq = seq_of(p, b, ROWS);
+  if (sq.nt == 0 || rt >= sq.nrt || join.z == 0) return;
+  const int parts = join.z, g = join.w;
   const int n_rows = min(ROWS, sq.lq * p.a.heads - rt * ROWS);
   auto store = [&](int sl, int r, const f32x4& o, float l) __attribute__((always_inline)) {
     if (r >= n_rows) return;
@@ -913,10 +914,10 @@ static int attn_launch(const char* name, AttnParams p, int64_t units, void* work
   latent_attn_kernel<R, DR, ROWS><<<dim3((unsigned)p.wgs), dim3(kLThreads), 0, s>>>(p);
   if (int rc = launch_status(name)) return rc;
   if (p.unit_tiles > 0) return PA_OK;
-  // at least eight workgroups a join, as many as there are slices for few joins
+  // a slice a wave, or a slice a workgroup for few joins (of many parts)
   const int64_t joins = p.row_tiles > 0 ? units : p.wgs;
   constexpr int kSlices = ROWS * R / 256;
-  const unsigned ny = (unsigned)std::max<int64_t>(8, std::min<int64_t>(kSlices, 1024 / joins));
+  const unsigned ny = (unsigned)std::max<int64_t>(16, std::min<int64_t>(kSlices, 1024 / joins));
   latent_merge_kernel<R, ROWS><<<dim3((unsigned)joins, ny), dim3(64 * kJoinWaves), 0, s>>>(p);
   return launch_status(name);
 }
