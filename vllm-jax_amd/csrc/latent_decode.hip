@@ -896,7 +896,9 @@ size_t latent_attn_workspace(int32_t batch, int32_t max_q, int32_t heads, int32_
   const int64_t tiles = (span + kTile - 1) / kTile;
   *why = nullptr;
   if (batch > kMaxBatch) *why = "more than 16384 sequences";
-  else if (span > 0x7fffffff - kTile || (int64_t)max_q * heads > 0x7fffffff - 64 || tiles > 0x7fffffff / std::max<int64_t>(1, row_tiles * batch))
+  else if (span > 0x7fffffff - 65 * kTile ||  // a loader makes row numbers up to 64 tiles ahead
+           (int64_t)max_q * heads > 0x7fffffff - 64 ||
+           tiles > 0x7fffffff / std::max<int64_t>(1, row_tiles * batch))
     *why = "more than 2^31 tiles of work";
   if (*why) return 0;
   const int wgs = wgs_of(row_tiles * batch * tiles);

@@ -101,7 +101,7 @@ latent_ragged_kernel(RaggedParams prm) {
   // Items from the last query tile down (the longest rows first); within a
   // level (sequence, head) pairs in order, so that with a multiple of eight
   // heads all query tiles of a pair run on one XCD and share its L2.
-  const int pairs = p.batch * p.heads;
+  const int pairs = max(p.batch * p.heads, 1);  // no sequences: nothing but rows to zero
   const int level = blockIdx.x / pairs, pair = blockIdx.x - level * pairs;
   if (level >= prm.n_qtiles) {
     zero_rows<DN>(p, ((int64_t)blockIdx.x - (int64_t)prm.n_qtiles * pairs) * kRThreads);
@@ -464,6 +464,7 @@ bool absorbed_form(int32_t batch, int32_t num_tokens, int32_t max_q, int32_t tot
 int plan(const char* name, int32_t batch, int32_t num_tokens, int32_t max_q, int32_t total_kv, int32_t pages_per_seq,
          int32_t page_size, int32_t heads, int32_t latent, int32_t rope, int32_t nope, PrefillPlan& p) {
   p = PrefillPlan{};
+  max_q = std::min(max_q, num_tokens);
   p.absorbed = absorbed_form(batch, num_tokens, max_q, total_kv, latent, rope, nope);
   p.cu = up256(4 * ((size_t)batch + 1));
   if (p.absorbed) {
@@ -554,6 +555,7 @@ extern "C" int pa_latent_prefill(const uint16_t* q_nope, int64_t qn_tok_stride, 
                         out_tok_stride | out_head_stride) % 8)
     return fail(PA_ERR_UNSUPPORTED, "%s: operands must be 16-byte aligned with strides multiple of 8", name);
   hipStream_t s = (hipStream_t)stream;
+  max_seqlen_q = std::min(max_seqlen_q, num_tokens);
   LatentRagged r;
   r.q_nope = q_nope;
   r.qn_ts = qn_tok_stride;

@@ -54,7 +54,6 @@ class LatentWeights:
         if self.w_kv.data_ptr() % 16:
             self.w_kv = self.w_kv.clone()
         self.w_uk_t = self.w_kv[:, :nope_dim].transpose(1, 2).contiguous()  # [H, R, Dn]
-        self.pointers = (self.w_uk_t.data_ptr(), self.w_kv.data_ptr())
 
 
 def _bf16(name: str, t: torch.Tensor, dims: int, like: Optional[torch.Tensor] = None) -> Tuple[int, ...]:
@@ -132,7 +131,7 @@ def latent_store(latent: torch.Tensor, k_rope: torch.Tensor, norm_weight: Option
         return latent_cache, q_out
     with on_device(latent):
         _lib.call("pa_latent_store", latent.data_ptr(), latent_stride[0], k_rope.data_ptr(), k_stride[0], norm,
-                  float(eps), freqs.pointer, freqs.amplitude, int(bool(interleaved)), pos.data_ptr(),
+                  float(eps), freqs.inv_freq.data_ptr(), freqs.amplitude, int(bool(interleaved)), pos.data_ptr(),
                   slots.data_ptr(), t_count, r, dr, *q_args, latent_cache.data_ptr(), nb, bs, *cache_stride,
                   stream_handle(latent))
     return latent_cache, q_out
@@ -226,8 +225,8 @@ def latent_decode_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_c
     ws, ws_bytes = _workspace(workspace, need, q_nope)
     with on_device(q_nope):
         _lib.call("pa_latent_decode", *rows, *table, lens.data_ptr(), batch, w.num_heads, w.latent_dim, dr, w.nope_dim,
-                  w.v_dim, *w.pointers, float(scale), out.data_ptr(), *out_stride, ws.data_ptr(), ws_bytes,
-                  stream_handle(q_nope))
+                  w.v_dim, w.w_uk_t.data_ptr(), w.w_kv.data_ptr(), float(scale), out.data_ptr(), *out_stride,
+                  ws.data_ptr(), ws_bytes, stream_handle(q_nope))
     return out
 
 
@@ -254,8 +253,8 @@ def latent_prefill_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_
     of a sequence are computed.  Rows outside the sequences are zero in a new output and
     left as they were in a given ``out``.
 
-    ``total_kv_tokens`` bounds the sum of the kv lengths on the host (rows
-    past it are dropped); without it ``max_seqlen_k``, or the block tables'
+    ``total_kv_tokens`` bounds the sum of the kv lengths on the host (it has to
+    hold: rows past it may be left out); without it ``max_seqlen_k``, or the block tables'
     span, times the sequences.  Tight bounds keep the workspace
     (``latent_prefill_workspace_bytes``) small and choose the form:
     expanded K and V rows (bf16) for a group of heads at a time, or the absorbed
@@ -290,8 +289,8 @@ def latent_prefill_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_
     with on_device(q_nope):
         _lib.call("pa_latent_prefill", *rows, *table, cu_q.data_ptr(), None if cu_k is None else cu_k.data_ptr(),
                   None if lens is None else lens.data_ptr(), batch, tokens, max_seqlen_q, total, w.num_heads,
-                  w.latent_dim, dr, w.nope_dim, w.v_dim, *w.pointers, float(scale), int(zero_rest), out.data_ptr(),
-                  *out_stride, ws.data_ptr(), ws_bytes, stream_handle(q_nope))
+                  w.latent_dim, dr, w.nope_dim, w.v_dim, w.w_uk_t.data_ptr(), w.w_kv.data_ptr(), float(scale),
+                  int(zero_rest), out.data_ptr(), *out_stride, ws.data_ptr(), ws_bytes, stream_handle(q_nope))
     return out
 
 

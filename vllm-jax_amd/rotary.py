@@ -41,7 +41,6 @@ class RotaryFrequencies:
 
         # (frozen: set once, read on every call)
         object.__setattr__(self, "rotary_dim", 2 * f.numel())
-        object.__setattr__(self, "pointer", f.data_ptr())
         object.__setattr__(self, "amplitude", float(self.amplitude))
 
 
@@ -173,7 +172,8 @@ def rotary_embedding(x: torch.Tensor, positions: torch.Tensor, freqs: RotaryFreq
     if t == 0 or h == 0:
         return out
     with on_device(x):
-        _lib.call("pa_rotary_embedding", code, x.data_ptr(), stride[0], stride[1], pos.data_ptr(), freqs.pointer,
+        _lib.call("pa_rotary_embedding", code, x.data_ptr(), stride[0], stride[1], pos.data_ptr(),
+                  freqs.inv_freq.data_ptr(),
                   freqs.amplitude, t, h, d, start, r, int(bool(interleaved)), out.data_ptr(), out_stride[0],
                   out_stride[1], stream_handle(x))
     return out
