@@ -22,6 +22,18 @@
 // laid end to end, are dealt to the workgroups in equal contiguous shares; a
 // workgroup that gets the whole of a unit writes its rows, one that gets a
 // part leaves O (float32), maximum and sum to latent_merge_kernel.
+//
+// P is rounded to bf16 for the matrix cores; the reference of a tile's P may lag
+// behind the row's maximum by 2^8, which costs no bits.  Scores, maxima, sums, O
+// and the parts are float32; the joined rows are rounded to bf16 once.
+//
+// Few heads are bound by the cache's reads: 256 sequences of 512-8 192 tokens by
+// 16 heads (1.28 GB) 220 us, 5.8 TB/s, of a call of 248.  At 64 rows a tile's step
+// is bound by LDS: 64 sequences by 128 heads 124 us, 650 TFLOP/s, of a call of
+// 158, at 2 300 clocks a tile of which the matrix instructions of a SIMD are
+// 1 090: the tile is read twice for the scores, once for the values and written
+// once, beside P.  One sequence of 32 k tokens by 64 heads: 20 us, and 5 us
+// joining 128 parts.
 #include <algorithm>
 #include <cmath>
 
@@ -40,13 +52,20 @@ constexpr int kLThreads = 512;
 constexpr int kMaxBatch = 16384;  // their prefix sums fit the ring
 constexpr float kSlack = 8.f;  // log2 units a tile's reference may lag behind the maximum of those before it
 constexpr float kJump = 64.f;  // and a half tile's behind its own
+constexpr int kDirect = 6, kDirectMany = 16;  // tiles of a sequence up to which it is not cut
 constexpr float kNoMax = -1e30f;
+
+// Tiles that a workgroup takes at least of `total`: more workgroups each do
+// less and leave more to join.  64 heads, one sequence of 32, 64, 128, 1 024
+// tiles, whole calls: 22.9, 24.2, 26.5 us with 2 (and 4 for the longest: 36.8),
+// 24.7, 25.4, 26.4, 36.8 with 4, 28.2, 29.2, 29.5, 35.3 with 8.
+__host__ __device__ inline int min_share(int64_t total) { return total <= 64 ? 2 : total <= 384 ? 4 : 8; }
 
 struct AttnParams {
   LatentAttn a;
   MagicDiv heads;
   float scale_log2;
-  int32_t min_share, wgs;
+  int32_t wgs;
   bool pages8;      // eight aligned rows lie in one page, within 32-bit byte offsets
   // What latent_merge_kernel has to join, [4] each: sequence, row tile, parts (0: nothing), first
   // workgroup; one entry a unit where there are no more units than workgroups
@@ -102,7 +121,8 @@ __device__ __forceinline__ int fresh(int x) {
 // A wave-uniform pointer, in scalar registers.
 __device__ __forceinline__ const uint16_t* uniform_ptr(const uint16_t* p) {
   const uint64_t x = (uint64_t)(uintptr_t)p;
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
   return (const uint16_t*)(uintptr_t)((uint64_t)hi << 32 | lo);
 }
 
@@ -120,7 +140,12 @@ __device__ __forceinline__ uint32_t fresh_addr(uint32_t x) {
 // them are there, a piece is one scalar base (made for 64 tiles at a time, one
 // a lane) and a lane offset kept in a register; other tiles are looked up row
 // by row (load_rows).
-template <typename D, int R, int DR, int kFirst, int kCount>
+//
+// kOnce (32 rows: one row tile a sequence, every cached row read by one
+// workgroup): loads that do not stay in the caches, 247 us against 267 for 256
+// sequences by 16 heads; at 64 rows they cost 168 against 158 (64 sequences by
+// 128 heads, two row tiles) and 35.5 against 32.8 (one of 32 k tokens, 64 heads).
+template <typename D, int R, int DR, int kFirst, int kCount, bool kOnce>
 struct TileLoader {
   static constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
   const LatentPool& pool;
@@ -128,7 +153,6 @@ struct TileLoader {
   uint32_t lds0;
   int w, lane, t0, lk;
   bool pages8;
-  bool once;  // (32 rows: one row tile a sequence) every cached row is read by one workgroup
   uint32_t voff[kCount];
   const uint16_t* base;
   uint32_t stage, base_lo, base_hi;
@@ -136,8 +160,8 @@ struct TileLoader {
   bool rows8;
 
   __device__ __forceinline__ TileLoader(const LatentPool& pool_, const int32_t* bt_, uint32_t lds0_, int w_, int lane_,
-                                        int t0_, int lk_, bool pages8_, bool once_)
-      : pool(pool_), bt(bt_), lds0(lds0_), w(w_), lane(lane_), t0(t0_), lk(lk_), pages8(pages8_), once(once_) {
+                                        int t0_, int lk_, bool pages8_)
+      : pool(pool_), bt(bt_), lds0(lds0_), w(w_), lane(lane_), t0(t0_), lk(lk_), pages8(pages8_) {
     base = nullptr;
     stage = base_lo = base_hi = 0;
     bases_at = t0 - 64;
@@ -182,7 +206,7 @@ struct TileLoader {
   // Piece k of this wave's (rows8).
   __device__ __forceinline__ void load(int k) {
     if (kFirst + k < D::kLatDma || 8 * kC == 64 || fresh(lane) < 8 * kC) {
-      if (once) lds_dma16s_once(voff[k], uniform_ptr(base), piece(kFirst + k));
+      if constexpr (kOnce) lds_dma16s_once(voff[k], uniform_ptr(base), piece(kFirst + k));
       else lds_dma16s(voff[k], uniform_ptr(base), piece(kFirst + k));
     }
   }
@@ -335,7 +359,7 @@ latent_attn_kernel(AttnParams p) {
       total += sum;
     }
     __syncthreads();
-    share = max(p.min_share, (total + p.wgs - 1) / p.wgs);
+    share = max(min_share(total), (total + p.wgs - 1) / p.wgs);
     int64_t at64 = (int64_t)g * share;
     if (at64 >= total) {  // uniform
       if (tid == 0 && p.row_tiles == 0) joins[g] = join;
@@ -415,7 +439,7 @@ latent_attn_kernel(AttnParams p) {
       // ================= scores
       const int tb = wave & 1, rw = (wave >> 1) * 16 * D::kNr;
       const int ln = fresh(lane), l16 = ln & 15, qd = ln >> 4;
-      TileLoader<D, R, DR, D::kVDma, D::kSDma> loader(pool, bt, lds0, wave, ln, t0, lk, p.pages8, ROWS == 32);
+      TileLoader<D, R, DR, D::kVDma, D::kSDma, ROWS == 32> loader(pool, bt, lds0, wave, ln, t0, lk, p.pages8);
 #pragma unroll 1
       for (int t = t0; t < min(t0 + 2, t1); ++t) loader.issue(t);
       bf16x8 q[D::kNr][D::kKs + D::kRs];
@@ -573,7 +597,7 @@ latent_attn_kernel(AttnParams p) {
       // ================= values
       const int pw = wave - 4;
       const int lv = fresh(lane), n = lv & 31, h = lv >> 5;
-      TileLoader<D, R, DR, 0, D::kVDma> loader(pool, bt, lds0, pw, lv, t0, lk, p.pages8, ROWS == 32);
+      TileLoader<D, R, DR, 0, D::kVDma, ROWS == 32> loader(pool, bt, lds0, pw, lv, t0, lk, p.pages8);
       f32x16 acc[D::kDt][D::kRb] = {};
       // transposing reads of V^T: lane 16 gamma + s reads row 4 h + s / 4 (+ 8)
       // of a 16-token step, columns 32 dt + 16 (gamma % 2) + 4 (s % 4)
@@ -875,14 +899,18 @@ __global__ void __launch_bounds__(64 * kJoinWaves) latent_merge_kernel(AttnParam
   }
 }
 
-// Rows of a workgroup: 64, or 32 where a sequence has no more.
+// Rows of a workgroup: 64, or 32 where a sequence has no more (4 096 tokens each,
+// 256 sequences by 16 heads: 206 us against 236 with 64 rows, 64 by 32 heads 72
+// against 82).
 int rows_of(int max_q, int heads) { return (int64_t)max_q * heads <= 32 ? 32 : 64; }
 
-constexpr int kMinShare = 8;  // tiles a workgroup takes at least
-constexpr int kDirect = 8;    // tiles of a sequence up to which it is not cut
-
+// Workgroups of a cut launch of at most `most_tiles`: as many as min_share
+// leaves work for, whatever there is.
 int wgs_of(int64_t most_tiles) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(kWgs, (most_tiles + kMinShare - 1) / kMinShare));
+  int64_t n = 1;
+  for (const int64_t t : {std::min<int64_t>(most_tiles, 64), std::min<int64_t>(most_tiles, 384), most_tiles})
+    n = std::max<int64_t>(n, (t + min_share(t) - 1) / min_share(t));
+  return (int)std::min<int64_t>(n, kWgs);
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -929,7 +957,6 @@ int latent_attn_launch(const char* name, const LatentAttn& a, int latent, int ro
   p.a = a;
   p.heads = magic_div((uint32_t)a.heads);
   p.scale_log2 = a.scale * kLog2e;
-  p.min_share = kMinShare;
   // eight rows' byte offsets from the first fit 32 bits
   p.pages8 = a.pool.page.d % 8 == 0 && a.pool.slot_stride >= 0 && a.pool.slot_stride < (1 << 27);
   const int rows = rows_of(a.max_q, a.heads);
@@ -938,14 +965,17 @@ int latent_attn_launch(const char* name, const LatentAttn& a, int latent, int ro
   const int64_t units = row_tiles * a.batch;
   p.wgs = wgs_of(units * ((span + kTile - 1) / kTile));
   p.row_tiles = units <= p.wgs ? (int)row_tiles : 0;
-  // Sequences of at most kDirect tiles: a workgroup each, which saves the cut's
-  // scan and the merge's launch.
-  p.unit_tiles = (span + kTile - 1) / kTile <= kDirect && units <= 0x7fffffff ? (int)row_tiles : 0;
+  // Short block tables take a workgroup a unit, without the cut's scan and the
+  // merge's launch.  16 heads, whole calls: 4 sequences of 4 tiles 18.3 us against
+  // 28.6, of 8 tiles 22.8 against 20.3 cut; 64 sequences of 8 tiles 26.6 against
+  // 30.1, of 16 tiles 33.1 against 35.7.
+  const int64_t tiles = (span + kTile - 1) / kTile;
+  p.unit_tiles = tiles <= (units < 64 ? kDirect : kDirectMany) && units <= 0x7fffffff ? (int)row_tiles : 0;
   if (p.unit_tiles > 0) p.wgs = (int)units;
   p.joins = nullptr;
   p.parts = p.stats = nullptr;
-#define PA_LATENT_CASE(R, DR)                                             \
-  if (latent == R && rope == DR)                                          \
+#define PA_LATENT_CASE(R, DR)                                                 \
+  if (latent == R && rope == DR)                                              \
     return rows == 32 ? attn_launch<R, DR, 32>(name, p, units, workspace, s)  \
                       : attn_launch<R, DR, 64>(name, p, units, workspace, s);
   PA_LATENT_CASE(512, 64)

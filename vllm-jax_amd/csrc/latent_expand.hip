@@ -12,6 +12,13 @@
 // LDS reads of the weights (32 KiB per wave and step) are as long as the
 // products.  Results go out through a wave's own 2 KiB of LDS, 64 bytes of a
 // token at a time.
+//
+// 24 k tokens by 64 heads (R = 512, Dn = 128): 0.55 ms, 750 TFLOP/s, of the
+// 8.4 ms that the call takes; both operands through LDS 64 deep at a time took
+// 0.85.  1 000 to 2 000 tokens by 16 heads: 18 to 22 us, most of them the
+// gather's chain (sequence, page, row) and its 16-byte reads of 32 rows at a
+// time.  K and V are rounded to bf16 here, as a cache of K and V rows per head
+// would hold them.
 #include <algorithm>
 
 #include "latent_attend.h"
@@ -61,15 +68,6 @@ latent_expand_kernel(LatentExpand p, int rope, int n, int blocks, int share, int
   const int t = t0 + 32 * wave + l;
   const bool live = t < total;
 
-  // ---- this wave's token rows: lane (l, h) holds chunks 2 ks + h of token l
-  const uint16_t* row = flat_row(p, min(t, total - 1));
-  bf16x8 x[kKs];
-#pragma unroll
-  for (int ks = 0; ks < kKs; ++ks) x[ks] = as_bf16x8(ld16(row + 16 * ks + 8 * h));
-  if (p.k_rope && part == 0 && live) {
-    for (int c = h; c < rope / 8; c += 2) st16(p.k_rope + (int64_t)t * rope + 8 * c, ld16(row + R + 8 * c));
-  }
-
   // ---- weight rows: block b's 32 rows are contiguous; a wave loads kDma KiB
   const uint16_t* w = p.w_kv + (int64_t)p.head0 * n * R;
   uint32_t woff[kDma];
@@ -84,6 +82,20 @@ latent_expand_kernel(LatentExpand p, int rope, int n, int blocks, int share, int
 #pragma unroll
     for (int i = 0; i < kDma; ++i) lds_dma16s(woff[i], src, st + (uint32_t)(1024 * (kDma * wave + i)));
   };
+  // (their latency passes under that of the gathered rows)
+  issue(first);
+  issue(first + 1);
+  issue(first + 2);
+
+  // ---- this wave's token rows: lane (l, h) holds chunks 2 ks + h of token l
+  const uint16_t* row = flat_row(p, min(t, total - 1));
+  bf16x8 x[kKs];
+#pragma unroll
+  for (int ks = 0; ks < kKs; ++ks) x[ks] = as_bf16x8(ld16(row + 16 * ks + 8 * h));
+  if (p.k_rope && part == 0 && live) {
+    for (int c = h; c < rope / 8; c += 2) st16(p.k_rope + (int64_t)t * rope + 8 * c, ld16(row + R + 8 * c));
+  }
+
   uint32_t aoff[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) aoff[i] = lds0 + l * kRowB + 16 * ((2 * i + h) ^ swz256(l));
@@ -91,9 +103,6 @@ latent_expand_kernel(LatentExpand p, int rope, int n, int blocks, int share, int
 
 #pragma unroll
   for (int ks = 0; ks < kKs; ++ks) asm volatile("" : "+v"(x[ks]));  // here, not waited for in the loop
-  issue(first);
-  issue(first + 1);
-  issue(first + 2);
   for (int b = first; b < last; ++b) {
     // block b has landed (loads complete in order, so at most those of the two
     // blocks behind it may be outstanding); everybody is done with block b - 1
@@ -150,10 +159,21 @@ latent_expand_kernel(LatentExpand p, int rope, int n, int blocks, int share, int
 int latent_expand_launch(const char* name, const LatentExpand& p, int latent, int rope, int nope, hipStream_t s) {
   const int n = 2 * nope, blocks = p.heads * n / 32;
   const int64_t tiles = ((int64_t)p.cap + kXTokens - 1) / kXTokens;
-  // three rounds of workgroups where there are tokens enough, at least two
-  // blocks each (the gathered rows cost about two steps)
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(blocks / 2, (3 * 256 + tiles - 1) / tiles));
-  const int share = (int)((blocks + parts - 1) / parts);
+  // Rounds of 256 workgroups by the time they take, in steps: each round gathers
+  // token rows (about eight steps) and multiplies its share.  One round for a
+  // few thousand tokens, more where one leaves CUs idle (2 044 tokens by 16 heads
+  // in one round 22 us, in two 32).
+  int share = blocks;
+  int64_t best = INT64_MAX;
+  for (int64_t rounds = 1; rounds <= 4; ++rounds) {
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(blocks, 256 * rounds / tiles));
+    const int64_t sh = (blocks + parts - 1) / parts;
+    const int64_t time = (tiles * ((blocks + sh - 1) / sh) + 255) / 256 * (8 + sh);
+    if (time < best) {
+      best = time;
+      share = (int)sh;
+    }
+  }
   const int64_t grid = tiles * ((blocks + share - 1) / share);
   if (grid > 0x7fffffff) return fail(PA_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)grid);
   const dim3 g((unsigned)grid), b(kXThreads);
