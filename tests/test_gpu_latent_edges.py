@@ -189,3 +189,45 @@ def test_prefill_no_rows_wanted_and_a_loose_bound(pkg, dev):
     out = torch.full((3, 2, 128), 7.0, dtype=torch.bfloat16, device=dev)
     assert (call(0, out=out) == 7).all()
     assert call(3).any() and torch.equal(call(3), call(0x7fffffff))
+
+
+@pytest.mark.parametrize("slots_apart", [False, True], ids=["pages-apart", "slots-apart"])
+def test_offsets_past_32_bits(pkg, dev, slots_apart):
+    """Rows of a pool, of q and of a rotated tensor more than 2^32 bytes apart: what a dense copy of them gives."""
+    heads, r, dr, dn = 3, 256, 32, 64
+    gen = torch.Generator(device=dev).manual_seed(8)
+    big = torch.empty((1 << 32) + 4096, dtype=torch.bfloat16, device=dev)
+    dense = torch.randn((4, 8, r + dr), generator=gen, device=dev).to(torch.bfloat16)
+    strides = (1 << 9, (1 << 29) + 2048, 1) if slots_apart else ((1 << 30) + 1024, 304, 1)
+    far = big.as_strided(dense.shape, strides)
+    far.copy_(dense)
+    w = pkg.LatentWeights((torch.randn((heads * 2 * dn, r), generator=gen, device=dev) * r ** -0.5).to(torch.bfloat16),
+                          num_heads=heads, nope_dim=dn, v_dim=dn)
+    table = torch.tensor([[3, 0, 2, 1], [1, 3, 0, 2]], dtype=torch.int32, device=dev)
+    lens = torch.tensor([32, 27], dtype=torch.int32, device=dev)
+    q = torch.randn((57, heads, dn + dr), generator=gen, device=dev).to(torch.bfloat16)
+    cu = torch.tensor([0, 30, 57], dtype=torch.int32, device=dev)
+
+    def decode(cache):
+        return pkg.latent_decode_attention(q[:2, :, :dn], q[:2, :, dn:], cache, w, table, lens, scale=0.1)
+
+    def prefill(cache, **kw):
+        return pkg.latent_prefill_attention(q[..., :dn], q[..., dn:], cache, w, table, cu, kv_lens=lens,
+                                            max_seqlen_q=30, scale=0.1, **kw)
+
+    # (a loose bound of the kv lengths makes the expanded form the dearer one)
+    route = pkg._lib.load().pa_latent_prefill_route
+    assert [route(2, 57, 30, total, 4, 8, heads, r, dr, dn) for total in (59, 1 << 20)] == [0, 1]
+    for call in (decode, lambda c: prefill(c, total_kv_tokens=59), lambda c: prefill(c, total_kv_tokens=1 << 20)):
+        want = call(dense)
+        assert want.any() and torch.equal(call(far), want)
+    freqs = pkg.rotary_frequencies(dr, 1e4, device=dev)
+    pos = torch.arange(4, dtype=torch.int32, device=dev)
+    latent, k = dense[:, 0, :r], dense[:, 0, r:]
+    slots = torch.tensor([31, 1, 9, 17], dtype=torch.int32, device=dev)
+    pkg.latent_store(latent, k, None, pos, slots, dense, freqs)
+    pkg.latent_store(far[:, 0, :r], far[:, 0, r:], None, pos, slots, far, freqs)
+    assert torch.equal(far, dense)
+    x = far.transpose(0, 1) if slots_apart else far
+    assert torch.equal(pkg.rotary_embedding(x, pos.repeat(2)[:x.shape[0]], freqs),
+                       pkg.rotary_embedding(x.contiguous(), pos.repeat(2)[:x.shape[0]], freqs))
