@@ -19,9 +19,10 @@
 // tile.  Both issue loads, two tiles ahead.
 //
 // Work is cut on the device: the kv tiles of all (sequence, row tile) units,
-// laid end to end, are dealt to the workgroups in equal contiguous shares; a
-// workgroup that gets the whole of a unit writes its rows, one that gets a
-// part leaves O (float32), maximum and sum to latent_merge_kernel.
+// laid end to end (a unit's start counted as some more of them), are dealt to the
+// workgroups in equal contiguous shares; a workgroup that gets the whole of a unit
+// writes its rows, one that gets a part leaves O (float32), maximum and sum to
+// latent_merge_kernel.
 //
 // P is rounded to bf16 for the matrix cores; the reference of a tile's P may lag
 // behind the row's maximum by 2^8, which costs no bits.  Scores, maxima, sums, O
@@ -29,10 +30,10 @@
 //
 // Few heads are bound by the cache's reads: 256 sequences of 512-8 192 tokens by
 // 16 heads (1.28 GB) 220 us, 5.8 TB/s, of a call of 248.  At 64 rows a tile's step
-// is bound by LDS: 64 sequences by 128 heads 124 us, 650 TFLOP/s, of a call of
-// 158, at 2 300 clocks a tile of which the matrix instructions of a SIMD are
-// 1 090: the tile is read twice for the scores, once for the values and written
-// once, beside P.  One sequence of 32 k tokens by 64 heads: 20 us, and 5 us
+// is bound by LDS: 64 sequences by 128 heads 106 us, 760 TFLOP/s, of a call of
+// 142, at 1.1 us a tile of which the matrix instructions of a SIMD are a half
+// (the tile is read twice for the scores, once for the values and written once,
+// beside P), and 15 us around them, much of it the parts' 50 MB.  One sequence of 32 k tokens by 64 heads: 20 us, and 5 us
 // joining 128 parts.
 #include <algorithm>
 #include <cmath>
@@ -52,6 +53,7 @@ constexpr int kLThreads = 512;
 constexpr int kMaxBatch = 16384;  // their prefix sums fit the ring
 constexpr float kSlack = 8.f;  // log2 units a tile's reference may lag behind the maximum of those before it
 constexpr float kJump = 64.f;  // and a half tile's behind its own
+constexpr int kLead = 7;
 constexpr int kDirect = 6, kDirectMany = 16;  // tiles of a sequence up to which it is not cut
 constexpr float kNoMax = -1e30f;
 
@@ -66,6 +68,7 @@ struct AttnParams {
   MagicDiv heads;
   float scale_log2;
   int32_t wgs;
+  int32_t lead;     // of a unit, in the cut: tiles that its start is counted as
   bool pages8;      // eight aligned rows lie in one page, within 32-bit byte offsets
   // What latent_merge_kernel has to join, [4] each: sequence, row tile, parts (0: nothing), first
   // workgroup; one entry a unit where there are no more units than workgroups
@@ -340,7 +343,7 @@ latent_attn_kernel(AttnParams p) {
       return;
     }
     seq_at = 0;
-    at = rt * sq.nt;
+    at = rt * sq.nt;  // (the lead is zero here)
     end = at + sq.nt;
   } else {
     int* pref = reinterpret_cast<int*>(smem);
@@ -351,7 +354,7 @@ latent_attn_kernel(AttnParams p) {
       int v = 0;
       if (b < p.a.batch) {
         const Seq s = seq_of(p, b, ROWS);
-        v = s.nt * s.nrt;
+        v = s.nt > 0 ? (s.nt + p.lead) * s.nrt : 0;
       }
       int sum;
       const int incl = block_scan(v, tmp, sum);
@@ -383,16 +386,17 @@ latent_attn_kernel(AttnParams p) {
 
   while (at < end) {
     const Seq sq = seq_of(p, b, ROWS);
-    const int seq_tiles = sq.nt * sq.nrt;
-    if (at >= seq_at + seq_tiles) {
-      seq_at += seq_tiles;
+    const int unit = sq.nt + p.lead, seq_span = sq.nt > 0 ? unit * sq.nrt : 0;
+    if (at >= seq_at + seq_span) {
+      seq_at += seq_span;
       ++b;
       continue;
     }
-    const int rt = __builtin_amdgcn_readfirstlane((at - seq_at) / sq.nt);
-    const int t0 = at - seq_at - rt * sq.nt;
-    const int t1 = min(sq.nt, t0 + end - at);
-    at += t1 - t0;
+    const int rt = __builtin_amdgcn_readfirstlane((at - seq_at) / unit);
+    const int off = at - seq_at - rt * unit, take = min(unit - off, end - at);
+    const int t0 = max(0, off - p.lead), t1 = off + take - p.lead;
+    at += take;
+    if (t1 <= t0) continue;  // the share ends before the unit's first tile
     // a unit that starts here and goes on: its parts are this one and those of
     // the workgroups behind
     if (t0 == 0 && p.unit_tiles == 0) {
@@ -921,7 +925,7 @@ size_t latent_attn_workspace(int32_t batch, int32_t max_q, int32_t heads, int32_
                              const char** why) {
   const int rows = rows_of(max_q, heads);
   const int64_t row_tiles = ((int64_t)max_q * heads + rows - 1) / rows;
-  const int64_t tiles = (span + kTile - 1) / kTile;
+  const int64_t tiles = (span + kTile - 1) / kTile + kLead;
   *why = nullptr;
   if (batch > kMaxBatch) *why = "more than 16384 sequences";
   else if (span > 0x7fffffff - 65 * kTile ||  // a loader makes row numbers up to 64 tiles ahead
@@ -929,7 +933,7 @@ size_t latent_attn_workspace(int32_t batch, int32_t max_q, int32_t heads, int32_
            tiles > 0x7fffffff / std::max<int64_t>(1, row_tiles * batch))
     *why = "more than 2^31 tiles of work";
   if (*why) return 0;
-  const int wgs = wgs_of(row_tiles * batch * tiles);
+  const int wgs = wgs_of(row_tiles * batch * (tiles - kLead));
   return align256((size_t)16 * wgs) + align256((size_t)2 * wgs * rows * 8) + (size_t)2 * wgs * rows * latent * 4;
 }
 
@@ -972,6 +976,12 @@ int latent_attn_launch(const char* name, const LatentAttn& a, int latent, int ro
   const int64_t tiles = (span + kTile - 1) / kTile;
   p.unit_tiles = tiles <= (units < 64 ? kDirect : kDirectMany) && units <= 0x7fffffff ? (int)row_tiles : 0;
   if (p.unit_tiles > 0) p.wgs = (int)units;
+  // The start and end of a unit (Q, the first tiles, O) take about as long as
+  // kLead tiles; counted as such, a workgroup that gets several short pieces
+  // gets fewer tiles: 64 sequences of 512-8 192 tokens by 128 heads 157.5 us with
+  // 0, 147.5, 141.8, 140.8 with 4, 7, 10; 256 by 16 heads 247.8, 244.7, 245.8,
+  // 246.6.  Where a workgroup has few tiles anyway they are dealt as they are.
+  p.lead = p.unit_tiles == 0 && units * tiles >= 16 * kWgs ? kLead : 0;
   p.joins = nullptr;
   p.parts = p.stats = nullptr;
 #define PA_LATENT_CASE(R, DR)                                                 \
