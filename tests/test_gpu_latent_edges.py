@@ -231,3 +231,45 @@ def test_offsets_past_32_bits(pkg, dev, slots_apart):
     x = far.transpose(0, 1) if slots_apart else far
     assert torch.equal(pkg.rotary_embedding(x, pos.repeat(2)[:x.shape[0]], freqs),
                        pkg.rotary_embedding(x.contiguous(), pos.repeat(2)[:x.shape[0]], freqs))
+
+
+def test_decode_uneven_units_in_wide_tables(pkg, dev):
+    """Several row tiles a sequence, lengths from nothing to long, more table than tokens: shares that end before, in
+    and behind a unit's counted start."""
+    import test_gpu_latent_decode as dec
+
+    lengths = [0, 1, 2999, 33, 1500, 64, 0, 640, 100, 2000, 31, 7]
+    c = dec.make(dev, lengths, 130, 256, 32, 64, 16, seed=12, width=256)
+    got = dec.run(pkg, c, 130, 64, 0.1)
+    w = c["w"].view(130, 2, 64, 256)
+    for b, n in enumerate(lengths):
+        if n == 0:
+            assert not got[b].any()
+            continue
+        for h in (0, 63, 64, 127, 129):
+            q = c["q"][b:b + 1, h]
+            o, s = ref.attend(q[:, :64], q[:, 64:], c["rows"][b], w[h, 0], w[h, 1], [n], 0.1, "absorbed")
+            ref.check(got[b:b + 1, h], o, s, f"sequence {b} head {h}")
+    assert torch.equal(got, dec.run(pkg, c, 130, 64, 0.1))
+
+
+def test_prefill_absorbed_many_uneven_units(pkg, dev):
+    """New tokens of eight row tiles a sequence behind contexts of all lengths, one of them longer than its context."""
+    import test_gpu_latent_prefill as pre
+
+    seqs = [(30, 4000), (9, 900), (1, 3000), (17, 2500), (30, 20), (25, 64), (0, 700), (12, 3500)]
+    c = pre.make(dev, seqs, 16, 256, 64, 128, 32, seed=13, behind=3)
+    assert pre.form(pkg, c, 16, 256, 64, 128, 32) == "absorbed"
+    for by in ("cu_k", "lens"):
+        pre.check(pkg, c, pre.run(pkg, c, 16, 128, 0.1, lengths=by), 16, 256, 64, 128, 32, 0.1, some_heads=[0, 15])
+
+
+def test_prefill_many_tokens_without_a_sequence(pkg, dev):
+    """More rows than a workgroup zeroes, before and behind the sequences, in both forms."""
+    import test_gpu_latent_prefill as pre
+
+    for heads, seqs, want in ((2, [(70, 70), (600, 600)], "expanded"), (16, [(4, 300), (3, 200)], "absorbed")):
+        c = pre.make(dev, seqs, heads, 256, 32, 64, 16, seed=14, before=700, behind=1100)
+        assert pre.form(pkg, c, heads, 256, 32, 64, 16) == want
+        pre.check(pkg, c, pre.run(pkg, c, heads, 64, 0.1), heads, 256, 32, 64, 16, 0.1, some_heads=[0, heads - 1],
+                  some_rows=20)

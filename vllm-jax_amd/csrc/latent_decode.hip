@@ -33,8 +33,8 @@
 // is bound by LDS: 64 sequences by 128 heads 106 us, 760 TFLOP/s, of a call of
 // 142, at 1.1 us a tile of which the matrix instructions of a SIMD are a half
 // (the tile is read twice for the scores, once for the values and written once,
-// beside P), and 15 us around them, much of it the parts' 50 MB.  One sequence of 32 k tokens by 64 heads: 20 us, and 5 us
-// joining 128 parts.
+// beside P), and 15 us around them, much of it the parts' 50 MB.  One sequence of
+// 32 k tokens by 64 heads: 20 us, and 5 us joining 128 parts.
 #include <algorithm>
 #include <cmath>
 
@@ -930,7 +930,7 @@ size_t latent_attn_workspace(int32_t batch, int32_t max_q, int32_t heads, int32_
   if (batch > kMaxBatch) *why = "more than 16384 sequences";
   else if (span > 0x7fffffff - 65 * kTile ||  // a loader makes row numbers up to 64 tiles ahead
            (int64_t)max_q * heads > 0x7fffffff - 64 ||
-           tiles > 0x7fffffff / std::max<int64_t>(1, row_tiles * batch))
+           tiles > (0x7fffffff - kWgs) / std::max<int64_t>(1, row_tiles * batch))
     *why = "more than 2^31 tiles of work";
   if (*why) return 0;
   const int wgs = wgs_of(row_tiles * batch * (tiles - kLead));
