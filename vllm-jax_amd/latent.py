@@ -212,7 +212,9 @@ def latent_decode_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_c
     split's partials go through ``workspace`` (``latent_decode_workspace_bytes``;
     made here if it is not given or too small).  Scores, softmax statistics and
     sums are float32; the absorbed q, the softmax weights and the latent-wide
-    result are rounded to bf16 for the matrix cores.
+    result are rounded to bf16 for the matrix cores.  How a sequence is cut
+    follows the batch's lengths and the table's width, and with it a row's last
+    bits.  Cached rows below a length have to be finite.
     """
     batch, dr, nb, bs, rows = _check_q(q_nope, q_rope, latent_cache, weights)
     table, _keep = _check_table(block_tables, batch, q_nope)
