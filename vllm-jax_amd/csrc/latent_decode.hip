@@ -24,9 +24,10 @@
 // writes its rows, one that gets a part leaves O (float32), maximum and sum to
 // latent_merge_kernel.
 //
-// P is rounded to bf16 for the matrix cores; the reference of a tile's P may lag
-// behind the row's maximum by 2^8, which costs no bits.  Scores, maxima, sums, O
-// and the parts are float32; the joined rows are rounded to bf16 once.
+// P is rounded to bf16 for the matrix cores; its reference may lag behind the
+// row's maximum (by 2^8 from tile to tile, 2^64 inside one), which costs range and
+// no bits.  Scores, maxima, sums, O and the parts are float32; the joined rows are
+// rounded to bf16 once.
 //
 // Few heads are bound by the cache's reads: 256 sequences of 512-8 192 tokens by
 // 16 heads (1.28 GB) 220 us, 5.8 TB/s, of a call of 248.  At 64 rows a tile's step
