@@ -1,11 +1,9 @@
-// LDS access of the latent-attention kernels: direct global->LDS loads,
-// reads of tile operands, waits and barriers.
-//
-// The direct loads are inline asm, so the compiler neither waits for them nor
-// orders them: a wave waits for its own with wait_vm, and a barrier behind the
-// wait makes them visible to the others.
+// LDS access of the latent-attention kernels: direct global->LDS loads
+// (lds_dma.h: a wave waits for its own with wait_vm), reads of tile operands,
+// waits and barriers.
 #pragma once
 
+#include "lds_dma.h"
 #include "pa_common.h"
 
 namespace pa {
@@ -20,19 +18,15 @@ __device__ __forceinline__ u32x4 lds_ld16(uint32_t a) {
 __device__ __forceinline__ u32x2 lds_tr8(uint32_t a) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(uintptr_t)a));
 }
+// Loads into a block whose address is made scalar here.
 __device__ __forceinline__ void lds_dma16(const void* g, uint32_t block) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(__builtin_amdgcn_readfirstlane(block)) : "memory", "m0");
+  lds_load16(g, __builtin_amdgcn_readfirstlane(block));
 }
-// The same from a scalar base: lane l loads the 16 bytes at base + voff.
 __device__ __forceinline__ void lds_dma16s(uint32_t voff, const void* base, uint32_t block) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(__builtin_amdgcn_readfirstlane(block))
-               : "memory", "m0");
+  lds_load16s(voff, base, __builtin_amdgcn_readfirstlane(block));
 }
-// The same for data that is read once: it does not displace other lines of L2.
 __device__ __forceinline__ void lds_dma16s_once(uint32_t voff, const void* base, uint32_t block) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voff), "s"(base),
-               "s"(__builtin_amdgcn_readfirstlane(block))
-               : "memory", "m0");
+  lds_load16s_once(voff, base, __builtin_amdgcn_readfirstlane(block));
 }
 // s_waitcnt vmcnt(N), other counters untouched
 template <int N>

@@ -40,6 +40,7 @@
 #pragma once
 #include <type_traits>
 
+#include "lds_dma.h"
 #include "pa_common.h"
 #include "pa_errors.h"
 
@@ -192,21 +193,6 @@ __device__ __forceinline__ void prefill_item(int bid, int batch, int hkv, int n_
     b = j / hkv;
     kvh = j - b * hkv;
   }
-}
-
-// One 16-byte-per-lane global->LDS load (global_load_lds_dwordx4): lane l's
-// 16 bytes land at LDS byte address lds_block + 16*l.  Issued as inline asm so
-// the compiler does not insert its conservative "wait for every LDS DMA"
-// before unrelated LDS reads; completion is tracked explicitly with
-// wait_vm_lgkm0 + s_barrier before any wave reads the stage.
-__device__ __forceinline__ void dma16(const void* gptr, uint32_t lds_block) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(gptr), "s"(lds_block) : "memory", "m0");
-}
-
-// The same from a scalar base: lane l loads the 16 bytes at sbase + voff.
-__device__ __forceinline__ void dma16s(uint32_t voff, const void* sbase, uint32_t lds_block) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_block)
-               : "memory", "m0");
 }
 
 // s_waitcnt with vmcnt = N (N < 16), lgkmcnt = 0, expcnt untouched (gfx9 encoding).
@@ -434,8 +420,8 @@ __device__ __forceinline__ void prefill_run(const PrefillParams& p, const Prefil
     const int hd = rw - tk * p.group;
     const int lt = min(tok0 + tk, lq_rows - 1);
     const int c = A::real_chunk((lane & (A::kRowChunks - 1)) ^ A::qswz(r));
-    dma16(p.q + (int64_t)(q0 + lt) * p.q_ts + (int64_t)(kvh * p.group + hd) * p.q_hs + 8 * c,
-          piece(kQSt, i / A::kBlk) + 1024 * (i % A::kBlk));
+    lds_load16(p.q + (int64_t)(q0 + lt) * p.q_ts + (int64_t)(kvh * p.group + hd) * p.q_hs + 8 * c,
+               piece(kQSt, i / A::kBlk) + 1024 * (i % A::kBlk));
   }
   const int qpos = row_ok ? qpos_ld : 0;
   // raw page ids of the first three kv tiles, read while the loads above fly
@@ -604,8 +590,8 @@ __device__ __forceinline__ void prefill_run(const PrefillParams& p, const Prefil
   };
   auto dma_issue = [&](const TileAddrs& a, int i, int stage) __attribute__((always_inline)) {
     const uint32_t lds = ((i & 1) ? v_lds0 : k_lds0) + (uint32_t)(stage * A::kStageB + (kBlk * wave + (i >> 1)) * 1024);
-    if constexpr (kAligned) dma16s(a.vo[i >> 1], (i & 1) ? a.vb : a.kb, lds);
-    else dma16(a.g[i], lds);
+    if constexpr (kAligned) lds_load16s(a.vo[i >> 1], (i & 1) ? a.vb : a.kb, lds);
+    else lds_load16(a.g[i], lds);
   };
   auto issue_tile_raw = [&](int j0, int32_t raw, int stage) __attribute__((always_inline)) {
     const TileAddrs a = tile_addrs(j0, raw, (j0 / kN) % tpp);
