@@ -210,8 +210,8 @@ struct TileLoader {
   // Piece k of this wave's (rows8).
   __device__ __forceinline__ void load(int k) {
     if (kFirst + k < D::kLatDma || 8 * kC == 64 || fresh(lane) < 8 * kC) {
-      if constexpr (kOnce) lds_dma16s_once(voff[k], uniform_ptr(base), piece(kFirst + k));
-      else lds_dma16s(voff[k], uniform_ptr(base), piece(kFirst + k));
+      if constexpr (kOnce) lds_dma16v_once(voff[k], uniform_ptr(base), piece(kFirst + k));
+      else lds_dma16v(voff[k], uniform_ptr(base), piece(kFirst + k));
     }
   }
   __device__ __forceinline__ void load_rows() {

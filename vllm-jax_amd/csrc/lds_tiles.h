@@ -25,8 +25,12 @@ __device__ __forceinline__ void lds_dma16(const void* g, uint32_t block) {
 __device__ __forceinline__ void lds_dma16s(uint32_t voff, const void* base, uint32_t block) {
   lds_load16s(voff, base, __builtin_amdgcn_readfirstlane(block));
 }
-__device__ __forceinline__ void lds_dma16s_once(uint32_t voff, const void* base, uint32_t block) {
-  lds_load16s_once(voff, base, __builtin_amdgcn_readfirstlane(block));
+// (a base that a vector instruction makes)
+__device__ __forceinline__ void lds_dma16v(uint32_t voff, const void* base, uint32_t block) {
+  lds_load16v(voff, base, __builtin_amdgcn_readfirstlane(block));
+}
+__device__ __forceinline__ void lds_dma16v_once(uint32_t voff, const void* base, uint32_t block) {
+  lds_load16v_once(voff, base, __builtin_amdgcn_readfirstlane(block));
 }
 // s_waitcnt vmcnt(N), other counters untouched
 template <int N>
