@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "magic_div.h"
 #include "pa_common.h"
 
 namespace pa {
@@ -14,30 +15,6 @@ inline bool latent_dims_ok(int latent, int rope) {
 }
 // Sizes of a head's unrotated key part and of its values (one size for both).
 inline bool latent_head_ok(int nope, int v) { return (nope == 64 || nope == 128) && v == nope; }
-
-// Quotient of numbers below 2^31 by a divisor of 1 .. 2^31 - 1 that is known on
-// the host: with l = ceil(log2 d) and m = ceil(2^(31 + l) / d) < 2^32 it is
-// (x * m) >> (31 + l), exactly (m d - 2^(31 + l) < d <= 2^l).
-struct MagicDiv {
-  uint32_t d, m, shift;
-};
-inline MagicDiv magic_div(uint32_t d) {
-  uint32_t l = 0;
-  while ((1ull << l) < d) ++l;
-  MagicDiv r;
-  r.d = d;
-  if (l == 0) {  // d == 1: (x * 2^31) >> 31
-    r.m = 1u << 31;
-    r.shift = 31;
-    return r;
-  }
-  r.m = (uint32_t)(((1ull << (31 + l)) + d - 1) / d);
-  r.shift = 31 + l;
-  return r;
-}
-__device__ __forceinline__ uint32_t div_by(uint32_t x, const MagicDiv& v) {
-  return (uint32_t)(((uint64_t)x * v.m) >> v.shift);
-}
 
 // Pool of latent rows: row (page, slot) is `latent` normalised elements, then
 // the rotated key part.

@@ -15,6 +15,7 @@
 //
 // HBM bound: those 159 us are 5.07 TB/s read and written, the rate of a large
 // copy.  Small calls (64 tokens, 32 heads: 7.7 us) are the host's time.
+#include "magic_div.h"
 #include "pa_errors.h"
 #include "../../include/latent_attention.h"
 #include "rotary.h"
@@ -30,7 +31,7 @@ struct RotaryParams {
   const double* inv_freq;
   const int32_t* positions;
   int32_t heads, dim, start, pairs, units;  // units: pieces of a head a thread takes one at a time
-  uint32_t units_magic;                     // ceil(2^32 / units)
+  MagicDiv per_head;                        // by units
   float amp;
 };
 
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_vec_kernel(RotaryParams p)
   for (int i = 0; i < kRotInFlight; ++i) {
     const int u = first + i * kRotThreads;
     if (u < total) {
-      head[i] = p.units == 1 ? u : (int)__umulhi((uint32_t)u, p.units_magic);
+      head[i] = (int)div_by((uint32_t)u, p.per_head);
       piece[i] = u - head[i] * p.units;
       const T* src = xt + head[i] * p.x_hs + offset(piece[i]);
       a[i] = ld16(src);
@@ -129,7 +130,7 @@ int launch(const RotaryParams& prm, int64_t tokens, bool inter, bool in_place, h
   const int rest = in_place ? 0 : p.dim - rot;  // copied elements of a head
   if (vec) {
     p.units = (inter ? rot : p.pairs) / kN + rest / kN;
-    p.units_magic = (uint32_t)((0x100000000ull + p.units - 1) / p.units);
+    p.per_head = magic_div((uint32_t)p.units);
     const int64_t parts = ((int64_t)p.heads * p.units + kRotThreads * kRotInFlight - 1) / (kRotThreads * kRotInFlight);
     const dim3 g((unsigned)tokens, (unsigned)parts);
     if (inter) rotary_vec_kernel<T, true><<<g, kRotThreads, 0, s>>>(p);
@@ -188,7 +189,7 @@ extern "C" int pa_rotary_embedding(int32_t dtype, const void* x, int64_t x_tok_s
   p.start = start;
   p.pairs = rotary_dim / 2;
   p.units = 0;
-  p.units_magic = 0;
+  p.per_head = MagicDiv{};
   p.amp = amplitude;
   const bool inter = interleaved != 0;
   hipStream_t s = (hipStream_t)stream;
