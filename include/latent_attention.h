@@ -52,8 +52,8 @@ int pa_rotary_embedding(int32_t dtype, const void* x, int64_t x_tok_stride, int6
  * cache[slot[t]] = [ latent[t] * norm_weight / rms(latent[t]) | rope(k_rope[t]) ]
  * for every token whose slot lies in the pool (others are skipped), and q_out
  * = rope(q_rope) for all tokens; norm_weight NULL stores the latent rows as
- * they come, num_heads 0 leaves q out, q_out may be q_rope.  Slots must be
- * unique.
+ * they come, num_heads 0 leaves q out, q_out may be q_rope (same strides).  Slots
+ * must be unique.
  */
 int pa_latent_store(const uint16_t* latent, int64_t latent_tok_stride, const uint16_t* k_rope,
                     int64_t k_rope_tok_stride, const uint16_t* norm_weight, float eps,

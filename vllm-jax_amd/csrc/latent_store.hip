@@ -159,6 +159,10 @@ extern "C" int pa_latent_store(const uint16_t* latent, int64_t latent_tok_stride
   }
   if ((align & 15u) || strides % 8)
     return fail(PA_ERR_UNSUPPORTED, "%s: operands must be 16-byte aligned with strides multiple of 8", name);
+  // a row is read and written by one workgroup only where both lie alike
+  if (num_heads && q_rope == q_out &&
+      ((num_tokens > 1 && q_tok_stride != q_out_tok_stride) || (num_heads > 1 && q_head_stride != q_out_head_stride)))
+    return fail(PA_ERR_INVALID_ARGUMENT, "%s: in place, q_rope and q_out must share strides", name);
   LatentStoreParams p;
   p.c = latent;
   p.c_ts = latent_tok_stride;

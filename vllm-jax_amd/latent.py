@@ -87,8 +87,9 @@ def latent_store(latent: torch.Tensor, k_rope: torch.Tensor, norm_weight: Option
     ``latent`` ``[T, R]`` and ``k_rope`` ``[T, Dr]`` may be slices of one
     projection; ``norm_weight`` ``[R]``, or ``None`` for rows that come
     normalised.  ``q_rope`` ``[T, H, Dr]`` (a slice of q's heads) is rotated
-    for every token, into ``q_out`` (``q_rope`` itself, or a new tensor).  Slots
-    outside the pool (padding tokens) are skipped.
+    for every token, into ``q_out`` (``q_rope`` itself, or a tensor that shares
+    no memory with it; a new one by default).  Slots outside the pool (padding
+    tokens) are skipped.
     """
     latent_stride = _bf16("latent", latent, 2)
     k_stride = _bf16("k_rope", k_rope, 2, latent)
