@@ -56,7 +56,8 @@ def rotary_frequencies(rotary_dim: int, base: float, *, scaling: Optional[dict] 
       ``original_max_position`` positions keep ``f_i``, those below
       ``beta_slow`` (1) turns take ``f_i / factor``, a linear ramp over the pair
       index between; cos and sin are multiplied by ``attention_factor``
-      (``0.1 ln(factor) + 1``).
+      (``0.1 ln(factor) + 1``, 1 for factors below 1).  Models that put that
+      factor into the softmax scale instead, squared, pass 1 here.
     """
     if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > MAX_ROTARY_DIM:
         raise ValueError(f"rotary_dim must be even and at most {MAX_ROTARY_DIM}, got {rotary_dim}")
@@ -96,7 +97,7 @@ def rotary_frequencies(rotary_dim: int, base: float, *, scaling: Optional[dict] 
         high = min(math.ceil(pair_of(slow)), rotary_dim - 1)
         ramp = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
         freq = freq / factor * ramp + freq * (1 - ramp)
-        amplitude = float(scaling.get("attention_factor", 0.1 * math.log(factor) + 1))
+        amplitude = float(scaling.get("attention_factor", 0.1 * math.log(max(factor, 1.0)) + 1))
     return RotaryFrequencies(freq.to(device), amplitude)
 
 
