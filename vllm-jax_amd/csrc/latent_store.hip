@@ -14,6 +14,8 @@
 // take 70 us, 4.5 TB/s.  A workgroup a token keeps the angles' float64 products
 // at one set a token; they pass under the rows' loads.  A decode step's four
 // tokens take 4 us, 13 us with the host's part.
+#include <algorithm>
+
 #include "pa_errors.h"
 #include "../../include/latent_attention.h"
 #include "latent.h"
@@ -189,14 +191,23 @@ extern "C" int pa_latent_store(const uint16_t* latent, int64_t latent_tok_stride
   p.latent = latent_dim;
   const bool inter = interleaved != 0;
   const int units = (num_heads + 1) * (inter ? rope_dim / 8 : rope_dim / 16);
-  const dim3 g((unsigned)num_tokens), b(units <= 64 ? 64 : (units <= 128 ? 128 : 256));
-  hipStream_t s = (hipStream_t)stream;
-  if (rope_dim == 64) {
-    if (inter) latent_store_kernel<64, true><<<g, b, 0, s>>>(p);
-    else latent_store_kernel<64, false><<<g, b, 0, s>>>(p);
-  } else {
-    if (inter) latent_store_kernel<32, true><<<g, b, 0, s>>>(p);
-    else latent_store_kernel<32, false><<<g, b, 0, s>>>(p);
+  const unsigned threads = units <= 64 ? 64 : (units <= 128 ? 128 : 256);
+  void (*kernel)(LatentStoreParams) = rope_dim == 64
+      ? (inter ? latent_store_kernel<64, true> : latent_store_kernel<64, false>)
+      : (inter ? latent_store_kernel<32, true> : latent_store_kernel<32, false>);
+  // a grid has fewer than 2^32 threads along x
+  constexpr int64_t kTokens = 1 << 23;
+  for (int64_t t0 = 0; t0 < num_tokens; t0 += kTokens) {
+    kernel<<<dim3((unsigned)std::min(num_tokens - t0, kTokens)), dim3(threads), 0, (hipStream_t)stream>>>(p);
+    if (int rc = launch_status(name)) return rc;
+    p.c += kTokens * p.c_ts;
+    p.k += kTokens * p.k_ts;
+    p.positions += kTokens;
+    p.slots += kTokens;
+    if (num_heads) {
+      p.q += kTokens * p.q_ts;
+      p.q_out += kTokens * p.qo_ts;
+    }
   }
-  return launch_status(name);
+  return PA_OK;
 }

@@ -15,6 +15,8 @@
 //
 // HBM bound: those 159 us are 5.07 TB/s read and written, the rate of a large
 // copy.  Small calls (64 tokens, 32 heads: 7.7 us) are the host's time.
+#include <algorithm>
+
 #include "magic_div.h"
 #include "pa_errors.h"
 #include "../../include/latent_attention.h"
@@ -37,6 +39,7 @@ struct RotaryParams {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotInFlight = 2;  // pieces a thread has in flight
+constexpr int64_t kRotTokens = 1 << 23;  // tokens of a launch: a grid has fewer than 2^32 threads along x
 
 __device__ __forceinline__ void rot_table(const RotaryParams& p, int64_t t, float* cs, float* sn) {
   const int32_t pos = p.positions[t];
@@ -120,6 +123,19 @@ __global__ void __launch_bounds__(kRotThreads) rotary_scalar_kernel(RotaryParams
 }
 
 template <typename T>
+int launch_tokens(RotaryParams p, int64_t tokens, int64_t parts, void (*kernel)(RotaryParams), hipStream_t s) {
+  for (int64_t t0 = 0; t0 < tokens; t0 += kRotTokens) {
+    const dim3 g((unsigned)std::min(tokens - t0, kRotTokens), (unsigned)parts);
+    kernel<<<g, kRotThreads, 0, s>>>(p);
+    if (int rc = launch_status("pa_rotary_embedding")) return rc;
+    p.x = (const T*)p.x + kRotTokens * p.x_ts;
+    p.out = (T*)p.out + kRotTokens * p.o_ts;
+    p.positions += kRotTokens;
+  }
+  return PA_OK;
+}
+
+template <typename T>
 int launch(const RotaryParams& prm, int64_t tokens, bool inter, bool in_place, hipStream_t s) {
   RotaryParams p = prm;
   constexpr int kN = RotVec<T>::kN;
@@ -132,17 +148,13 @@ int launch(const RotaryParams& prm, int64_t tokens, bool inter, bool in_place, h
     p.units = (inter ? rot : p.pairs) / kN + rest / kN;
     p.per_head = magic_div((uint32_t)p.units);
     const int64_t parts = ((int64_t)p.heads * p.units + kRotThreads * kRotInFlight - 1) / (kRotThreads * kRotInFlight);
-    const dim3 g((unsigned)tokens, (unsigned)parts);
-    if (inter) rotary_vec_kernel<T, true><<<g, kRotThreads, 0, s>>>(p);
-    else rotary_vec_kernel<T, false><<<g, kRotThreads, 0, s>>>(p);
+    return launch_tokens<T>(p, tokens, parts, inter ? rotary_vec_kernel<T, true> : rotary_vec_kernel<T, false>, s);
   } else {
     p.units = p.pairs + rest;
     const int64_t parts = ((int64_t)p.heads * p.units + kRotThreads * 8 - 1) / (kRotThreads * 8);
-    const dim3 g((unsigned)tokens, (unsigned)parts);
-    if (inter) rotary_scalar_kernel<T, true><<<g, kRotThreads, 0, s>>>(p);
-    else rotary_scalar_kernel<T, false><<<g, kRotThreads, 0, s>>>(p);
+    return launch_tokens<T>(p, tokens, parts, inter ? rotary_scalar_kernel<T, true> : rotary_scalar_kernel<T, false>,
+                            s);
   }
-  return launch_status("pa_rotary_embedding");
 }
 
 }  // namespace
