@@ -975,7 +975,8 @@ int latent_attn_launch(const char* name, const LatentAttn& a, int latent, int ro
   // 28.6, of 8 tiles 22.8 against 20.3 cut; 64 sequences of 8 tiles 26.6 against
   // 30.1, of 16 tiles 33.1 against 35.7.
   const int64_t tiles = (span + kTile - 1) / kTile;
-  p.unit_tiles = tiles <= (units < 64 ? kDirect : kDirectMany) && units <= 0x7fffffff ? (int)row_tiles : 0;
+  // (a grid has fewer than 2^32 threads along x)
+  p.unit_tiles = tiles <= (units < 64 ? kDirect : kDirectMany) && units * kLThreads <= 0xffffffffll ? (int)row_tiles : 0;
   if (p.unit_tiles > 0) p.wgs = (int)units;
   // The start and end of a unit (Q, the first tiles, O) take about as long as
   // kLead tiles; counted as such, a workgroup that gets several short pieces

@@ -175,7 +175,7 @@ int latent_expand_launch(const char* name, const LatentExpand& p, int latent, in
     }
   }
   const int64_t grid = tiles * ((blocks + share - 1) / share);
-  if (grid > 0x7fffffff) return fail(PA_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)grid);
+  if (grid * kXThreads > 0xffffffffll) return fail(PA_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)grid);
   const dim3 g((unsigned)grid), b(kXThreads);
   if (latent == 512) latent_expand_kernel<512><<<g, b, 0, s>>>(p, rope, n, blocks, share, (int)tiles);
   else latent_expand_kernel<256><<<g, b, 0, s>>>(p, rope, n, blocks, share, (int)tiles);

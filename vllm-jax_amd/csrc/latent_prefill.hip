@@ -45,10 +45,14 @@ constexpr int kRWaves = 8, kRThreads = 64 * kRWaves, kRRows = 32 * kRWaves;
 constexpr int kRTile = 64, kRStages = 3;
 constexpr float kRSlack = 8.f;
 
+// Workgroups of a launch: a grid has fewer than 2^32 threads along x.
+constexpr int64_t kRGrid = (1 << 22) - 1;  // and as many to zero rows
+
 struct RaggedParams {
   LatentRagged r;
   float scale_log2;
   int32_t n_qtiles;
+  int32_t level0;  // first level of this launch
 };
 
 template <int DN, int DR>
@@ -110,9 +114,11 @@ latent_ragged_kernel(RaggedParams prm) {
   // level (sequence, head) pairs in order, so that with a multiple of eight
   // heads all query tiles of a pair run on one XCD and share its L2.
   const int pairs = max(p.batch * p.heads, 1);  // no sequences: nothing but rows to zero
-  const int level = blockIdx.x / pairs, pair = blockIdx.x - level * pairs;
+  int level = blockIdx.x / pairs;
+  const int pair = blockIdx.x - level * pairs;
+  level += prm.level0;
   if (level >= prm.n_qtiles) {
-    zero_rows<DN>(p, ((int64_t)blockIdx.x - (int64_t)prm.n_qtiles * pairs) * kRThreads);
+    zero_rows<DN>(p, ((int64_t)blockIdx.x - (int64_t)(prm.n_qtiles - prm.level0) * pairs) * kRThreads);
     return;
   }
   const int qt = prm.n_qtiles - 1 - level;
@@ -399,13 +405,26 @@ latent_ragged_kernel(RaggedParams prm) {
 }
 
 template <int DN, int DR>
-int ragged_launch(const char* name, const RaggedParams& p, hipStream_t s) {
+int ragged_launch(const char* name, RaggedParams p, hipStream_t s) {
   const int64_t zero = p.r.zero_out ? ((int64_t)p.r.num_tokens + kRThreads - 1) / kRThreads : 0;
-  const int64_t blocks = (int64_t)p.n_qtiles * p.r.batch * p.r.heads + zero;
-  if (blocks > 0x7fffffff) return fail(PA_ERR_UNSUPPORTED, "%s: %lld workgroups", name, (long long)blocks);
-  if (blocks == 0) return PA_OK;
-  latent_ragged_kernel<DN, DR><<<dim3((unsigned)blocks), kRThreads, 0, s>>>(p);
-  return launch_status(name);
+  const int64_t pairs = (int64_t)p.r.batch * p.r.heads;
+  if (pairs > kRGrid) return fail(PA_ERR_UNSUPPORTED, "%s: %d sequences", name, p.r.batch);
+  // as many levels at a time as a grid holds, the rows to zero behind the last
+  int32_t left = pairs ? p.n_qtiles : 0;
+  p.level0 = p.n_qtiles - left;
+  for (bool rows = zero > 0; left > 0 || rows;) {
+    const int64_t take = pairs ? std::min<int64_t>(left, kRGrid / pairs) : 0;
+    int64_t blocks = take * pairs;
+    if (take == left) {
+      blocks += zero;
+      rows = false;
+    }
+    latent_ragged_kernel<DN, DR><<<dim3((unsigned)blocks), kRThreads, 0, s>>>(p);
+    if (int rc = launch_status(name)) return rc;
+    p.level0 += (int32_t)take;
+    left -= (int32_t)take;
+  }
+  return PA_OK;
 }
 
 }  // namespace
@@ -414,7 +433,8 @@ int latent_ragged_launch(const char* name, const LatentRagged& r, int nope, int 
   RaggedParams p;
   p.r = r;
   p.scale_log2 = r.scale * kLog2e;
-  p.n_qtiles = (r.max_q + kRRows - 1) / kRRows;
+  p.n_qtiles = (int32_t)(((int64_t)r.max_q + kRRows - 1) / kRRows);
+  p.level0 = 0;
   if (nope == 128) return rope == 64 ? ragged_launch<128, 64>(name, p, s) : ragged_launch<128, 32>(name, p, s);
   return rope == 64 ? ragged_launch<64, 64>(name, p, s) : ragged_launch<64, 32>(name, p, s);
 }
@@ -492,6 +512,7 @@ int plan(const char* name, int32_t batch, int32_t num_tokens, int32_t max_q, int
   const size_t head = (size_t)total_kv * 2 * nope * 2;
   size_t g = head ? kGroupBytes / head : heads;
   if (g >= 8) g &= ~(size_t)7;
+  g = std::min<size_t>(g, (size_t)std::max<int64_t>(1, kRGrid / batch));
   p.group = (int32_t)std::max<size_t>(1, std::min<size_t>(g, heads));
   p.k_rope = up256((size_t)total_kv * rope * 2);
   p.kv = up256(head * p.group);
