@@ -95,7 +95,9 @@ int pa_latent_decode(const uint16_t* q_nope, int64_t qn_tok_stride, int64_t qn_h
  *
  * pa_latent_prefill_route says which form a launch takes: K and V expanded for
  * a group of heads at a time, or the absorbed form of pa_latent_decode for few
- * new tokens behind long contexts; the workspace follows it.  1 .. 65535 heads.
+ * new tokens behind long contexts and, where it needs less memory, for a total_kv
+ * whose expanded rows of one head would pass 8 GiB; the workspace follows it.
+ * 1 .. 65535 heads.
  */
 #define PA_LATENT_EXPANDED 0
 #define PA_LATENT_ABSORBED 1

@@ -75,7 +75,9 @@ class MixedAttentionMetadata:
     new token, as ``context_lens`` of qwen3.py:17-22), the rest prefill
     sequences (q rows ``cu_seqlens_q[b] .. cu_seqlens_q[b+1]``, kv length
     ``kv_lens[b]``, positions as qwen3.py:25-34).  ``max_seqlen_q`` bounds
-    every prefill q length."""
+    every prefill q length.  ``max_seqlen_k`` (read by ``latent_attention``
+    only) is what the host knows of the prefill sequences' longest kv length,
+    as in ``PrefillAttentionMetadata``."""
     input_positions: torch.Tensor
     slot_mapping: torch.Tensor
     block_tables: torch.Tensor
@@ -83,6 +85,7 @@ class MixedAttentionMetadata:
     kv_lens: torch.Tensor
     num_decodes: int
     max_seqlen_q: int
+    max_seqlen_k: Union[torch.Tensor, int, None] = None
 
 
 AttentionMetadata = Union[DecodeAttentionMetadata, PrefillAttentionMetadata, MixedAttentionMetadata]

@@ -465,7 +465,11 @@ using namespace pa;
 
 namespace {
 
-constexpr size_t kGroupBytes = (size_t)2 << 30;  // K and V rows expanded at a time
+constexpr size_t kGroupBytes = (size_t)2 << 30;  // K and V rows expanded at a time, one head's at least
+// A bound of the kv lengths that makes one head's rows longer than this is the
+// width of block tables rather than lengths (16.8 M tokens at Dn = 128 are 19 GB
+// of cache a layer): the form with the smaller workspace runs.
+constexpr size_t kHeadMost = (size_t)8 << 30;
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
@@ -498,17 +502,6 @@ int plan(const char* name, int32_t batch, int32_t num_tokens, int32_t max_q, int
   max_q = std::min(max_q, num_tokens);
   p.absorbed = absorbed_form(batch, num_tokens, max_q, total_kv, latent, rope, nope);
   p.cu = up256(4 * ((size_t)batch + 1));
-  if (p.absorbed) {
-    const char* why;
-    p.attn = latent_attn_workspace(batch, max_q, heads, latent, (int64_t)pages_per_seq * page_size, &why);
-    if (why) {
-      p.absorbed = false;  // sizes past the absorbed kernel's: the expanded form takes them
-    } else {
-      p.q_lat = up256((size_t)num_tokens * heads * latent * 2);
-      p.need = 2 * p.q_lat + p.attn;
-      return PA_OK;
-    }
-  }
   const size_t head = (size_t)total_kv * 2 * nope * 2;
   size_t g = head ? kGroupBytes / head : heads;
   if (g >= 8) g &= ~(size_t)7;
@@ -517,6 +510,14 @@ int plan(const char* name, int32_t batch, int32_t num_tokens, int32_t max_q, int
   p.k_rope = up256((size_t)total_kv * rope * 2);
   p.kv = up256(head * p.group);
   p.need = p.cu + p.k_rope + p.kv;
+  if (!p.absorbed && head <= kHeadMost) return PA_OK;
+  const char* why;
+  p.attn = latent_attn_workspace(batch, max_q, heads, latent, (int64_t)pages_per_seq * page_size, &why);
+  p.q_lat = up256((size_t)num_tokens * heads * latent * 2);
+  const size_t need = 2 * p.q_lat + p.attn;
+  if (!p.absorbed) p.absorbed = need < p.need;
+  if (why) p.absorbed = false;  // sizes past the absorbed kernel's: the expanded form takes them
+  if (p.absorbed) p.need = need;
   (void)name;
   return PA_OK;
 }

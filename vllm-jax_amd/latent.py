@@ -261,7 +261,8 @@ def latent_prefill_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_
     span, times the sequences.  Tight bounds keep the workspace
     (``latent_prefill_workspace_bytes``) small and choose the form:
     expanded K and V rows (bf16) for a group of heads at a time, or the absorbed
-    form where few new tokens stand behind long contexts.
+    form where few new tokens stand behind long contexts (or where one head's
+    rows would pass 8 GiB and the absorbed form's workspace is smaller).
     """
     tokens, dr, nb, bs, rows = _check_q(q_nope, q_rope, latent_cache, weights)
     w = weights
@@ -298,16 +299,16 @@ def latent_prefill_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_
 
 
 def _total_kv(batch, tokens, span, max_seqlen_k, total_kv_tokens, fresh) -> int:
-    """Bound of the kv lengths' sum, from what the host knows."""
+    """Bound of the kv lengths' sum, from what the host knows; the C entries' largest number where that is more."""
     if total_kv_tokens is not None:
         total = int(total_kv_tokens)
     elif fresh:
         total = tokens
     else:
         total = batch * min(span, span if max_seqlen_k is None else int(max_seqlen_k))
-    if total < 0 or total > 0x7fffffff:
-        raise ValueError(f"the kv lengths' sum is bounded by {total}: give total_kv_tokens (at most 2^31 - 1)")
-    return total
+    if total < 0:
+        raise ValueError(f"the kv lengths' sum is bounded by {total}")
+    return min(total, 0x7fffffff)
 
 
 def latent_prefill_workspace_bytes(batch: int, num_tokens: int, max_seqlen_q: int, total_kv_tokens: int,
@@ -321,13 +322,19 @@ def latent_prefill_workspace_bytes(batch: int, num_tokens: int, max_seqlen_q: in
 def latent_attention(latent_cache: torch.Tensor, q: torch.Tensor, latent: torch.Tensor, k_rope: torch.Tensor,
                      norm_weight: Optional[torch.Tensor], weights: LatentWeights, freqs: RotaryFrequencies,
                      metadata: AttentionMetadata, *, scale: float, eps: float = 1e-6,
-                     interleaved: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+                     interleaved: bool = True,
+                     total_kv_tokens: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """A layer's whole step between its projections, beside ``attention()``:
     the latent store with both rotations (:func:`latent_store`), then decode,
     prefill or a mixed step by ``metadata``, whose three types and fields are
     ``attention()``'s.  q is ``[T, H, Dn + Dr]`` (not rotated; not changed).
     Returns ``(latent_cache, out [T, H, Dv])``; rows outside the sequences are
     zero.
+
+    ``total_kv_tokens`` and the metadata's ``max_seqlen_k`` bound the kv lengths
+    of the step's prefill sequences, their sum and each, and have to hold (see
+    :func:`latent_prefill_attention`); a step that gives neither is planned for
+    the block tables' whole width.
     """
     if not isinstance(weights, LatentWeights):
         raise TypeError(f"weights must be LatentWeights, got {type(weights).__name__}")
@@ -342,10 +349,11 @@ def latent_attention(latent_cache: torch.Tensor, q: torch.Tensor, latent: torch.
         return latent_cache, latent_decode_attention(q_nope, q_rope, latent_cache, weights, m.block_tables,
                                                      m.context_lens, scale=scale)
     if isinstance(m, PrefillAttentionMetadata):
-        longest = _host_bound(m.max_seqlen_k) or None
         out = latent_prefill_attention(q_nope, q_rope, latent_cache, weights, m.block_tables, m.cu_seqlens_q,
                                        None if m.cu_seqlens_k is m.cu_seqlens_q else m.cu_seqlens_k,
-                                       max_seqlen_q=m.max_seqlen_bucket, max_seqlen_k=longest, scale=scale)
+                                       max_seqlen_q=m.max_seqlen_bucket, scale=scale,
+                                       max_seqlen_k=_host_bound(m.max_seqlen_k) or None,
+                                       total_kv_tokens=total_kv_tokens)
         return latent_cache, out
     if not isinstance(m, MixedAttentionMetadata):
         raise TypeError(f"metadata of type {type(m).__name__}")
@@ -357,7 +365,8 @@ def latent_attention(latent_cache: torch.Tensor, q: torch.Tensor, latent: torch.
     else:
         out = latent_prefill_attention(q_nope, q_rope, latent_cache, weights, m.block_tables[nd:],
                                        m.cu_seqlens_q[nd:], kv_lens=m.kv_lens[nd:], max_seqlen_q=m.max_seqlen_q,
-                                       scale=scale)
+                                       max_seqlen_k=_host_bound(m.max_seqlen_k) or None,
+                                       total_kv_tokens=total_kv_tokens, scale=scale)
     if nd:
         latent_decode_attention(q_nope[:nd], q_rope[:nd], latent_cache, weights, m.block_tables[:nd], m.kv_lens[:nd],
                                 scale=scale, out=out[:nd])
