@@ -299,16 +299,17 @@ def latent_prefill_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_
 
 
 def _total_kv(batch, tokens, span, max_seqlen_k, total_kv_tokens, fresh) -> int:
-    """Bound of the kv lengths' sum, from what the host knows; the C entries' largest number where that is more."""
+    """Bound of the kv lengths' sum, from what the host knows; where only widths are known, at most the C entries'
+    largest number."""
     if total_kv_tokens is not None:
         total = int(total_kv_tokens)
     elif fresh:
         total = tokens
     else:
-        total = batch * min(span, span if max_seqlen_k is None else int(max_seqlen_k))
-    if total < 0:
-        raise ValueError(f"the kv lengths' sum is bounded by {total}")
-    return min(total, 0x7fffffff)
+        total = min(batch * min(span, span if max_seqlen_k is None else int(max_seqlen_k)), 0x7fffffff)
+    if total < 0 or total > 0x7fffffff:
+        raise ValueError(f"the kv lengths' sum is bounded by {total} (0 to 2^31 - 1 can be given)")
+    return total
 
 
 def latent_prefill_workspace_bytes(batch: int, num_tokens: int, max_seqlen_q: int, total_kv_tokens: int,
