@@ -24,9 +24,10 @@
 // writes its rows, one that gets a part leaves O (float32), maximum and sum to
 // latent_merge_kernel.
 //
-// P is rounded to bf16 for the matrix cores; its reference may lag behind the
-// row's maximum (by 2^8 from tile to tile, 2^64 inside one), which costs range and
-// no bits.  Scores, maxima, sums, O and the parts are float32; the joined rows are
+// P is rounded to bf16 for the matrix cores, once: its reference is a whole number
+// of log2 units, so that bringing P or O from one to another multiplies by a power
+// of two.  It may lag behind the row's maximum (by 2^8 from tile to tile, 2^64
+// inside one), which costs range and no bits.  Scores, maxima, sums, O and the parts are float32; the joined rows are
 // rounded to bf16 once.
 //
 // Few heads are bound by the cache's reads: 256 sequences of 512-8 192 tokens by
@@ -460,7 +461,7 @@ latent_attn_kernel(AttnParams p) {
       // The reference of a half tile's P: the one the value waves ask for (the
       // maximum two tiles ago, where that passes O's reference by the slack) or
       // this wave's own last one; a half tile whose maximum passes that by kJump
-      // takes its maximum.  The value waves bring the halves together.
+      // takes its maximum, rounded up.  The value waves bring the halves together.
       float own_ref[D::kNr], l_sum[D::kNr];
 #pragma unroll
       for (int r = 0; r < D::kNr; ++r) {
@@ -558,7 +559,7 @@ latent_attn_kernel(AttnParams p) {
         for (int r = 0; r < D::kNr; ++r) {
           mx[r] *= p.scale_log2;  // positive
           const float base = t > t0 + 1 ? __builtin_fmaxf(own_ref[r], ask[r]) : own_ref[r];
-          const float ref = mx[r] > base + kJump ? mx[r] : base;
+          const float ref = mx[r] > base + kJump ? __builtin_ceilf(mx[r]) : base;
           corr[r] = fast_exp2(own_ref[r] - ref);
           own_ref[r] = ref;
         }
@@ -709,7 +710,8 @@ latent_attn_kernel(AttnParams p) {
           for (int rb = 0; rb < D::kRb; ++rb)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              const float f = fast_exp2((u ? a1[rb] : a0[rb]) - m_ref[rb]);
+              // a power of two: bf16 values times it are exact
+              const float f = __builtin_amdgcn_ldexpf(1.f, (int)fmaxf((u ? a1[rb] : a0[rb]) - m_ref[rb], -256.f));
               u32x4 w = as_u32x4(pt[rb][u]);
 #pragma unroll
               for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(bf16_lo(w[e]) * f, bf16_hi(w[e]) * f);
@@ -731,7 +733,7 @@ latent_attn_kernel(AttnParams p) {
           for (int rb = 0; rb < D::kRb; ++rb) {
             const float mx = __builtin_fmaxf(m0[rb], m1[rb]);
             *reinterpret_cast<float*>(smem + D::kAskOff + (t & 1) * (ROWS * 4) + (32 * rb + n) * 4) =
-                mx > m_ref[rb] + kSlack ? mx : m_ref[rb];
+                mx > m_ref[rb] + kSlack ? __builtin_ceilf(mx) : m_ref[rb];
           }
         }
         landed<D::kVDma>(t + 2 < t1);
