@@ -91,7 +91,8 @@ int pa_latent_decode(const uint16_t* q_nope, int64_t qn_tok_stride, int64_t qn_h
  * computed) over lk cached ones, itself among them, given by cu_seqlens_k or by
  * kv_lens (one of the two); row i sees the first lk - lq + i + 1.  A row that sees none is
  * zero; rows outside the sequences are zeroed with zero_rest, else left alone.
- * total_kv bounds the sum of the kv lengths and has to hold (rows past it may be left out).
+ * total_kv bounds the sum of the kv lengths (of cu_seqlens_k as it stands, or batch
+ * times the block table's span) and has to hold (rows past it may be left out).
  *
  * pa_latent_prefill_route says which form a launch takes: K and V expanded for
  * a group of heads at a time, or the absorbed form of pa_latent_decode for few

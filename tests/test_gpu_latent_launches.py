@@ -51,3 +51,29 @@ def test_absorbed_more_units_than_one_grid_holds(pkg, dev):
         for h in (0, 63, heads - 1):
             o, s = ref.attend(q[:, h, :dn], q[:, h, dn:], c["rows"][b], w[h, 0], w[h, 1], range(1, 21), scale, "absorbed")
             ref.check(out[20 * i:20 * i + 20, h], o, s, f"sequence {b} head {h}")
+
+
+@pytest.mark.parametrize("lengths", ["cu_k", "lens"])
+@pytest.mark.parametrize("heads,seqs,want", [
+    (3, [(90, 150), (96, 96), (80, 300), (90, 96), (95, 97), (0, 200), (96, 96)], "expanded"),
+    (16, [(3, 150), (2, 50), (1, 300), (4, 96)], "absorbed")])
+def test_prefill_lengths_past_the_tables(pkg, dev, heads, seqs, want, lengths):
+    """A kv length past its table row's span is clamped to it, and takes nothing from the sequences behind."""
+    r, dr, dn, page, span = 512, 64, 128, 16, 96
+    c = make(dev, seqs, heads, r, dr, dn, page, seed=12)
+    c["table"] = c["table"][:, :span // page]
+    code = pkg._lib.load().pa_latent_prefill_route(len(seqs), c["q"].shape[0], max(n for n, _ in seqs), len(seqs) * span,
+                                                   span // page, page, heads, r, dr, dn)
+    assert ["expanded", "absorbed"][code] == want
+    scale = (dn + dr) ** -0.5
+    out = run(pkg, c, heads, dn, scale, lengths=lengths, total_kv_tokens=None)
+    w = c["w"].view(heads, 2, dn, r)
+    at = 0
+    for b, (n, t) in enumerate(seqs):
+        t = min(t, span)
+        for h in (0, heads - 1) if n else ():
+            q = c["q"][at:at + n, h]
+            o, s = ref.attend(q[:, :dn], q[:, dn:], c["rows"][b][:t], w[h, 0], w[h, 1],
+                              [t - n + i + 1 for i in range(n)], scale, want)
+            ref.check(out[at:at + n, h], o, s, f"sequence {b} head {h}")
+        at += n

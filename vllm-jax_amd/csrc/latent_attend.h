@@ -63,6 +63,13 @@ int latent_attn_launch(const char* name, const LatentAttn& a, int latent, int ro
 // sequences, laid end to end by cu_k, become K and V rows of `heads` heads from
 // `head0` on: kv [heads][cap][nope + v], and (k_rope not null) the rotary parts
 // k_rope [cap][rope].  Tokens from cap on are dropped.
+//
+// First row of sequence b among them.  cu_k may hold lengths past the span of a
+// block-table row, which are clamped to it: rows start where the lengths before
+// would end, but no later than b spans (the clamped lengths still fit between).
+__device__ __forceinline__ int64_t flat_start(const int32_t* cu_k, int b, int64_t span) {
+  return min((int64_t)cu_k[b] - cu_k[0], (int64_t)b * span);
+}
 struct LatentExpand {
   LatentPool pool;
   const int32_t* cu_k;

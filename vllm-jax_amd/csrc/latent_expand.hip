@@ -35,15 +35,14 @@ constexpr int kXStages = 4;
 
 // Cache row of flat token t (of the sequences laid end to end by cu_k).
 __device__ __forceinline__ const uint16_t* flat_row(const LatentExpand& p, int t) {
-  int lo = 0, hi = p.batch;  // last b with cu_k[b] - cu_k[0] <= t
-  const int base = p.cu_k[0];
+  const int64_t span = (int64_t)p.pool.pages_per_seq * p.pool.page.d;
+  int lo = 0, hi = p.batch;  // last b whose rows start at t or before
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (p.cu_k[mid] - base <= t) lo = mid;
+    if (flat_start(p.cu_k, mid, span) <= t) lo = mid;
     else hi = mid;
   }
-  const int64_t span = (int64_t)p.pool.pages_per_seq * p.pool.page.d;
-  const int j = (int)max((int64_t)0, min((int64_t)t - (p.cu_k[lo] - base), span - 1));
+  const int j = (int)max((int64_t)0, min(t - flat_start(p.cu_k, lo, span), span - 1));
   const int pg = (int)div_by((uint32_t)j, p.pool.page);
   const int page = safe_page(p.pool.tables + lo * p.pool.bt_stride, pg, p.pool.num_pages);
   return p.pool.cache + page * p.pool.page_stride + (int64_t)(j - pg * (int)p.pool.page.d) * p.pool.slot_stride;
@@ -61,7 +60,8 @@ latent_expand_kernel(LatentExpand p, int rope, int n, int blocks, int share, int
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // workgroups that run together work on all tokens and few weight rows
   const int part = blockIdx.x / tiles, t0 = (blockIdx.x - part * tiles) * kXTokens;
-  const int total = min(p.cap, p.cu_k[p.batch] - p.cu_k[0]);
+  const int64_t end = flat_start(p.cu_k, p.batch, (int64_t)p.pool.pages_per_seq * p.pool.page.d);
+  const int total = (int)max((int64_t)0, min((int64_t)p.cap, end));
   if (t0 >= total) return;
   const int first = part * share, last = min(blocks, first + share);
   const int l = lane & 31, h = lane >> 5;

@@ -127,9 +127,9 @@ latent_ragged_kernel(RaggedParams prm) {
   const int lq_all = p.cu_q[b + 1] - q0;
   const int lq = q0 < 0 || q0 >= p.num_tokens ? 0 : min(min(lq_all, p.max_q), p.num_tokens - q0);
   if (qt * kRRows >= lq) return;
-  const int kbase = p.cu_k[b] - p.cu_k[0];
+  const int64_t kbase = flat_start(p.cu_k, b, p.span);
   const int lk_all = max(0, min(p.cu_k[b + 1] - p.cu_k[b], p.span));
-  const int lk = kbase < 0 || kbase >= p.cap ? 0 : min(lk_all, p.cap - kbase);
+  const int lk = kbase < 0 || kbase >= p.cap ? 0 : min(lk_all, p.cap - (int)kbase);
   const int first = lk_all - lq_all;  // row i sees first + i + 1 keys
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -145,7 +145,7 @@ latent_ragged_kernel(RaggedParams prm) {
   const int n_free = min(lk, max(0, first + qt * kRRows + 1)) / kRTile;
 
   const uint16_t* kv = p.kv + ((int64_t)head * p.cap + kbase) * (2 * DN);
-  const uint16_t* kr = p.k_rope + (int64_t)kbase * DR;
+  const uint16_t* kr = p.k_rope + kbase * DR;
 
   // ---- tile loads: this wave's rows of a tile are 8 wave .. 8 wave + 7, each load
   // a scalar tile base and a lane offset kept in a register.  Piece i of kDma:
