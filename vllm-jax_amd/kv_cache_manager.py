@@ -132,20 +132,26 @@ class KVCacheManager:
 def copy_blocks(kv_cache, src: Sequence[int], dst: Sequence[int]) -> None:
     """Execute page copies ``kv_cache[:, dst[i]] <- kv_cache[:, src[i]]`` on
     the device (copy-on-write), in place; ``kv_cache`` is one layer's
-    ``[2, NB, BS, Hkv, d]`` bf16 pool."""
+    ``[2, NB, BS, Hkv, d]`` bf16 pool, or its pool of latent rows
+    ``[NB, BS, R + Dr]`` (``kv_cache[dst[i]] <- kv_cache[src[i]]``)."""
     import torch
 
     from .kernels._common import require_bf16, require_device, stream_handle
     require_device("kv_cache", kv_cache)
     require_bf16("kv_cache", kv_cache)
-    if kv_cache.dim() != 5 or kv_cache.shape[0] != 2:
-        raise ValueError(f"kv_cache must be [2, NB, BS, Hkv, d], got {tuple(kv_cache.shape)}")
+    if kv_cache.dim() == 3 and kv_cache.shape[2] > 0 and kv_cache.shape[2] % 16 == 0:
+        # latent rows: their halves are the two pools, of one head
+        half = kv_cache.shape[2] // 2
+        kc, vc = kv_cache[..., :half].unsqueeze(2), kv_cache[..., half:].unsqueeze(2)
+    elif kv_cache.dim() == 5 and kv_cache.shape[0] == 2:
+        kc, vc = kv_cache[0], kv_cache[1]
+    else:
+        raise ValueError(f"kv_cache must be [2, NB, BS, Hkv, d] or [NB, BS, R + Dr], got {tuple(kv_cache.shape)}")
     if len(src) != len(dst):
         raise ValueError("src and dst must have the same length")
     if len(src) == 0:
         return
-    _, nb, bs, hkv, d = kv_cache.shape
+    nb, bs, hkv, d = kc.shape
     idx = torch.as_tensor(np.stack([np.asarray(src, np.int32), np.asarray(dst, np.int32)]), device=kv_cache.device)
-    kc, vc = kv_cache[0], kv_cache[1]
     _lib.call("pa_copy_blocks", kc.data_ptr(), vc.data_ptr(), nb, bs, kc.stride(0), kc.stride(1), kc.stride(2),
               hkv, d, idx[0].data_ptr(), idx[1].data_ptr(), len(src), stream_handle(kv_cache))
