@@ -13,7 +13,8 @@
  * synchronisation, PA_* return codes).  Pools are [num_pages, page_size,
  * latent_dim + rope_dim] with caller-given page and slot strides; negative
  * block-table entries read page 0, entries past the pool are clamped into it,
- * kv lengths are clamped to the block table's span.  Supported: latent_dim 256
+ * kv lengths are clamped to the block table's span.  Cached rows below a kv
+ * length have to be finite.  Supported: latent_dim 256
  * or 512, rope_dim 32 or 64, nope_dim = v_dim = 64 or 128, any page size, any
  * number of heads; all operands 16-byte aligned with strides multiple of 8.
  */

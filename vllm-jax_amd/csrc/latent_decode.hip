@@ -31,12 +31,15 @@
 // rounded to bf16 once.
 //
 // Few heads are bound by the cache's reads: 256 sequences of 512-8 192 tokens by
-// 16 heads (1.28 GB) 220 us, 5.8 TB/s, of a call of 248.  At 64 rows a tile's step
-// is bound by LDS: 64 sequences by 128 heads 106 us, 760 TFLOP/s, of a call of
-// 142, at 1.1 us a tile of which the matrix instructions of a SIMD are a half
-// (the tile is read twice for the scores, once for the values and written once,
-// beside P), and 15 us around them, much of it the parts' 50 MB.  One sequence of
-// 32 k tokens by 64 heads: 20 us, and 5 us joining 128 parts.
+// 16 heads (1.28 GB) 220 us, 5.8 TB/s, of a call of 246.  At 64 rows nothing is
+// full: 64 sequences by 128 heads 108 us, 740 TFLOP/s, of a call of 139, at 1.1 us
+// a tile; over next turns of eight conversations (350 us) the counters have the
+// matrix cores busy for 41 % of the time, LDS for 34 % (a third of that bank
+// conflicts) and a wave waiting for 32 % of its own, most likely in the chain
+// through the one barrier a tile: the scores' products, their exponentials, the
+// values' products.  15 us of the 108 are around the loop, much of it the parts'
+// 50 MB.  One sequence of 32 k tokens by 64 heads: 21 us, and 5 us joining 128
+// parts.
 #include <algorithm>
 #include <cmath>
 
@@ -60,9 +63,9 @@ constexpr int kDirect = 6, kDirectMany = 16;  // tiles of a sequence up to which
 constexpr float kNoMax = -1e30f;
 
 // Tiles that a workgroup takes at least of `total`: more workgroups each do
-// less and leave more to join.  64 heads, one sequence of 32, 64, 128, 1 024
-// tiles, whole calls: 22.9, 24.2, 26.5 us with 2 (and 4 for the longest: 36.8),
-// 24.7, 25.4, 26.4, 36.8 with 4, 28.2, 29.2, 29.5, 35.3 with 8.
+// less and leave more to join.  64 heads, one sequence of 32, 64, 128, 256, 512,
+// 1 024 tiles, whole calls: 23.4, 24.2, 26.4, 29.8, 34.4, 36.4 us with 2, 25.0,
+// 25.5, 26.6, 28.3, 31.0, 36.3 with 4, 28.7, 29.9, 30.0, 30.7, 32.0, 34.9 with 8.
 __host__ __device__ inline int min_share(int64_t total) { return total <= 64 ? 2 : total <= 384 ? 4 : 8; }
 
 struct AttnParams {
@@ -147,9 +150,9 @@ __device__ __forceinline__ uint32_t fresh_addr(uint32_t x) {
 // by row (load_rows).
 //
 // kOnce (32 rows: one row tile a sequence, every cached row read by one
-// workgroup): loads that do not stay in the caches, 247 us against 267 for 256
-// sequences by 16 heads; at 64 rows they cost 168 against 158 (64 sequences by
-// 128 heads, two row tiles) and 35.5 against 32.8 (one of 32 k tokens, 64 heads).
+// workgroup): loads that do not stay in the caches, 239 us against 258 for 256
+// sequences by 16 heads; at 64 rows they cost 152 against 139 (64 sequences by
+// 128 heads, two row tiles) and 37.2 against 34.9 (one of 32 k tokens, 64 heads).
 template <typename D, int R, int DR, int kFirst, int kCount, bool kOnce>
 struct TileLoader {
   static constexpr int kC = D::kRopeB / 16;  // chunks of a rotary row
@@ -907,8 +910,8 @@ __global__ void __launch_bounds__(64 * kJoinWaves) latent_merge_kernel(AttnParam
 }
 
 // Rows of a workgroup: 64, or 32 where a sequence has no more (4 096 tokens each,
-// 256 sequences by 16 heads: 206 us against 236 with 64 rows, 64 by 32 heads 72
-// against 82).
+// 256 sequences by 16 heads: 203 us against 234 with 64 rows, 64 by 32 heads 78
+// against 91).
 int rows_of(int max_q, int heads) { return (int64_t)max_q * heads <= 32 ? 32 : 64; }
 
 // Workgroups of a cut launch of at most `most_tiles`: as many as min_share
@@ -973,18 +976,19 @@ int latent_attn_launch(const char* name, const LatentAttn& a, int latent, int ro
   p.wgs = wgs_of(units * ((span + kTile - 1) / kTile));
   p.row_tiles = units <= p.wgs ? (int)row_tiles : 0;
   // Short block tables take a workgroup a unit, without the cut's scan and the
-  // merge's launch.  16 heads, whole calls: 4 sequences of 4 tiles 18.3 us against
-  // 28.6, of 8 tiles 22.8 against 20.3 cut; 64 sequences of 8 tiles 26.6 against
-  // 30.1, of 16 tiles 33.1 against 35.7.
+  // merge's launch.  16 heads, whole calls: 4 sequences of 4 tiles 18.9 us against
+  // 20.1, of 8 tiles 22.5 against 20.5 cut; 64 sequences of 8 tiles 26.6 against
+  // 30.6, of 16 tiles 33.1 against 35.7, of 24 tiles 39.6 against 37.9.
   const int64_t tiles = (span + kTile - 1) / kTile;
   // (a grid has fewer than 2^32 threads along x)
   p.unit_tiles = tiles <= (units < 64 ? kDirect : kDirectMany) && units * kLThreads <= 0xffffffffll ? (int)row_tiles : 0;
   if (p.unit_tiles > 0) p.wgs = (int)units;
   // The start and end of a unit (Q, the first tiles, O) take about as long as
   // kLead tiles; counted as such, a workgroup that gets several short pieces
-  // gets fewer tiles: 64 sequences of 512-8 192 tokens by 128 heads 157.5 us with
-  // 0, 147.5, 141.8, 140.8 with 4, 7, 10; 256 by 16 heads 247.8, 244.7, 245.8,
-  // 246.6.  Where a workgroup has few tiles anyway they are dealt as they are.
+  // gets fewer tiles: 64 sequences of 512-8 192 tokens by 128 heads 157.7 us with
+  // 0, 143.8, 138.7, 138.0 with 4, 7, 10; by 32 heads 89.2, 84.8, 78.6, 78.2; 256
+  // by 16 heads 247.0, 240.3, 239.5, 242.7.  Where a workgroup has few tiles anyway
+  // they are dealt as they are.
   p.lead = p.unit_tiles == 0 && units * tiles >= 16 * kWgs ? kLead : 0;
   p.joins = nullptr;
   p.parts = p.stats = nullptr;

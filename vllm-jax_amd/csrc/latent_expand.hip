@@ -8,14 +8,14 @@
 // once through the block tables, and streams its share of the weight rows
 // through a four-stage LDS ring, 32 rows a step: v_mfma_f32_32x32x16_bf16 with A
 // = weight rows (16-byte LDS reads, shared by the eight waves) and B = token
-// rows.  Token rows are read once per share, weights once per 256 tokens; the
-// LDS reads of the weights (32 KiB per wave and step) are as long as the
-// products.  Results go out through a wave's own 2 KiB of LDS, 64 bytes of a
+// rows.  Token rows are read once per share, weights once per 256 tokens
+// (32 KiB of LDS reads per wave and step).  Results go out through a wave's own 2 KiB of LDS, 64 bytes of a
 // token at a time.
 //
-// 24 k tokens by 64 heads (R = 512, Dn = 128): 0.55 ms, 750 TFLOP/s, of the
-// 8.4 ms that the call takes; both operands through LDS 64 deep at a time took
-// 0.85.  1 000 to 2 000 tokens by 16 heads: 18 to 22 us, most of them the
+// 24 k tokens by 64 heads (R = 512, Dn = 128): 0.49 to 0.55 ms, 750 to 840
+// TFLOP/s, of the 8.5 ms that the call takes, the matrix cores busy for 56 % of
+// the time at 1.75 GHz, LDS for 37 %; both operands through LDS 64 deep at a time
+// took 0.85.  1 000 to 2 000 tokens by 16 heads: 18 to 22 us, most of them the
 // gather's chain (sequence, page, row) and its 16-byte reads of 32 rows at a
 // time.  K and V are rounded to bf16 here, as a cache of K and V rows per head
 // would hold them.

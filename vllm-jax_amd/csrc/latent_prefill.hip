@@ -25,10 +25,10 @@
 // rounded to bf16 for the matrix cores (2^8 at most, so far from its range's
 // ends); its sum, the statistics and O are float32.
 //
-// Bound by LDS reads and the power limit: a product segment is 40 matrix
-// instructions (1 280 clocks) in about 1 540, beside 40 KiB of LDS reads a wave.
-// Two documents of 8-16 k tokens by 64 heads: 7.9 ms, 1 160 TFLOP/s, where a
-// large library product reaches 1 230.
+// Bound by the power limit: two documents of 8-16 k tokens by 64 heads take 7.8 to
+// 8.1 ms, 1 170 to 1 210 TFLOP/s issued, where a large library product reaches
+// 1 230, with the matrix cores busy for 74 % of the time at 1.5 GHz and LDS reads
+// for 37 %, without bank conflicts.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -484,9 +484,12 @@ struct PrefillPlan {
 // Which form runs, by the operations of both with sequences of equal length:
 // the absorbed form multiplies each (query, key) pair R + Dr and R wide, the
 // expanded one Dn + Dr and Dn wide but expands every cached token first.
-// Measured (8 sequences of 4 096 cached tokens, 32 heads, R = 512, Dn = 128;
-// the rule changes at 167 new tokens each): 16, 64, 128, 192, 256 new tokens
-// take 71, 183, 346, 513, 679 us absorbed and 417, 439, 452, 464, 481 expanded.
+// Measured, absorbed against expanded, in us by the new tokens of a sequence:
+// 8 sequences of 4 096 cached tokens by 32 heads (R = 512, Dn = 128; the rule
+// changes behind 167 new tokens): 64: 196 / 447, 128: 373 / 463, 192: 559 / 484,
+// 256: 751 / 495; 2 of 8 192 by 128 heads (168): 64: 341 / 820, 128: 682 / 851, 192:
+// 988 / 873, 256: 1 310 / 936; 16 of 2 048 by 16 heads (R = 256, Dn = 64; 83): 64:
+// 86 / 94, 128: 153 / 100.
 bool absorbed_form(int32_t batch, int32_t num_tokens, int32_t max_q, int32_t total_kv, int32_t latent, int32_t rope,
                    int32_t nope) {
   const double tokens = std::min((double)num_tokens, (double)batch * max_q);

@@ -5,8 +5,8 @@
 // v_mfma_f32_32x32x16_bf16: A = weight rows, B = token rows, both 16 bytes a
 // lane straight from memory (each weight is used once per wave, so LDS would
 // only add a hop).  With few tokens the weights' read bounds it, with many the
-// latent-wide rows': 128 heads by 64 tokens, 128 to 512 and back, take 9.7 and
-// 8.0 us (27 MB each, 2.8 and 3.4 TB/s), 16 heads by 256 tokens 5.5 and 6.3 us.
+// latent-wide rows': 128 heads by 64 tokens, 128 to 512 and back, take 9.8 and
+// 8.1 us (27 MB each, 2.8 and 3.3 TB/s), 16 heads by 256 tokens 5.8 and 6.0 us.
 //
 // Sums are float32.  Results are rounded to bf16 once: the next product, on the
 // matrix cores, takes bf16.  Of q_lat that moves a score by 2^-9 of its size
@@ -107,8 +107,8 @@ template <int kDepth, int kSplit>
 void launch(const HeadProduct& p, hipStream_t s) {
   const int n_groups = p.n / (kSplit == 1 ? 128 : 64);
   // 64 tokens a wave from 33 on: 33, 64 and 256 tokens by 128 heads, both
-  // products and the attention of two tiles between them: 29.0, 32.0, 81.8 us
-  // against 33.6, 35.3, 90.5 with 32; 16 tokens 26.8 against 25.5
+  // products and the attention of two tiles between them: 29.1, 31.9, 81.4 us
+  // against 33.8, 35.0, 90.0 with 32; 16 tokens 27.2 against 25.6
   const bool two = p.tokens > 32;
   const int m_blocks = (p.tokens + (two ? 63 : 31)) / (two ? 64 : 32);
   const dim3 g((unsigned)(n_groups * m_blocks), (unsigned)p.heads);

@@ -252,7 +252,8 @@ def latent_prefill_attention(q_nope: torch.Tensor, q_rope: torch.Tensor, latent_
     The kv lengths ``lk`` (cached rows, the new ones included; already stored) come as
     ``cu_seqlens_k`` (differences), as ``kv_lens`` ``[B]``, or, with neither,
     equal the new tokens'; row ``i`` of a sequence sees its first ``lk - lq +
-    i + 1`` rows, and is zero if that is none.  At most ``max_seqlen_q`` rows
+    i + 1`` rows, and is zero if that is none.  Cached rows below a length
+    have to be finite (those that a row does not see, too).  At most ``max_seqlen_q`` rows
     of a sequence are computed.  Rows outside the sequences are zero in a new output and
     left as they were in a given ``out``.
 
