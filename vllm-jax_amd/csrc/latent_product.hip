@@ -9,7 +9,7 @@
 // 8.1 us (27 MB each, 2.8 and 3.3 TB/s), 16 heads by 256 tokens 5.8 and 6.0 us.
 //
 // Sums are float32.  Results are rounded to bf16 once: the next product, on the
-// matrix cores, takes bf16.  Of q_lat that moves a score by 2^-9 of its size
+// matrix cores, takes bf16.  Of q_lat that moves a score by 2^-8 of its size at most
 // (both parts of a split q_lat would double the scores' products), of o_lat
 // the result by as much as its own rounding does.
 #include "latent_attend.h"
