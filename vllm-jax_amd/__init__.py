@@ -16,6 +16,9 @@ Public surface (mirrors simpissa/vllm-jax):
 * ``latent_attention`` with ``LatentWeights`` -- the layer seam for models
   whose cache holds one latent vector a token, over ``latent_store``,
   ``latent_decode_attention`` and ``latent_prefill_attention``;
+* ``block_sparse_attention`` -- the layer seam with decode over the blocks of
+  a long context that a cheap score selects, over ``update_block_bounds``,
+  ``block_scores``, ``select_blocks`` and ``block_sparse_decode_attention``;
 * ``KVCacheManager`` / ``copy_blocks`` -- the block manager of
   vllm/src/kv_cache_manager.py on a native allocator, with optional prefix
   caching and fork / copy-on-write.
@@ -32,6 +35,9 @@ module name ``vllm_jax_amd``::
 from .attention import (DecodeAttentionMetadata, MixedAttentionMetadata, PrefillAttentionMetadata,  # noqa: F401
                         attention, attention_stored, gather_kv, qk_norm_rope_store, qwen3_attention_core,
                         update_kv_cache, update_kv_cache_fp8)
+from .block_sparse import (block_scores, block_sparse_attention, block_sparse_decode_attention,  # noqa: F401
+                           block_sparse_workspace_bytes, copy_block_bounds, new_block_bounds, select_blocks,
+                           update_block_bounds)
 from .kernels.decode_paged_attention import decode_paged_attention  # noqa: F401
 from .kernels.mixed_paged_attention import mixed_paged_attention  # noqa: F401
 from .kernels.prefill_paged_attention import prefill_paged_attention  # noqa: F401

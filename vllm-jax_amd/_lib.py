@@ -209,6 +209,43 @@ SIGNATURES = {
         c_vp, c_i64, c_i64,            # out
         c_vp, c_sz, c_vp,              # workspace, bytes, stream
     ]),
+    # long contexts (include/long_context.h)
+    "pa_block_bounds": (ctypes.c_int, [
+        c_vp, c_i32, c_i32,            # k_cache, num_pages, page_size
+        c_i64, c_i64, c_i64,           # page/slot/head strides
+        c_vp, c_i64, c_i32,            # block_tables, bt_stride, pages_per_seq
+        c_vp, c_vp, c_i32, c_i32,      # lengths, cu_seqlens_q, batch, max_seqlen_q
+        c_i32, c_i32, c_i32,           # kv heads, head_dim, block
+        c_vp, c_i64, c_i64, c_i64,     # bounds, page/block/head strides
+        c_vp,                          # stream
+    ]),
+    "pa_block_scores": (ctypes.c_int, [
+        c_vp, c_i64, c_i64,            # q
+        c_vp, c_i32, c_i32,            # bounds, num_pages, page_size
+        c_i64, c_i64, c_i64,           # page/block/head strides
+        c_vp, c_i64, c_i32,            # block_tables, bt_stride, pages_per_seq
+        c_vp, c_i32, c_i32, c_i32,     # lengths, batch, heads, kv heads
+        c_i32, c_i32, c_f32,           # head_dim, block, scale
+        c_vp, c_i64, c_i64, c_vp,      # scores, strides, stream
+    ]),
+    "pa_select_blocks": (ctypes.c_int, [
+        c_vp, c_i64, c_i64, c_i32,     # scores, strides, width
+        c_vp, c_i32, c_i32, c_i32,     # lengths, batch, kv heads, block
+        c_i32, c_i32, c_i32,           # num_selected, first, recent
+        c_vp, c_i64, c_i64, c_vp,      # selected, strides, stream
+    ]),
+    "pa_block_sparse_decode_workspace_size": (c_sz, [c_i32] * 6),
+    "pa_block_sparse_decode": (ctypes.c_int, [
+        c_vp, c_i64, c_i64,            # q
+        c_vp, c_vp, c_i32, c_i32,      # caches, num_pages, page_size
+        c_i64, c_i64, c_i64,           # strides
+        c_vp, c_i64, c_i32,            # block_tables, bt_stride, pages_per_seq
+        c_vp, c_i32, c_i32, c_i32,     # lengths, batch, heads, kv heads
+        c_i32, c_vp, c_i64, c_i64,     # head_dim, selected, strides
+        c_i32, c_i32, c_f32, c_f32,    # num_selected, block, scale, soft_cap
+        c_vp, c_i64, c_i64,            # out
+        c_vp, c_sz, c_vp,              # workspace, bytes, stream
+    ]),
 }
 # pa_decode_quant / pa_prefill_quant: a code_type (PA_CODE_*) before the
 # arguments of pa_decode_fp8 / pa_prefill_fp8

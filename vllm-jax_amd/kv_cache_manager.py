@@ -134,9 +134,7 @@ def copy_blocks(kv_cache, src: Sequence[int], dst: Sequence[int]) -> None:
     the device (copy-on-write), in place; ``kv_cache`` is one layer's
     ``[2, NB, BS, Hkv, d]`` bf16 pool, or its pool of latent rows
     ``[NB, BS, R + Dr]`` (``kv_cache[dst[i]] <- kv_cache[src[i]]``)."""
-    import torch
-
-    from .kernels._common import require_bf16, require_device, stream_handle
+    from .kernels._common import require_bf16, require_device
     require_device("kv_cache", kv_cache)
     require_bf16("kv_cache", kv_cache)
     if kv_cache.dim() == 3 and kv_cache.shape[2] > 0 and kv_cache.shape[2] % 16 == 0:
@@ -147,11 +145,20 @@ def copy_blocks(kv_cache, src: Sequence[int], dst: Sequence[int]) -> None:
         kc, vc = kv_cache[0], kv_cache[1]
     else:
         raise ValueError(f"kv_cache must be [2, NB, BS, Hkv, d] or [NB, BS, R + Dr], got {tuple(kv_cache.shape)}")
+    copy_pages(kc, vc, src, dst)
+
+
+def copy_pages(kc, vc, src: Sequence[int], dst: Sequence[int]) -> None:
+    """``kc[dst[i]] <- kc[src[i]]`` and the same for ``vc``: two bf16 pools
+    ``[NB, slots, heads, d]`` on a device, of one shape and strides."""
+    import torch
+
+    from .kernels._common import stream_handle
     if len(src) != len(dst):
         raise ValueError("src and dst must have the same length")
     if len(src) == 0:
         return
     nb, bs, hkv, d = kc.shape
-    idx = torch.as_tensor(np.stack([np.asarray(src, np.int32), np.asarray(dst, np.int32)]), device=kv_cache.device)
+    idx = torch.as_tensor(np.stack([np.asarray(src, np.int32), np.asarray(dst, np.int32)]), device=kc.device)
     _lib.call("pa_copy_blocks", kc.data_ptr(), vc.data_ptr(), nb, bs, kc.stride(0), kc.stride(1), kc.stride(2),
-              hkv, d, idx[0].data_ptr(), idx[1].data_ptr(), len(src), stream_handle(kv_cache))
+              hkv, d, idx[0].data_ptr(), idx[1].data_ptr(), len(src), stream_handle(kc))
