@@ -93,6 +93,35 @@ int pa_block_sparse_decode(const uint16_t* q, int64_t q_batch_stride, int64_t q_
                            float soft_cap, uint16_t* out, int64_t out_batch_stride, int64_t out_head_stride,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Attention of new tokens whose sequences share prefixes in groups: group g is
+ * sequences cu_groups[g] .. cu_groups[g + 1] - 1, whose first shared_lens[g]
+ * tokens lie in the same pages.  Sequence b's new tokens are rows
+ * cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 of q and out (at most
+ * max_seqlen_q of them; cu_seqlens_q NULL: row b, one new token each); row i
+ * of n sees the first lengths[b] - n + i + 1 of the sequence's tokens, as in
+ * pa_decode and pa_prefill, and is zero if that is none.  The shared tokens are
+ * read once a group, through the block table of its first sequence that has
+ * tokens; shared_lens is rounded down to 64 tokens, cut to the group's shortest
+ * length (sequences without tokens aside), and taken for 0 in groups of fewer than
+ * two sequences.  Sequences outside all groups share nothing; cu_groups does not fall.
+ * Rows outside the sequences are zeroed with zero_rest and left as they were
+ * without.  head_dim 128, up to 256 q heads a kv head, any page size.  The
+ * workspace (256-byte aligned) is sized with ragged = (cu_seqlens_q != NULL).
+ */
+size_t pa_shared_prefix_workspace_size(int32_t batch, int32_t num_groups, int32_t num_tokens, int32_t max_seqlen_q,
+                                       int32_t ragged, int32_t num_heads, int32_t num_kv_heads,
+                                       int32_t pages_per_seq, int32_t page_size);
+int pa_shared_prefix(const uint16_t* q, int64_t q_tok_stride, int64_t q_head_stride, const uint16_t* k_cache,
+                     const uint16_t* v_cache, int32_t num_pages, int32_t page_size, int64_t page_stride,
+                     int64_t slot_stride, int64_t head_stride, const int32_t* block_tables, int64_t bt_stride,
+                     int32_t pages_per_seq, const int32_t* lengths, const int32_t* cu_groups,
+                     const int32_t* shared_lens, int32_t num_groups, const int32_t* cu_seqlens_q, int32_t batch,
+                     int32_t num_tokens, int32_t max_seqlen_q, int32_t num_heads, int32_t num_kv_heads,
+                     int32_t head_dim, float scale, float soft_cap, int32_t zero_rest, uint16_t* out,
+                     int64_t out_tok_stride, int64_t out_head_stride, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

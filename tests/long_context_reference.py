@@ -38,19 +38,45 @@ def rows(half, table, t0, t1):
     return half[page, t % half.shape[1]].double().transpose(0, 1)
 
 
-def attend(q, k, v, scale, cap=None, roundings=1):
+def attend(q, k, v, scale, cap=None, limit=None, scaled_q=False):
     """softmax(scale q k) v of q [n, d], k [t, d], v [t, d] in 64 bits, and the bound of a kernel's error: the weights
-    rounded to bf16 (``roundings`` times, counting q's scaling as one of the logits' own), the output once, logits from
-    32-bit sums."""
+    rounded to bf16 once, the output once, logits from 32-bit sums.  ``limit`` [n]: the tokens that each row sees
+    (none: a zero row).  ``scaled_q``: q times the scale is rounded to bf16 too, which moves a logit by at most half a
+    step of its terms' magnitudes."""
     x = scale * (q @ k.t())
     mag = scale * (q.abs() @ k.abs().t()).max().item() if k.shape[0] else 0.0
     if cap:
         x = cap * torch.tanh(x / cap)
-    p = torch.softmax(x, -1)
+    if limit is not None:
+        hidden = torch.arange(k.shape[0]) >= limit[:, None]
+        x = x.masked_fill(hidden, -math.inf)
+    p = torch.nan_to_num(torch.softmax(x, -1), nan=0.0)
     out = p @ v
     spread = p @ v.abs()
-    logit = 2 * (q.shape[1] + 8) * F32 * mag + (16 * F32 * cap if cap else 0.0)  # of a weight, relative, both ways
-    tol = (roundings * BF16 * 1.01 + logit + 32 * F32) * spread + BF16 * out.abs() * 1.02 + 1e-30
+    # relative, of a weight; twice: of the weight and of the sum
+    logit = 2 * ((q.shape[1] + 8) * F32 + (BF16 if scaled_q else 0.0)) * mag + (16 * F32 * cap if cap else 0.0)
+    tol = (BF16 * 1.01 + math.expm1(logit) + (32 + k.shape[0] / 16) * F32) * spread + BF16 * out.abs() * 1.02 + 1e-30
+    return out, tol
+
+
+def shared(q, cache, table, lengths, new, scale, cap=None, scaled_q=True):
+    """Attention of the last ``new[b]`` tokens of every sequence, rows in order."""
+    heads, kv = q.shape[1], cache.shape[3]
+    g = heads // kv
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    tol = torch.full(q.shape, 1e-30, dtype=torch.float64)
+    at = 0
+    for b, n in enumerate(new):
+        t = max(0, min(int(lengths[b]), table.shape[1] * cache.shape[2]))
+        if n and t:
+            safe = table[b].clamp(0, cache.shape[1] - 1)
+            k, v = (rows(cache[i], safe, 0, t) for i in (0, 1))
+            limit = torch.arange(t - n + 1, t + 1).clamp(min=0).repeat_interleave(g)
+            for j in range(kv):
+                x = q[at:at + n, j * g:(j + 1) * g].double().reshape(n * g, -1)
+                o, e = attend(x, k[j], v[j], scale, cap, limit, scaled_q)
+                out[at:at + n, j * g:(j + 1) * g], tol[at:at + n, j * g:(j + 1) * g] = (y.view(n, g, -1) for y in (o, e))
+        at += n
     return out, tol
 
 

@@ -19,6 +19,9 @@ Public surface (mirrors simpissa/vllm-jax):
 * ``block_sparse_attention`` -- the layer seam with decode over the blocks of
   a long context that a cheap score selects, over ``update_block_bounds``,
   ``block_scores``, ``select_blocks`` and ``block_sparse_decode_attention``;
+* ``shared_prefix_attention`` with ``SharedPrefixes`` -- attention of a batch
+  whose sequences share prefixes, each read once (``attention()`` takes it by
+  the metadata's ``shared``);
 * ``KVCacheManager`` / ``copy_blocks`` -- the block manager of
   vllm/src/kv_cache_manager.py on a native allocator, with optional prefix
   caching and fork / copy-on-write.
@@ -45,4 +48,5 @@ from .latent import (LatentWeights, latent_attention, latent_decode_attention,  
                      latent_decode_workspace_bytes, latent_prefill_attention, latent_prefill_workspace_bytes,
                      latent_store)
 from .rotary import RotaryFrequencies, rotary_embedding, rotary_frequencies  # noqa: F401
+from .shared_prefix import SharedPrefixes, shared_prefix_attention, shared_prefix_workspace_bytes  # noqa: F401
 from .kv_cache_manager import Block, KVCacheManager, copy_blocks  # noqa: F401

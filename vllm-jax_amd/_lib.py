@@ -246,6 +246,19 @@ SIGNATURES = {
         c_vp, c_i64, c_i64,            # out
         c_vp, c_sz, c_vp,              # workspace, bytes, stream
     ]),
+    "pa_shared_prefix_workspace_size": (c_sz, [c_i32] * 9),
+    "pa_shared_prefix": (ctypes.c_int, [
+        c_vp, c_i64, c_i64,            # q
+        c_vp, c_vp, c_i32, c_i32,      # caches, num_pages, page_size
+        c_i64, c_i64, c_i64,           # strides
+        c_vp, c_i64, c_i32,            # block_tables, bt_stride, pages_per_seq
+        c_vp, c_vp, c_vp, c_i32,       # lengths, cu_groups, shared_lens, groups
+        c_vp, c_i32, c_i32, c_i32,     # cu_seqlens_q, batch, num_tokens, max_seqlen_q
+        c_i32, c_i32, c_i32,           # heads, kv heads, head_dim
+        c_f32, c_f32, c_i32,           # scale, soft_cap, zero_rest
+        c_vp, c_i64, c_i64,            # out
+        c_vp, c_sz, c_vp,              # workspace, bytes, stream
+    ]),
 }
 # pa_decode_quant / pa_prefill_quant: a code_type (PA_CODE_*) before the
 # arguments of pa_decode_fp8 / pa_prefill_fp8

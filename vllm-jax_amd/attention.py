@@ -29,10 +29,12 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib
-from .kernels._common import bf16_round, pool_pointers, require_bf16, require_device, stream_handle
+from .kernels._common import (bf16_round, inv_sqrt_head_dim_bf16, pool_pointers, require_bf16, require_device,
+                              stream_handle)
 from .kernels.decode_paged_attention import decode_paged_attention, decode_pool
 from .kernels.mixed_paged_attention import mixed_paged_attention
 from .kernels.prefill_paged_attention import prefill_paged_attention, prefill_pool
+from .shared_prefix import SharedPrefixes, shared_prefix_attention
 
 USE_DECODE_PAGED_ATTENTION_KERNEL = True
 USE_PREFILL_PAGED_ATTENTION_KERNEL = True
@@ -40,11 +42,13 @@ USE_PREFILL_PAGED_ATTENTION_KERNEL = True
 
 @dataclass
 class DecodeAttentionMetadata:
-    """qwen3.py:17-22."""
+    """qwen3.py:17-22.  ``shared``: the groups of sequences that share their
+    first pages, each shared page then read once (no reference counterpart)."""
     input_positions: torch.Tensor
     slot_mapping: torch.Tensor
     block_tables: torch.Tensor
     context_lens: torch.Tensor
+    shared: Optional[SharedPrefixes] = None
 
 
 @dataclass
@@ -57,7 +61,8 @@ class PrefillAttentionMetadata:
     by the width); anything else, such as a device tensor, which is not read,
     says that it is not known, ``None`` that the table is as wide as the
     longest.  Where nothing is cached, ``cu_seqlens_k`` may be
-    ``cu_seqlens_q`` itself: the new tokens then bound the kv lengths."""
+    ``cu_seqlens_q`` itself: the new tokens then bound the kv lengths.
+    ``shared`` as in ``DecodeAttentionMetadata``."""
     input_positions: torch.Tensor
     slot_mapping: torch.Tensor
     block_tables: torch.Tensor
@@ -66,6 +71,7 @@ class PrefillAttentionMetadata:
     max_seqlen_q: torch.Tensor
     max_seqlen_k: Union[torch.Tensor, int, None]
     max_seqlen_bucket: int = field(default=0)
+    shared: Optional[SharedPrefixes] = None
 
 
 @dataclass
@@ -293,6 +299,10 @@ def attention_stored(kv_cache: torch.Tensor, q: torch.Tensor, metadata: Attentio
     # the engine's pool goes in as it is; anything else that has a K and a V
     # half goes in as page views
     pool = isinstance(kv_cache, torch.Tensor) and kv_cache.dim() == 5 and kv_cache.shape[0] >= 2
+    if getattr(metadata, "shared", None) is not None:
+        if not pool:
+            raise ValueError("shared prefixes need the pool [2, NB, BS, Hkv, d]")
+        return _attention_shared(kv_cache, q, metadata)
     if isinstance(metadata, MixedAttentionMetadata) or not pool:
         k_pages = kv_cache[0].permute(2, 0, 1, 3)   # [Hkv, NB, BS, d] view
         v_pages = kv_cache[1].permute(2, 0, 1, 3)
@@ -318,6 +328,18 @@ def attention_stored(kv_cache: torch.Tensor, q: torch.Tensor, metadata: Attentio
             outputs = decode_paged_attention(q, k_pages, v_pages, metadata.block_tables, metadata.context_lens,
                                              scale=scale)
     return outputs
+
+
+def _attention_shared(kv_cache: torch.Tensor, q: torch.Tensor, metadata) -> torch.Tensor:
+    """``attention_stored`` of a decode or prefill step whose sequences share prefixes; same scales."""
+    head_dim = q.shape[-1]
+    if isinstance(metadata, DecodeAttentionMetadata):
+        return shared_prefix_attention(q, kv_cache, metadata.block_tables, metadata.context_lens, metadata.shared,
+                                       scale=1.0 / bf16_round(float(head_dim) ** 0.5))
+    cu_k = metadata.cu_seqlens_k
+    return shared_prefix_attention(q, kv_cache, metadata.block_tables, cu_k[1:] - cu_k[:-1], metadata.shared,
+                                   metadata.cu_seqlens_q, max_seqlen_q=metadata.max_seqlen_bucket,
+                                   scale=inv_sqrt_head_dim_bf16(head_dim))
 
 
 def gather_kv(cache: torch.Tensor, block_tables: torch.Tensor, lengths: torch.Tensor) -> torch.Tensor:

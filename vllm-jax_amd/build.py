@@ -29,7 +29,7 @@ ARCH = "gfx950"
 SOURCES = ["pa_errors.cpp", "block_manager.cpp", "kv_store.hip", "decode.hip", "prefill.hip", "prefill_heads.hip",
            "prefill_split.hip", "qk_norm_rope.hip", "mixed.hip", "any_head.hip", "rotary.hip", "latent_store.hip",
            "latent_product.hip", "latent_decode.hip", "latent_expand.hip", "latent_prefill.hip",
-           "block_select.hip", "block_sparse.hip"]
+           "block_select.hip", "block_sparse.hip", "shared_prefix.hip"]
 PHASES_SOURCES = ["pa_errors.cpp", "prefill.hip", "any_head.hip"]  # any_head: the head-size check of the quantized entries
 
 # Packed-FP32 VALU forms are disabled for every device compile: the build

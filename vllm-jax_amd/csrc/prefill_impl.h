@@ -351,12 +351,13 @@ __device__ __forceinline__ bool prefill_resolve(const PrefillParams& p, int bid,
 struct PrefillPart {
   int lo, hi, slot;
 };
-// A partial's O: 16 bytes (four d) per lane and (32-row block, chunk), as the
-// accumulators hold them; then (reference max, row sum) of its 256 rows.
+// A partial is one unit a wave (32 rows), from unit `slot` on: its O, 16 bytes
+// (four d) per lane and chunk, as the accumulators hold them; then (reference
+// max, row sum) of its rows.  Waves without a row write nothing.
 template <int D>
-constexpr int kPartO = kRows * ((D + 31) / 32 * 32);  // floats
+constexpr int kPartO = 32 * ((D + 31) / 32 * 32);  // floats
 template <int D>
-constexpr int kPartFloats = kPartO<D> + 2 * kRows;
+constexpr int kPartFloats = kPartO<D> + 2 * 32;
 
 // One prefill work item (kSplit: one part of it), run by a whole 512-thread
 // workgroup.
@@ -948,18 +949,19 @@ __device__ __forceinline__ void prefill_run(const PrefillParams& p, const Prefil
                               : sum_xor32(l_part[0] + l_part[1]);
   if constexpr (kSplit) {
     if (part.slot >= 0) {  // uniform over the workgroup
-      float* dst = p.parts + (int64_t)part.slot * kPartFloats<D>;
+      if (!wave_live) return;
+      float* dst = p.parts + (int64_t)(part.slot + wave) * kPartFloats<D>;
 #pragma unroll
       for (int dt = 0; dt < A::kDt; ++dt)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
           const f32x16& a = acc_o[dt];
-          *reinterpret_cast<f32x4*>(dst + 4 * (((wave * A::kDt + dt) * 4 + q4) * 64 + lane)) =
+          *reinterpret_cast<f32x4*>(dst + 4 * ((dt * 4 + q4) * 64 + lane)) =
               f32x4{a[4 * q4], a[4 * q4 + 1], a[4 * q4 + 2], a[4 * q4 + 3]};
         }
       // a row that saw no key here carries no weight, whatever its reference
       if (h == 0)
-        *reinterpret_cast<f32x2*>(dst + kPartO<D> + 2 * row) = f32x2{l_run > 0.f ? m_ref : -INFINITY, l_run};
+        *reinterpret_cast<f32x2*>(dst + kPartO<D> + 2 * n) = f32x2{l_run > 0.f ? m_ref : -INFINITY, l_run};
       return;
     }
   }

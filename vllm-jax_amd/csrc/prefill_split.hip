@@ -187,7 +187,7 @@ prefill_split_kernel(PrefillParams p, int grid_parts) {
   part.lo = work(6);
   part.hi = work(7);
   part.slot = work(8);
-  if (part.slot >= 0) part.slot += w.kvh;
+  if (part.slot >= 0) part.slot = (part.slot + w.kvh) * kWaves;
   prefill_run<kSoftCap, kPaging, kPHeadDim, true>(p, w, part);
 }
 
@@ -205,15 +205,15 @@ prefill_split_merge_kernel(PrefillParams p) {
   if (rank >= p.split[0]) return;
   const int4 rec = *reinterpret_cast<const int4*>(p.split + 4 * (1 + rank));  // parts and q tile, first slot, q0, rows
   const int parts = rec.x & 0xffff;
-  const float* src = p.parts + (int64_t)(rec.y + kvh) * kPartFloats<kPHeadDim>;
-  const int64_t step = (int64_t)hkv * kPartFloats<kPHeadDim>;
+  const float* src = p.parts + ((int64_t)(rec.y + kvh) * kWaves + block) * kPartFloats<kPHeadDim>;
+  const int64_t step = (int64_t)hkv * kWaves * kPartFloats<kPHeadDim>;
   const int lane = threadIdx.x & 63;
   const int dt = threadIdx.x >> 6;
   const int n = lane & 31, h = lane >> 5;
   const int row = 32 * block + n;
   const int rtok = (rec.x >> 16) * p.tile_tokens + row / p.group;
-  const float* ml = src + kPartO<kPHeadDim> + 2 * row;
-  const float* po = src + 4 * ((block * 4 + dt) * 4 * 64 + lane);
+  const float* ml = src + kPartO<kPHeadDim> + 2 * n;
+  const float* po = src + 4 * (dt * 4 * 64 + lane);
   f32x4 o[4] = {};
   float m_run = -INFINITY, lsum = 0.f;
   // the sums follow a running max, so that no load waits for another part's
@@ -246,7 +246,7 @@ size_t prefill_split_bytes(int32_t batch, int32_t n_qtiles, int32_t num_kv_heads
   if (pairs <= 0 || pairs > kSplitMaxPairs || pairs * num_kv_heads > kSplitMaxGrid ||
       span < (int64_t)kSplitMinSpan * kTileN)
     return 0;
-  return kSplitHeader + (size_t)split_max_slots(pairs, num_kv_heads) * kPartFloats<kPHeadDim> * sizeof(float);
+  return kSplitHeader + (size_t)split_max_slots(pairs, num_kv_heads) * kWaves * kPartFloats<kPHeadDim> * sizeof(float);
 }
 
 // With N items, the longest of T tiles (N an upper bound, T a lower one), a

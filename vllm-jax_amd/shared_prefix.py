@@ -1,0 +1,117 @@
+"""Attention of a batch whose sequences share prefixes.
+
+Prefix caching lets sequences share the pages of a common prefix, and forks
+those of their parent, but decode and prefill still read a shared page once for
+every sequence.  :func:`shared_prefix_attention` takes the batch in groups of
+sequences that share their first pages: all rows of a group attend to the
+shared tokens together, as the rows of one matrix product over pages that are
+read once, each sequence to its own tokens behind them, and the two are added
+by their log-sum-exp.  The result is that of ``decode_paged_attention`` and
+``prefill_paged_attention`` up to rounding.
+
+The block manager finds the groups of a step (``KVCacheManager.shared_prefixes``);
+a step's metadata carries them to ``attention()`` (``shared=``).
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Sequence
+
+import torch
+
+from . import _lib
+from ._operands import check_heads, check_output, check_pool, check_table, check_workspace
+from .kernels._common import pool_pointers, stream_handle
+from .rotary import check_tokens, on_device
+
+
+@dataclass
+class SharedPrefixes:
+    """Groups of a batch's sequences: group ``g`` is sequences ``cu_groups[g] ..
+    cu_groups[g + 1] - 1``, and their first ``shared_lens[g]`` tokens lie in the
+    same pages.  int32 ``[groups + 1]`` and ``[groups]`` on the device."""
+    cu_groups: torch.Tensor
+    shared_lens: torch.Tensor
+
+    @classmethod
+    def of(cls, cu_groups: Sequence[int], shared_lens: Sequence[int], device) -> "SharedPrefixes":
+        """From the numbers that ``KVCacheManager.shared_prefixes`` returns."""
+        return cls(torch.as_tensor(list(cu_groups), dtype=torch.int32, device=device),
+                   torch.as_tensor(list(shared_lens), dtype=torch.int32, device=device))
+
+
+def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor,
+                            lengths: torch.Tensor, prefixes: SharedPrefixes,
+                            cu_seqlens_q: Optional[torch.Tensor] = None, *, max_seqlen_q: int = 1, scale: float,
+                            attn_logits_soft_cap: Optional[float] = None,
+                            workspace: Optional[torch.Tensor] = None,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """New tokens of sequences that share prefixes in groups: q ``[T, H, 128]``
+    over the pool ``[2, NB, BS, Hkv, 128]``, whose rows for the new tokens are
+    stored, -> ``[T, H, 128]`` bf16.
+
+    Without ``cu_seqlens_q`` each sequence has one new token, row ``b`` of q
+    (a length of zero gives a zero row).  With it the rows of sequence ``b`` are
+    ``cu_seqlens_q[b] .. cu_seqlens_q[b + 1]``, at most ``max_seqlen_q`` of them
+    are computed, and row ``i`` of ``n`` sees the first ``lengths[b] - n + i + 1``
+    tokens (and is zero if that is none).  Rows outside the sequences are zero
+    in a new output and left as they were in a given ``out``.
+
+    ``prefixes.shared_lens`` is a promise about the block tables: it is rounded
+    down to 64 tokens and cut to the shortest length of its group (sequences
+    of no tokens aside), and the shared tokens are read through the table of the group's
+    first sequence that has tokens.  Groups do not overlap; sequences outside them
+    share nothing.  Cached rows below a length have to be finite.
+
+    Scores, softmax statistics and sums are 32-bit; the scaled q of the shared
+    part (and of several new tokens) and the weights are rounded to bf16 for the
+    matrix cores.  How the parts are cut follows the whole batch, and with it a
+    row's last bits.  The workspace (``shared_prefix_workspace_bytes``) is made
+    here if it is not given or too small.
+    """
+    (nb, bs, hkv, d), cache_stride = check_pool(kv_cache)
+    q_stride = check_heads(q, hkv, d)
+    if kv_cache.get_device() != q.get_device():
+        raise ValueError(f"kv_cache lives on {kv_cache.device}, q on {q.device}")
+    if not isinstance(prefixes, SharedPrefixes):
+        raise TypeError(f"prefixes must be SharedPrefixes, got {type(prefixes).__name__}")
+    tokens, heads, _ = q.shape
+    if cu_seqlens_q is None:
+        batch, cu, longest = tokens, None, 1
+    else:
+        if cu_seqlens_q.dim() != 1 or cu_seqlens_q.numel() < 1:
+            raise ValueError(f"cu_seqlens_q must be int32 [B + 1], got {tuple(cu_seqlens_q.shape)}")
+        batch, longest = cu_seqlens_q.numel() - 1, max_seqlen_q
+        cu = check_tokens("cu_seqlens_q", cu_seqlens_q, batch + 1, q)
+    if not 0 <= max_seqlen_q <= 0x7fffffff:
+        raise ValueError(f"max_seqlen_q {max_seqlen_q}")
+    table, _keep = check_table(block_tables, batch, q)
+    lens = check_tokens("lengths", lengths, batch, q)
+    groups = prefixes.shared_lens.numel()
+    cu_groups = check_tokens("cu_groups", prefixes.cu_groups, groups + 1, q)
+    shared = check_tokens("shared_lens", prefixes.shared_lens, groups, q)
+    zero_rest = out is None
+    out, out_stride = check_output(out, q)
+    if tokens == 0:
+        return out
+    if batch == 0 or longest == 0:
+        return out.zero_() if zero_rest else out
+    need = shared_prefix_workspace_bytes(batch, groups, tokens, heads, hkv, table[2], bs,
+                                         max_seqlen_q=None if cu is None else longest)
+    _ws, ws_args = check_workspace(workspace, need, q)
+    k, v = pool_pointers(kv_cache)
+    cap = 0.0 if attn_logits_soft_cap is None else float(attn_logits_soft_cap)
+    with on_device(q):
+        _lib.call("pa_shared_prefix", q.data_ptr(), q_stride[0], q_stride[1], k, v, nb, bs, *cache_stride, *table,
+                  lens.data_ptr(), cu_groups.data_ptr(), shared.data_ptr(), groups,
+                  None if cu is None else cu.data_ptr(), batch, tokens, longest, heads, hkv, d, float(scale), cap,
+                  int(zero_rest), out.data_ptr(), *out_stride, *ws_args, stream_handle(q))
+    return out
+
+
+def shared_prefix_workspace_bytes(batch: int, num_groups: int, num_tokens: int, num_heads: int, num_kv_heads: int,
+                                  pages_per_seq: int, page_size: int, *, max_seqlen_q: Optional[int] = None) -> int:
+    """Bytes of the workspace of a :func:`shared_prefix_attention` call; ``max_seqlen_q`` None: without cu_seqlens_q."""
+    return int(_lib.load().pa_shared_prefix_workspace_size(
+        batch, num_groups, num_tokens, 1 if max_seqlen_q is None else max_seqlen_q, int(max_seqlen_q is not None),
+        num_heads, num_kv_heads, pages_per_seq, page_size))
