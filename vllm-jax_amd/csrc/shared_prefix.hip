@@ -11,11 +11,11 @@
 // Launches:
 //   shared_plan_kernel    reads the lengths, cuts prefixes and own parts for the
 //                         chip and writes the lists of work
-//   shared_tile_kernel    prefill_run's loop over one part of a prefix (256 rows
-//                         against 64-token tiles), and, where sequences have
-//                         several new tokens, over their own part too
-//   shared_decode_kernel  decode_run over a sequence's own part, where each has
-//                         one new token
+//   shared_part_kernel    parts of prefixes (128 rows against 32-token tiles,
+//                         shared_tile.h), then of the sequences' own tokens: where
+//                         each has one new token by decode_run, else by row tiles
+//   shared_tile_kernel    both by prefill_run's loop (256 rows against 64-token
+//                         tiles), where sequences have many new tokens
 //   shared_merge_kernel   adds the parts up
 #include <algorithm>
 #include <type_traits>
@@ -24,22 +24,28 @@
 #include "decode_impl.h"
 #include "long_context.h"
 #include "prefill_impl.h"
+#include "shared_tile.h"
 
 namespace pa {
 namespace {
 
 constexpr int kShPlanThreads = 1024;
-constexpr int kShPlanWaves = kShPlanThreads / 64;
-constexpr int kShTileSlots = 256;    // tile workgroups resident at once (one a CU)
-constexpr int kShDecodeSlots = 512;  // decode workgroups resident at once (two a CU)
-constexpr int kShMinTiles = 8;       // shortest part of a tile item
-constexpr int kShMinChunk = 512;     // shortest part of a decode item, tokens
+constexpr int kShPlanMax = 2048;     // sequences (and groups) that the plan keeps in LDS
+constexpr int kShTileSlots = 256;    // workgroups resident at once: of shared_tile_kernel (one a CU)
+constexpr int kShPartSlots = 512;    // ... of shared_part_kernel (two a CU)
+constexpr int kShMinTiles = 8;       // shortest part of a row tile, in 64-token tiles
+constexpr int kShMinChunk = 512;     // shortest part of a sequence's own tokens, in tokens
+// Time of a 64-token step of a row tile and of a chunk in shared_part_kernel
+#ifndef PA_SH_TILE_COST
+#define PA_SH_TILE_COST 3
+#endif
+constexpr int kShTileCost = PA_SH_TILE_COST, kShChunkCost = 4;
 
-// One part of a (row range, q tile) pair; every kv head has it.
+// One part of a (row range, row tile) pair; every kv head has it.
 struct alignas(16) ShTile {
-  int32_t table, qt, q0, rows;    // block-table row, q tile, first token, tokens
-  int32_t lk, lo, hi, unit;       // kv length, kv tiles [lo, hi), first unit of kv head 0
-  int32_t step, pad[3];           // units a kv head
+  int32_t table, tile, q0, tokens;  // block-table row, row tile, first token, tokens
+  int32_t lk, lo, hi, unit;         // kv length, 64-token tiles [lo, hi), first unit of kv head 0
+  int32_t step, pad[3];             // units a kv head
 };
 // One part of a sequence's own tokens.
 struct alignas(16) ShChunk {
@@ -48,10 +54,7 @@ struct alignas(16) ShChunk {
 // Where the rows of a sequence find their parts.
 struct alignas(16) ShSeq {
   int32_t p_unit, p_parts, p_step, p_q0;  // prefix: first unit, parts, units a kv head, first token of the group
-  int32_t s_unit, s_parts, s_step, s_q0;  // own part likewise (decode: first slot)
-};
-struct alignas(16) ShGroup {
-  int32_t shared, table, q0, tokens;  // shared tokens (whole tiles), table row, first token, tokens
+  int32_t s_unit, s_parts, s_step, s_q0;  // own part likewise (chunks: first slot; s_step: no parts to add up)
 };
 constexpr int kShHeader = 64;  // ints: number of tile parts, of chunks
 
@@ -62,11 +65,13 @@ struct SharedParams {
   const int32_t* lengths;
   const int32_t* cu_groups;
   const int32_t* shared_lens;
-  int32_t batch, groups, num_tokens, num_kv_heads, group, tile_tokens, span, max_seqlen_q;
+  int32_t batch, groups, num_tokens, num_kv_heads, group, span, max_seqlen_q;
+  int32_t light;        // row tiles of 128 rows (shared_part_kernel), else of tile_tokens tokens in 256 rows
+  int32_t tile_tokens;
   int32_t chunk_cap, zero_rest;
   int32_t cap_tiles, cap_chunks, cap_units;  // what the workspace holds
   int32_t* header;
-  ShGroup* group_info;
+  int32_t* group_shared;  // [groups] and [batch], where the plan's LDS does not hold them
   ShSeq* seqs;
   ShTile* tiles;
   ShChunk* chunks;
@@ -74,7 +79,7 @@ struct SharedParams {
   int32_t* owner;      // [num_tokens] its sequence, or -1 (with cu_q)
 };
 
-// Sequence b: first token, new tokens, tokens in all.
+// Sequence b: first token, new tokens that are computed, tokens in all.
 __device__ __forceinline__ int3 sh_sequence(const SharedParams& p, int b) {
   const int len = clamp_len(p.lengths, b, p.span);
   if (!p.cu_q) return make_int3(b, len > 0 ? 1 : 0, len);
@@ -84,44 +89,47 @@ __device__ __forceinline__ int3 sh_sequence(const SharedParams& p, int b) {
   return make_int3(q0, max(n, 0), len);
 }
 
-// Exclusive scan over the workgroup of one number a thread; `total`: their sum.
-__device__ __forceinline__ int sh_scan(int v, int* s_wave, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int upto = (int)wave_scan((uint32_t)v);
-  __syncthreads();  // the last scan's sums have been read
-  if (lane == 63) s_wave[wave] = upto;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < kShPlanWaves; ++i) {
-    before += i < wave ? s_wave[i] : 0;
-    total += s_wave[i];
-  }
-  return before + upto - v;
+__host__ __device__ __forceinline__ int sh_ceil(int a, int b) { return (a + b - 1) / b; }
+// Row tiles of `tokens` tokens in a row, and the units (32 rows) of each.
+__device__ __forceinline__ int sh_row_tiles(const SharedParams& p, int tokens) {
+  return p.light ? sh_ceil(tokens * p.group, kLtRows) : sh_ceil(tokens, p.tile_tokens);
 }
-__device__ __forceinline__ long long sh_sum(long long v, long long* s_wave) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if (lane == 0) s_wave[wave] = v;
-  __syncthreads();
-  v = 0;
-#pragma unroll
-  for (int i = 0; i < kShPlanWaves; ++i) v += s_wave[i];
-  return v;
+__device__ __forceinline__ int sh_units(const SharedParams& p, int tokens, int n) {
+  const int most = p.light ? kLtWaves : kWaves;
+  return n > 1 ? most : min(most, sh_ceil(tokens * p.group, 32));
 }
+// 64-token tiles [0, n) that the part k of `parts` ends before.
+__device__ __forceinline__ int sh_cut(int n, int k, int parts) { return (int)((double)n * k / parts); }
 
-__device__ __forceinline__ int sh_ceil(int a, int b) { return (a + b - 1) / b; }
+// Sums and exclusive sums over the workgroup of three numbers a thread.
+struct Sh3 {
+  int a, b, c;
+};
+__device__ __forceinline__ Sh3 sh_scan(const Sh3& v, Sh3* s_wave, Sh3& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const Sh3 u = {(int)wave_scan((uint32_t)v.a), (int)wave_scan((uint32_t)v.b), (int)wave_scan((uint32_t)v.c)};
+  __syncthreads();  // the last scan's sums have been read
+  if (lane == 63) s_wave[wave] = u;
+  __syncthreads();
+  Sh3 before = {0, 0, 0};
+  total = {0, 0, 0};
+  for (int i = 0; i < waves; ++i) {
+    const Sh3 w = s_wave[i];
+    if (i < wave) before = {before.a + w.a, before.b + w.b, before.c + w.c};
+    total = {total.a + w.a, total.b + w.b, total.c + w.c};
+  }
+  return {before.a + u.a - v.a, before.b + u.b - v.b, before.c + u.c - v.c};
+}
 
 // Workgroup 0 plans; the others (with cu_q) map tokens to sequences and kv
-// positions, a token a thread.
+// positions, a token a thread.  kLds: sequences and groups fit the plan's LDS,
+// and are read from memory once.
+template <bool kLds>
 __global__ void __launch_bounds__(kShPlanThreads)
 shared_plan_kernel(SharedParams p) {
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, threads = blockDim.x;
   if (blockIdx.x > 0) {
-    const int t = (blockIdx.x - 1) * kShPlanThreads + tid;
+    const int t = (blockIdx.x - 1) * threads + tid;
     if (t >= p.num_tokens) return;
     int lo = 0, hi = p.batch;  // last b with cu_q[b] <= t
     while (hi - lo > 1) {
@@ -137,16 +145,44 @@ shared_plan_kernel(SharedParams p) {
     p.positions[t] = in ? s.z - (p.cu_q[lo + 1] - s.x) + i : -1;
     return;
   }
-  __shared__ int s_wave[kShPlanWaves];
-  __shared__ long long s_long[kShPlanWaves];
-  const int lane = tid & 63, wave = tid >> 6;
+  constexpr int kMax = kLds ? kShPlanMax : 1;
+  __shared__ int32_t s_len[kMax], s_q0[kMax], s_n[kMax];     // sequences
+  __shared__ int16_t s_of[kMax];                             // their group, or -1
+  __shared__ int32_t s_cu[kMax + 1], s_want[kMax];           // groups: cu_groups, then shared tokens
+  __shared__ int32_t s_table[kMax], s_gunit[kMax];           // first sequence with tokens, first unit
+  __shared__ Sh3 s_wave[kShPlanThreads / 64];
+  __shared__ unsigned long long s_total[3];
+  const int lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
   const int hkv = p.num_kv_heads;
-  // ---- groups: a wave each
-  for (int g = wave; g < p.groups; g += kShPlanWaves) {
-    const int g0 = max(0, p.cu_groups[g]), g1 = min(p.batch, p.cu_groups[g + 1]);
+  if (tid < 3) s_total[tid] = 0;
+  if constexpr (kLds) {
+    for (int b = tid; b < p.batch; b += threads) {
+      const int3 s = sh_sequence(p, b);
+      s_q0[b] = s.x;
+      s_n[b] = s.y;
+      s_len[b] = s.z;
+      s_of[b] = -1;
+    }
+    for (int g = tid; g <= p.groups; g += threads) s_cu[g] = p.cu_groups[g];
+    for (int g = tid; g < p.groups; g += threads) s_want[g] = p.shared_lens[g];
+  }
+  auto seq = [&](int b) { return kLds ? make_int3(s_q0[b], s_n[b], s_len[b]) : sh_sequence(p, b); };
+  auto cu_group = [&](int g) { return kLds ? s_cu[g] : p.cu_groups[g]; };
+  auto shared_of = [&](int g) { return kLds ? s_want[g] : p.group_shared[g]; };
+  // first token and tokens of a group
+  auto group_rows = [&](int g) {
+    const int g0 = max(0, cu_group(g)), g1 = min(p.batch, cu_group(g + 1));
+    return p.cu_q ? make_int2(p.cu_q[g0], p.cu_q[g1] - p.cu_q[g0]) : make_int2(g0, g1 - g0);
+  };
+  __syncthreads();
+  // ---- groups, a wave each: the shared tokens (whole 64-token tiles, no further
+  // than the shortest sequence)
+  for (int g = wave; g < p.groups; g += waves) {
+    const int g0 = max(0, cu_group(g)), g1 = min(p.batch, cu_group(g + 1));
     int active = 0, least = INT_MAX, first = INT_MAX;
     for (int b = g0 + lane; b < g1; b += 64) {
-      const int3 s = sh_sequence(p, b);
+      const int3 s = seq(b);
+      if constexpr (kLds) s_of[b] = (int16_t)g;
       if (s.y > 0 && s.z > 0) {
         ++active;
         least = min(least, s.z);
@@ -160,21 +196,24 @@ shared_plan_kernel(SharedParams p) {
       first = min(first, __shfl_xor(first, o));
     }
     if (lane == 0) {
-      ShGroup r = {0, 0, 0, 0};
+      int shared = 0;
       if (active > 1) {
-        r.table = first;
-        r.q0 = p.cu_q ? p.cu_q[g0] : g0;
-        r.tokens = (p.cu_q ? p.cu_q[g1] : g1) - r.q0;
-        // whole tiles, and no further than the shortest sequence
-        r.shared = min(p.shared_lens[g], least) & ~(kTileN - 1);
-        if (r.shared <= 0 || r.q0 < 0 || r.tokens <= 0 || r.tokens > p.num_tokens - r.q0) r = {0, 0, 0, 0};
+        const int2 r = group_rows(g);
+        if (r.x >= 0 && r.y > 0 && r.y <= p.num_tokens - r.x)
+          shared = max(0, min(kLds ? s_want[g] : p.shared_lens[g], least)) & ~(kTileN - 1);
       }
-      p.group_info[g] = r;
+      if constexpr (kLds) {
+        s_want[g] = shared;
+        s_table[g] = first;
+      } else {
+        p.group_shared[g] = shared;
+        p.group_shared[p.groups + g] = first;
+      }
     }
   }
   __syncthreads();
-  auto group_pairs = [&](const ShGroup& r) { return r.shared ? sh_ceil(r.tokens, p.tile_tokens) : 0; };
   auto group_of = [&](int b) {
+    if constexpr (kLds) return (int)s_of[b];
     int lo = 0, hi = p.groups;  // last g with cu_groups[g] <= b
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -183,137 +222,154 @@ shared_plan_kernel(SharedParams p) {
     }
     return p.groups > 0 && p.cu_groups[lo] <= b && b < p.cu_groups[lo + 1] ? lo : -1;
   };
-  // kv tiles of q tile qt of sequence s behind `shared` tokens
-  auto own_tiles = [&](const int3& s, int full, int shared, int qt) {
-    const int hi = min(s.z, s.z - full + min((qt + 1) * p.tile_tokens, s.y));
+  auto group_tiles = [&](int g) { return shared_of(g) ? sh_row_tiles(p, group_rows(g).y) : 0; };
+  // 64-token tiles of row tile i of n of sequence s behind `shared` tokens
+  auto own_tiles = [&](int b, const int3& s, int shared, int i) {
+    const int end = p.light ? sh_ceil((i + 1) * kLtRows, p.group) : (i + 1) * p.tile_tokens;  // tokens up to it
+    const int hi = min(s.z, s.z - (p.cu_q[b + 1] - p.cu_q[b]) + min(end, s.y));
     return hi <= shared ? 0 : sh_ceil(hi, kTileN) - shared / kTileN;
   };
-  // ---- work in all
-  long long tiles = 0, pairs = 0, own = 0;
-  for (int g = tid; g < p.groups; g += kShPlanThreads) {
-    const ShGroup r = p.group_info[g];
-    const int n = group_pairs(r);
+  // ---- work in all: 64-token tiles of row tiles, row tiles, tokens of chunks
+  unsigned long long tiles = 0, pairs = 0, own = 0;
+  for (int g = tid; g < p.groups; g += threads) {
+    const int n = group_tiles(g);
     pairs += n;
-    tiles += (long long)n * (r.shared / kTileN);
+    tiles += (unsigned long long)n * (shared_of(g) / kTileN);
   }
-  for (int b = tid; b < p.batch; b += kShPlanThreads) {
-    const int3 s = sh_sequence(p, b);
+  for (int b = tid; b < p.batch; b += threads) {
+    const int3 s = seq(b);
     const int g = group_of(b);
-    const int shared = g >= 0 ? p.group_info[g].shared : 0;
+    const int shared = g >= 0 ? shared_of(g) : 0;
     if (!p.cu_q) {
       own += max(0, s.z - shared);
-    } else {
-      const int full = p.cu_q[b + 1] - s.x, n = sh_ceil(s.y, p.tile_tokens);
+    } else if (s.y > 0) {
+      const int n = sh_row_tiles(p, s.y);
       pairs += n;
-      if (n) tiles += (long long)n * own_tiles(s, full, shared, n - 1);  // (its q tiles are cut alike)
+      tiles += (unsigned long long)n * own_tiles(b, s, shared, n - 1);  // (its row tiles are cut alike)
     }
   }
-  tiles = sh_sum(tiles, s_long);
-  pairs = sh_sum(pairs, s_long);
-  own = sh_sum(own, s_long);
-  // Parts of at most `most` tiles: every pair rounds up, so where there are few
-  // pairs an even share of the slots that they leave over makes one round;
-  // else a share of all.
-  const int slots = kShTileSlots / hkv;
-  const long long left = slots - pairs;
-  const long long share = (2 * left >= slots && left > 0) ? (tiles + left - 1) / left : (tiles + slots - 1) / max(1, slots);
-  const int most = (int)max((long long)kShMinTiles, share);
-  const long long chunk_share = (own * hkv * p.dec.hblocks + kShDecodeSlots - 1) / kShDecodeSlots;
-  const int chunk = min(p.chunk_cap, max(kShMinChunk, (int)min(chunk_share, (long long)INT_MAX - 16) + 15 & ~15));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    tiles += __shfl_xor(tiles, o);
+    pairs += __shfl_xor(pairs, o);
+    own += __shfl_xor(own, o);
+  }
+  if (lane == 0) {
+    atomicAdd(&s_total[0], tiles);
+    atomicAdd(&s_total[1], pairs);
+    atomicAdd(&s_total[2], own);
+  }
+  __syncthreads();
+  const double all_tiles = (double)s_total[0] * hkv, all_pairs = (double)s_total[1] * hkv;
+  const double all_own = (double)s_total[2] * hkv * p.dec.hblocks;
+  // Parts of at most `most` tiles and `chunk` tokens.  Every row tile rounds up,
+  // so where there are few of them, and nothing else, an even share of the
+  // slots that they leave over makes one round; else a share of all.
+  const int slots = p.light ? kShPartSlots : kShTileSlots;
+  double share;
+  if (all_own == 0. && 2. * all_pairs <= slots) share = all_tiles / (slots - all_pairs);
+  else share = (all_tiles * kShTileCost + all_own / kTileN * kShChunkCost) / ((double)slots * kShTileCost);
+  const int most = max(kShMinTiles, (int)fmin(share, 1e9) + 1);
+  const int chunk = min(p.chunk_cap, max(kShMinChunk, ((int)fmin(all_own / slots, 1e9) + 16) & ~15));
   // ---- the lists
-  int n_tiles = 0, n_units = 0;  // before this round (units of one kv head)
-  for (int g0 = 0; g0 < p.groups; g0 += kShPlanThreads) {
+  Sh3 base = {0, 0, 0}, sum;  // tile parts, units (of one kv head) and chunks before this round
+  for (int g0 = 0; g0 < p.groups; g0 += threads) {
     const int g = g0 + tid;
-    ShGroup r = {0, 0, 0, 0};
-    if (g < p.groups) r = p.group_info[g];
-    const int n = group_pairs(r), kv = r.shared / kTileN;
-    const int parts = n ? sh_ceil(kv, most) : 0;
-    const int step = n > 1 ? kWaves : min(kWaves, sh_ceil(r.tokens * p.group, 32));
-    int all_t, all_u;
-    const int at = n_tiles + sh_scan(n * parts, s_wave, all_t);
-    const int unit = n_units + sh_scan(n * parts * step, s_wave, all_u);
-    n_tiles += all_t;
-    n_units += all_u;
-    for (int i = 0; i < n * parts; ++i) {
-      if (at + i >= p.cap_tiles) break;
-      const int qt = i / parts, k = i - qt * parts;
-      p.tiles[at + i] = ShTile{r.table, qt, r.q0, r.tokens, r.shared, (int)((long long)kv * k / parts),
-                               (int)((long long)kv * (k + 1) / parts), (unit + i * step) * hkv, step, {0, 0, 0}};
+    int n = 0, parts = 0, step = 0;
+    if (g < p.groups) {
+      n = group_tiles(g);
+      parts = n ? sh_ceil(shared_of(g) / kTileN, most) : 0;
+      step = n ? sh_units(p, group_rows(g).y, n) : 0;
     }
-    if (g < p.groups) p.group_info[g].table = unit * hkv;  // (read below: the prefix's first unit)
-    __syncthreads();
+    const Sh3 at = sh_scan({n * parts, n * parts * step, 0}, s_wave, sum);
+    // a wave writes the entries of each of its groups
+    uint64_t todo = __ballot(n > 0);
+    while (todo) {
+      const int l = __ffsll((unsigned long long)todo) - 1;
+      todo &= todo - 1;
+      const int gg = __shfl(g, l), nn = __shfl(n, l), pp = __shfl(parts, l), st = __shfl(step, l);
+      const int first = base.a + __shfl(at.a, l), unit = base.b + __shfl(at.b, l);
+      const int shared = shared_of(gg), kv = shared / kTileN;
+      const int table = kLds ? s_table[gg] : p.group_shared[p.groups + gg];
+      const int2 r = group_rows(gg);
+      for (int i = lane; i < nn * pp && first + i < p.cap_tiles; i += 64) {
+        // the parts of one range of tokens stand together: its row tiles share them
+        const int k = i / nn, t = i - k * nn;
+        p.tiles[first + i] = ShTile{table, t, r.x, r.y, shared, sh_cut(kv, k, pp), sh_cut(kv, k + 1, pp),
+                                    (unit + (t * pp + k) * st) * hkv, st, {0, 0, 0}};
+      }
+      if (lane == l) {
+        if constexpr (kLds) s_gunit[gg] = unit * hkv;
+        else p.group_shared[2 * p.groups + gg] = unit * hkv;
+      }
+    }
+    base = {base.a + sum.a, base.b + sum.b, 0};
   }
-  int n_chunks = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += kShPlanThreads) {
+  __syncthreads();
+  for (int b0 = 0; b0 < p.batch; b0 += threads) {
     const int b = b0 + tid;
     int3 s = make_int3(0, 0, 0);
     ShSeq q = {0, 0, 0, 0, 0, 0, 0, 0};
     int shared = 0;
     if (b < p.batch) {
-      s = sh_sequence(p, b);
+      s = seq(b);
       const int g = s.y > 0 ? group_of(b) : -1;
-      if (g >= 0) {
-        const ShGroup r = p.group_info[g];
-        const int n = group_pairs(r);
-        if (n) {
-          shared = r.shared;
-          q.p_unit = r.table;
-          q.p_parts = sh_ceil(r.shared / kTileN, most);
-          q.p_step = n > 1 ? kWaves : min(kWaves, sh_ceil(r.tokens * p.group, 32));
-          q.p_q0 = r.q0;
-        }
+      const int n = g >= 0 ? group_tiles(g) : 0;
+      if (n) {
+        const int2 r = group_rows(g);
+        shared = shared_of(g);
+        q.p_unit = kLds ? s_gunit[g] : p.group_shared[2 * p.groups + g];
+        q.p_parts = sh_ceil(shared / kTileN, most);
+        q.p_step = sh_units(p, r.y, n);
+        q.p_q0 = r.x;
       }
     }
     if (!p.cu_q) {
       const int tokens = max(0, s.z - shared);
-      const int parts = sh_ceil(tokens, chunk), size = parts ? sh_ceil(tokens, parts) + 15 & ~15 : 0;
-      int all;
-      const int at = n_chunks + sh_scan(parts, s_wave, all);
-      n_chunks += all;
-      q.s_unit = at;
+      const int parts = sh_ceil(tokens, chunk), size = parts ? (sh_ceil(tokens, parts) + 15) & ~15 : 0;
+      const Sh3 at = sh_scan({0, 0, parts}, s_wave, sum);
+      const int first = base.c + at.c;
+      q.s_unit = first;
       q.s_parts = parts;
       const bool whole = parts == 1 && q.p_parts == 0;
       q.s_step = whole;
-      for (int k = 0; k < parts && at + k < p.cap_chunks; ++k)
-        p.chunks[at + k] = ShChunk{b, shared + k * size, min(shared + (k + 1) * size, s.z),
-                                   (int)((uint32_t)(at + k) | (whole ? 0x80000000u : 0u))};
+      for (int k = 0; k < parts && first + k < p.cap_chunks; ++k)
+        p.chunks[first + k] = ShChunk{b, shared + k * size, min(shared + (k + 1) * size, s.z),
+                                      (int)((uint32_t)(first + k) | (whole ? 0x80000000u : 0u))};
     } else {
-      const int n = sh_ceil(s.y, p.tile_tokens);
-      const int full = b < p.batch ? p.cu_q[b + 1] - s.x : 0;
-      const int longest = n ? own_tiles(s, full, shared, n - 1) : 0;
-      const int parts = sh_ceil(longest, most);
-      const int step = n > 1 ? kWaves : min(kWaves, sh_ceil(s.y * p.group, 32));
-      int all_t, all_u;
-      const int at = n_tiles + sh_scan(n * parts, s_wave, all_t);
-      const int unit = n_units + sh_scan(n * parts * step, s_wave, all_u);
-      n_tiles += all_t;
-      n_units += all_u;
+      const int n = s.y > 0 ? sh_row_tiles(p, s.y) : 0;
+      const int parts = n ? sh_ceil(own_tiles(b, s, shared, n - 1), most) : 0;
+      const int step = n ? sh_units(p, s.y, n) : 0;
+      const Sh3 at = sh_scan({n * parts, n * parts * step, 0}, s_wave, sum);
+      const int first = base.a + at.a, unit = base.b + at.b;
       q.s_unit = unit * hkv;
       q.s_parts = parts;
       q.s_step = step;
       q.s_q0 = s.x;
-      for (int i = 0; i < n * parts; ++i) {
-        if (at + i >= p.cap_tiles) break;
-        const int qt = i / parts, k = i - qt * parts;
-        const int kv = own_tiles(s, full, shared, qt), lo = shared / kTileN;
-        p.tiles[at + i] = ShTile{b, qt, s.x, s.y, s.z, lo + (int)((long long)kv * k / parts),
-                                 lo + (int)((long long)kv * (k + 1) / parts), (unit + i * step) * hkv, step, {0, 0, 0}};
+      const int lo = shared / kTileN;
+      for (int i = 0; i < n * parts && first + i < p.cap_tiles; ++i) {
+        const int k = i / n, t = i - k * n;
+        const int kv = own_tiles(b, s, shared, t);
+        p.tiles[first + i] = ShTile{b, t, s.x, s.y, s.z, lo + sh_cut(kv, k, parts), lo + sh_cut(kv, k + 1, parts),
+                                    (unit + (t * parts + k) * step) * hkv, step, {0, 0, 0}};
       }
     }
     if (b < p.batch) p.seqs[b] = q;
-    __syncthreads();
+    base = {base.a + sum.a, base.b + sum.b, base.c + sum.c};
   }
-  // lists that do not fit (cu_groups that fall) are not run: every row is zero
-  const bool fits = n_tiles <= p.cap_tiles && n_chunks <= p.cap_chunks && (long long)n_units * hkv <= p.cap_units;
+  // lists that do not fit (cu_groups or cu_q that fall) are not run: every row is zero
+  const bool fits = base.a <= p.cap_tiles && base.c <= p.cap_chunks && (long long)base.b * hkv <= p.cap_units;
   if (tid == 0) {
-    p.header[0] = fits ? n_tiles : 0;
-    p.header[1] = fits ? n_chunks : 0;
+    p.header[0] = fits ? base.a : 0;
+    p.header[1] = fits ? base.c : 0;
   }
-  if (!fits)
-    for (int b = tid; b < p.batch; b += kShPlanThreads) p.seqs[b] = ShSeq{0, 0, 0, 0, 0, 0, 0, 0};
+  if (!fits) {
+    __syncthreads();
+    for (int b = tid; b < p.batch; b += threads) p.seqs[b] = ShSeq{0, 0, 0, 0, 0, 0, 0, 0};
+  }
 }
 
-// Parts of tile items: workgroup = (part, kv head).
+// Parts of 256-row tiles: workgroup = (part, kv head).
 template <bool kSoftCap, int kPaging>
 __global__ void __launch_bounds__(kThreads, 1)
 shared_tile_kernel(SharedParams p) {
@@ -338,17 +394,54 @@ shared_tile_kernel(SharedParams p) {
   prefill_run<kSoftCap, kPaging, kPHeadDim, true>(p.pre, w, part);
 }
 
-// Chunks of own parts, one new token a sequence.  XCD x = bid % 8 takes chunks
-// x, x + 8, ..., all kv heads of one in a row (they are adjacent in the pool).
-template <bool kAligned, bool kSoftCap, bool kShared>
+// Parts of 128-row tiles (the first tile_ranks ranks of all kv heads), then
+// chunks of sequences' own tokens, one new token a sequence.  The tiles are bound
+// by the matrix cores and the chunks by their reads, and a CU has one of each.
+// XCD x = bid % 8 takes chunks x, x + 8, ..., all kv heads of one in a row (they
+// are adjacent in the pool).
+template <bool kSoftCap, bool kShared>
 __global__ void __launch_bounds__(64 * kDecodeWaves, 2)
-shared_decode_kernel(SharedParams p) {
-  __shared__ DecodeLds red;
-  const int vheads = p.num_kv_heads * p.dec.hblocks;
-  const int k = blockIdx.x >> 3;
+shared_part_kernel(SharedParams p, int tile_blocks) {
+  __shared__ __attribute__((aligned(1024))) char lds[kLtLdsB];
+  static_assert(sizeof(DecodeLds) <= kLtLdsB, "a chunk's combine fits the ring");
+  const __attribute__((address_space(4))) int32_t* hd = (const __attribute__((address_space(4))) int32_t*)p.header;
+  const int hkv = p.num_kv_heads;
+  if ((int)blockIdx.x < tile_blocks) {
+    const int rank = blockIdx.x / hkv, kvh = blockIdx.x - rank * hkv;
+    if (rank >= hd[0]) return;  // uniform over the workgroup, as below
+    const __attribute__((address_space(4))) int32_t* e =
+        (const __attribute__((address_space(4))) int32_t*)(p.tiles + rank);
+    LtParams a;
+    a.q = p.pre.q;
+    a.q_ts = p.pre.q_ts;
+    a.q_hs = p.pre.q_hs;
+    a.k = p.pre.k_cache;
+    a.v = p.pre.v_cache;
+    a.num_pages = p.pre.num_pages;
+    a.page_size = p.pre.page_size;
+    a.page_stride = p.pre.page_stride;
+    a.slot_stride = p.pre.slot_stride;
+    a.head_stride = p.pre.head_stride;
+    a.pages_per_seq = p.pre.pages_per_seq;
+    a.group = p.group;
+    a.logit_scale = p.pre.logit_scale;
+    a.soft_cap = p.pre.soft_cap;
+    a.parts = p.pre.parts;
+    const int row0 = e[1] * kLtRows, q0 = e[2], rows = e[3] * p.group;
+    const int t0 = e[5] * kTileN, t1 = min(e[6] * kTileN, e[4]);
+    const int r = min(row0 + (int)(threadIdx.x >> 6) * 32 + (int)(threadIdx.x & 31), rows - 1);
+    const int token = q0 + r / p.group;
+    const int limit = p.cu_q ? p.positions[token] + 1 : clamp_len(p.lengths, token, p.span);
+    lt_run<kSoftCap>(a, p.pre.block_tables + (int64_t)e[0] * p.pre.bt_stride, kvh, q0, rows, row0, t0, t1, limit,
+                     e[7] + kvh * e[8], (uint32_t)(uintptr_t)(lds_void)&lds[0]);
+    return;
+  }
+  const int vheads = hkv * p.dec.hblocks;
+  const int bid = blockIdx.x - tile_blocks;
+  const int k = bid >> 3;
   const int kr = k / vheads;
-  const int rank = 8 * kr + (blockIdx.x & 7);
-  if (rank >= p.header[1]) return;  // uniform
+  const int rank = 8 * kr + (bid & 7);
+  if (rank >= hd[1]) return;
   const ShChunk c = p.chunks[rank];
   DecodeWork w;
   w.b = __builtin_amdgcn_readfirstlane(c.b);
@@ -358,12 +451,34 @@ shared_decode_kernel(SharedParams p) {
   w.len = w.t_end;
   const int slot = __builtin_amdgcn_readfirstlane(c.slot);
   w.single = slot < 0;
+  w.part = (int64_t)(slot & 0x7fffffff) * hkv + w.vh / p.dec.hblocks;
+  DecodeLds& red = *reinterpret_cast<DecodeLds*>(&lds[0]);
+  decode_run<kDecodeWaves, true, kSoftCap, false, kShared>(p.dec, w, &red.o[0][0][0], &red.m[0][0], &red.l[0][0]);
+}
+
+// The chunks alone, over pages that are not of whole 16-token steps.
+template <bool kSoftCap, bool kShared>
+__global__ void __launch_bounds__(64 * kDecodeWaves, 2)
+shared_chunk_kernel(SharedParams p) {
+  __shared__ DecodeLds red;
+  const int vheads = p.num_kv_heads * p.dec.hblocks;
+  const int rank = blockIdx.x / vheads;
+  if (rank >= p.header[1]) return;  // uniform
+  const ShChunk c = p.chunks[rank];
+  DecodeWork w;
+  w.b = __builtin_amdgcn_readfirstlane(c.b);
+  w.vh = blockIdx.x - rank * vheads;
+  w.t_begin = __builtin_amdgcn_readfirstlane(c.t0);
+  w.t_end = __builtin_amdgcn_readfirstlane(c.t1);
+  w.len = w.t_end;
+  const int slot = __builtin_amdgcn_readfirstlane(c.slot);
+  w.single = slot < 0;
   w.part = (int64_t)(slot & 0x7fffffff) * p.num_kv_heads + w.vh / p.dec.hblocks;
-  decode_run<kDecodeWaves, kAligned, kSoftCap, false, kShared>(p.dec, w, &red.o[0][0][0], &red.m[0][0], &red.l[0][0]);
+  decode_run<kDecodeWaves, false, kSoftCap, false, kShared>(p.dec, w, &red.o[0][0][0], &red.m[0][0], &red.l[0][0]);
 }
 
 // One workgroup a (32 rows, kv head), one wave per 32 d: a lane has row n, d =
-// 32 dt + 8 q4 + 4 h .. + 4, as prefill_run's accumulators.
+// 32 dt + 8 q4 + 4 h .. + 4, as the tiles' accumulators.
 __global__ void __launch_bounds__(256)
 shared_merge_kernel(SharedParams p) {
   const int hkv = p.num_kv_heads;
@@ -389,13 +504,19 @@ shared_merge_kernel(SharedParams p) {
   };
   auto add_tiles = [&](int unit, int parts, int step, int q0) __attribute__((always_inline)) {
     const int at = token - q0;
-    const int qt = at / p.tile_tokens;
-    const int r = (at - qt * p.tile_tokens) * p.group + head;
-    const float* src = p.pre.parts + ((int64_t)unit + ((int64_t)qt * parts * hkv + kvh) * step + (r >> 5)) *
-                                         kPartFloats<kPHeadDim>;
+    int t, r;  // row tile, row of it
+    if (p.light) {
+      r = at * p.group + head;
+      t = r / kLtRows;
+      r -= t * kLtRows;
+    } else {
+      t = at / p.tile_tokens;
+      r = (at - t * p.tile_tokens) * p.group + head;
+    }
+    const float* src = p.pre.parts + ((int64_t)unit + ((int64_t)t * parts * hkv + kvh) * step + (r >> 5)) * kLtUnit;
     const float* po = src + 4 * (dt * 4 * 64 + 32 * h + (r & 31));
-    const float* ml = src + kPartO<kPHeadDim> + 2 * (r & 31);
-    const int64_t next = (int64_t)hkv * step * kPartFloats<kPHeadDim>;
+    const float* ml = src + 32 * kHeadDim + 2 * (r & 31);
+    const int64_t next = (int64_t)hkv * step * kLtUnit;
 #pragma unroll 4
     for (int k = 0; k < parts; ++k) {
       const f32x2 v = *reinterpret_cast<const f32x2*>(ml + k * next);
@@ -425,9 +546,17 @@ shared_merge_kernel(SharedParams p) {
     *reinterpret_cast<u32x2*>(dst + 8 * q4) =
         u32x2{pack_bf16x2(o[q4][0] * inv, o[q4][1] * inv), pack_bf16x2(o[q4][2] * inv, o[q4][3] * inv)};
 }
+static_assert(kPartFloats<kPHeadDim> == kLtUnit, "both kinds of tiles leave partials of one layout");
+
+// Whether a launch takes 128-row tiles that share a CU.
+bool shared_light(bool ragged, int64_t max_q, int64_t group, int64_t page) {
+  if (page % 16) return false;
+  return !ragged || max_q * group < kRows;
+}
 
 // What a launch of a shape needs: entries of the lists and bytes of the workspace.
 struct ShSizes {
+  bool light;
   int64_t tiles, units, chunks;
   int32_t chunk_cap;
   size_t header, groups, seqs, list, chunk_list, positions, owner, parts, dec_o, dec_ml, bytes;
@@ -437,22 +566,30 @@ size_t sh_up(size_t x) { return (x + 255) & ~(size_t)255; }
 ShSizes shared_sizes(int64_t batch, int64_t groups, int64_t tokens, int64_t max_q, bool ragged, int64_t heads,
                      int64_t hkv, int64_t pages, int64_t page) {
   ShSizes z = {};
-  const int64_t group = heads / hkv, tile = kRows / group;
+  const int64_t group = heads / hkv;
+  z.light = shared_light(ragged, max_q, group, page);
+  const int64_t most = z.light ? kLtWaves : kWaves;  // units of a row tile
+  const int64_t slots = z.light ? kShPartSlots : kShTileSlots;
   const int64_t span = pages * page;
-  const int64_t extra = std::max<int64_t>(1, kShTileSlots / hkv);
-  // q tiles of groups, and of sequences: a range of n tokens has ceil(n / tile)
-  const int64_t prefix = std::min(groups, tokens) + tokens / tile;
-  const int64_t mine = ragged ? std::min(batch, tokens) + tokens / tile : 0;
-  const int64_t step = std::min<int64_t>(kWaves, (std::min(max_q, tokens) * group + 31) / 32);
-  // parts of a share of the slots: one a pair and `extra` more
-  z.tiles = prefix + mine + extra;
-  z.units = hkv * (kWaves * (prefix + extra) + (max_q > tile ? kWaves : step) * mine);
+  // row tiles of groups, and of sequences: a range of n tokens rounds up once
+  auto row_tiles = [&](int64_t ranges) {
+    const int64_t whole = z.light ? tokens * group / kLtRows : tokens / (kRows / group);
+    return std::min(ranges, tokens) + whole;
+  };
+  const int64_t prefix = groups ? row_tiles(groups) : 0, mine = ragged ? row_tiles(batch) : 0;
+  // units of a sequence's row tile: of those of one tile what its rows take
+  const int64_t rows = std::min(max_q, tokens) * group;
+  const int64_t step = std::min(most, (rows + 31) / 32);
+  // parts of a share of the slots: one a row tile and `extra` more
+  const int64_t extra = slots / hkv + 1;
+  z.tiles = prefix + mine ? prefix + mine + extra : 0;
+  z.units = hkv * (most * (prefix + extra) + step * mine);
   z.chunk_cap = (int32_t)std::max<int64_t>(16, std::min<int64_t>(2048, 62 * page) & ~(int64_t)15);
   if (!ragged) {
-    const int64_t per = (span + z.chunk_cap - 1) / z.chunk_cap;  // of the longest sequence at the longest chunk
     const int64_t least = std::min<int64_t>(kShMinChunk, z.chunk_cap);
+    const int64_t per = (span + z.chunk_cap - 1) / z.chunk_cap;  // of the longest sequence at the longest chunk
     z.chunks = std::min(batch * ((span + least - 1) / least),
-                        batch + std::max(kShDecodeSlots / hkv + 1, batch * per));
+                        batch + std::max(kShPartSlots / hkv + 1, batch * per));
   }
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -461,13 +598,13 @@ ShSizes shared_sizes(int64_t batch, int64_t groups, int64_t tokens, int64_t max_
     return r;
   };
   z.header = take(kShHeader * sizeof(int32_t));
-  z.groups = take(groups * sizeof(ShGroup));
+  z.groups = take(3 * groups * sizeof(int32_t));
   z.seqs = take(batch * sizeof(ShSeq));
   z.list = take(z.tiles * sizeof(ShTile));
   z.chunk_list = take((z.chunks + 8) * sizeof(ShChunk));
   z.positions = take(ragged ? tokens * sizeof(int32_t) : 0);
   z.owner = take(ragged ? tokens * sizeof(int32_t) : 0);
-  z.parts = take((size_t)z.units * kPartFloats<kPHeadDim> * sizeof(float));
+  z.parts = take(z.tiles ? (size_t)z.units * kLtUnit * sizeof(float) : 0);
   z.dec_o = take((size_t)z.chunks * heads * kHeadDim * sizeof(float));
   z.dec_ml = take((size_t)z.chunks * heads * 2 * sizeof(float));
   z.bytes = at;
@@ -547,6 +684,7 @@ extern "C" int pa_shared_prefix(const uint16_t* q, int64_t q_tok_stride, int64_t
   p.num_tokens = num_tokens;
   p.num_kv_heads = num_kv_heads;
   p.group = group;
+  p.light = z.light;
   p.tile_tokens = kRows / group;
   p.span = pages_per_seq * page_size;
   p.max_seqlen_q = max_seqlen_q;
@@ -556,7 +694,7 @@ extern "C" int pa_shared_prefix(const uint16_t* q, int64_t q_tok_stride, int64_t
   p.cap_chunks = (int32_t)z.chunks;
   p.cap_units = (int32_t)z.units;
   p.header = (int32_t*)(ws + z.header);
-  p.group_info = (ShGroup*)(ws + z.groups);
+  p.group_shared = (int32_t*)(ws + z.groups);
   p.seqs = (ShSeq*)(ws + z.seqs);
   p.tiles = (ShTile*)(ws + z.list);
   p.chunks = (ShChunk*)(ws + z.chunk_list);
@@ -622,38 +760,50 @@ extern "C" int pa_shared_prefix(const uint16_t* q, int64_t q_tok_stride, int64_t
       merges > 4 * kMaxGrid)
     return fail(PA_ERR_UNSUPPORTED, "%s: %lld parts of %lld rows", name, (long long)(z.tiles + z.chunks),
                 (long long)merges * 32);
-  const int64_t maps = ragged ? (num_tokens + kShPlanThreads - 1) / kShPlanThreads : 0;
-  shared_plan_kernel<<<dim3((unsigned)(1 + maps)), dim3(kShPlanThreads), 0, s>>>(p);
+  const bool small = batch <= 256 && num_groups <= 256;  // (short barriers where few threads do)
+  const int threads = small ? 256 : kShPlanThreads;
+  const int64_t maps = ragged ? (num_tokens + threads - 1) / threads : 0;
+  const bool fits = batch <= kShPlanMax && num_groups <= kShPlanMax;
+  auto plan = fits ? shared_plan_kernel<true> : shared_plan_kernel<false>;
+  plan<<<dim3((unsigned)(1 + maps)), dim3(threads), 0, s>>>(p);
   if (int rc = launch_status(name)) return rc;
-  if (num_groups > 0 || ragged) {
-    const dim3 grid((unsigned)(z.tiles * num_kv_heads)), blk(kThreads);
-    auto launch = [&](auto c) {
-      constexpr bool kCap = decltype(c)::value;
-      const int paging = prefill_paging(page_size, slot_stride);
-      if (paging == kPageTile) shared_tile_kernel<kCap, kPageTile><<<grid, blk, 0, s>>>(p);
-      else if (paging == kPageWave) shared_tile_kernel<kCap, kPageWave><<<grid, blk, 0, s>>>(p);
-      else shared_tile_kernel<kCap, kPageLane><<<grid, blk, 0, s>>>(p);
-    };
-    if (cap) launch(std::true_type{});
-    else launch(std::false_type{});
-    if (int rc = launch_status(name)) return rc;
-  }
-  if (!ragged) {
-    const dim3 grid((unsigned)((z.chunks + 7) / 8 * 8 * num_kv_heads * d.hblocks)), blk(64 * kDecodeWaves);
-    auto launch = [&](auto al, auto c, auto sh) {
-      shared_decode_kernel<decltype(al)::value, decltype(c)::value, decltype(sh)::value><<<grid, blk, 0, s>>>(p);
-    };
-    auto by_cap = [&](auto al, auto sh) {
-      if (cap) launch(al, std::true_type{}, sh);
-      else launch(al, std::false_type{}, sh);
-    };
-    auto by_group = [&](auto al) {
-      if (d.hblocks > 1) by_cap(al, std::true_type{});
-      else by_cap(al, std::false_type{});
-    };
-    if (page_size % kDecodeStep == 0) by_group(std::true_type{});
-    else by_group(std::false_type{});
-    if (int rc = launch_status(name)) return rc;
+  const int64_t tile_blocks = z.tiles * num_kv_heads;
+  auto by_flags = [&](auto launch) {
+    if (cap && d.hblocks > 1) launch(std::true_type{}, std::true_type{});
+    else if (cap) launch(std::true_type{}, std::false_type{});
+    else if (d.hblocks > 1) launch(std::false_type{}, std::true_type{});
+    else launch(std::false_type{}, std::false_type{});
+    return launch_status(name);
+  };
+  const dim3 small_blk(64 * kDecodeWaves);
+  if (z.light) {
+    const int64_t chunk_blocks = (z.chunks + 7) / 8 * 8 * num_kv_heads * d.hblocks;
+    const int rc = by_flags([&](auto c, auto sh) {
+      shared_part_kernel<decltype(c)::value, decltype(sh)::value>
+          <<<dim3((unsigned)(tile_blocks + chunk_blocks)), small_blk, 0, s>>>(p, (int)tile_blocks);
+    });
+    if (rc) return rc;
+  } else {
+    if (tile_blocks) {
+      const dim3 grid((unsigned)tile_blocks), blk(kThreads);
+      auto launch = [&](auto c) {
+        constexpr bool kCap = decltype(c)::value;
+        const int paging = prefill_paging(page_size, slot_stride);
+        if (paging == kPageTile) shared_tile_kernel<kCap, kPageTile><<<grid, blk, 0, s>>>(p);
+        else if (paging == kPageWave) shared_tile_kernel<kCap, kPageWave><<<grid, blk, 0, s>>>(p);
+        else shared_tile_kernel<kCap, kPageLane><<<grid, blk, 0, s>>>(p);
+      };
+      if (cap) launch(std::true_type{});
+      else launch(std::false_type{});
+      if (int rc = launch_status(name)) return rc;
+    }
+    if (!ragged) {
+      const int rc = by_flags([&](auto c, auto sh) {
+        shared_chunk_kernel<decltype(c)::value, decltype(sh)::value>
+            <<<dim3((unsigned)(z.chunks * num_kv_heads * d.hblocks)), small_blk, 0, s>>>(p);
+      });
+      if (rc) return rc;
+    }
   }
   shared_merge_kernel<<<dim3((unsigned)merges), dim3(256), 0, s>>>(p);
   return launch_status(name);
