@@ -10,6 +10,12 @@ from conftest import PKG
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def _share(monkeypatch):
+    """The small steps here go through the kernels of shared prefixes, not through the plain decode."""
+    monkeypatch.setattr(PKG.shared_prefix, "shared_prefix_pays", lambda *a: True)
+
+
 def _gen(seed):
     return torch.Generator().manual_seed(seed)
 
@@ -128,6 +134,33 @@ def test_matches_the_entries_it_stands_beside(dev):
     none = PKG.SharedPrefixes.of([0], [], dev)
     assert ((PKG.shared_prefix_attention(q.to(dev), cache, table, lens, none, scale=0.09).double()
              - dense.double()).abs().cpu() <= 2 * tol).all()
+
+
+def test_plain_decode_where_sharing_does_not_pay(dev, monkeypatch):
+    """The route of small steps: the plain decode's bits, out and soft cap included."""
+    monkeypatch.undo()
+    gen = _gen(11)
+    batch = Batch([(6, [50, 200, 3, None])], 64, 4, gen)
+    q = torch.randn((4, 16, 128), generator=gen).to(torch.bfloat16).to(dev)
+    assert not PKG.shared_prefix_pays(4, 1, 4, batch.table.shape[1] * 64)
+    cache, table, lens, prefixes = batch.args(dev)
+    pages = (cache[0].permute(2, 0, 1, 3), cache[1].permute(2, 0, 1, 3))
+    out = torch.empty((4, 18, 128), dtype=torch.bfloat16, device=dev)
+    for cap in (None, 9.0):
+        dense = PKG.decode_paged_attention(q, *pages, table, lens, scale=0.09, attn_logits_soft_cap=cap)
+        got = PKG.shared_prefix_attention(q, cache, table, lens, prefixes, scale=0.09, attn_logits_soft_cap=cap)
+        assert torch.equal(got, dense)
+        PKG.shared_prefix_attention(q, cache, table, lens, prefixes, scale=0.09, attn_logits_soft_cap=cap,
+                                    out=out[:, 1:17])
+        assert torch.equal(out[:, 1:17], dense)
+    # and where it pays, by the tables' width, the shared kernels'
+    wide = torch.full((4, 4000), -1, dtype=torch.int32, device=dev)
+    wide[:, :table.shape[1]] = table
+    assert PKG.shared_prefix_pays(4, 1, 4, 4000 * 64) and not PKG.shared_prefix_pays(4, 4, 4, 4000 * 64)
+    got = PKG.shared_prefix_attention(q, cache, wide, lens, prefixes, scale=0.09)
+    monkeypatch.setattr(PKG.shared_prefix, "shared_prefix_pays", lambda *a: True)
+    want, tol = ref.shared(q.cpu(), batch.cache, batch.table, batch.lengths, [1] * 4, 0.09)
+    assert ((got.cpu().double() - want).abs() <= tol).all()
 
 
 def test_attention_takes_the_groups(dev):

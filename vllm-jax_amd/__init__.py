@@ -48,5 +48,6 @@ from .latent import (LatentWeights, latent_attention, latent_decode_attention,  
                      latent_decode_workspace_bytes, latent_prefill_attention, latent_prefill_workspace_bytes,
                      latent_store)
 from .rotary import RotaryFrequencies, rotary_embedding, rotary_frequencies  # noqa: F401
-from .shared_prefix import SharedPrefixes, shared_prefix_attention, shared_prefix_workspace_bytes  # noqa: F401
+from .shared_prefix import (SharedPrefixes, shared_prefix_attention, shared_prefix_pays,  # noqa: F401
+                            shared_prefix_workspace_bytes)
 from .kv_cache_manager import Block, KVCacheManager, copy_blocks  # noqa: F401

@@ -29,10 +29,11 @@ struct BoundsParams {
 
 // Bounds of one block for 64 chunks (8 elements each) of its tokens' keys: wave
 // w takes rows w, w + 4, ..., and the four meet in LDS.  Bound by the reads of
-// the block's rows (whole 16-byte chunks of consecutive lanes), eight of them
-// in flight a lane.  A block is computed from all its rows in the pool, not
+// the block's rows (whole 16-byte chunks of consecutive lanes), four (blocks of 16
+// tokens) or eight of them in flight a lane.  A block is computed from all its rows in the pool, not
 // from its old bounds and the new rows: a block that a page held before never
 // shows through, and the order in which tokens came does not matter.
+template <int kRowsInFlight>
 __global__ void __launch_bounds__(256)
 block_bounds_kernel(BoundsParams p) {
   __shared__ u32x4 s_min[4][64], s_max[4][64];
@@ -61,12 +62,13 @@ block_bounds_kernel(BoundsParams p) {
     if (has) {
       const uint16_t* src = p.k + (int64_t)page * p.page_stride + (int64_t)(t0 % p.page_size) * p.slot_stride +
                             (int64_t)h * p.head_stride + e;
-      for (int r0 = wave; r0 < rows; r0 += 32) {
-        u32x4 v[8];
+      for (int r0 = wave; r0 < rows; r0 += 4 * kRowsInFlight) {
+        u32x4 v[kRowsInFlight];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = ld16(src + (int64_t)min(r0 + 4 * i, rows - 1) * p.slot_stride);
+        for (int i = 0; i < kRowsInFlight; ++i)
+          v[i] = ld16(src + (int64_t)min(r0 + 4 * i, rows - 1) * p.slot_stride);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < kRowsInFlight; ++i)
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const float a = bf16_lo(v[i][w]), z = bf16_hi(v[i][w]);
@@ -123,10 +125,15 @@ struct ScoresParams {
   int64_t s_bs, s_hs;
 };
 
-constexpr int kScoreBlocks = 16;  // blocks of a wave task: the rows of an MFMA
+constexpr int kScoreBlocks = 16;  // blocks of an MFMA's rows
+#ifndef PA_SCORE_TILES
+#define PA_SCORE_TILES 2
+#endif
+template <int D>
+constexpr int kScoreTiles = D == 256 ? 1 : PA_SCORE_TILES;  // row tiles of a wave, all in flight
 
-// One wave: 16 blocks of one sequence and kv head against the kv head's q
-// heads, 16 at a time.  With q+ = max(q, 0) and q- = min(q, 0) the bound
+// One wave: kScoreTiles x 16 blocks of one sequence and kv head against the kv
+// head's q heads, 16 at a time.  With q+ = max(q, 0) and q- = min(q, 0) the bound
 // sum_d max(q lo, q hi) is q+ . hi + q- . lo: products of a 16 x 2d matrix of
 // bounds with 2d x 16 of q, whose products are exact and whose sums are 32-bit.
 // Bound by the reads of the bounds (4 d bytes a block and kv head).
@@ -134,6 +141,7 @@ template <int D>
 __global__ void __launch_bounds__(256)
 block_scores_kernel(ScoresParams p) {
   constexpr int kS = D / 32;  // k-steps of one bound
+  constexpr int kT = kScoreTiles<D>;
   const int lane = threadIdx.x & 63;
   const int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hkv = p.num_kv_heads;
@@ -141,24 +149,39 @@ block_scores_kernel(ScoresParams p) {
   const int kvh = (int)(task - bt * hkv);
   const int b = (int)(bt / p.tiles);
   if (b >= p.batch) return;
-  const int j0 = kScoreBlocks * (int)(bt - (int64_t)b * p.tiles);
+  const int j0 = kScoreBlocks * kT * (int)(bt - (int64_t)b * p.tiles);
   const int len = clamp_len(p.lengths, b, (int64_t)p.pages_per_seq * p.page_size);
   const int n_blocks = (len + p.block - 1) / p.block;
   const int n = lane & 15, g = lane >> 4;
   float* dst = p.scores + b * p.s_bs + kvh * p.s_hs;
-  float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  if (j0 < n_blocks) {  // uniform
-    const int j = min(j0 + n, n_blocks - 1);
-    const int lp = (int)div_by((uint32_t)j, p.per);
-    const int32_t page = safe_page(p.block_tables + b * p.bt_stride, lp, p.num_pages);
-    const uint16_t* row = p.bounds + page * p.b_ps + (int64_t)(j - lp * (int)p.per.d) * p.b_bs + kvh * p.b_hs;
-    u32x4 a[2 * kS];
+  float best[kT][4];
 #pragma unroll
-    for (int s = 0; s < 2 * kS; ++s) a[s] = ld16(row + 8 * (4 * s + g));
+  for (int t = 0; t < kT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) best[t][i] = -INFINITY;
+  if (j0 < n_blocks) {  // uniform
+    int32_t page[kT];
+    int part[kT];
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      const int j = min(j0 + kScoreBlocks * t + n, n_blocks - 1);
+      const int lp = (int)div_by((uint32_t)j, p.per);
+      part[t] = j - lp * (int)p.per.d;
+      page[t] = safe_page(p.block_tables + b * p.bt_stride, lp, p.num_pages);
+    }
+    u32x4 a[kT][2 * kS];
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      const uint16_t* row = p.bounds + page[t] * p.b_ps + part[t] * p.b_bs + kvh * p.b_hs;
+#pragma unroll
+      for (int s = 0; s < 2 * kS; ++s) a[t][s] = ld16(row + 8 * (4 * s + g));
+    }
     for (int c0 = 0; c0 < p.group; c0 += 16) {
       const bool live = c0 + n < p.group;
       const uint16_t* qrow = p.q + b * p.q_bs + (int64_t)(kvh * p.group + (live ? c0 + n : c0)) * p.q_hs;
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      f32x4 acc[kT];
+#pragma unroll
+      for (int t = 0; t < kT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
         const u32x4 qv = ld16(qrow + 8 * (4 * s + g));
@@ -169,19 +192,29 @@ block_scores_kernel(ScoresParams p) {
           neg[w] = qv[w] & m;
           pos[w] = qv[w] & ~m;
         }
-        acc = mfma16(as_bf16x8(a[s]), as_bf16x8(neg), acc);
-        acc = mfma16(as_bf16x8(a[kS + s]), as_bf16x8(pos), acc);
-      }
-      // lane holds the bound of q head c0 + n in block j0 + 4g + i
 #pragma unroll
-      for (int i = 0; i < 4; ++i) best[i] = fmaxf(best[i], live ? acc[i] : -INFINITY);
+        for (int t = 0; t < kT; ++t) {
+          acc[t] = mfma16(as_bf16x8(a[t][s]), as_bf16x8(neg), acc[t]);
+          acc[t] = mfma16(as_bf16x8(a[t][kS + s]), as_bf16x8(pos), acc[t]);
+        }
+      }
+      // lane holds the bound of q head c0 + n in block j0 + 16 t + 4 g + i
+#pragma unroll
+      for (int t = 0; t < kT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) best[t][i] = fmaxf(best[t][i], live ? acc[t][i] : -INFINITY);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) best[i] = max_row16(best[i]);
+    for (int t = 0; t < kT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) best[t][i] = max_row16(best[t][i]);
   }
-  const int i = n & 3, at = j0 + 4 * g + i;
-  const float x = i == 0 ? best[0] : (i == 1 ? best[1] : (i == 2 ? best[2] : best[3]));
-  if (n < 4 && at < p.width) dst[at] = at < n_blocks ? x * p.scale : -INFINITY;
+#pragma unroll
+  for (int t = 0; t < kT; ++t) {
+    const int i = n & 3, at = j0 + kScoreBlocks * t + 4 * g + i;
+    const float x = i == 0 ? best[t][0] : (i == 1 ? best[t][1] : (i == 2 ? best[t][2] : best[t][3]));
+    if (n < 4 && at < p.width) dst[at] = at < n_blocks ? x * p.scale : -INFINITY;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -213,7 +246,6 @@ __global__ void __launch_bounds__(64 * kWavesN)
 select_blocks_kernel(SelectParams p) {
   constexpr int kThreadsN = 64 * kWavesN;
   __shared__ uint32_t s_count[2][kWavesN];
-  __shared__ uint32_t s_gt[kWavesN], s_eq[kWavesN];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x - b * p.num_kv_heads;
@@ -230,7 +262,6 @@ select_blocks_kernel(SelectParams p) {
   for (int i = tid; i < p.recent; i += kThreadsN) out[p.num - p.recent + i] = n - p.recent + i;
   if (k == 0) return;
   const uint32_t* src = reinterpret_cast<const uint32_t*>(p.scores + b * p.s_bs + kvh * p.s_hs) + p.first;
-  const int rounds = kPer ? kPer : (m + kThreadsN - 1) / kThreadsN;
   uint32_t keys[kPer ? kPer : 1];
   if constexpr (kPer > 0) {
 #pragma unroll
@@ -248,6 +279,7 @@ select_blocks_kernel(SelectParams p) {
     else key = i < m ? score_key(src[i]) : 0;
     return i < m;
   };
+  const int used = (m + kThreadsN - 1) / kThreadsN;  // rounds that hold candidates
   // the largest t with at least k keys >= t
   uint32_t t = 0;
   int turn = 0;
@@ -257,9 +289,9 @@ select_blocks_kernel(SelectParams p) {
 #pragma unroll
     for (int j = 0; j < (kPer ? kPer : 1); ++j) {
       if constexpr (kPer > 0) {
-        count += (uint32_t)__popcll(__ballot(keys[j] >= cand));  // (cand > 0: places past m hold 0)
+        if (j < used) count += (uint32_t)__popcll(__ballot(keys[j] >= cand));  // (cand > 0: places past m hold 0)
       } else {
-        for (int r = 0; r < rounds; ++r) {
+        for (int r = 0; r < used; ++r) {
           uint32_t key;
           const bool is = key_of(r, key);
           count += (uint32_t)__popcll(__ballot(is && key >= cand));
@@ -277,66 +309,81 @@ select_blocks_kernel(SelectParams p) {
     if ((int)count >= k) t = cand;
     if ((int)count == k) break;  // uniform
   }
-  // all keys above t, and of those equal to it the first ones
-  uint32_t above = 0;
+  // all keys above t, and of those equal to it the first ones: their places are
+  // sums over the (round, wave) pairs before
+  constexpr int kPairs = kPer ? kPer * kWavesN : kWavesN;  // pairs of a scan (kPer 0: of one round)
+  static_assert(kPairs <= 64 * 4, "at most four pairs a lane");
+  constexpr int kEach = (kPairs + 63) / 64;
+  __shared__ uint32_t s_pair[kPairs];  // above t in the low half, equal in the high half (of 64 at most)
+  int gt_base = 0, eq_base = 0;        // (kPer 0) above t and equal to it before this round
+  uint32_t before_gt[kEach], before_eq[kEach];
+  int all_gt = 0;
+  auto scan_pairs = [&]() __attribute__((always_inline)) {
+    int gt_run = 0, eq_run = 0;
 #pragma unroll
-  for (int j = 0; j < rounds; ++j) {
-    uint32_t key = 0;
-    bool is;
-    if constexpr (kPer > 0) {
-      is = j * kThreadsN + tid < m;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) key = i == j ? keys[i] : key;
-    } else {
-      is = key_of(j, key);
+    for (int e = 0; e < kEach; ++e) {
+      const uint32_t v = 64 * e + lane < kPairs ? s_pair[64 * e + lane] : 0;
+      const uint32_t gt = wave_scan(v & 0xffffu), eq = wave_scan(v >> 16);
+      before_gt[e] = gt_run + gt - (v & 0xffffu);
+      before_eq[e] = eq_run + eq - (v >> 16);
+      gt_run += __builtin_amdgcn_readlane((int)gt, 63);
+      eq_run += __builtin_amdgcn_readlane((int)eq, 63);
     }
-    above += (uint32_t)__popcll(__ballot(is && key > t));
-  }
-  if constexpr (kWavesN > 1) {
-    if (lane == 0) s_gt[wave] = above;
-    __syncthreads();
-    above = 0;
-#pragma unroll
-    for (int w = 0; w < kWavesN; ++w) above += s_gt[w];
-  }
-  const int ties = k - (int)above;
-  int gt_base = 0, eq_base = 0;  // above t and equal to it before this round
-#pragma unroll
-  for (int j = 0; j < rounds; ++j) {
-    uint32_t key = 0;
-    bool is;
-    if constexpr (kPer > 0) {
-      is = j * kThreadsN + tid < m;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) key = i == j ? keys[i] : key;
-    } else {
-      is = key_of(j, key);
-    }
-    const uint64_t gt = __ballot(is && key > t), eq = __ballot(is && key == t);
+    all_gt = gt_run;
+    return eq_run;
+  };
+  auto write = [&](int pair, int j, uint64_t gt, uint64_t eq, int ties) __attribute__((always_inline)) {
     int gt_at = gt_base, eq_at = eq_base;
-    if constexpr (kWavesN > 1) {
-      __syncthreads();  // the last round's counts have been read
-      if (lane == 0) {
-        s_gt[wave] = (uint32_t)__popcll(gt);
-        s_eq[wave] = (uint32_t)__popcll(eq);
-      }
-      __syncthreads();
 #pragma unroll
-      for (int w = 0; w < kWavesN; ++w) {
-        gt_at += w < wave ? (int)s_gt[w] : 0;
-        eq_at += w < wave ? (int)s_eq[w] : 0;
-        gt_base += (int)s_gt[w];
-        eq_base += (int)s_eq[w];
+    for (int e = 0; e < kEach; ++e)
+      if (pair >> 6 == e) {  // uniform
+        gt_at += __builtin_amdgcn_readlane((int)before_gt[e], pair & 63);
+        eq_at += __builtin_amdgcn_readlane((int)before_eq[e], pair & 63);
       }
-    } else {
-      gt_base += __popcll(gt);
-      eq_base += __popcll(eq);
-    }
     const uint64_t below = (1ull << lane) - 1;
     gt_at += __popcll(gt & below);
     eq_at += __popcll(eq & below);
-    const bool mine_gt = gt >> lane & 1, mine_eq = (eq >> lane & 1) && eq_at < ties;
-    if (mine_gt || mine_eq) out[p.first + gt_at + min(eq_at, ties)] = p.first + j * kThreadsN + tid;
+    if ((gt >> lane & 1) || ((eq >> lane & 1) && eq_at < ties))
+      out[p.first + gt_at + min(eq_at, ties)] = p.first + j * kThreadsN + tid;
+  };
+  if constexpr (kPer > 0) {
+    uint64_t gt[kPer], eq[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const bool is = j * kThreadsN + tid < m;
+      gt[j] = __ballot(is && keys[j] > t);
+      eq[j] = __ballot(is && keys[j] == t);
+      if (lane == 0) s_pair[j * kWavesN + wave] = (uint32_t)__popcll(gt[j]) | (uint32_t)__popcll(eq[j]) << 16;
+    }
+    __syncthreads();
+    scan_pairs();
+    const int ties = k - all_gt;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) write(j * kWavesN + wave, j, gt[j], eq[j], ties);
+  } else {
+    uint32_t above = 0;
+    for (int j = 0; j < used; ++j) {
+      uint32_t key;
+      const bool is = key_of(j, key);
+      above += (uint32_t)__popcll(__ballot(is && key > t));
+    }
+    if (lane == 0) s_count[turn][wave] = above;
+    __syncthreads();
+    int ties = k;
+#pragma unroll
+    for (int w = 0; w < kWavesN; ++w) ties -= (int)s_count[turn][w];
+    for (int j = 0; j < used; ++j) {
+      uint32_t key;
+      const bool is = key_of(j, key);
+      const uint64_t gt = __ballot(is && key > t), eq = __ballot(is && key == t);
+      __syncthreads();  // the last round's counts have been read
+      if (lane == 0) s_pair[wave] = (uint32_t)__popcll(gt) | (uint32_t)__popcll(eq) << 16;
+      __syncthreads();
+      const int eqs = scan_pairs();
+      write(wave, j, gt, eq, ties);
+      gt_base += all_gt;
+      eq_base += eqs;
+    }
   }
 }
 
@@ -405,11 +452,11 @@ extern "C" int pa_block_bounds(const uint16_t* k_cache, int32_t num_pages, int32
   p.b_ps = bounds_page_stride;
   p.b_bs = bounds_block_stride;
   p.b_hs = bounds_head_stride;
+  auto kernel = block == 16 ? block_bounds_kernel<4> : block_bounds_kernel<8>;
   const int64_t per = (int64_t)p.parts * p.blocks_per_seq;
   const int64_t seqs = std::max<int64_t>(1, kMaxGrid / per);
   for (int64_t b0 = 0; b0 < batch; b0 += seqs) {
-    block_bounds_kernel<<<dim3((unsigned)(std::min<int64_t>(batch - b0, seqs) * per)), dim3(256), 0,
-                          (hipStream_t)stream>>>(p);
+    kernel<<<dim3((unsigned)(std::min<int64_t>(batch - b0, seqs) * per)), dim3(256), 0, (hipStream_t)stream>>>(p);
     if (int rc = launch_status(name)) return rc;
     p.block_tables += seqs * bt_stride;
     p.lengths += seqs;
@@ -456,7 +503,8 @@ extern "C" int pa_block_scores(const uint16_t* q, int64_t q_batch_stride, int64_
   p.group = num_heads / num_kv_heads;
   p.per = magic_div((uint32_t)(page_size / block));
   p.width = (int32_t)((int64_t)pages_per_seq * (page_size / block));
-  p.tiles = (p.width + kScoreBlocks - 1) / kScoreBlocks;
+  const int wave_blocks = kScoreBlocks * (head_dim == 64 ? kScoreTiles<64> : (head_dim == 128 ? kScoreTiles<128> : kScoreTiles<256>));
+  p.tiles = (p.width + wave_blocks - 1) / wave_blocks;
   p.scale = scale;
   p.scores = scores;
   p.s_bs = scores_batch_stride;

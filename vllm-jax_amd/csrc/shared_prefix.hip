@@ -35,11 +35,10 @@ constexpr int kShTileSlots = 256;    // workgroups resident at once: of shared_t
 constexpr int kShPartSlots = 512;    // ... of shared_part_kernel (two a CU)
 constexpr int kShMinTiles = 8;       // shortest part of a row tile, in 64-token tiles
 constexpr int kShMinChunk = 512;     // shortest part of a sequence's own tokens, in tokens
+constexpr int64_t kShMergeFew = 128; // (32 rows, kv head) pairs up to which the merge takes four teams
+constexpr int kShBins = 256;         // classes of chunks by length, of 16 tokens
 // Time of a 64-token step of a row tile and of a chunk in shared_part_kernel
-#ifndef PA_SH_TILE_COST
-#define PA_SH_TILE_COST 3
-#endif
-constexpr int kShTileCost = PA_SH_TILE_COST, kShChunkCost = 4;
+constexpr int kShTileCost = 3, kShChunkCost = 4;
 
 // One part of a (row range, row tile) pair; every kv head has it.
 struct alignas(16) ShTile {
@@ -121,6 +120,35 @@ __device__ __forceinline__ Sh3 sh_scan(const Sh3& v, Sh3* s_wave, Sh3& total) {
   return {before.a + u.a - v.a, before.b + u.b - v.b, before.c + u.c - v.c};
 }
 
+// Sum and minimum over the wave's lanes (DPP, as wave_scan); every lane gets it.
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ float add_dpp(float x) {
+  return x + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), kCtrl, kRowMask, 0xF,
+                                                                   false));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x = add_dpp<0x111, 0xF>(x);
+  x = add_dpp<0x112, 0xF>(x);
+  x = add_dpp<0x114, 0xF>(x);
+  x = add_dpp<0x118, 0xF>(x);
+  x = add_dpp<0x142, 0xA>(x);
+  x = add_dpp<0x143, 0xC>(x);
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), 63));
+}
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ int min_dpp(int x) {
+  return min(x, __builtin_amdgcn_update_dpp(INT_MAX, x, kCtrl, kRowMask, 0xF, false));
+}
+__device__ __forceinline__ int wave_min(int x) {
+  x = min_dpp<0x111, 0xF>(x);
+  x = min_dpp<0x112, 0xF>(x);
+  x = min_dpp<0x114, 0xF>(x);
+  x = min_dpp<0x118, 0xF>(x);
+  x = min_dpp<0x142, 0xA>(x);
+  x = min_dpp<0x143, 0xC>(x);
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 // Workgroup 0 plans; the others (with cu_q) map tokens to sequences and kv
 // positions, a token a thread.  kLds: sequences and groups fit the plan's LDS,
 // and are read from memory once.
@@ -150,11 +178,12 @@ shared_plan_kernel(SharedParams p) {
   __shared__ int16_t s_of[kMax];                             // their group, or -1
   __shared__ int32_t s_cu[kMax + 1], s_want[kMax];           // groups: cu_groups, then shared tokens
   __shared__ int32_t s_table[kMax], s_gunit[kMax];           // first sequence with tokens, first unit
+  __shared__ int32_t s_bins[kShBins];
   __shared__ Sh3 s_wave[kShPlanThreads / 64];
-  __shared__ unsigned long long s_total[3];
+  __shared__ float s_total[3][kShPlanThreads / 64];
   const int lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
   const int hkv = p.num_kv_heads;
-  if (tid < 3) s_total[tid] = 0;
+  for (int i = tid; i < kShBins; i += threads) s_bins[i] = 0;
   if constexpr (kLds) {
     for (int b = tid; b < p.batch; b += threads) {
       const int3 s = sh_sequence(p, b);
@@ -179,22 +208,21 @@ shared_plan_kernel(SharedParams p) {
   // than the shortest sequence)
   for (int g = wave; g < p.groups; g += waves) {
     const int g0 = max(0, cu_group(g)), g1 = min(p.batch, cu_group(g + 1));
-    int active = 0, least = INT_MAX, first = INT_MAX;
-    for (int b = g0 + lane; b < g1; b += 64) {
-      const int3 s = seq(b);
-      if constexpr (kLds) s_of[b] = (int16_t)g;
-      if (s.y > 0 && s.z > 0) {
-        ++active;
-        least = min(least, s.z);
-        first = min(first, b);
+    int active = 0, least = INT_MAX, first = INT_MAX;  // active, first: uniform
+    for (int b0 = g0; b0 < g1; b0 += 64) {
+      const int b = b0 + lane;
+      int3 s = make_int3(0, 0, 0);
+      if (b < g1) {
+        s = seq(b);
+        if constexpr (kLds) s_of[b] = (int16_t)g;
       }
+      const bool has = s.y > 0 && s.z > 0;
+      const uint64_t who = __ballot(has);
+      if (who && !active) first = b0 + __ffsll((unsigned long long)who) - 1;
+      active += __popcll(who);
+      if (has) least = min(least, s.z);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      active += __shfl_xor(active, o);
-      least = min(least, __shfl_xor(least, o));
-      first = min(first, __shfl_xor(first, o));
-    }
+    least = wave_min(least);
     if (lane == 0) {
       int shared = 0;
       if (active > 1) {
@@ -230,47 +258,51 @@ shared_plan_kernel(SharedParams p) {
     return hi <= shared ? 0 : sh_ceil(hi, kTileN) - shared / kTileN;
   };
   // ---- work in all: 64-token tiles of row tiles, row tiles, tokens of chunks
-  unsigned long long tiles = 0, pairs = 0, own = 0;
+  float tiles = 0.f, pairs = 0.f, own = 0.f;
   for (int g = tid; g < p.groups; g += threads) {
     const int n = group_tiles(g);
-    pairs += n;
-    tiles += (unsigned long long)n * (shared_of(g) / kTileN);
+    pairs += (float)n;
+    tiles += (float)n * (float)(shared_of(g) / kTileN);
   }
   for (int b = tid; b < p.batch; b += threads) {
     const int3 s = seq(b);
     const int g = group_of(b);
     const int shared = g >= 0 ? shared_of(g) : 0;
     if (!p.cu_q) {
-      own += max(0, s.z - shared);
+      own += (float)max(0, s.z - shared);
     } else if (s.y > 0) {
       const int n = sh_row_tiles(p, s.y);
-      pairs += n;
-      tiles += (unsigned long long)n * own_tiles(b, s, shared, n - 1);  // (its row tiles are cut alike)
+      pairs += (float)n;
+      tiles += (float)n * (float)own_tiles(b, s, shared, n - 1);  // (its row tiles are cut alike)
     }
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    tiles += __shfl_xor(tiles, o);
-    pairs += __shfl_xor(pairs, o);
-    own += __shfl_xor(own, o);
-  }
+  tiles = wave_sum(tiles);
+  pairs = wave_sum(pairs);
+  own = wave_sum(own);
   if (lane == 0) {
-    atomicAdd(&s_total[0], tiles);
-    atomicAdd(&s_total[1], pairs);
-    atomicAdd(&s_total[2], own);
+    s_total[0][wave] = tiles;
+    s_total[1][wave] = pairs;
+    s_total[2][wave] = own;
   }
   __syncthreads();
-  const double all_tiles = (double)s_total[0] * hkv, all_pairs = (double)s_total[1] * hkv;
-  const double all_own = (double)s_total[2] * hkv * p.dec.hblocks;
+  tiles = pairs = own = 0.f;
+  for (int i = 0; i < waves; ++i) {
+    tiles += s_total[0][i];
+    pairs += s_total[1][i];
+    own += s_total[2][i];
+  }
+  // (the sums' roundings, below 2^-15 of them, must not make the shares short)
+  const float all_tiles = tiles * (float)hkv * 1.0001f, all_pairs = pairs * (float)hkv * 1.0001f;
+  const float all_own = own * (float)(hkv * p.dec.hblocks) * 1.0001f;
   // Parts of at most `most` tiles and `chunk` tokens.  Every row tile rounds up,
   // so where there are few of them, and nothing else, an even share of the
   // slots that they leave over makes one round; else a share of all.
-  const int slots = p.light ? kShPartSlots : kShTileSlots;
-  double share;
-  if (all_own == 0. && 2. * all_pairs <= slots) share = all_tiles / (slots - all_pairs);
-  else share = (all_tiles * kShTileCost + all_own / kTileN * kShChunkCost) / ((double)slots * kShTileCost);
-  const int most = max(kShMinTiles, (int)fmin(share, 1e9) + 1);
-  const int chunk = min(p.chunk_cap, max(kShMinChunk, ((int)fmin(all_own / slots, 1e9) + 16) & ~15));
+  const float slots = (float)(p.light ? kShPartSlots : kShTileSlots);
+  float share;
+  if (all_own == 0.f && 2.f * all_pairs <= slots) share = all_tiles / (slots - all_pairs);
+  else share = (all_tiles * kShTileCost + all_own / kTileN * kShChunkCost) / (slots * kShTileCost);
+  const int most = max(kShMinTiles, (int)fminf(share, 1e9f) + 1);
+  const int chunk = min(p.chunk_cap, max(kShMinChunk, ((int)fminf(all_own / slots, 1e9f) + 16) & ~15));
   // ---- the lists
   Sh3 base = {0, 0, 0}, sum;  // tile parts, units (of one kv head) and chunks before this round
   for (int g0 = 0; g0 < p.groups; g0 += threads) {
@@ -333,9 +365,26 @@ shared_plan_kernel(SharedParams p) {
       q.s_parts = parts;
       const bool whole = parts == 1 && q.p_parts == 0;
       q.s_step = whole;
-      for (int k = 0; k < parts && first + k < p.cap_chunks; ++k)
-        p.chunks[first + k] = ShChunk{b, shared + k * size, min(shared + (k + 1) * size, s.z),
-                                      (int)((uint32_t)(first + k) | (whole ? 0x80000000u : 0u))};
+      // the longest first, by the tokens of a sequence's parts
+      const int bin = kShBins - 1 - min(size / 16, kShBins - 1);
+      if (parts) atomicAdd(&s_bins[bin], parts);
+      __syncthreads();
+      if (wave == 0) {  // ranks before each bin
+        int run = base.c;
+        for (int i = 0; i < kShBins; i += 64) {
+          const int have = s_bins[i + lane], upto = (int)wave_scan((uint32_t)have);
+          s_bins[i + lane] = run + upto - have;
+          run += __builtin_amdgcn_readlane(upto, 63);
+        }
+      }
+      __syncthreads();
+      const int rank = parts ? atomicAdd(&s_bins[bin], parts) : 0;
+      for (int k = 0; k < parts && rank + k < p.cap_chunks; ++k)
+        p.chunks[rank + k] = ShChunk{b, shared + k * size, min(shared + (k + 1) * size, s.z),
+                                     (int)((uint32_t)(first + k) | (whole ? 0x80000000u : 0u))};
+      __syncthreads();
+      for (int i = tid; i < kShBins; i += threads) s_bins[i] = 0;
+      __syncthreads();
     } else {
       const int n = s.y > 0 ? sh_row_tiles(p, s.y) : 0;
       const int parts = n ? sh_ceil(own_tiles(b, s, shared, n - 1), most) : 0;
@@ -394,11 +443,25 @@ shared_tile_kernel(SharedParams p) {
   prefill_run<kSoftCap, kPaging, kPHeadDim, true>(p.pre, w, part);
 }
 
+// The chunk of a rank, for the kv head and block of 16 q heads vh.
+template <bool kAligned, bool kSoftCap, bool kShared>
+__device__ __forceinline__ void shared_chunk(const SharedParams& p, int rank, int vh, DecodeLds& red) {
+  const ShChunk c = p.chunks[rank];
+  DecodeWork w;
+  w.b = __builtin_amdgcn_readfirstlane(c.b);
+  w.vh = vh;
+  w.t_begin = __builtin_amdgcn_readfirstlane(c.t0);
+  w.t_end = __builtin_amdgcn_readfirstlane(c.t1);
+  w.len = w.t_end;
+  const int slot = __builtin_amdgcn_readfirstlane(c.slot);
+  w.single = slot < 0;
+  w.part = (int64_t)(slot & 0x7fffffff) * p.num_kv_heads + vh / p.dec.hblocks;
+  decode_run<kDecodeWaves, kAligned, kSoftCap, false, kShared>(p.dec, w, &red.o[0][0][0], &red.m[0][0], &red.l[0][0]);
+}
+
 // Parts of 128-row tiles (the first tile_ranks ranks of all kv heads), then
 // chunks of sequences' own tokens, one new token a sequence.  The tiles are bound
 // by the matrix cores and the chunks by their reads, and a CU has one of each.
-// XCD x = bid % 8 takes chunks x, x + 8, ..., all kv heads of one in a row (they
-// are adjacent in the pool).
 template <bool kSoftCap, bool kShared>
 __global__ void __launch_bounds__(64 * kDecodeWaves, 2)
 shared_part_kernel(SharedParams p, int tile_blocks) {
@@ -437,23 +500,12 @@ shared_part_kernel(SharedParams p, int tile_blocks) {
     return;
   }
   const int vheads = hkv * p.dec.hblocks;
-  const int bid = blockIdx.x - tile_blocks;
-  const int k = bid >> 3;
-  const int kr = k / vheads;
-  const int rank = 8 * kr + (bid & 7);
-  if (rank >= hd[1]) return;
-  const ShChunk c = p.chunks[rank];
-  DecodeWork w;
-  w.b = __builtin_amdgcn_readfirstlane(c.b);
-  w.vh = k - kr * vheads;
-  w.t_begin = __builtin_amdgcn_readfirstlane(c.t0);
-  w.t_end = __builtin_amdgcn_readfirstlane(c.t1);
-  w.len = w.t_end;
-  const int slot = __builtin_amdgcn_readfirstlane(c.slot);
-  w.single = slot < 0;
-  w.part = (int64_t)(slot & 0x7fffffff) * hkv + w.vh / p.dec.hblocks;
-  DecodeLds& red = *reinterpret_cast<DecodeLds*>(&lds[0]);
-  decode_run<kDecodeWaves, true, kSoftCap, false, kShared>(p.dec, w, &red.o[0][0][0], &red.m[0][0], &red.l[0][0]);
+  const int bid = blockIdx.x - tile_blocks, step = (gridDim.x - tile_blocks) / vheads;
+  const int first = bid / vheads, vh = bid - first * vheads;
+  for (int rank = first; rank < hd[1]; rank += step) {
+    if (rank != first) __syncthreads();  // the last chunk's combine has been read
+    shared_chunk<true, kSoftCap, kShared>(p, rank, vh, *reinterpret_cast<DecodeLds*>(&lds[0]));
+  }
 }
 
 // The chunks alone, over pages that are not of whole 16-token steps.
@@ -462,34 +514,29 @@ __global__ void __launch_bounds__(64 * kDecodeWaves, 2)
 shared_chunk_kernel(SharedParams p) {
   __shared__ DecodeLds red;
   const int vheads = p.num_kv_heads * p.dec.hblocks;
-  const int rank = blockIdx.x / vheads;
-  if (rank >= p.header[1]) return;  // uniform
-  const ShChunk c = p.chunks[rank];
-  DecodeWork w;
-  w.b = __builtin_amdgcn_readfirstlane(c.b);
-  w.vh = blockIdx.x - rank * vheads;
-  w.t_begin = __builtin_amdgcn_readfirstlane(c.t0);
-  w.t_end = __builtin_amdgcn_readfirstlane(c.t1);
-  w.len = w.t_end;
-  const int slot = __builtin_amdgcn_readfirstlane(c.slot);
-  w.single = slot < 0;
-  w.part = (int64_t)(slot & 0x7fffffff) * p.num_kv_heads + w.vh / p.dec.hblocks;
-  decode_run<kDecodeWaves, false, kSoftCap, false, kShared>(p.dec, w, &red.o[0][0][0], &red.m[0][0], &red.l[0][0]);
+  const int first = blockIdx.x / vheads;
+  for (int rank = first; rank < p.header[1]; rank += gridDim.x / vheads) {
+    if (rank != first) __syncthreads();
+    shared_chunk<false, kSoftCap, kShared>(p, rank, blockIdx.x - first * vheads, red);
+  }
 }
 
-// One workgroup a (32 rows, kv head), one wave per 32 d: a lane has row n, d =
-// 32 dt + 8 q4 + 4 h .. + 4, as the tiles' accumulators.
-__global__ void __launch_bounds__(256)
+// One workgroup a (32 rows, kv head), 4 kTeams waves: a wave has 32 d (a lane row n,
+// d = 32 dt + 8 q4 + 4 h .. + 4, as the tiles' accumulators) of every kTeams'th
+// part; the teams meet in LDS.  Launches of few rows have many parts a row and
+// take four teams (57 parts of two sequences' 32k shared tokens: 74 -> 49 us the call).
+template <int kTeams>
+__global__ void __launch_bounds__(256 * kTeams)
 shared_merge_kernel(SharedParams p) {
   const int hkv = p.num_kv_heads;
   const int block = blockIdx.x / hkv, kvh = blockIdx.x - block * hkv;
-  const int lane = threadIdx.x & 63, dt = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, dt = threadIdx.x >> 6 & 3;
+  const int team = kTeams == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
   const int n = lane & 31, h = lane >> 5;
   const int64_t row = (int64_t)32 * block + n;
-  const int token = (int)(row / p.group), head = (int)(row - (int64_t)token * p.group);
-  if (token >= p.num_tokens) return;
+  const int token = (int)min(row / p.group, (int64_t)p.num_tokens - 1), head = (int)(row - row / p.group * p.group);
+  const bool is = row < (int64_t)p.num_tokens * p.group;
   const int b = p.cu_q ? p.owner[token] : token;
-  if (b < 0 && !p.zero_rest) return;
   f32x4 o[4] = {};
   float m_run = -INFINITY, lsum = 0.f;
   auto add = [&](const float* po, int stride, float m, float l) __attribute__((always_inline)) {
@@ -518,26 +565,44 @@ shared_merge_kernel(SharedParams p) {
     const float* ml = src + 32 * kHeadDim + 2 * (r & 31);
     const int64_t next = (int64_t)hkv * step * kLtUnit;
 #pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
+    for (int k = team; k < parts; k += kTeams) {
       const f32x2 v = *reinterpret_cast<const f32x2*>(ml + k * next);
       add(po + k * next, 256, v[0], v[1]);
     }
   };
-  if (b >= 0) {
+  bool done = !is || (b < 0 && !p.zero_rest);
+  if (!done && b >= 0) {
     const ShSeq s = p.seqs[b];
-    if (!p.cu_q && s.s_step) return;  // its one part wrote the row
-    if (s.p_parts) add_tiles(s.p_unit, s.p_parts, s.p_step, s.p_q0);
-    if (p.cu_q) {
-      if (s.s_parts) add_tiles(s.s_unit, s.s_parts, s.s_step, s.s_q0);
-    } else {
+    done = !p.cu_q && s.s_step;  // its one part wrote the row
+    if (!done) {
+      if (s.p_parts) add_tiles(s.p_unit, s.p_parts, s.p_step, s.p_q0);
+      if (p.cu_q) {
+        if (s.s_parts) add_tiles(s.s_unit, s.s_parts, s.s_step, s.s_q0);
+      } else {
 #pragma unroll 2
-      for (int k = 0; k < s.s_parts; ++k) {
-        const int64_t at = ((int64_t)(s.s_unit + k) * hkv + kvh) * p.group + head;
-        const f32x2 v = *reinterpret_cast<const f32x2*>(p.dec.ws_ml + 2 * at);
-        add(p.dec.ws_o + at * kHeadDim + 32 * dt + 4 * h, 8, v[0], v[1]);
+        for (int k = team; k < s.s_parts; k += kTeams) {
+          const int64_t at = ((int64_t)(s.s_unit + k) * hkv + kvh) * p.group + head;
+          const f32x2 v = *reinterpret_cast<const f32x2*>(p.dec.ws_ml + 2 * at);
+          add(p.dec.ws_o + at * kHeadDim + 32 * dt + 4 * h, 8, v[0], v[1]);
+        }
       }
     }
   }
+  if constexpr (kTeams > 1) {
+    __shared__ __attribute__((aligned(16))) float s_o[kTeams - 1][4][4][64][4];
+    __shared__ float s_ml[kTeams - 1][4][64][2];
+    if (team) {
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) *reinterpret_cast<f32x4*>(s_o[team - 1][dt][q4][lane]) = o[q4];
+      s_ml[team - 1][dt][lane][0] = m_run;
+      s_ml[team - 1][dt][lane][1] = lsum;
+    }
+    __syncthreads();
+    if (team) return;
+#pragma unroll
+    for (int k = 0; k + 1 < kTeams; ++k) add(s_o[k][dt][0][lane], 256, s_ml[k][dt][lane][0], s_ml[k][dt][lane][1]);
+  }
+  if (done) return;
   const float inv = lsum > 0.f ? 1.f / lsum : 0.f;  // rows that see no key are zeros
   uint16_t* dst = p.pre.out + (int64_t)token * p.pre.o_ts + (int64_t)(kvh * p.group + head) * p.pre.o_hs + 32 * dt +
                   4 * h;
@@ -756,7 +821,7 @@ extern "C" int pa_shared_prefix(const uint16_t* q, int64_t q_tok_stride, int64_t
   hipStream_t s = (hipStream_t)stream;
   const bool cap = soft_cap > 0.f;
   const int64_t merges = ((int64_t)num_tokens * group + 31) / 32 * num_kv_heads;
-  if (z.tiles * num_kv_heads > kMaxGrid || (z.chunks + 7) / 8 * 8 * num_kv_heads * d.hblocks > 4 * kMaxGrid ||
+  if (z.tiles * num_kv_heads > kMaxGrid || z.chunks * num_kv_heads * d.hblocks > 4 * kMaxGrid ||
       merges > 4 * kMaxGrid)
     return fail(PA_ERR_UNSUPPORTED, "%s: %lld parts of %lld rows", name, (long long)(z.tiles + z.chunks),
                 (long long)merges * 32);
@@ -768,6 +833,9 @@ extern "C" int pa_shared_prefix(const uint16_t* q, int64_t q_tok_stride, int64_t
   plan<<<dim3((unsigned)(1 + maps)), dim3(threads), 0, s>>>(p);
   if (int rc = launch_status(name)) return rc;
   const int64_t tile_blocks = z.tiles * num_kv_heads;
+  // ranks that have a workgroup (further ones come behind in their loops): where
+  // the chunk is a share of the slots there are no more
+  const int64_t ranks = std::min<int64_t>(z.chunks, ((batch + kShPartSlots / (num_kv_heads * d.hblocks) + 1) + 7) / 8 * 8);
   auto by_flags = [&](auto launch) {
     if (cap && d.hblocks > 1) launch(std::true_type{}, std::true_type{});
     else if (cap) launch(std::true_type{}, std::false_type{});
@@ -777,7 +845,7 @@ extern "C" int pa_shared_prefix(const uint16_t* q, int64_t q_tok_stride, int64_t
   };
   const dim3 small_blk(64 * kDecodeWaves);
   if (z.light) {
-    const int64_t chunk_blocks = (z.chunks + 7) / 8 * 8 * num_kv_heads * d.hblocks;
+    const int64_t chunk_blocks = ranks * num_kv_heads * d.hblocks;
     const int rc = by_flags([&](auto c, auto sh) {
       shared_part_kernel<decltype(c)::value, decltype(sh)::value>
           <<<dim3((unsigned)(tile_blocks + chunk_blocks)), small_blk, 0, s>>>(p, (int)tile_blocks);
@@ -800,11 +868,12 @@ extern "C" int pa_shared_prefix(const uint16_t* q, int64_t q_tok_stride, int64_t
     if (!ragged) {
       const int rc = by_flags([&](auto c, auto sh) {
         shared_chunk_kernel<decltype(c)::value, decltype(sh)::value>
-            <<<dim3((unsigned)(z.chunks * num_kv_heads * d.hblocks)), small_blk, 0, s>>>(p);
+            <<<dim3((unsigned)(ranks * num_kv_heads * d.hblocks)), small_blk, 0, s>>>(p);
       });
       if (rc) return rc;
     }
   }
-  shared_merge_kernel<<<dim3((unsigned)merges), dim3(256), 0, s>>>(p);
+  if (merges <= kShMergeFew) shared_merge_kernel<4><<<dim3((unsigned)merges), dim3(1024), 0, s>>>(p);
+  else shared_merge_kernel<1><<<dim3((unsigned)merges), dim3(256), 0, s>>>(p);
   return launch_status(name);
 }

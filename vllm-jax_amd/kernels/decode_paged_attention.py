@@ -20,6 +20,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
+from ..rotary import on_device
 from ._common import (DEFAULT_MASK_VALUE, as_i32, check_quantized_pages, pages_strides, pool_pointers, require_bf16,
                       require_device, stream_handle)
 
@@ -86,6 +87,13 @@ def decode_pool(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Ten
     _, ps, ss, hs, _ = kv_cache.stride()
     return _decode(q, (num_kv_heads, num_pages, page_size, head_dim), pool_pointers(kv_cache), (ps, ss, hs), None, (),
                    block_tables, lengths, None, scale, None, None)
+
+
+def decode_checked(q, pages, pointers, strides, block_tables, lengths, attn_logits_soft_cap, scale, workspace, out):
+    """The launch over bf16 pages whose operands an entry beside this one has checked (``_decode``'s arguments)."""
+    with on_device(q):
+        return _decode(q, pages, pointers, strides, None, (), block_tables, lengths, attn_logits_soft_cap, scale,
+                       workspace, out)
 
 
 def _check_shapes(q, pages, block_tables, lengths):
