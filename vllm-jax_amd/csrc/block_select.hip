@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "../../include/long_context.h"
+#include "lds_tiles.h"
 #include "long_context.h"
 #include "magic_div.h"
 
@@ -125,96 +126,85 @@ struct ScoresParams {
   int64_t s_bs, s_hs;
 };
 
-constexpr int kScoreBlocks = 16;  // blocks of an MFMA's rows
-#ifndef PA_SCORE_TILES
-#define PA_SCORE_TILES 2
-#endif
-template <int D>
-constexpr int kScoreTiles = D == 256 ? 1 : PA_SCORE_TILES;  // row tiles of a wave, all in flight
+constexpr int kScoreBlocks = 16;  // blocks of a wave task: the rows of an MFMA
 
-// One wave: kScoreTiles x 16 blocks of one sequence and kv head against the kv
-// head's q heads, 16 at a time.  With q+ = max(q, 0) and q- = min(q, 0) the bound
-// sum_d max(q lo, q hi) is q+ . hi + q- . lo: products of a 16 x 2d matrix of
-// bounds with 2d x 16 of q, whose products are exact and whose sums are 32-bit.
-// Bound by the reads of the bounds (4 d bytes a block and kv head).
+// One wave: 16 blocks of one sequence and kv head against the kv head's q heads,
+// 16 at a time.  With q+ = max(q, 0) and q- = min(q, 0) the bound sum_d max(q lo,
+// q hi) is q+ . hi + q- . lo: products of a 16 x 2d matrix of bounds with 2d x 16
+// of q, whose products are exact and whose sums are 32-bit.  Bound by the reads of
+// the bounds (4 d bytes a block and kv head), which come through LDS as whole rows
+// (chunk c of row r at c ^ r, so that 16 rows' reads of one chunk land on distinct
+// banks).
 template <int D>
 __global__ void __launch_bounds__(256)
 block_scores_kernel(ScoresParams p) {
-  constexpr int kS = D / 32;  // k-steps of one bound
-  constexpr int kT = kScoreTiles<D>;
+  constexpr int kS = D / 32;            // k-steps of one bound
+  constexpr int kRowB = 4 * D;          // bytes of a row: min and max
+  constexpr int kLoads = 16 * kRowB / 1024, kRowLanes = 64 * kLoads / 16;
+  __shared__ __attribute__((aligned(1024))) char lds[4][16 * kRowB];
   const int lane = threadIdx.x & 63;
-  const int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t task = (int64_t)blockIdx.x * 4 + wave;
   const int hkv = p.num_kv_heads;
   const int64_t bt = task / hkv;
   const int kvh = (int)(task - bt * hkv);
   const int b = (int)(bt / p.tiles);
   if (b >= p.batch) return;
-  const int j0 = kScoreBlocks * kT * (int)(bt - (int64_t)b * p.tiles);
+  const int j0 = kScoreBlocks * (int)(bt - (int64_t)b * p.tiles);
   const int len = clamp_len(p.lengths, b, (int64_t)p.pages_per_seq * p.page_size);
   const int n_blocks = (len + p.block - 1) / p.block;
   const int n = lane & 15, g = lane >> 4;
   float* dst = p.scores + b * p.s_bs + kvh * p.s_hs;
-  float best[kT][4];
-#pragma unroll
-  for (int t = 0; t < kT; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) best[t][i] = -INFINITY;
+  float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
   if (j0 < n_blocks) {  // uniform
-    int32_t page[kT];
-    int part[kT];
+    const uint32_t mine = (uint32_t)(uintptr_t)(lds_void)&lds[wave][0];
+    const int j = min(j0 + n, n_blocks - 1);
+    const int lp = (int)div_by((uint32_t)j, p.per);
+    const int32_t page = safe_page(p.block_tables + b * p.bt_stride, lp, p.num_pages);
+    const int64_t off = page * p.b_ps + (int64_t)(j - lp * (int)p.per.d) * p.b_bs + kvh * p.b_hs;
+    const int lo = (int)(uint32_t)off, hi = (int)(off >> 32);
 #pragma unroll
-    for (int t = 0; t < kT; ++t) {
-      const int j = min(j0 + kScoreBlocks * t + n, n_blocks - 1);
-      const int lp = (int)div_by((uint32_t)j, p.per);
-      part[t] = j - lp * (int)p.per.d;
-      page[t] = safe_page(p.block_tables + b * p.bt_stride, lp, p.num_pages);
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = (64 * i + lane) / kRowLanes, c = (64 * i + lane) % kRowLanes;
+      const int64_t row = (int64_t)(uint32_t)__builtin_amdgcn_ds_bpermute(4 * r, lo) |
+                          (int64_t)__builtin_amdgcn_ds_bpermute(4 * r, hi) << 32;
+      lds_dma16(p.bounds + row + 8 * (c ^ r), mine + 1024 * i);
     }
-    u32x4 a[kT][2 * kS];
-#pragma unroll
-    for (int t = 0; t < kT; ++t) {
-      const uint16_t* row = p.bounds + page[t] * p.b_ps + part[t] * p.b_bs + kvh * p.b_hs;
-#pragma unroll
-      for (int s = 0; s < 2 * kS; ++s) a[t][s] = ld16(row + 8 * (4 * s + g));
-    }
+    bool first = true;
     for (int c0 = 0; c0 < p.group; c0 += 16) {
       const bool live = c0 + n < p.group;
       const uint16_t* qrow = p.q + b * p.q_bs + (int64_t)(kvh * p.group + (live ? c0 + n : c0)) * p.q_hs;
-      f32x4 acc[kT];
+      u32x4 qv[kS];
 #pragma unroll
-      for (int t = 0; t < kT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < kS; ++s) qv[s] = ld16(qrow + 8 * (4 * s + g));
+      if (first) {
+        wait_vm<0>();  // the rows have landed
+        asm volatile("" ::: "memory");
+        first = false;
+      }
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
-        const u32x4 qv = ld16(qrow + 8 * (4 * s + g));
         u32x4 neg, pos;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const uint32_t m = ((qv[w] & 0x80008000u) >> 15) * 0xffffu;
-          neg[w] = qv[w] & m;
-          pos[w] = qv[w] & ~m;
+          const uint32_t m = ((qv[s][w] & 0x80008000u) >> 15) * 0xffffu;
+          neg[w] = qv[s][w] & m;
+          pos[w] = qv[s][w] & ~m;
         }
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-          acc[t] = mfma16(as_bf16x8(a[t][s]), as_bf16x8(neg), acc[t]);
-          acc[t] = mfma16(as_bf16x8(a[t][kS + s]), as_bf16x8(pos), acc[t]);
-        }
+        acc = mfma16(as_bf16x8(lds_ld16(mine + kRowB * n + 16 * ((4 * s + g) ^ n))), as_bf16x8(neg), acc);
+        acc = mfma16(as_bf16x8(lds_ld16(mine + kRowB * n + 16 * ((4 * (kS + s) + g) ^ n))), as_bf16x8(pos), acc);
       }
-      // lane holds the bound of q head c0 + n in block j0 + 16 t + 4 g + i
+      // lane holds the bound of q head c0 + n in block j0 + 4g + i
 #pragma unroll
-      for (int t = 0; t < kT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) best[t][i] = fmaxf(best[t][i], live ? acc[t][i] : -INFINITY);
+      for (int i = 0; i < 4; ++i) best[i] = fmaxf(best[i], live ? acc[i] : -INFINITY);
     }
 #pragma unroll
-    for (int t = 0; t < kT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) best[t][i] = max_row16(best[t][i]);
+    for (int i = 0; i < 4; ++i) best[i] = max_row16(best[i]);
   }
-#pragma unroll
-  for (int t = 0; t < kT; ++t) {
-    const int i = n & 3, at = j0 + kScoreBlocks * t + 4 * g + i;
-    const float x = i == 0 ? best[t][0] : (i == 1 ? best[t][1] : (i == 2 ? best[t][2] : best[t][3]));
-    if (n < 4 && at < p.width) dst[at] = at < n_blocks ? x * p.scale : -INFINITY;
-  }
+  const int i = n & 3, at = j0 + 4 * g + i;
+  const float x = i == 0 ? best[0] : (i == 1 ? best[1] : (i == 2 ? best[2] : best[3]));
+  if (n < 4 && at < p.width) dst[at] = at < n_blocks ? x * p.scale : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -237,15 +227,16 @@ __device__ __forceinline__ uint32_t score_key(uint32_t u) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One workgroup a (sequence, kv head): the k-th largest key by bisection over
-// its 32 bits, then the blocks in order.  A thread keeps its keys in registers
+// One workgroup a (sequence, kv head): the k-th largest key, bit by bit (one
+// wave) or by histograms of its digits, then the blocks in order.  A thread keeps its keys in registers
 // (kPer of them; 0: reads them again), key j of thread t being candidate j *
 // threads + t, so that counts are ballots and their sums scalar.
 template <int kWavesN, int kPer>
 __global__ void __launch_bounds__(64 * kWavesN)
 select_blocks_kernel(SelectParams p) {
   constexpr int kThreadsN = 64 * kWavesN;
-  __shared__ uint32_t s_count[2][kWavesN];
+  constexpr int kDigits = 2048;
+  __shared__ int s_hist[kWavesN > 1 ? kDigits : 1], s_count[kWavesN], s_found[3];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x - b * p.num_kv_heads;
@@ -280,34 +271,70 @@ select_blocks_kernel(SelectParams p) {
     return i < m;
   };
   const int used = (m + kThreadsN - 1) / kThreadsN;  // rounds that hold candidates
-  // the largest t with at least k keys >= t
+  // t: the k-th largest key, or a lower one that no key lies between
   uint32_t t = 0;
-  int turn = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t cand = t | 1u << bit;
-    uint32_t count = 0;
+  if constexpr (kWavesN == 1) {
+    // bit by bit, the largest t with at least k keys >= t (t > 0: places past m hold 0)
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = t | 1u << bit;
+      int count = 0;
 #pragma unroll
-    for (int j = 0; j < (kPer ? kPer : 1); ++j) {
+      for (int j = 0; j < kPer; ++j) count += __popcll(__ballot(keys[j] >= cand));
+      if (count >= k) t = cand;
+      if (count == k) break;  // uniform
+    }
+  } else {
+    // by digits of 11, 11 and 10 bits: a histogram of the keys with the digits
+    // found so far, and the digit in which the r-th largest of them lies
+    constexpr int kMine = kDigits / kThreadsN;  // bins of a thread, from the top down
+    int r = k;
+    int shift = 21;
+    for (int pass = 0; pass < 3; ++pass) {
+      const uint32_t known = pass == 0 ? 0 : ~0u << (pass == 1 ? 21 : 10);  // bits of t found
+      for (int i = tid; i < kDigits; i += kThreadsN) s_hist[i] = 0;
+      __syncthreads();
       if constexpr (kPer > 0) {
-        if (j < used) count += (uint32_t)__popcll(__ballot(keys[j] >= cand));  // (cand > 0: places past m hold 0)
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (j * kThreadsN + tid < m && (keys[j] & known) == t) atomicAdd(&s_hist[keys[j] >> shift & (kDigits - 1)], 1);
       } else {
-        for (int r = 0; r < used; ++r) {
+        for (int j = 0; j < used; ++j) {
           uint32_t key;
-          const bool is = key_of(r, key);
-          count += (uint32_t)__popcll(__ballot(is && key >= cand));
+          if (key_of(j, key) && (key & known) == t) atomicAdd(&s_hist[key >> shift & (kDigits - 1)], 1);
         }
       }
-    }
-    if constexpr (kWavesN > 1) {
-      if (lane == 0) s_count[turn][wave] = count;
       __syncthreads();
-      count = 0;
+      const int top = kDigits - 1 - kMine * tid;
+      int have[kMine], total = 0;
 #pragma unroll
-      for (int w = 0; w < kWavesN; ++w) count += s_count[turn][w];
-      turn ^= 1;
+      for (int i = 0; i < kMine; ++i) {
+        have[i] = s_hist[top - i];
+        total += have[i];
+      }
+      int upto = (int)wave_scan((uint32_t)total);
+      if (lane == 63) s_count[wave] = upto;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWavesN; ++w) upto += w < wave ? s_count[w] : 0;
+      int above = upto - total;  // keys in higher bins
+      if (above < r && upto >= r) {  // one thread
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          if (above < r && above + have[i] >= r) {
+            s_found[0] = top - i;
+            s_found[1] = above;
+            s_found[2] = have[i];
+          }
+          above += have[i];
+        }
+      }
+      __syncthreads();
+      // (the last pass has 10 bits: its digit's top bit is known, and kept out of t)
+      t |= ((uint32_t)s_found[0] << shift) & ~known;
+      r -= s_found[1];
+      if (s_found[2] == r) break;  // all keys of the bin: uniform
+      shift = pass == 0 ? 10 : 0;
     }
-    if ((int)count >= k) t = cand;
-    if ((int)count == k) break;  // uniform
   }
   // all keys above t, and of those equal to it the first ones: their places are
   // sums over the (round, wave) pairs before
@@ -367,11 +394,11 @@ select_blocks_kernel(SelectParams p) {
       const bool is = key_of(j, key);
       above += (uint32_t)__popcll(__ballot(is && key > t));
     }
-    if (lane == 0) s_count[turn][wave] = above;
+    if (lane == 0) s_count[wave] = (int)above;
     __syncthreads();
     int ties = k;
 #pragma unroll
-    for (int w = 0; w < kWavesN; ++w) ties -= (int)s_count[turn][w];
+    for (int w = 0; w < kWavesN; ++w) ties -= s_count[w];
     for (int j = 0; j < used; ++j) {
       uint32_t key;
       const bool is = key_of(j, key);
@@ -503,8 +530,7 @@ extern "C" int pa_block_scores(const uint16_t* q, int64_t q_batch_stride, int64_
   p.group = num_heads / num_kv_heads;
   p.per = magic_div((uint32_t)(page_size / block));
   p.width = (int32_t)((int64_t)pages_per_seq * (page_size / block));
-  const int wave_blocks = kScoreBlocks * (head_dim == 64 ? kScoreTiles<64> : (head_dim == 128 ? kScoreTiles<128> : kScoreTiles<256>));
-  p.tiles = (p.width + wave_blocks - 1) / wave_blocks;
+  p.tiles = (p.width + kScoreBlocks - 1) / kScoreBlocks;
   p.scale = scale;
   p.scores = scores;
   p.s_bs = scores_batch_stride;
@@ -559,6 +585,7 @@ extern "C" int pa_select_blocks(const float* scores, int64_t scores_batch_stride
   const int64_t items = (int64_t)batch * num_kv_heads;
   const int64_t most = (int64_t)width - first - recent;  // candidates
   hipStream_t s = (hipStream_t)stream;
+  if (most <= 64 * 4) return select_launch<1, 4>(name, p, items, s);
   if (most <= 64 * 16) return select_launch<1, 16>(name, p, items, s);
   if (most <= 256 * 16) return select_launch<4, 16>(name, p, items, s);
   if (most <= 1024 * 16) return select_launch<16, 16>(name, p, items, s);
