@@ -73,6 +73,16 @@ int32_t pa_bm_ref_count(pa_block_manager* bm, int32_t block_id);
  * otherwise nothing is taken. */
 int32_t pa_bm_take_copies(pa_block_manager* bm, int32_t* src, int32_t* dst, int32_t capacity);
 
+/* Groups of sequences that share their leading blocks, for pa_shared_prefix:
+ * the n sequences seq_ids are taken in their order (a batch's), and neighbours
+ * whose tables begin with the same blocks are put together as long as that
+ * does not lower (members - 1) x (blocks common to all), the block reads saved.
+ * Writes group g's first sequence to cu_groups[g] (and n behind the last) and
+ * its common tokens, whole blocks, to shared_lens[g] (0 for a sequence alone);
+ * room for n + 1 and n entries (host arrays).  Returns the number of groups. */
+int32_t pa_bm_shared_prefixes(pa_block_manager* bm, const int64_t* seq_ids, int32_t n, int32_t* cu_groups,
+                              int32_t* shared_lens);
+
 /* Device page copy for copy-on-write: page dst_blocks[i] <- page
  * src_blocks[i] in both K and V pools (device int32 arrays, num_copies <=
  * 65535), the pool addressed as in pa_kv_store.  Destinations must be

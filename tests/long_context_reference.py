@@ -59,7 +59,7 @@ def attend(q, k, v, scale, cap=None, limit=None, scaled_q=False):
     return out, tol
 
 
-def shared(q, cache, table, lengths, new, scale, cap=None, scaled_q=True):
+def shared(q, cache, table, lengths, new, scale, cap=None, scaled_q=False):
     """Attention of the last ``new[b]`` tokens of every sequence, rows in order."""
     heads, kv = q.shape[1], cache.shape[3]
     g = heads // kv

@@ -8,6 +8,8 @@ import long_context_reference as ref
 from conftest import PKG
 
 pytestmark = pytest.mark.gpu
+DECODE_SCALE = 1 / 11.3125       # what attention() applies: 1 / bf16(128 ** 0.5)
+PREFILL_SCALE = 0.08837890625    # bf16(128 ** -0.5)
 
 
 @pytest.fixture(autouse=True)
@@ -178,19 +180,23 @@ def test_attention_takes_the_groups(dev):
     outs = []
     for shared in (None, batch.prefixes(dev)):
         cache, table, _, _ = batch.args(dev)
-        meta = PKG.PrefillAttentionMetadata(_i32(pos, dev), slots, table, cu_q, cu_k, None, None, 4, shared=shared)
+        meta = PKG.SharedPrefillAttentionMetadata(_i32(pos, dev), slots, table, cu_q, cu_k, None, None, 4, shared=shared)
         pool, out = PKG.attention(cache, q, k, v, meta)
         outs.append((pool.cpu(), out.cpu().double()))
     assert torch.equal(outs[0][0], outs[1][0])
-    _, tol = ref.shared(q.cpu(), outs[0][0], batch.table, batch.lengths, new, 128 ** -0.5)
-    assert ((outs[0][1] - outs[1][1]).abs() <= 2 * tol + 2 * ref.BF16 * 0.01).all()
+    # (the plain prefill rounds its scaled q)
+    _, tol = ref.shared(q.cpu(), outs[0][0], batch.table, batch.lengths, new, PREFILL_SCALE, scaled_q=True)
+    assert ((outs[0][1] - outs[1][1]).abs() <= 2 * tol).all()
     first = [0, 4, 5]
     outs = []
     for shared in (None, batch.prefixes(dev)):
         cache, table, lens, _ = batch.args(dev)
-        meta = PKG.DecodeAttentionMetadata(_i32(pos, dev)[first], slots[first], table, lens, shared=shared)
-        outs.append(PKG.attention(cache, q[first], k[first], v[first], meta)[1].cpu().double())
-    assert ((outs[0] - outs[1]).abs() <= 2 * tol[first] + 2 * ref.BF16 * 0.01).all()
+        meta = PKG.SharedDecodeAttentionMetadata(_i32(pos, dev)[first], slots[first], table, lens, shared=shared)
+        pool, out = PKG.attention(cache, q[first], k[first], v[first], meta)
+        outs.append((pool.cpu(), out.cpu().double()))
+    assert torch.equal(outs[0][0], outs[1][0])
+    _, tol = ref.shared(q[first].cpu(), outs[0][0], batch.table, batch.lengths, [1] * 3, DECODE_SCALE)
+    assert ((outs[0][1] - outs[1][1]).abs() <= 2 * tol).all()
 
 
 def test_rows_outside_and_strides(dev):
@@ -294,3 +300,56 @@ def test_captured(several, dev):
         assert torch.equal(replayed, eager)
         want, tol = ref.shared(q.cpu(), batch.cache, batch.table, lens.cpu(), [2] * 4 if several else [1] * 4, 0.1)
         assert ((out.cpu().double() - want).abs() <= tol).all()
+
+
+def test_a_step_of_the_block_manager(dev):
+    """Prompts behind a cached system prompt, then decode steps, with the groups that the manager finds: each step's
+    output against the plain form."""
+    from test_long_context_api import Request
+    gen = _gen(12)
+    mgr = PKG.KVCacheManager(64, 64, enable_prefix_caching=True)
+    cache = torch.zeros((2, 64, 64, 2, 128), dtype=torch.bfloat16, device=dev)
+    model = torch.zeros((2, 64, 64, 2, 128), dtype=torch.bfloat16)
+    system = list(range(300))
+    first = Request(0, system + [900] * 30)
+    rest = [Request(i, system + [1000 + i] * (20 + 9 * i)) for i in range(1, 5)]
+
+    def step(batch, new, decode):
+        lens = [len(r) for r in batch]
+        tables = [mgr.block_ids(r) for r in batch]
+        table = torch.full((len(batch), max(map(len, tables))), -1, dtype=torch.int32)
+        for i, t in enumerate(tables):
+            table[i, :len(t)] = torch.tensor(t, dtype=torch.int32)
+        pos = [t for n, c in zip(lens, new) for t in range(n - c, n)]
+        seq = [i for i, c in enumerate(new) for _ in range(c)]
+        slots = [int(table[i, t // 64]) * 64 + t % 64 for i, t in zip(seq, pos)]
+        q = torch.randn((len(pos), 8, 128), generator=gen).to(torch.bfloat16)
+        k, v = (torch.randn((len(pos), 2, 128), generator=gen).to(torch.bfloat16) for _ in range(2))
+        model[0].view(-1, 2, 128)[slots], model[1].view(-1, 2, 128)[slots] = k, v
+        groups = mgr.shared_prefixes(batch)
+        shared = PKG.SharedPrefixes.of(*groups, dev)
+        common = (_i32(pos, dev), _i32(slots, dev), table.to(dev))
+        if decode:
+            meta = PKG.SharedDecodeAttentionMetadata(*common, _i32(lens, dev), shared=shared)
+        else:
+            cu = lambda x: _i32([0, *torch.tensor(x).cumsum(0).tolist()], dev)  # noqa: E731
+            meta = PKG.SharedPrefillAttentionMetadata(*common, cu(new), cu(lens), None, None, max(new), shared=shared)
+        _, out = PKG.attention(cache, q.to(dev), k.to(dev), v.to(dev), meta)
+        want, tol = ref.shared(q, model, table, lens, new, DECODE_SCALE if decode else PREFILL_SCALE)
+        assert torch.equal(cache.cpu(), model)
+        assert ((out.cpu().double() - want).abs() <= tol).all()
+        return groups
+
+    mgr.allocate_slots(first, True)
+    step([first], [330], False)
+    for r in rest:
+        mgr.allocate_slots(r, True)
+    assert all(mgr.num_cached_tokens(r) == 256 for r in rest)
+    groups = step(rest, [len(r) - 256 for r in rest], False)
+    assert groups == ([0, 4], [256])
+    everyone = [first, *rest]
+    for _ in range(3):
+        for r in everyone:
+            r.token_ids.append(7)
+            mgr.allocate_slots(r, False)
+        assert step(everyone, [1] * 5, True) == ([0, 5], [256])

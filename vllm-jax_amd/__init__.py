@@ -20,8 +20,8 @@ Public surface (mirrors simpissa/vllm-jax):
   a long context that a cheap score selects, over ``update_block_bounds``,
   ``block_scores``, ``select_blocks`` and ``block_sparse_decode_attention``;
 * ``shared_prefix_attention`` with ``SharedPrefixes`` -- attention of a batch
-  whose sequences share prefixes, each read once (``attention()`` takes it by
-  the metadata's ``shared``);
+  whose sequences share prefixes, each read once (``attention()`` takes the
+  groups in ``SharedDecodeAttentionMetadata`` / ``SharedPrefillAttentionMetadata``);
 * ``KVCacheManager`` / ``copy_blocks`` -- the block manager of
   vllm/src/kv_cache_manager.py on a native allocator, with optional prefix
   caching and fork / copy-on-write.
@@ -36,6 +36,7 @@ module name ``vllm_jax_amd``::
         submodule_search_locations=["<repo>/vllm-jax_amd"])
 """
 from .attention import (DecodeAttentionMetadata, MixedAttentionMetadata, PrefillAttentionMetadata,  # noqa: F401
+                        SharedDecodeAttentionMetadata, SharedPrefillAttentionMetadata,
                         attention, attention_stored, gather_kv, qk_norm_rope_store, qwen3_attention_core,
                         update_kv_cache, update_kv_cache_fp8)
 from .block_sparse import (block_scores, block_sparse_attention, block_sparse_decode_attention,  # noqa: F401

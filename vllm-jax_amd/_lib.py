@@ -140,6 +140,7 @@ SIGNATURES = {
     "pa_bm_fork": (ctypes.c_int, [c_vp, c_i64, c_i64]),
     "pa_bm_deallocate": (ctypes.c_int, [c_vp, c_i64]),
     "pa_bm_ref_count": (c_i32, [c_vp, c_i32]),
+    "pa_bm_shared_prefixes": (c_i32, [c_vp, c_vp, c_i32, c_vp, c_vp]),
     "pa_bm_take_copies": (c_i32, [c_vp, c_vp, c_vp, c_i32]),
     "pa_copy_blocks": (ctypes.c_int, [
         c_vp, c_vp, c_i32, c_i32,      # caches, num_pages, page_size

@@ -42,13 +42,11 @@ USE_PREFILL_PAGED_ATTENTION_KERNEL = True
 
 @dataclass
 class DecodeAttentionMetadata:
-    """qwen3.py:17-22.  ``shared``: the groups of sequences that share their
-    first pages, each shared page then read once (no reference counterpart)."""
+    """qwen3.py:17-22."""
     input_positions: torch.Tensor
     slot_mapping: torch.Tensor
     block_tables: torch.Tensor
     context_lens: torch.Tensor
-    shared: Optional[SharedPrefixes] = None
 
 
 @dataclass
@@ -61,8 +59,7 @@ class PrefillAttentionMetadata:
     by the width); anything else, such as a device tensor, which is not read,
     says that it is not known, ``None`` that the table is as wide as the
     longest.  Where nothing is cached, ``cu_seqlens_k`` may be
-    ``cu_seqlens_q`` itself: the new tokens then bound the kv lengths.
-    ``shared`` as in ``DecodeAttentionMetadata``."""
+    ``cu_seqlens_q`` itself: the new tokens then bound the kv lengths."""
     input_positions: torch.Tensor
     slot_mapping: torch.Tensor
     block_tables: torch.Tensor
@@ -71,6 +68,19 @@ class PrefillAttentionMetadata:
     max_seqlen_q: torch.Tensor
     max_seqlen_k: Union[torch.Tensor, int, None]
     max_seqlen_bucket: int = field(default=0)
+
+
+@dataclass
+class SharedDecodeAttentionMetadata(DecodeAttentionMetadata):
+    """A decode step with the groups of its sequences that share their first
+    pages (``KVCacheManager.shared_prefixes``): ``attention()`` reads each shared
+    page once a group.  No reference counterpart."""
+    shared: Optional[SharedPrefixes] = None
+
+
+@dataclass
+class SharedPrefillAttentionMetadata(PrefillAttentionMetadata):
+    """The same for a prefill step (new tokens behind shared, cached ones)."""
     shared: Optional[SharedPrefixes] = None
 
 

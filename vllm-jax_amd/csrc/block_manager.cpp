@@ -16,6 +16,7 @@
 // With prefix caching off and no forks, every call returns exactly what the
 // reference returns for the same sequence of calls (block ids, order,
 // reference counts, free-queue order).
+#include <algorithm>
 #include <cstdint>
 #include <cstring>
 #include <mutex>
@@ -310,6 +311,37 @@ extern "C" int32_t pa_bm_ref_count(pa_block_manager* h, int32_t block_id) {
     return fail(PA_ERR_INVALID_ARGUMENT, "pa_bm_ref_count: bad block id");
   std::lock_guard<std::mutex> g(h->m.mu);
   return h->m.ref[block_id];
+}
+
+extern "C" int32_t pa_bm_shared_prefixes(pa_block_manager* h, const int64_t* seq_ids, int32_t n, int32_t* cu_groups,
+                                         int32_t* shared_lens) {
+  if (!h || n < 0 || !cu_groups || (n > 0 && (!seq_ids || !shared_lens)))
+    return fail(PA_ERR_INVALID_ARGUMENT, "pa_bm_shared_prefixes: bad arguments");
+  BlockManager& m = h->m;
+  std::lock_guard<std::mutex> g(m.mu);
+  static const std::vector<int32_t> kNone;
+  auto table = [&](int32_t i) -> const std::vector<int32_t>& {
+    auto it = m.seqs.find(seq_ids[i]);
+    return it == m.seqs.end() ? kNone : it->second.table;
+  };
+  int32_t groups = 0;
+  for (int32_t first = 0; first < n;) {
+    const std::vector<int32_t>& head = table(first);
+    int64_t common = (int64_t)head.size(), members = 1;
+    for (int32_t i = first + 1; i < n; ++i) {
+      const std::vector<int32_t>& t = table(i);
+      int64_t c = 0;
+      while (c < common && c < (int64_t)t.size() && t[c] == head[c]) ++c;
+      if (c == 0 || members * c < (members - 1) * common) break;
+      common = c;
+      ++members;
+    }
+    cu_groups[groups] = first;
+    shared_lens[groups++] = members > 1 ? (int32_t)std::min<int64_t>(common * m.block_size, INT32_MAX) : 0;
+    first += (int32_t)members;
+  }
+  cu_groups[groups] = n;
+  return groups;
 }
 
 extern "C" int32_t pa_bm_take_copies(pa_block_manager* h, int32_t* src, int32_t* dst, int32_t capacity) {

@@ -360,8 +360,10 @@ template <int D>
 constexpr int kPartFloats = kPartO<D> + 2 * 32;
 
 // One prefill work item (kSplit: one part of it), run by a whole 512-thread
-// workgroup.
-template <bool kSoftCap, int kPaging, int D = kPHeadDim, bool kSplit = false>
+// workgroup.  kExactQ: q keeps its bits and the scale is a factor of the
+// exponent (a multiplication an element more), where the parts meet others that
+// do not round q either.
+template <bool kSoftCap, int kPaging, int D = kPHeadDim, bool kSplit = false, bool kExactQ = false>
 __device__ __forceinline__ void prefill_run(const PrefillParams& p, const PrefillWork& w,
                                             const PrefillPart& part = {0, INT_MAX, -1}) {
   const int base = kSplit ? part.lo : 0;  // first tile; the loop counts from it
@@ -472,7 +474,16 @@ __device__ __forceinline__ void prefill_run(const PrefillParams& p, const Prefil
   // read before any wave passes the barrier below (then tile 2 may overwrite
   // stage 2)
   wait_vm_lgkm0<0>();
-  if constexpr (!kSoftCap) {
+  // (kExactQ) the exponent's factor: positive, q takes a negative scale's sign
+  const float q_factor = kExactQ && !kSoftCap ? fmaxf(fabsf(p.logit_scale), 1e-30f) : 1.f;
+  if constexpr (kExactQ && !kSoftCap) {
+    const uint32_t sign = p.logit_scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int ks = 0; ks < A::kKs; ++ks) {
+      const u32x4 w = __builtin_bit_cast(u32x4, qt_op[ks]);
+      qt_op[ks] = as_bf16x8(u32x4{w[0] ^ sign, w[1] ^ sign, w[2] ^ sign, w[3] ^ sign});
+    }
+  } else if constexpr (!kSoftCap) {
     // Q^T scaled by scale * log2 e (rounded to bf16), so that S = K Q^T is in
     // log2 units
 #pragma unroll
@@ -745,10 +756,10 @@ __device__ __forceinline__ void prefill_run(const PrefillParams& p, const Prefil
       // S is already relative to m_ref.  The first tile sets m_ref to the row
       // max (a row that sees no key keeps 0); later the reference moves only
       // when a row max exceeds it by more than the slack (any lane).
-      if (t == 0 || __any(mx > kRescaleSlack)) {
+      if (t == 0 || __any(mx * q_factor > kRescaleSlack)) {
         const float d = t == 0 ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
         if (t != 0) {
-          const float corr = fast_exp2(-d);
+          const float corr = fast_exp2(-d * q_factor);
 #pragma unroll
           for (int u = 0; u < kL; ++u) l_part[u] *= corr;
 #pragma unroll
@@ -771,8 +782,8 @@ __device__ __forceinline__ void prefill_run(const PrefillParams& p, const Prefil
       u32x4 w;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float a = fast_exp2(s_acc[mt][base + 2 * e]);
-        const float c = fast_exp2(s_acc[mt][base + 2 * e + 1]);
+        const float a = fast_exp2(s_acc[mt][base + 2 * e] * q_factor);
+        const float c = fast_exp2(s_acc[mt][base + 2 * e + 1] * q_factor);
         w[e] = pack_bf16x2(a, c);
         l_part[u % kL] += a + c;
       }
@@ -961,7 +972,7 @@ __device__ __forceinline__ void prefill_run(const PrefillParams& p, const Prefil
         }
       // a row that saw no key here carries no weight, whatever its reference
       if (h == 0)
-        *reinterpret_cast<f32x2*>(dst + kPartO<D> + 2 * n) = f32x2{l_run > 0.f ? m_ref : -INFINITY, l_run};
+        *reinterpret_cast<f32x2*>(dst + kPartO<D> + 2 * n) = f32x2{l_run > 0.f ? m_ref * q_factor : -INFINITY, l_run};
       return;
     }
   }

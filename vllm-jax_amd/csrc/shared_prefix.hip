@@ -440,7 +440,7 @@ shared_tile_kernel(SharedParams p) {
   part.lo = e[5];
   part.hi = e[6];
   part.slot = e[7] + kvh * e[8];
-  prefill_run<kSoftCap, kPaging, kPHeadDim, true>(p.pre, w, part);
+  prefill_run<kSoftCap, kPaging, kPHeadDim, true, true>(p.pre, w, part);
 }
 
 // The chunk of a rank, for the kv head and block of 16 q heads vh.

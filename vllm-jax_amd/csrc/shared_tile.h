@@ -71,7 +71,7 @@ __device__ __forceinline__ void lt_run(const LtParams& p, const int32_t* bt_row,
     for (int ks = 0; ks < 8; ++ks) qt[ks] = as_bf16x8(ld16(src + 16 * ks));
   }
   // the exponent's factor is positive: q takes a negative scale's sign
-  const float c = kSoftCap ? 1.f : fabsf(p.logit_scale);
+  const float c = kSoftCap ? 1.f : fmaxf(fabsf(p.logit_scale), 1e-30f);  // (-inf times it stays -inf)
   if (!kSoftCap && p.logit_scale < 0.f) {
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {

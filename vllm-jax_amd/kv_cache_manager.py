@@ -116,6 +116,20 @@ class KVCacheManager:
     def ref_count(self, block_id: int) -> int:
         return int(self._lib.pa_bm_ref_count(self._h, int(block_id)))
 
+    def shared_prefixes(self, requests: Sequence) -> Tuple[List[int], List[int]]:
+        """Groups of a batch's requests, in its order, that share their leading
+        blocks, as ``SharedPrefixes.of`` takes them: ``(cu_groups, shared_lens)``,
+        group ``g`` being requests ``cu_groups[g] .. cu_groups[g + 1] - 1``.
+        Neighbours are put together as long as that saves block reads; a request
+        alone shares 0 tokens."""
+        n = len(requests)
+        ids = np.fromiter((int(r.id) for r in requests), np.int64, n)
+        cu, shared = np.zeros(n + 1, np.int32), np.zeros(max(n, 1), np.int32)
+        groups = self._lib.pa_bm_shared_prefixes(self._h, ids.ctypes.data, n, cu.ctypes.data, shared.ctypes.data)
+        if groups < 0:
+            _lib.check("pa_bm_shared_prefixes", groups)
+        return cu[:groups + 1].tolist(), shared[:groups].tolist()
+
     def take_block_copies(self) -> Tuple[List[int], List[int]]:
         """Queued copy-on-write page copies (src, dst); the queue is cleared."""
         n = self._lib.pa_bm_take_copies(self._h, None, None, 0)

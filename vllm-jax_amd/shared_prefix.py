@@ -10,7 +10,8 @@ by their log-sum-exp.  The result is that of ``decode_paged_attention`` and
 ``prefill_paged_attention`` up to rounding.
 
 The block manager finds the groups of a step (``KVCacheManager.shared_prefixes``);
-a step's metadata carries them to ``attention()`` (``shared=``).
+a step's metadata carries them to ``attention()`` (``SharedDecodeAttentionMetadata``,
+``SharedPrefillAttentionMetadata``).
 """
 from __future__ import annotations
 
@@ -77,9 +78,8 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     first sequence that has tokens.  Groups do not overlap; sequences outside them
     share nothing.  Cached rows below a length have to be finite.
 
-    Scores, softmax statistics and sums are 32-bit; the scaled q of the shared
-    part (and of several new tokens) and the weights are rounded to bf16 for the
-    matrix cores.  How the parts are cut follows the whole batch, and with it a
+    Scores, softmax statistics and sums are 32-bit; the weights are rounded to
+    bf16 for the matrix cores, and q is not rounded again.  How the parts are cut follows the whole batch, and with it a
     row's last bits.  One new token a sequence is computed by the plain decode
     where sharing does not pay (:func:`shared_prefix_pays`).  The workspace (``shared_prefix_workspace_bytes``) is made
     here if it is not given or too small.
