@@ -56,9 +56,10 @@ def test_bounds_of_more_new_tokens_than_said(dev):
     table, nb = ref.tables([900, 40], 64, gen)
     cache = ref.pool(nb, 64, 2, 128, gen)
     before = torch.zeros((nb, 4, 2, 2, 128), dtype=torch.bfloat16)
-    got = PKG.update_block_bounds(before.to(dev), cache.to(dev), table.to(dev), _i32([900, 40], dev),
-                                  _i32([0, 900, 940], dev), max_seqlen_q=1)
-    assert torch.equal(got.cpu(), ref.bounds(cache, table, [900, 40], [900, 40], 16, before))
+    for most in (0, 1, 900, 1 << 30):
+        got = PKG.update_block_bounds(before.to(dev), cache.to(dev), table.to(dev), _i32([900, 40], dev),
+                                      _i32([0, 900, 940], dev), max_seqlen_q=most)
+        assert torch.equal(got.cpu(), ref.bounds(cache, table, [900, 40], [900, 40], 16, before))
 
 
 def test_bounds_leave_other_pages(dev):
@@ -392,7 +393,7 @@ def test_a_conversation(dev):
         q, k, v, slots, pos = step([1] * 3, now)
         lens = _i32(now, dev)
         if i == 2:  # as part of a mixed step without prefill sequences
-            meta = PKG.MixedAttentionMetadata(pos, slots, tdev, _i32([0, 1, 2, 3], dev), lens, 3, 1)
+            meta = PKG.MixedAttentionMetadata(pos, slots, tdev, _i32([0, 1, 2, 3], dev), lens, 3, 0)
         else:
             meta = PKG.DecodeAttentionMetadata(pos, slots, tdev, lens)
         _, out = PKG.block_sparse_attention(cache, bounds, q.to(dev), k, v, meta, num_selected=num)

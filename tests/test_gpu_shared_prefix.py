@@ -121,6 +121,35 @@ def test_long_prefix(dev):
     _check(Batch([(300, [5, 90, 700, 1])], 64, 2, gen), 8, dev, gen, new=[5, 20, 3, 1], zero_q=True)
 
 
+@pytest.mark.parametrize("new", [None, 2])
+def test_more_sequences_than_the_plan_keeps_in_lds(new, dev):
+    gen = _gen(13)
+    batch = Batch([(4, [1 + (g + i) % 30 for i in range(3)]) for g in range(700)], 16, 1, gen)
+    _check(batch, 2, dev, gen, new=new and [min(new, n - 64) for n in batch.lengths], zero_q=True)
+
+
+def test_more_chunks_than_workgroups(dev):
+    """Long own parts of 256 q heads a kv head: a workgroup takes several chunks."""
+    gen = _gen(14)
+    _check(Batch([(0, [20000]), (4, [9000, 100])], 16, 2, gen), 512, dev, gen, zero_q=True)
+
+
+def test_scales_of_any_sign(dev):
+    gen = _gen(15)
+    for new in (None, [3, 1, 2], [70, 1, 100]):
+        batch = Batch([(4, [100, 7 if new is None else 107, 300])], 64, 2, gen)
+        n = sum(new) if new else 3
+        q = torch.randn((n, 8, 128), generator=gen).to(torch.bfloat16)
+        cu = None if new is None else _i32([0, *torch.tensor(new).cumsum(0).tolist()], dev)
+        for scale in (-0.09, 0.0):
+            want, _ = ref.shared(q, batch.cache, batch.table, batch.lengths, new or [1] * 3, scale)
+            flipped, tol = ref.shared(-q if scale < 0 else q, batch.cache, batch.table, batch.lengths, new or [1] * 3,
+                                      abs(scale))
+            assert torch.allclose(flipped, want)
+            got = PKG.shared_prefix_attention(q.to(dev), *batch.args(dev), cu, max_seqlen_q=max(new or [1]), scale=scale)
+            assert ((got.cpu().double() - want).abs() <= tol).all(), (new, scale)
+
+
 def test_matches_the_entries_it_stands_beside(dev):
     """Decode and prefill of the same sequences without sharing, up to both kernels' roundings."""
     gen = _gen(5)

@@ -76,7 +76,7 @@ def test_block_refusals(call):
 
 
 def test_bounds_refusals():
-    assert _bounds(most=0) == 0 and _bounds(pps=0) == 0
+    assert _bounds(pps=0) == 0
     assert _bounds(most=-1) == -1
     assert _bounds(k=FAKE + 8) == -2 and "aligned" in _err()
     assert _bounds(bounds=FAKE + 2) == -2

@@ -75,7 +75,8 @@ def update_block_bounds(bounds: torch.Tensor, kv_cache: torch.Tensor, block_tabl
     The tokens' keys are in the pool already (``update_kv_cache``).  A block is
     computed from all its keys below the length, so that what a reused page held
     before does not show; other blocks' bounds are left as they were.  Blocks
-    whose table entry is not a page of the pool are left out.
+    whose table entry is not a page of the pool are left out.  Two sequences of
+    a call with new tokens in one block race, as their stores do.
     """
     (nb, per, hkv, _, d), bounds_stride = _check_bounds(bounds)
     (cache_nb, bs, cache_hkv, cache_d), cache_stride = check_pool(kv_cache, bounds)

@@ -447,7 +447,7 @@ extern "C" int pa_block_bounds(const uint16_t* k_cache, int32_t num_pages, int32
     return rc;
   if (max_seqlen_q < 0) return fail(PA_ERR_INVALID_ARGUMENT, "%s: max_seqlen_q %d", name, max_seqlen_q);
   if (num_kv_heads > (1 << 16)) return fail(PA_ERR_UNSUPPORTED, "%s: %d kv heads", name, num_kv_heads);
-  if (batch == 0 || pages_per_seq == 0 || max_seqlen_q == 0) return PA_OK;
+  if (batch == 0 || pages_per_seq == 0) return PA_OK;
   if (!k_cache || !block_tables || !lengths || !bounds)
     return fail(PA_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
   if ((((uintptr_t)k_cache | (uintptr_t)bounds) & 15u) ||
@@ -470,7 +470,7 @@ extern "C" int pa_block_bounds(const uint16_t* k_cache, int32_t num_pages, int32
   p.chunks = num_kv_heads * p.chunks_per_head;
   p.parts = (p.chunks + 63) / 64;
   const int64_t span = (int64_t)pages_per_seq * page_size;
-  const int64_t most = cu_seqlens_q ? std::min<int64_t>(max_seqlen_q, span) : 1;
+  const int64_t most = cu_seqlens_q ? std::min<int64_t>(std::max(max_seqlen_q, 1), span) : 1;
   // blocks that so many tokens touch; a workgroup takes several where one
   // launch could not hold them all
   const int64_t touched = std::min<int64_t>((most + block - 2) / block + 1, (span + block - 1) / block);

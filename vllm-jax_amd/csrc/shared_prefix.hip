@@ -821,8 +821,7 @@ extern "C" int pa_shared_prefix(const uint16_t* q, int64_t q_tok_stride, int64_t
   hipStream_t s = (hipStream_t)stream;
   const bool cap = soft_cap > 0.f;
   const int64_t merges = ((int64_t)num_tokens * group + 31) / 32 * num_kv_heads;
-  if (z.tiles * num_kv_heads > kMaxGrid || z.chunks * num_kv_heads * d.hblocks > 4 * kMaxGrid ||
-      merges > 4 * kMaxGrid)
+  if (z.tiles * num_kv_heads > kMaxGrid || z.chunks * num_kv_heads * d.hblocks > 2 * kMaxGrid || merges > 4 * kMaxGrid)
     return fail(PA_ERR_UNSUPPORTED, "%s: %lld parts of %lld rows", name, (long long)(z.tiles + z.chunks),
                 (long long)merges * 32);
   const bool small = batch <= 256 && num_groups <= 256;  // (short barriers where few threads do)
