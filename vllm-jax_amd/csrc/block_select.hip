@@ -31,9 +31,11 @@ struct BoundsParams {
 // Bounds of one block for 64 chunks (8 elements each) of its tokens' keys: wave
 // w takes rows w, w + 4, ..., and the four meet in LDS.  Bound by the reads of
 // the block's rows (whole 16-byte chunks of consecutive lanes), four (blocks of 16
-// tokens) or eight of them in flight a lane.  A block is computed from all its rows in the pool, not
-// from its old bounds and the new rows: a block that a page held before never
-// shows through, and the order in which tokens came does not matter.
+// tokens) or eight of them in flight a lane.  A block is computed from all its
+// rows in the pool, not from its old bounds and the new rows: a block that a page
+// held before never shows through, and the order in which tokens came does not
+// matter.  256 sequences' newest token, blocks of 32, 8 kv heads of 128: 4.8 us;
+// 20k new tokens of 8 prompts, blocks of 16: 11.5 us, 4.3 TB/s.
 template <int kRowsInFlight>
 __global__ void __launch_bounds__(256)
 block_bounds_kernel(BoundsParams p) {
@@ -134,7 +136,9 @@ constexpr int kScoreBlocks = 16;  // blocks of a wave task: the rows of an MFMA
 // of q, whose products are exact and whose sums are 32-bit.  Bound by the reads of
 // the bounds (4 d bytes a block and kv head), which come through LDS as whole rows
 // (chunk c of row r at c ^ r, so that 16 rows' reads of one chunk land on distinct
-// banks).
+// banks).  64 contexts of 16k to 64k tokens, blocks of 32, 8 kv heads of 128: 60
+// us, 5.3 TB/s; loaded straight into the operand's layout, 64 bytes of a row at a
+// time, 14 us more, and then two or four times the blocks a wave 2 and 21 more.
 template <int D>
 __global__ void __launch_bounds__(256)
 block_scores_kernel(ScoresParams p) {
@@ -228,9 +232,11 @@ __device__ __forceinline__ uint32_t score_key(uint32_t u) {
 }
 
 // One workgroup a (sequence, kv head): the k-th largest key, bit by bit (one
-// wave) or by histograms of its digits, then the blocks in order.  A thread keeps its keys in registers
-// (kPer of them; 0: reads them again), key j of thread t being candidate j *
-// threads + t, so that counts are ballots and their sums scalar.
+// wave) or by histograms of its digits, then the blocks in order.  A thread keeps
+// its keys in registers (kPer of them; 0: reads them again), key j of thread t
+// being candidate j * threads + t, so that counts are ballots and their sums
+// scalar.  Bound by its chain of steps: 250 candidates 4.2 us, of which 3.5 are the
+// launch and the loads; 512 workgroups of up to 4096 10 us, bit by bit 17.8.
 template <int kWavesN, int kPer>
 __global__ void __launch_bounds__(64 * kWavesN)
 select_blocks_kernel(SelectParams p) {

@@ -17,6 +17,10 @@
 //   shared_tile_kernel    both by prefill_run's loop (256 rows against 64-token
 //                         tiles), where sequences have many new tokens
 //   shared_merge_kernel   adds the parts up
+//
+// 128 sequences of 64 to 1024 own tokens behind 8192 shared ones, 32 / 8 heads: plan
+// 6.7 us, parts 64 (the tiles alone 42, the chunks alone 50), merge 6.0; the plain
+// decode of the same step takes 573.
 #include <algorithm>
 #include <type_traits>
 
@@ -418,7 +422,10 @@ shared_plan_kernel(SharedParams p) {
   }
 }
 
-// Parts of 256-row tiles: workgroup = (part, kv head).
+// Parts of 256-row tiles: workgroup = (part, kv head).  64 questions of 20 to 100
+// tokens about 32 768 shared ones, 32 / 8 heads: 1.1 PFLOP/s; with q rounded once
+// more, scale included, as the plain prefill has it, 6 % less time and an error of
+// 0.29 % of the output's norm in place of 0.23 %.
 template <bool kSoftCap, int kPaging>
 __global__ void __launch_bounds__(kThreads, 1)
 shared_tile_kernel(SharedParams p) {

@@ -13,7 +13,10 @@
 // and at most 256 registers a wave: two workgroups a CU, so that one's products
 // run under the other's softmax, or, beside decode_run's workgroups, under their
 // loads.  q is not scaled (and not rounded again): the scale is a factor of the
-// exponent.
+// exponent.  512 rows a kv head (32 / 8 heads): 895 TFLOP/s from one shared length
+// to the next, two workgroups a CU; by their counts, LDS reads (an operand feeds
+// one wave's 32 rows) and matrix instructions then take the same time.  A fifth
+// stage gained nothing.
 #pragma once
 
 #include <type_traits>
