@@ -159,6 +159,8 @@ def test_tensors_off_the_device():
                  lambda: PKG.shared_prefix_attention(q, cache, table, lens, prefixes, scale=1.0)):
         with pytest.raises(ValueError, match="HIP device"):
             call()
+    with pytest.raises(TypeError, match="SharedPrefixes"):
+        PKG.shared_prefix_attention(q, cache, table, lens, ([0, 2], [64]), scale=1.0)
     for block in (0, 8, 24, 128, 16.0):
         with pytest.raises(ValueError, match="multiple of 16"):
             PKG.new_block_bounds(cache, block)

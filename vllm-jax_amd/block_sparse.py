@@ -82,8 +82,9 @@ def update_block_bounds(bounds: torch.Tensor, kv_cache: torch.Tensor, block_tabl
     (cache_nb, bs, cache_hkv, cache_d), cache_stride = check_pool(kv_cache, bounds)
     if (cache_nb, cache_hkv, cache_d) != (nb, hkv, d) or per == 0 or bs % per:
         raise ValueError(f"bounds {tuple(bounds.shape)} do not fit a pool {tuple(kv_cache.shape)}")
-    lens = check_tokens("lengths", lengths, lengths.shape[0], bounds)
-    batch = lens.shape[0]
+    require_device("lengths", lengths)
+    batch = lengths.numel()
+    lens = check_tokens("lengths", lengths, batch, bounds)
     table, _keep = check_table(block_tables, batch, bounds)
     cu = None if cu_seqlens_q is None else check_tokens("cu_seqlens_q", cu_seqlens_q, batch + 1, bounds)
     if not 0 <= max_seqlen_q <= 0x7fffffff:

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from ._operands import check_heads, check_output, check_pool, check_table, check_workspace
-from .kernels._common import pool_pointers, stream_handle
+from .kernels._common import pool_pointers, require_device, stream_handle
 from .kernels.decode_paged_attention import decode_checked
 from .rotary import check_tokens, on_device
 
@@ -84,16 +84,17 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     where sharing does not pay (:func:`shared_prefix_pays`).  The workspace (``shared_prefix_workspace_bytes``) is made
     here if it is not given or too small.
     """
+    if not isinstance(prefixes, SharedPrefixes):
+        raise TypeError(f"prefixes must be SharedPrefixes, got {type(prefixes).__name__}")
     (nb, bs, hkv, d), cache_stride = check_pool(kv_cache)
     q_stride = check_heads(q, hkv, d)
     if kv_cache.get_device() != q.get_device():
         raise ValueError(f"kv_cache lives on {kv_cache.device}, q on {q.device}")
-    if not isinstance(prefixes, SharedPrefixes):
-        raise TypeError(f"prefixes must be SharedPrefixes, got {type(prefixes).__name__}")
     tokens, heads, _ = q.shape
     if cu_seqlens_q is None:
         batch, cu, longest = tokens, None, 1
     else:
+        require_device("cu_seqlens_q", cu_seqlens_q)
         if cu_seqlens_q.dim() != 1 or cu_seqlens_q.numel() < 1:
             raise ValueError(f"cu_seqlens_q must be int32 [B + 1], got {tuple(cu_seqlens_q.shape)}")
         batch, longest = cu_seqlens_q.numel() - 1, max_seqlen_q
@@ -102,6 +103,7 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
         raise ValueError(f"max_seqlen_q {max_seqlen_q}")
     table, _keep = check_table(block_tables, batch, q)
     lens = check_tokens("lengths", lengths, batch, q)
+    require_device("shared_lens", prefixes.shared_lens)
     groups = prefixes.shared_lens.numel()
     cu_groups = check_tokens("cu_groups", prefixes.cu_groups, groups + 1, q)
     shared = check_tokens("shared_lens", prefixes.shared_lens, groups, q)
