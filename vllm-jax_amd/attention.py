@@ -34,7 +34,7 @@ from .kernels._common import (bf16_round, inv_sqrt_head_dim_bf16, pool_pointers,
 from .kernels.decode_paged_attention import decode_paged_attention, decode_pool
 from .kernels.mixed_paged_attention import mixed_paged_attention
 from .kernels.prefill_paged_attention import prefill_paged_attention, prefill_pool
-from .shared_prefix import SharedPrefixes, shared_prefix_attention
+from .shared_prefix import SharedPrefixes, check_shared, shared_prefix_attention
 
 USE_DECODE_PAGED_ATTENTION_KERNEL = True
 USE_PREFILL_PAGED_ATTENTION_KERNEL = True
@@ -271,6 +271,8 @@ def update_kv_cache_fp8(kv_codes: torch.Tensor, kv_scales: torch.Tensor, slot_ma
 def attention(kv_cache: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
               metadata: AttentionMetadata) -> Tuple[torch.Tensor, torch.Tensor]:
     """qwen3.py:172-218 on gfx950 kernels; returns ``(kv_cache, out)``."""
+    if getattr(metadata, "shared", None) is not None:
+        check_shared(q, kv_cache, metadata.shared)
     kv_cache = update_kv_cache(kv_cache, metadata.slot_mapping, k, v)
     return kv_cache, attention_stored(kv_cache, q, metadata)
 
@@ -283,6 +285,8 @@ def qwen3_attention_core(kv_cache: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     projections and o_proj (qwen3.py:287-299): q/k RMSNorm + RoPE and the KV
     store in one fused kernel, then paged attention.  Returns
     ``(kv_cache, out)``."""
+    if getattr(metadata, "shared", None) is not None:
+        check_shared(q, kv_cache, metadata.shared)
     q_rot, kv_cache = qk_norm_rope_store(q, k, v, q_norm_weight, k_norm_weight, metadata.input_positions,
                                          metadata.slot_mapping, kv_cache, eps=eps, rope_theta=rope_theta,
                                          rope_scaling=rope_scaling)
@@ -310,8 +314,6 @@ def attention_stored(kv_cache: torch.Tensor, q: torch.Tensor, metadata: Attentio
     # half goes in as page views
     pool = isinstance(kv_cache, torch.Tensor) and kv_cache.dim() == 5 and kv_cache.shape[0] >= 2
     if getattr(metadata, "shared", None) is not None:
-        if not pool:
-            raise ValueError("shared prefixes need the pool [2, NB, BS, Hkv, d]")
         return _attention_shared(kv_cache, q, metadata)
     if isinstance(metadata, MixedAttentionMetadata) or not pool:
         k_pages = kv_cache[0].permute(2, 0, 1, 3)   # [Hkv, NB, BS, d] view

@@ -27,6 +27,10 @@ from .kernels.decode_paged_attention import decode_checked
 from .rotary import check_tokens, on_device
 
 
+HEAD_DIM = 128   # the head size of the kernels of shared prefixes
+MAX_GROUP = 256  # and the most q heads a kv head
+
+
 @dataclass
 class SharedPrefixes:
     """Groups of a batch's sequences: group ``g`` is sequences ``cu_groups[g] ..
@@ -55,6 +59,20 @@ def shared_prefix_pays(batch: int, num_groups: int, num_kv_heads: int, span: int
     return batch > num_groups > 0 and batch * span * num_kv_heads * 512 >= 256 << 20
 
 
+def check_shared(q: torch.Tensor, kv_cache: torch.Tensor, prefixes: SharedPrefixes) -> None:
+    """Refuses what the kernels of shared prefixes do not take, by shapes alone: the answer does not follow the
+    route that a step's size chooses, and ``attention()`` has it before it stores the step's keys and values."""
+    if not isinstance(prefixes, SharedPrefixes):
+        raise TypeError(f"prefixes must be SharedPrefixes, got {type(prefixes).__name__}")
+    if not isinstance(kv_cache, torch.Tensor) or kv_cache.dim() != 5 or kv_cache.shape[0] != 2:
+        raise ValueError("shared prefixes need the pool [2, NB, BS, Hkv, d]")
+    hkv, d = kv_cache.shape[3:]
+    if d != HEAD_DIM:
+        raise ValueError(f"shared prefixes need a head size of {HEAD_DIM}, got {d}")
+    if q.dim() == 3 and q.shape[1] > MAX_GROUP * hkv:
+        raise ValueError(f"shared prefixes take up to {MAX_GROUP} q heads a kv head, got {q.shape[1]} for {hkv}")
+
+
 def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor,
                             lengths: torch.Tensor, prefixes: SharedPrefixes,
                             cu_seqlens_q: Optional[torch.Tensor] = None, *, max_seqlen_q: int = 1, scale: float,
@@ -76,7 +94,8 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     down to 64 tokens and cut to the shortest length of its group (sequences
     of no tokens aside), and the shared tokens are read through the table of the group's
     first sequence that has tokens.  Groups do not overlap; sequences outside them
-    share nothing.  Cached rows below a length have to be finite.
+    share nothing.  Cached rows below a length have to be finite.  Other head sizes
+    and more than 256 q heads a kv head are refused, whatever the tables' width.
 
     Scores, softmax statistics and sums are 32-bit; the weights are rounded to
     bf16 for the matrix cores, and q is not rounded again.  How the parts are cut follows the whole batch, and with it a
@@ -84,8 +103,7 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     where sharing does not pay (:func:`shared_prefix_pays`).  The workspace (``shared_prefix_workspace_bytes``) is made
     here if it is not given or too small.
     """
-    if not isinstance(prefixes, SharedPrefixes):
-        raise TypeError(f"prefixes must be SharedPrefixes, got {type(prefixes).__name__}")
+    check_shared(q, kv_cache, prefixes)
     (nb, bs, hkv, d), cache_stride = check_pool(kv_cache)
     q_stride = check_heads(q, hkv, d)
     if kv_cache.get_device() != q.get_device():
