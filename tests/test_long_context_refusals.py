@@ -62,3 +62,71 @@ def test_attention_refuses_groups_before_the_store(prefill, monkeypatch):
         with pytest.raises(error, match=message):
             PKG.qwen3_attention_core(cache, q, k, k, w, w, meta(shared), eps=1e-6, rope_theta=1e6)
     assert not stored
+
+
+# ---------------------------------------------------------------------------
+# selected blocks
+# ---------------------------------------------------------------------------
+SPARSE = importlib.import_module(PKG.__name__ + ".block_sparse")
+
+
+def _steps(batch, pages, shared=None):
+    """A decode, a prefill and a mixed step of ``batch`` sequences by one token."""
+    row, table, cu = _i32(batch), _i32(batch, pages), _i32(batch + 1)
+    return [PKG.SharedDecodeAttentionMetadata(row, row, table, row, shared=shared),
+            PKG.SharedPrefillAttentionMetadata(row, row, table, cu, cu, None, None, 1, shared=shared),
+            PKG.MixedAttentionMetadata(row, row, table, cu, row, batch, 1)]
+
+
+@pytest.mark.parametrize("pages", [1, 300])
+def test_sparse_attention_refuses_before_the_store(pages, monkeypatch):
+    """Tables narrower than the selection (whole contexts, by attention()) and wider ones."""
+    stored = []
+    monkeypatch.setattr(SPARSE, "update_kv_cache", lambda cache, *a: stored.append(1) or cache)
+    monkeypatch.setattr(SPARSE, "update_block_bounds", lambda *a, **k: stored.append(1))
+    cache = _bf16(2, 3, 512, 2, 128)
+    fine = dict(cache=cache, bounds=_bf16(3, 4, 2, 2, 128), num=8)
+
+    def call(m, cache, bounds, num, **kw):
+        d = cache.shape[-1]
+        PKG.block_sparse_attention(cache, bounds, _bf16(2, 8, d), _bf16(2, 2, d), _bf16(2, 2, d), m, num_selected=num, **kw)
+
+    cases = [(dict(bounds=_bf16(3, 1, 2, 2, 128)), "blocks of 512"),
+             (dict(cache=_bf16(2, 3, 512, 2, 96), bounds=_bf16(3, 4, 2, 2, 96)), "head size 96"),
+             (dict(bounds=_bf16(3, 64, 2, 2, 128)), "multiple of 16"),
+             (dict(bounds=_bf16(3, 3, 2, 2, 128)), "do not fit"),
+             (dict(bounds=_bf16(3, 0, 2, 2, 128)), "do not fit"),
+             (dict(bounds=_bf16(2, 4, 2, 2, 128)), "do not fit"),
+             (dict(bounds=_bf16(3, 4, 2, 128)), "bounds must be"),
+             (dict(cache=cache[0]), "kv_cache must be"),
+             (dict(num=0), "num_selected 0"),
+             (dict(num=2), "num_selected 2"),
+             (dict(num=4, first=3, recent=2), "the first 3")]
+    for m in _steps(2, pages):
+        for over, message in cases:
+            with pytest.raises(ValueError, match=message):
+                call(m, **{**fine, **over})
+    groups = PKG.SharedPrefixes.of([0, 2], [64], "cpu")
+    for m in _steps(2, pages, groups)[:2]:
+        with pytest.raises(ValueError, match="head size"):
+            call(m, _bf16(2, 3, 512, 2, 64), _bf16(3, 4, 2, 2, 64), 8)
+    for decodes in (-1, 3):
+        m = _steps(2, pages)[2]
+        m.num_decodes = decodes
+        with pytest.raises(ValueError, match=f"num_decodes {decodes}"):
+            call(m, **fine)
+    m = _steps(3, pages)[2]  # three decode sequences, two tokens
+    with pytest.raises(ValueError, match="num_decodes 3"):
+        call(m, **fine)
+    with pytest.raises(TypeError, match="metadata"):
+        call(None, **fine)
+    assert not stored
+
+
+def test_bounds_that_no_decode_takes():
+    for block in (512, 1024):
+        with pytest.raises(ValueError, match=f"blocks of {block}"):
+            PKG.new_block_bounds(_bf16(2, 3, 1024, 2, 128), block)
+    with pytest.raises(ValueError, match="head size 96"):
+        PKG.new_block_bounds(_bf16(2, 3, 64, 2, 96), 16)
+    assert PKG.new_block_bounds(_bf16(2, 3, 512, 2, 256), 256).shape == (3, 2, 2, 2, 256)

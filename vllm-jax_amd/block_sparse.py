@@ -32,6 +32,7 @@ from .kernels._common import bf16_round, pool_pointers, require_device, stream_h
 from .kernels.mixed_paged_attention import mixed_paged_attention
 from .kv_cache_manager import copy_pages
 from .rotary import check_tokens, on_device
+from .shared_prefix import check_shared
 
 HEAD_DIMS = (64, 128, 256)
 MAX_BLOCK = 256  # tokens of a block that block_sparse_decode_attention takes
@@ -43,6 +44,20 @@ def _check_block(block: int, page_size: int) -> int:
     return block
 
 
+def _check_decode(block: int, head_dim: int) -> None:
+    """What the decode over selected blocks takes."""
+    if block > MAX_BLOCK:
+        raise ValueError(f"blocks of {block} tokens, {MAX_BLOCK} at most")
+    if head_dim not in HEAD_DIMS:
+        raise ValueError(f"head size {head_dim} not supported ({', '.join(map(str, HEAD_DIMS))})")
+
+
+def _check_picks(num_selected: int, first: int, recent: int) -> None:
+    if num_selected <= 0 or first < 0 or recent < 0 or first + recent > num_selected:
+        raise ValueError(f"num_selected {num_selected} must be positive and hold the first {first} and the last "
+                         f"{recent} blocks")
+
+
 def _check_bounds(bounds: torch.Tensor, like: Optional[torch.Tensor] = None):
     """Shape and (page, block, head) strides of bounds ``[NB, blocks, Hkv, 2, d]``."""
     stride = operand("bounds", bounds, 5, like)
@@ -52,15 +67,22 @@ def _check_bounds(bounds: torch.Tensor, like: Optional[torch.Tensor] = None):
     return bounds.shape, stride[:3]
 
 
+def _check_fit(bounds: torch.Tensor, kv_cache: torch.Tensor) -> None:
+    nb, per, hkv, _, d = bounds.shape
+    if (nb, hkv, d) != (kv_cache.shape[1], *kv_cache.shape[3:]) or per == 0 or kv_cache.shape[2] % per:
+        raise ValueError(f"bounds {tuple(bounds.shape)} do not fit a pool {tuple(kv_cache.shape)}")
+
+
 def new_block_bounds(kv_cache: torch.Tensor, block: int) -> torch.Tensor:
     """Bounds for every block of ``block`` tokens of a layer's pool ``[2, NB,
     BS, Hkv, d]``: bf16 ``[NB, BS / block, Hkv, 2, d]``, zero until
     :func:`update_block_bounds` writes them.  ``block`` is a multiple of 16 that
-    divides ``BS``."""
+    divides ``BS``, 256 at most, and ``d`` one of 64, 128 and 256."""
     if kv_cache.dim() != 5 or kv_cache.shape[0] != 2:
         raise ValueError(f"kv_cache must be [2, NB, BS, Hkv, d], got {tuple(kv_cache.shape)}")
     _, nb, bs, hkv, d = kv_cache.shape
     _check_block(block, bs)
+    _check_decode(block, d)
     return torch.zeros((nb, bs // block, hkv, 2, d), dtype=torch.bfloat16, device=kv_cache.device)
 
 
@@ -79,9 +101,8 @@ def update_block_bounds(bounds: torch.Tensor, kv_cache: torch.Tensor, block_tabl
     a call with new tokens in one block race, as their stores do.
     """
     (nb, per, hkv, _, d), bounds_stride = _check_bounds(bounds)
-    (cache_nb, bs, cache_hkv, cache_d), cache_stride = check_pool(kv_cache, bounds)
-    if (cache_nb, cache_hkv, cache_d) != (nb, hkv, d) or per == 0 or bs % per:
-        raise ValueError(f"bounds {tuple(bounds.shape)} do not fit a pool {tuple(kv_cache.shape)}")
+    (_, bs, _, _), cache_stride = check_pool(kv_cache, bounds)
+    _check_fit(bounds, kv_cache)
     require_device("lengths", lengths)
     batch = lengths.numel()
     lens = check_tokens("lengths", lengths, batch, bounds)
@@ -158,9 +179,7 @@ def select_blocks(scores: torch.Tensor, lengths: torch.Tensor, num_selected: int
         raise ValueError(f"scores must be float32 [B, Hkv, blocks], contiguous in the last dimension, got "
                          f"{scores.dtype} {tuple(scores.shape)}")
     batch, hkv, width = scores.shape
-    if num_selected <= 0 or first < 0 or recent < 0 or first + recent > num_selected:
-        raise ValueError(f"num_selected {num_selected} must be positive and hold the first {first} and the last "
-                         f"{recent} blocks")
+    _check_picks(num_selected, first, recent)
     if block <= 0:
         raise ValueError(f"block {block}")
     lens = check_tokens("lengths", lengths, batch, scores)
@@ -236,6 +255,24 @@ def block_sparse_workspace_bytes(batch: int, num_heads: int, num_kv_heads: int, 
                                                                  num_selected, block))
 
 
+def _check_step(kv_cache, bounds, q, m, num_selected, first, recent) -> None:
+    """The seam's arguments by shapes alone, whatever the step and however wide its tables."""
+    if not isinstance(m, (DecodeAttentionMetadata, PrefillAttentionMetadata, MixedAttentionMetadata)):
+        raise TypeError(f"metadata of type {type(m).__name__}")
+    for name, t, pair, shape in (("kv_cache", kv_cache, 0, "[2, NB, BS, Hkv, d]"),
+                                 ("bounds", bounds, 3, "[NB, BS / block, Hkv, 2, d]")):
+        if not isinstance(t, torch.Tensor) or t.dim() != 5 or t.shape[pair] != 2:
+            raise ValueError(f"{name} must be {shape}")
+    _check_fit(bounds, kv_cache)
+    bs, d = kv_cache.shape[2], kv_cache.shape[4]
+    _check_decode(_check_block(bs // bounds.shape[1], bs), d)
+    _check_picks(num_selected, first, recent)
+    if getattr(m, "shared", None) is not None:
+        check_shared(q, kv_cache, m.shared)
+    if isinstance(m, MixedAttentionMetadata) and not 0 <= m.num_decodes <= min(m.block_tables.shape[0], q.shape[0]):
+        raise ValueError(f"num_decodes {m.num_decodes} of {m.block_tables.shape[0]} sequences and {q.shape[0]} tokens")
+
+
 def block_sparse_attention(kv_cache: torch.Tensor, bounds: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
                            v: torch.Tensor, metadata: AttentionMetadata, *, num_selected: int, first: int = 1,
                            recent: int = 2) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -245,8 +282,10 @@ def block_sparse_attention(kv_cache: torch.Tensor, bounds: torch.Tensor, q: torc
     to their whole context.  Returns ``(kv_cache, out)``.
 
     Where the block tables are no wider than ``num_selected`` blocks, decode is
-    ``attention()``'s.
+    ``attention()``'s.  What wider tables would be refused for is refused here too,
+    before anything is stored.
     """
+    _check_step(kv_cache, bounds, q, metadata, num_selected, first, recent)
     kv_cache = update_kv_cache(kv_cache, metadata.slot_mapping, k, v)
     m = metadata
     bs, per = kv_cache.shape[2], bounds.shape[1]
@@ -266,14 +305,10 @@ def block_sparse_attention(kv_cache: torch.Tensor, bounds: torch.Tensor, q: torc
         lens = m.cu_seqlens_k[1:] - m.cu_seqlens_k[:-1]
         update_block_bounds(bounds, kv_cache, m.block_tables, lens, m.cu_seqlens_q, max_seqlen_q=m.max_seqlen_bucket)
         return kv_cache, attention_stored(kv_cache, q, m)
-    if not isinstance(m, MixedAttentionMetadata):
-        raise TypeError(f"metadata of type {type(m).__name__}")
     update_block_bounds(bounds, kv_cache, m.block_tables, m.kv_lens, m.cu_seqlens_q, max_seqlen_q=m.max_seqlen_q)
     nd = m.num_decodes
     if whole or nd == 0:
         return kv_cache, attention_stored(kv_cache, q, m)
-    if not 0 < nd <= m.block_tables.shape[0] or nd > q.shape[0]:
-        raise ValueError(f"num_decodes {nd} of {m.block_tables.shape[0]} sequences and {q.shape[0]} tokens")
     if nd < m.block_tables.shape[0]:
         pages = (kv_cache[0].permute(2, 0, 1, 3), kv_cache[1].permute(2, 0, 1, 3))
         out = mixed_paged_attention(q, *pages, m.block_tables[nd:], m.cu_seqlens_q[nd:], m.kv_lens[nd:],
