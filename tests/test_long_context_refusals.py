@@ -1,6 +1,7 @@
 """What the entries over long contexts refuse, they refuse at every size and before they change anything (no device)."""
 from __future__ import annotations
 
+import contextlib
 import importlib
 
 import pytest
@@ -130,3 +131,57 @@ def test_bounds_that_no_decode_takes():
     with pytest.raises(ValueError, match="head size 96"):
         PKG.new_block_bounds(_bf16(2, 3, 64, 2, 96), 16)
     assert PKG.new_block_bounds(_bf16(2, 3, 512, 2, 256), 256).shape == (3, 2, 2, 2, 256)
+
+
+# ---------------------------------------------------------------------------
+# workspaces
+# ---------------------------------------------------------------------------
+@pytest.fixture
+def host_tensors(monkeypatch):
+    """The entries' checks take host tensors; nothing is launched."""
+    for module in ("shared_prefix", "_operands", "rotary"):
+        monkeypatch.setattr(importlib.import_module(f"{PKG.__name__}.{module}"), "require_device", lambda *a: None)
+    monkeypatch.setattr(PKG.shared_prefix, "on_device", lambda t: contextlib.nullcontext())
+    monkeypatch.setattr(PKG.shared_prefix, "stream_handle", lambda t: None)
+
+
+@pytest.mark.parametrize("pays", [False, True])
+def test_workspaces_that_do_not_fit_are_replaced(pays, host_tensors, monkeypatch):
+    """The plain decode writes through the workspace's address: on either route only one that is contiguous, aligned and
+    large enough gets there."""
+    used = []
+    sp = PKG.shared_prefix
+    monkeypatch.setattr(sp, "decode_checked", lambda *a: used.append((a[8].data_ptr(), a[8].numel() * a[8].element_size(),
+                                                                      a[8].is_contiguous())))
+    monkeypatch.setattr(sp._lib, "call", lambda name, *a: used.append((a[-3], a[-2], True)))
+    monkeypatch.setattr(sp, "shared_prefix_pays", lambda *a: pays)
+    q, cache, table = _bf16(2, 8, 128), _bf16(2, 4, 256, 2, 128), _i32(2, 64)
+    prefixes = PKG.SharedPrefixes.of([0, 2], [64], "cpu")
+    need = PKG.shared_prefix_workspace_bytes(2, 1, 2, 8, 2, 64, 256) if pays else \
+        importlib.import_module(PKG.__name__ + ".kernels.decode_paged_attention").decode_workspace_bytes(2, 8, 128, 64, 256)
+    assert need > 512
+    room = torch.empty(4 * need + 1024, dtype=torch.uint8)
+    at = -room.data_ptr() % 256
+    fits = room[at:at + need]
+    unfit = [room[at + 16:at + 16 + need], room[at:at + need - 1], room[at:at + 2 * need:2], room[:0]]
+    for ws in (fits, room[at:].view(torch.int8)):
+        PKG.shared_prefix_attention(q, cache, table, _i32(2), prefixes, scale=1.0, workspace=ws)
+        assert used.pop()[0] == ws.data_ptr()
+    # (what a new one's address is on the host is the host allocator's matter)
+    for ws in unfit:
+        PKG.shared_prefix_attention(q, cache, table, _i32(2), prefixes, scale=1.0, workspace=ws)
+        ptr, given, contiguous = used.pop()
+        assert given >= need and contiguous and not room.data_ptr() <= ptr < room.data_ptr() + room.numel()
+
+
+@pytest.mark.gpu
+def test_workspaces_off_the_device(dev):
+    """Refused on both routes, by name."""
+    groups = PKG.SharedPrefixes.of([0, 2], [64], dev)
+    q, cache = _bf16(2, 8, 128).to(dev), _bf16(2, 1, 16, 2, 128).to(dev)
+    for pages in (4, 1 << 20):
+        table = _i32(2, 1).to(dev).expand(2, pages)
+        assert PKG.shared_prefix_pays(2, 1, 2, 16 * pages) == (pages > 4)
+        with pytest.raises(ValueError, match="workspace must live on a HIP device"):
+            PKG.shared_prefix_attention(q, cache, table, _i32(2).to(dev), groups, scale=1.0,
+                                        workspace=torch.empty(1 << 20, dtype=torch.uint8))

@@ -23,7 +23,7 @@ import torch
 from . import _lib
 from ._operands import check_heads, check_output, check_pool, check_table, check_workspace
 from .kernels._common import pool_pointers, require_device, stream_handle
-from .kernels.decode_paged_attention import decode_checked
+from .kernels.decode_paged_attention import decode_checked, decode_workspace_bytes
 from .rotary import check_tokens, on_device
 
 
@@ -100,8 +100,9 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     Scores, softmax statistics and sums are 32-bit; the weights are rounded to
     bf16 for the matrix cores, and q is not rounded again.  How the parts are cut follows the whole batch, and with it a
     row's last bits.  One new token a sequence is computed by the plain decode
-    where sharing does not pay (:func:`shared_prefix_pays`).  The workspace (``shared_prefix_workspace_bytes``) is made
-    here if it is not given or too small.
+    where sharing does not pay (:func:`shared_prefix_pays`).  The workspace
+    (``shared_prefix_workspace_bytes``; the plain decode's is smaller) is made here if
+    none is given, or one that is too small, not contiguous or not 256-byte aligned.
     """
     check_shared(q, kv_cache, prefixes)
     (nb, bs, hkv, d), cache_stride = check_pool(kv_cache)
@@ -132,6 +133,8 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     if batch == 0 or longest == 0:
         return out.zero_() if zero_rest else out
     if cu is None and not shared_prefix_pays(batch, groups, hkv, table[2] * bs):
+        if workspace is not None:
+            workspace, _ = check_workspace(workspace, max(1, decode_workspace_bytes(batch, heads, d, table[2], bs)), q)
         return decode_checked(q, (hkv, nb, bs, d), pool_pointers(kv_cache), cache_stride, _keep, lens,
                               attn_logits_soft_cap, scale, workspace, out)
     need = shared_prefix_workspace_bytes(batch, groups, tokens, heads, hkv, table[2], bs,
