@@ -185,3 +185,51 @@ def test_workspaces_off_the_device(dev):
         with pytest.raises(ValueError, match="workspace must live on a HIP device"):
             PKG.shared_prefix_attention(q, cache, table, _i32(2).to(dev), groups, scale=1.0,
                                         workspace=torch.empty(1 << 20, dtype=torch.uint8))
+
+
+# ---------------------------------------------------------------------------
+# steps that share nothing
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("cu_groups", [[0], [0, 1, 2], [0, 0, 2, 2]])
+def test_attention_without_a_shared_token_is_the_plain_one(cu_groups, host_tensors, monkeypatch):
+    """As many groups as sequences (what the block manager returns for unrelated requests), or none: the plain kernels,
+    which put no partials aside; a group of two takes the shared ones."""
+    took = []
+    monkeypatch.setattr(ATTENTION, "prefill_pool", lambda *a, **k: took.append("prefill"))
+    monkeypatch.setattr(ATTENTION, "decode_pool", lambda *a, **k: took.append("decode"))
+    monkeypatch.setattr(ATTENTION, "shared_prefix_attention", lambda *a, **k: took.append("shared"))
+    q, cache = _bf16(2, 8, 128), _bf16(2, 4, 16, 2, 128)
+    groups = PKG.SharedPrefixes.of(cu_groups, [16] * (len(cu_groups) - 1), "cpu")
+    pair = PKG.SharedPrefixes.of([0, 2], [16], "cpu")
+    decode, prefill = _steps(2, 4, groups)[:2]
+    PKG.attention_stored(cache, q, decode)
+    PKG.attention_stored(cache, q, prefill)
+    for m in _steps(2, 4, pair)[:2]:
+        PKG.attention_stored(cache, q, m)
+    assert took == ["decode", "prefill", "shared", "shared"]
+    # groups that do not fit together are refused there too
+    for m in (decode, prefill):
+        m.shared = PKG.SharedPrefixes(_i32(3), _i32(3))
+        with pytest.raises(ValueError, match="cu_groups"):
+            PKG.attention_stored(cache, q, m)
+    assert len(took) == 4
+
+
+@pytest.mark.gpu
+def test_a_step_of_unrelated_requests(dev):
+    """The bits of the same step without groups."""
+    gen = torch.Generator().manual_seed(21)
+    rand = lambda *s: torch.randn(s, generator=gen).to(torch.bfloat16).to(dev)  # noqa: E731
+    i32 = lambda x: torch.as_tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    cache, table = rand(2, 12, 64, 2, 128), i32([[3, 1, 7], [0, 9, 2], [11, 4, 5]])
+    lens, new = [150, 64, 190], [70, 1, 33]
+    q, k, v = rand(104, 8, 128), rand(104, 2, 128), rand(104, 2, 128)
+    pos = [t for n, c in zip(lens, new) for t in range(n - c, n)]
+    slots = [int(table[b, t // 64]) * 64 + t % 64 for b, (n, c) in enumerate(zip(lens, new)) for t in range(n - c, n)]
+    outs = []
+    for shared in (None, PKG.SharedPrefixes.of([0, 1, 2, 3], [0, 0, 0], dev), PKG.SharedPrefixes.of([0], [], dev)):
+        meta = PKG.SharedPrefillAttentionMetadata(i32(pos), i32(slots), table, i32([0, 70, 71, 104]), i32([0, 150, 214, 404]),
+                                                  None, None, 70, shared=shared)
+        outs.append(PKG.attention(cache.clone(), q, k, v, meta))
+    for pool, out in outs[1:]:
+        assert torch.equal(pool, outs[0][0]) and torch.equal(out, outs[0][1])

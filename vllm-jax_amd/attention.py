@@ -34,7 +34,7 @@ from .kernels._common import (bf16_round, inv_sqrt_head_dim_bf16, pool_pointers,
 from .kernels.decode_paged_attention import decode_paged_attention, decode_pool
 from .kernels.mixed_paged_attention import mixed_paged_attention
 from .kernels.prefill_paged_attention import prefill_paged_attention, prefill_pool
-from .shared_prefix import SharedPrefixes, check_shared, shared_prefix_attention
+from .shared_prefix import SharedPrefixes, check_groups, check_shared, shared_prefix_attention
 
 USE_DECODE_PAGED_ATTENTION_KERNEL = True
 USE_PREFILL_PAGED_ATTENTION_KERNEL = True
@@ -74,7 +74,8 @@ class PrefillAttentionMetadata:
 class SharedDecodeAttentionMetadata(DecodeAttentionMetadata):
     """A decode step with the groups of its sequences that share their first
     pages (``KVCacheManager.shared_prefixes``): ``attention()`` reads each shared
-    page once a group.  No reference counterpart."""
+    page once a group.  With as many groups as sequences, or none, it is a step
+    without ``shared``.  No reference counterpart."""
     shared: Optional[SharedPrefixes] = None
 
 
@@ -314,7 +315,11 @@ def attention_stored(kv_cache: torch.Tensor, q: torch.Tensor, metadata: Attentio
     # half goes in as page views
     pool = isinstance(kv_cache, torch.Tensor) and kv_cache.dim() == 5 and kv_cache.shape[0] >= 2
     if getattr(metadata, "shared", None) is not None:
-        return _attention_shared(kv_cache, q, metadata)
+        check_shared(q, kv_cache, metadata.shared)
+        # as many groups as sequences: no two share, and the plain kernels need no partials
+        if 0 < metadata.shared.shared_lens.numel() < metadata.block_tables.shape[0]:
+            return _attention_shared(kv_cache, q, metadata)
+        check_groups(metadata.shared, q)
     if isinstance(metadata, MixedAttentionMetadata) or not pool:
         k_pages = kv_cache[0].permute(2, 0, 1, 3)   # [Hkv, NB, BS, d] view
         v_pages = kv_cache[1].permute(2, 0, 1, 3)

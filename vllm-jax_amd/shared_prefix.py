@@ -73,6 +73,14 @@ def check_shared(q: torch.Tensor, kv_cache: torch.Tensor, prefixes: SharedPrefix
         raise ValueError(f"shared prefixes take up to {MAX_GROUP} q heads a kv head, got {q.shape[1]} for {hkv}")
 
 
+def check_groups(prefixes: SharedPrefixes, like: torch.Tensor):
+    """(groups, cu_groups, shared_lens): their number, and both as the kernels take them."""
+    require_device("shared_lens", prefixes.shared_lens)
+    groups = prefixes.shared_lens.numel()
+    return (groups, check_tokens("cu_groups", prefixes.cu_groups, groups + 1, like),
+            check_tokens("shared_lens", prefixes.shared_lens, groups, like))
+
+
 def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor,
                             lengths: torch.Tensor, prefixes: SharedPrefixes,
                             cu_seqlens_q: Optional[torch.Tensor] = None, *, max_seqlen_q: int = 1, scale: float,
@@ -100,7 +108,9 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     Scores, softmax statistics and sums are 32-bit; the weights are rounded to
     bf16 for the matrix cores, and q is not rounded again.  How the parts are cut follows the whole batch, and with it a
     row's last bits.  One new token a sequence is computed by the plain decode
-    where sharing does not pay (:func:`shared_prefix_pays`).  The workspace
+    where sharing does not pay (:func:`shared_prefix_pays`).  With ``cu_seqlens_q``
+    every row goes through 32-bit partials in the workspace, also where nothing is
+    shared; ``attention()`` takes the plain prefill there.  The workspace
     (``shared_prefix_workspace_bytes``; the plain decode's is smaller) is made here if
     none is given, or one that is too small, not contiguous or not 256-byte aligned.
     """
@@ -122,10 +132,7 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
         raise ValueError(f"max_seqlen_q {max_seqlen_q}")
     table, _keep = check_table(block_tables, batch, q)
     lens = check_tokens("lengths", lengths, batch, q)
-    require_device("shared_lens", prefixes.shared_lens)
-    groups = prefixes.shared_lens.numel()
-    cu_groups = check_tokens("cu_groups", prefixes.cu_groups, groups + 1, q)
-    shared = check_tokens("shared_lens", prefixes.shared_lens, groups, q)
+    groups, cu_groups, shared = check_groups(prefixes, q)
     zero_rest = out is None
     out, out_stride = check_output(out, q)
     if tokens == 0:
