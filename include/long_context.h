@@ -104,7 +104,8 @@ int pa_block_sparse_decode(const uint16_t* q, int64_t q_batch_stride, int64_t q_
  * read once a group, through the block table of its first sequence that has
  * tokens; shared_lens is rounded down to 64 tokens, cut to the group's shortest
  * length (sequences without tokens aside), and taken for 0 in groups of fewer than
- * two sequences.  Sequences outside all groups share nothing; cu_groups does not fall.
+ * two sequences.  Sequences outside all groups share nothing; cu_groups and cu_seqlens_q
+ * do not fall (where they do, rows may be zero).
  * Rows outside the sequences are zeroed with zero_rest and left as they were
  * without.  head_dim 128, up to 256 q heads a kv head, any page size.  The
  * workspace (256-byte aligned) is sized with ragged = (cu_seqlens_q != NULL).

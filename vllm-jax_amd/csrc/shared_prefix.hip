@@ -295,6 +295,17 @@ shared_plan_kernel(SharedParams p) {
     pairs += s_total[1][i];
     own += s_total[2][i];
   }
+  // lists that do not fit (cu_groups or cu_q that fall) are not run: every row is
+  // zero.  More row tiles than any that do not fall have are known here already, and
+  // below that number the sums of the lists stay far from 2^31.
+  auto run_nothing = [&]() {
+    if (tid == 0) p.header[0] = p.header[1] = 0;
+    for (int b = tid; b < p.batch; b += threads) p.seqs[b] = ShSeq{0, 0, 0, 0, 0, 0, 0, 0};
+  };
+  if (pairs > (float)p.cap_tiles * 1.001f) {  // uniform
+    run_nothing();
+    return;
+  }
   // (the sums' roundings, below 2^-15 of them, must not make the shares short)
   const float all_tiles = tiles * (float)hkv * 1.0001f, all_pairs = pairs * (float)hkv * 1.0001f;
   const float all_own = own * (float)(hkv * p.dec.hblocks) * 1.0001f;
@@ -351,8 +362,10 @@ shared_plan_kernel(SharedParams p) {
       s = seq(b);
       const int g = s.y > 0 ? group_of(b) : -1;
       const int n = g >= 0 ? group_tiles(g) : 0;
-      if (n) {
-        const int2 r = group_rows(g);
+      const int2 r = n ? group_rows(g) : make_int2(0, 0);
+      if (n && (s.x < r.x || s.x + s.y > r.x + r.y)) {
+        s.y = s.z = 0;  // (cu_q falls) rows that the group's tiles do not have: zeros
+      } else if (n) {
         shared = shared_of(g);
         q.p_unit = kLds ? s_gunit[g] : p.group_shared[2 * p.groups + g];
         q.p_parts = sh_ceil(shared / kTileN, most);
@@ -410,15 +423,15 @@ shared_plan_kernel(SharedParams p) {
     if (b < p.batch) p.seqs[b] = q;
     base = {base.a + sum.a, base.b + sum.b, base.c + sum.c};
   }
-  // lists that do not fit (cu_groups or cu_q that fall) are not run: every row is zero
   const bool fits = base.a <= p.cap_tiles && base.c <= p.cap_chunks && (long long)base.b * hkv <= p.cap_units;
-  if (tid == 0) {
-    p.header[0] = fits ? base.a : 0;
-    p.header[1] = fits ? base.c : 0;
-  }
-  if (!fits) {
-    __syncthreads();
-    for (int b = tid; b < p.batch; b += threads) p.seqs[b] = ShSeq{0, 0, 0, 0, 0, 0, 0, 0};
+  if (fits) {
+    if (tid == 0) {
+      p.header[0] = base.a;
+      p.header[1] = base.c;
+    }
+  } else {
+    __syncthreads();  // the entries of all sequences have been written
+    run_nothing();
   }
 }
 

@@ -95,7 +95,7 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     (a length of zero gives a zero row).  With it the rows of sequence ``b`` are
     ``cu_seqlens_q[b] .. cu_seqlens_q[b + 1]``, at most ``max_seqlen_q`` of them
     are computed, and row ``i`` of ``n`` sees the first ``lengths[b] - n + i + 1``
-    tokens (and is zero if that is none).  Rows outside the sequences are zero
+    tokens (and is zero if that is none; ``cu_seqlens_q`` does not fall).  Rows outside the sequences are zero
     in a new output and left as they were in a given ``out``.
 
     ``prefixes.shared_lens`` is a promise about the block tables: it is rounded
