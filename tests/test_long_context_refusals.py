@@ -233,3 +233,28 @@ def test_a_step_of_unrelated_requests(dev):
         outs.append(PKG.attention(cache.clone(), q, k, v, meta))
     for pool, out in outs[1:]:
         assert torch.equal(pool, outs[0][0]) and torch.equal(out, outs[0][1])
+
+
+# ---------------------------------------------------------------------------
+# devices
+# ---------------------------------------------------------------------------
+def test_page_copies_launch_on_the_pools_device(host_tensors, monkeypatch):
+    """Bounds and pools on another device than the current one: the launch is made with theirs current."""
+    events = []
+    common = importlib.import_module(PKG.__name__ + ".kernels._common")
+
+    @contextlib.contextmanager
+    def on_device(t):
+        events.append("enter")
+        yield
+        events.append("leave")
+
+    monkeypatch.setattr(importlib.import_module(PKG.__name__ + ".rotary"), "on_device", on_device)
+    monkeypatch.setattr(common, "require_device", lambda *a: None)
+    monkeypatch.setattr(common, "stream_handle", lambda t: None)
+    monkeypatch.setattr(PKG.kv_cache_manager._lib, "call", lambda name, *a: events.append(name))
+    PKG.copy_block_bounds(_bf16(3, 4, 2, 2, 128), [0], [2])
+    PKG.copy_blocks(_bf16(2, 3, 16, 2, 128), [0], [2])
+    assert events == ["enter", "pa_copy_blocks", "leave"] * 2
+    PKG.copy_block_bounds(_bf16(3, 4, 2, 2, 128), [], [])
+    assert len(events) == 6

@@ -168,11 +168,13 @@ def copy_pages(kc, vc, src: Sequence[int], dst: Sequence[int]) -> None:
     import torch
 
     from .kernels._common import stream_handle
+    from .rotary import on_device
     if len(src) != len(dst):
         raise ValueError("src and dst must have the same length")
     if len(src) == 0:
         return
     nb, bs, hkv, d = kc.shape
     idx = torch.as_tensor(np.stack([np.asarray(src, np.int32), np.asarray(dst, np.int32)]), device=kc.device)
-    _lib.call("pa_copy_blocks", kc.data_ptr(), vc.data_ptr(), nb, bs, kc.stride(0), kc.stride(1), kc.stride(2),
-              hkv, d, idx[0].data_ptr(), idx[1].data_ptr(), len(src), stream_handle(kc))
+    with on_device(kc):
+        _lib.call("pa_copy_blocks", kc.data_ptr(), vc.data_ptr(), nb, bs, kc.stride(0), kc.stride(1), kc.stride(2),
+                  hkv, d, idx[0].data_ptr(), idx[1].data_ptr(), len(src), stream_handle(kc))
