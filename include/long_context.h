@@ -49,7 +49,8 @@ int pa_block_bounds(const uint16_t* k_cache, int32_t num_pages, int32_t page_siz
 
 /*
  * scores[b, kv head, j] = scale * max over the kv head's q heads of
- * sum_d max(q_d min_d, q_d max_d), which no scaled logit of block j exceeds;
+ * sum_d max(q_d min_d, q_d max_d), which no scaled logit of block j exceeds
+ * (but for the roundings of the 32-bit sums);
  * -inf for blocks that start at or past lengths[b].  scale > 0.  q: [batch,
  * num_heads, head_dim]; scores: float32 [batch, num_kv_heads, pages_per_seq *
  * page_size / block].

@@ -69,11 +69,10 @@ def check_workspace(workspace: Optional[torch.Tensor], need: int, like: torch.Te
     return workspace, (workspace.data_ptr(), need)
 
 
-def check_heads(q: torch.Tensor, num_kv_heads: int, head_dim: int, batch: Optional[int] = None):
-    """Checked strides of q ``[T, H, d]`` (``T`` = ``batch`` if given) for a pool of these heads."""
+def check_heads(q: torch.Tensor, num_kv_heads: int, head_dim: int):
+    """Checked strides of q ``[T, H, d]`` for a pool of these heads."""
     stride = operand("q", q, 3)
-    tokens, heads, dim = q.shape
-    if dim != head_dim or heads == 0 or heads % num_kv_heads or (batch is not None and tokens != batch):
-        raise ValueError(f"q must be [{'T' if batch is None else batch}, H, {head_dim}] with H a multiple of "
-                         f"{num_kv_heads}, got {tuple(q.shape)}")
+    _, heads, dim = q.shape
+    if dim != head_dim or heads == 0 or heads % num_kv_heads:
+        raise ValueError(f"q must be [T, H, {head_dim}] with H a multiple of {num_kv_heads}, got {tuple(q.shape)}")
     return stride

@@ -236,7 +236,10 @@ __device__ __forceinline__ uint32_t score_key(uint32_t u) {
 // its keys in registers (kPer of them; 0: reads them again), key j of thread t
 // being candidate j * threads + t, so that counts are ballots and their sums
 // scalar.  Bound by its chain of steps: 250 candidates 4.2 us, of which 3.5 are the
-// launch and the loads; 512 workgroups of up to 4096 10 us, bit by bit 17.8.
+// launch and the loads; 512 workgroups of up to 4096 10 us, bit by bit 17.8.  One wave
+// and bits up to 1024 candidates, against four and histograms, calls in a graph: 32
+// workgroups of 260 10.2 and 8.3 us, of 1000 10.7 and 8.3; 512 of 260 10.3 and 9.2, of
+// 1000 11.7 and 10.2: the bits cost up to a quarter of the call at every size measured.
 template <int kWavesN, int kPer>
 __global__ void __launch_bounds__(64 * kWavesN)
 select_blocks_kernel(SelectParams p) {

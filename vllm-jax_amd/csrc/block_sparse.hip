@@ -18,8 +18,10 @@
 // block_sparse_merge_kernel.  P is rounded to bf16 for the matrix cores; scores,
 // sums and O are 32-bit.
 //
-// Bound by the reads of the selected rows (256 bytes at a stride of all kv heads):
-// 128 sequences by 64 blocks of 32 tokens, 32 / 8 heads of 128, 167 us, 6.4 TB/s.
+// Bound by the reads of the selected rows (2 d bytes at a stride of all kv heads):
+// 128 sequences by 64 blocks of 32 tokens, 32 / 8 heads of 128, 167 us, 6.4 TB/s; of
+// 64 98 us, 5.5 TB/s; of 256 346 us, 6.2 TB/s (9 registers go to scratch, 13 with the
+// soft cap).
 // One sequence's 64 blocks, in 16 parts, take 7.4 us, a chain of loads (length,
 // selection, table, K and V), and 2.2 us of merge.
 #include <algorithm>

@@ -19,8 +19,8 @@
 //   shared_merge_kernel   adds the parts up
 //
 // 128 sequences of 64 to 1024 own tokens behind 8192 shared ones, 32 / 8 heads: plan
-// 6.7 us, parts 64 (the tiles alone 42, the chunks alone 50), merge 6.0; the plain
-// decode of the same step takes 573.
+// 6.8 us, parts 64 (behind the prefix alone 42, the own tokens alone 50), merge 6.0;
+// the plain decode takes 560 for the same step.
 #include <algorithm>
 #include <type_traits>
 
@@ -633,7 +633,16 @@ shared_merge_kernel(SharedParams p) {
 }
 static_assert(kPartFloats<kPHeadDim> == kLtUnit, "both kinds of tiles leave partials of one layout");
 
-// Whether a launch takes 128-row tiles that share a CU.
+// Whether a launch takes 128-row tiles that share a CU: pages of whole 16-token steps,
+// and one new token a sequence or fewer than 256 rows of one.  Calls in a graph, 128-row
+// tiles then 256-row tiles, 32 / 8 heads, pages of 64.  One new token: 128 sequences of
+// 64 to 1024 own tokens behind 8192 shared ones 87 and 129 us (the chunks have a launch
+// of their own beside 256-row tiles), 256 behind 32768 255 and 320; with hardly any own
+// tokens the tiles alone count: 128 behind 2048 36 and 42, behind 32768 110 and 98.
+// Several: 32 sequences by 2 behind 8192 38 and 41, by 5 55 and 54, by 20 145 and 113,
+// by 60 329 and 283, by 64 (256 rows) 334 and 283, by 200 1085 and 927; 64 by 5 behind
+// 32768 288 and 192.  So below 256 rows of a sequence the rule gives up to a third away
+// where the groups are large.
 bool shared_light(bool ragged, int64_t max_q, int64_t group, int64_t page) {
   if (page % 16) return false;
   return !ragged || max_q * group < kRows;
