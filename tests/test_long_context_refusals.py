@@ -54,6 +54,9 @@ def test_attention_refuses_groups_before_the_store(prefill, monkeypatch):
     groups = PKG.SharedPrefixes.of([0, 2], [64], "cpu")
     cases = [(_bf16(2, 1, 16, hkv, dim), heads, groups, ValueError, message) for hkv, heads, dim, message in NOT_SHARED]
     cases += [(_bf16(2, 1, 16, 2, 128), 8, ([0, 2], [64]), TypeError, "SharedPrefixes"),
+              (_bf16(2, 1, 16, 2, 128), 8, PKG.SharedPrefixes([0, 2], [64]), TypeError, "cu_groups"),
+              (_bf16(2, 1, 16, 2, 128), 8, PKG.SharedPrefixes(_i32(3), _i32(1)), ValueError, "cu_groups"),
+              (_bf16(2, 1, 16, 2, 128), 8, PKG.SharedPrefixes(_i32(2), _i32(1, 1)), ValueError, "shared_lens"),
               (_bf16(3, 1, 16, 2, 128), 8, groups, ValueError, "the pool")]
     for cache, heads, shared, error, message in cases:
         hkv, dim = cache.shape[3:]

@@ -275,7 +275,7 @@ def attention(kv_cache: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     if getattr(metadata, "shared", None) is not None:
         check_shared(q, kv_cache, metadata.shared)
     kv_cache = update_kv_cache(kv_cache, metadata.slot_mapping, k, v)
-    return kv_cache, attention_stored(kv_cache, q, metadata)
+    return kv_cache, _attend(kv_cache, q, metadata)
 
 
 def qwen3_attention_core(kv_cache: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -291,7 +291,7 @@ def qwen3_attention_core(kv_cache: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     q_rot, kv_cache = qk_norm_rope_store(q, k, v, q_norm_weight, k_norm_weight, metadata.input_positions,
                                          metadata.slot_mapping, kv_cache, eps=eps, rope_theta=rope_theta,
                                          rope_scaling=rope_scaling)
-    return kv_cache, attention_stored(kv_cache, q_rot, metadata)
+    return kv_cache, _attend(kv_cache, q_rot, metadata)
 
 
 def _host_bound(longest) -> Optional[int]:
@@ -308,6 +308,13 @@ def _host_bound(longest) -> Optional[int]:
 
 def attention_stored(kv_cache: torch.Tensor, q: torch.Tensor, metadata: AttentionMetadata) -> torch.Tensor:
     """The attention part of qwen3.py:175-218 for K/V already in the pool."""
+    if getattr(metadata, "shared", None) is not None:
+        check_shared(q, kv_cache, metadata.shared)
+    return _attend(kv_cache, q, metadata)
+
+
+def _attend(kv_cache: torch.Tensor, q: torch.Tensor, metadata: AttentionMetadata) -> torch.Tensor:
+    """``attention_stored`` of metadata whose groups, if any, ``check_shared`` has seen."""
     if not (USE_PREFILL_PAGED_ATTENTION_KERNEL and USE_DECODE_PAGED_ATTENTION_KERNEL):
         raise NotImplementedError("the dense fallbacks of qwen3.py:120-169 are not part of this library")
     head_dim = q.shape[-1]
@@ -315,7 +322,6 @@ def attention_stored(kv_cache: torch.Tensor, q: torch.Tensor, metadata: Attentio
     # half goes in as page views
     pool = isinstance(kv_cache, torch.Tensor) and kv_cache.dim() == 5 and kv_cache.shape[0] >= 2
     if getattr(metadata, "shared", None) is not None:
-        check_shared(q, kv_cache, metadata.shared)
         # as many groups as sequences: no two share, and the plain kernels need no partials
         if 0 < metadata.shared.shared_lens.numel() < metadata.block_tables.shape[0]:
             return _attention_shared(kv_cache, q, metadata)

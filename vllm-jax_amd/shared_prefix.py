@@ -71,6 +71,12 @@ def check_shared(q: torch.Tensor, kv_cache: torch.Tensor, prefixes: SharedPrefix
     route that a step's size chooses, and ``attention()`` has it before it stores the step's keys and values."""
     if not isinstance(prefixes, SharedPrefixes):
         raise TypeError(f"prefixes must be SharedPrefixes, got {type(prefixes).__name__}")
+    cu_groups, shared_lens = prefixes.cu_groups, prefixes.shared_lens
+    if not isinstance(cu_groups, torch.Tensor) or not isinstance(shared_lens, torch.Tensor):
+        raise TypeError("cu_groups and shared_lens must be torch.Tensors")
+    if shared_lens.dim() != 1 or cu_groups.shape != (shared_lens.shape[0] + 1,):
+        raise ValueError(f"cu_groups {tuple(cu_groups.shape)} and shared_lens {tuple(shared_lens.shape)} must be "
+                         "[groups + 1] and [groups]")
     if not isinstance(kv_cache, torch.Tensor) or kv_cache.dim() != 5 or kv_cache.shape[0] != 2:
         raise ValueError("shared prefixes need the pool [2, NB, BS, Hkv, d]")
     hkv, d = kv_cache.shape[3:]
