@@ -20,6 +20,15 @@ def _i32(*shape):
     return torch.zeros(shape, dtype=torch.int32)
 
 
+@pytest.fixture
+def host_tensors(monkeypatch):
+    """The entries' checks take host tensors; nothing is launched."""
+    for module in ("shared_prefix", "_operands", "rotary"):
+        monkeypatch.setattr(importlib.import_module(f"{PKG.__name__}.{module}"), "require_device", lambda *a: None)
+    monkeypatch.setattr(PKG.shared_prefix, "on_device", lambda t: contextlib.nullcontext())
+    monkeypatch.setattr(PKG.shared_prefix, "stream_handle", lambda t: None)
+
+
 NOT_SHARED = [  # kv heads, q heads, head size, what the message names
     (2, 8, 64, "head size"),
     (2, 8, 256, "head size"),
@@ -29,7 +38,7 @@ NOT_SHARED = [  # kv heads, q heads, head size, what the message names
 
 @pytest.mark.parametrize("pages", [1, 1 << 20])
 @pytest.mark.parametrize("hkv,heads,dim,message", NOT_SHARED)
-def test_shared_prefixes_of_other_heads_at_every_width(hkv, heads, dim, message, pages):
+def test_shared_prefixes_of_other_heads_at_every_width(hkv, heads, dim, message, pages, host_tensors):
     """Tables narrow enough for the plain decode, and wide ones."""
     prefixes = PKG.SharedPrefixes.of([0, 2], [64], "cpu")
     q, cache, table = _bf16(2, heads, dim), _bf16(2, 1, 16, hkv, dim), _i32(1, 1).expand(2, pages)
@@ -139,15 +148,6 @@ def test_bounds_that_no_decode_takes():
 # ---------------------------------------------------------------------------
 # workspaces
 # ---------------------------------------------------------------------------
-@pytest.fixture
-def host_tensors(monkeypatch):
-    """The entries' checks take host tensors; nothing is launched."""
-    for module in ("shared_prefix", "_operands", "rotary"):
-        monkeypatch.setattr(importlib.import_module(f"{PKG.__name__}.{module}"), "require_device", lambda *a: None)
-    monkeypatch.setattr(PKG.shared_prefix, "on_device", lambda t: contextlib.nullcontext())
-    monkeypatch.setattr(PKG.shared_prefix, "stream_handle", lambda t: None)
-
-
 @pytest.mark.parametrize("pays", [False, True])
 def test_workspaces_that_do_not_fit_are_replaced(pays, host_tensors, monkeypatch):
     """The plain decode writes through the workspace's address: on either route only one that is contiguous, aligned and

@@ -67,23 +67,27 @@ def shared_prefix_pays(batch: int, num_groups: int, num_kv_heads: int, span: int
 
 
 def check_shared(q: torch.Tensor, kv_cache: torch.Tensor, prefixes: SharedPrefixes) -> None:
-    """Refuses what the kernels of shared prefixes do not take, by shapes alone: the answer does not follow the
-    route that a step's size chooses, and ``attention()`` has it before it stores the step's keys and values."""
+    """Refuses what the kernels of shared prefixes do not take, by types and shapes alone: ``attention()`` has the
+    answer before it stores the step's keys and values."""
     if not isinstance(prefixes, SharedPrefixes):
         raise TypeError(f"prefixes must be SharedPrefixes, got {type(prefixes).__name__}")
-    cu_groups, shared_lens = prefixes.cu_groups, prefixes.shared_lens
-    if not isinstance(cu_groups, torch.Tensor) or not isinstance(shared_lens, torch.Tensor):
+    cu_groups, shared_lens = getattr(prefixes.cu_groups, "shape", None), getattr(prefixes.shared_lens, "shape", None)
+    if cu_groups is None or shared_lens is None:
         raise TypeError("cu_groups and shared_lens must be torch.Tensors")
-    if shared_lens.dim() != 1 or cu_groups.shape != (shared_lens.shape[0] + 1,):
-        raise ValueError(f"cu_groups {tuple(cu_groups.shape)} and shared_lens {tuple(shared_lens.shape)} must be "
-                         "[groups + 1] and [groups]")
-    if not isinstance(kv_cache, torch.Tensor) or kv_cache.dim() != 5 or kv_cache.shape[0] != 2:
+    if len(shared_lens) != 1 or cu_groups != (shared_lens[0] + 1,):
+        raise ValueError(f"cu_groups {tuple(cu_groups)} and shared_lens {tuple(shared_lens)} must be [groups + 1] and "
+                         "[groups]")
+    pool, rows = getattr(kv_cache, "shape", ()), getattr(q, "shape", ())
+    if len(pool) != 5 or pool[0] != 2:
         raise ValueError("shared prefixes need the pool [2, NB, BS, Hkv, d]")
-    hkv, d = kv_cache.shape[3:]
-    if d != HEAD_DIM:
-        raise ValueError(f"shared prefixes need a head size of {HEAD_DIM}, got {d}")
-    if q.dim() == 3 and q.shape[1] > MAX_GROUP * hkv:
-        raise ValueError(f"shared prefixes take up to {MAX_GROUP} q heads a kv head, got {q.shape[1]} for {hkv}")
+    check_sharing_heads(rows[1] if len(rows) == 3 else 0, pool[3], pool[4])
+
+
+def check_sharing_heads(heads: int, num_kv_heads: int, head_dim: int) -> None:
+    if head_dim != HEAD_DIM:
+        raise ValueError(f"shared prefixes need a head size of {HEAD_DIM}, got {head_dim}")
+    if heads > MAX_GROUP * num_kv_heads:
+        raise ValueError(f"shared prefixes take up to {MAX_GROUP} q heads a kv head, got {heads} for {num_kv_heads}")
 
 
 def check_groups(prefixes: SharedPrefixes, like: torch.Tensor):
@@ -127,9 +131,11 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     (``shared_prefix_workspace_bytes``; the plain decode's is smaller) is made here if
     none is given, or one that is too small, not contiguous or not 256-byte aligned.
     """
-    check_shared(q, kv_cache, prefixes)
+    if not isinstance(prefixes, SharedPrefixes):
+        raise TypeError(f"prefixes must be SharedPrefixes, got {type(prefixes).__name__}")
     (nb, bs, hkv, d), cache_stride = check_pool(kv_cache)
     q_stride = check_heads(q, hkv, d)
+    check_sharing_heads(q.shape[1], hkv, d)
     if kv_cache.get_device() != q.get_device():
         raise ValueError(f"kv_cache lives on {kv_cache.device}, q on {q.device}")
     tokens, heads, _ = q.shape
