@@ -122,3 +122,30 @@ def test_sparse_decode_with_a_soft_cap(dim, heads, kv, dev):
     got = PKG.block_sparse_decode_attention(q.to(dev), cache.to(dev), table.to(dev), _i32(lengths, dev), sel.to(dev),
                                             block=block, scale=dim ** -0.5, attn_logits_soft_cap=20.0)
     assert ((got.cpu().double() - want).abs() <= tol).all()
+
+
+def test_routes_of_a_prefill_step(dev, monkeypatch):
+    """attention() of a step with groups: few rows a sequence behind wide tables by the shared kernels, many by the plain
+    prefill, with its bits."""
+    gen = _gen(36)
+    calls = []
+    call = PKG._lib.call
+    monkeypatch.setattr(PKG._lib, "call", lambda name, *a: calls.append(name) or call(name, *a))
+    for new, name in (([3, 150, 16], "pa_shared_prefix"), ([199, 100, 86], "pa_prefill")):
+        batch = Batch([(4, [250, 200, 130])], 64, 2, gen)
+        cache, table, _, shared = batch.args(dev)
+        wide = torch.full((3, 1400), -1, dtype=torch.int32, device=dev)
+        wide[:, :table.shape[1]] = table
+        n = sum(new)
+        q = torch.randn((n, 32, 128), generator=gen).to(torch.bfloat16).to(dev)
+        pos = [t for c, t0 in zip(new, batch.lengths) for t in range(t0 - c, t0)]
+        cu = lambda x: _i32([0, *torch.tensor(x).cumsum(0).tolist()], dev)  # noqa: E731
+        args = (_i32(pos, dev), _i32([-1] * n, dev), wide, cu(new), cu(batch.lengths), None, 0, max(new))
+        plain = PKG.attention_stored(cache, q, PKG.PrefillAttentionMetadata(*args))
+        calls.clear()
+        got = PKG.attention_stored(cache, q, PKG.SharedPrefillAttentionMetadata(*args, shared=shared))
+        assert calls == [name]
+        assert torch.equal(got, plain) == (name == "pa_prefill")
+        want, tol = ref.shared(q.cpu(), batch.cache, batch.table, batch.lengths, new, 0.08837890625,
+                               scaled_q=name == "pa_prefill")
+        assert ((got.cpu().double() - want).abs() <= tol).all()

@@ -196,7 +196,7 @@ def test_workspaces_off_the_device(dev):
 @pytest.mark.parametrize("cu_groups", [[0], [0, 1, 2], [0, 0, 2, 2]])
 def test_attention_without_a_shared_token_is_the_plain_one(cu_groups, host_tensors, monkeypatch):
     """As many groups as sequences (what the block manager returns for unrelated requests), or none: the plain kernels,
-    which put no partials aside; a group of two takes the shared ones."""
+    which put no partials aside; a group of two takes the shared ones where they pay."""
     took = []
     monkeypatch.setattr(ATTENTION, "prefill_pool", lambda *a, **k: took.append("prefill"))
     monkeypatch.setattr(ATTENTION, "decode_pool", lambda *a, **k: took.append("decode"))
@@ -209,13 +209,37 @@ def test_attention_without_a_shared_token_is_the_plain_one(cu_groups, host_tenso
     PKG.attention_stored(cache, q, prefill)
     for m in _steps(2, 4, pair)[:2]:
         PKG.attention_stored(cache, q, m)
-    assert took == ["decode", "prefill", "shared", "shared"]
+    assert took == ["decode", "prefill", "shared", "prefill"]  # (the entry itself chooses for decode)
     # groups that do not fit together are refused there too
     for m in (decode, prefill):
         m.shared = PKG.SharedPrefixes(_i32(3), _i32(3))
         with pytest.raises(ValueError, match="cu_groups"):
             PKG.attention_stored(cache, q, m)
     assert len(took) == 4
+
+
+@pytest.mark.parametrize("qwen", [False, True])
+def test_prefill_steps_with_groups_take_the_faster_kernels(qwen, host_tensors, monkeypatch):
+    """Few rows a sequence behind wide tables: the shared kernels; many rows, whose partials would take time and room, or
+    narrow tables: the plain prefill."""
+    took = []
+    monkeypatch.setattr(ATTENTION, "prefill_pool", lambda *a, **k: took.append("prefill"))
+    monkeypatch.setattr(ATTENTION, "shared_prefix_attention", lambda *a, **k: took.append("shared"))
+    monkeypatch.setattr(ATTENTION, "update_kv_cache", lambda cache, *a: cache)
+    monkeypatch.setattr(ATTENTION, "qk_norm_rope_store", lambda q, *a, **k: (q, cache))
+    cache = _bf16(2, 1, 256, 8, 128)
+    groups = PKG.SharedPrefixes.of([0, 16], [4096], "cpu")
+    for heads, pages, tokens, name in ((32, 17, 16, "shared"), (32, 17, 8191, "shared"), (32, 17, 8192, "prefill"),
+                                       (32, 15, 16, "prefill"), (64, 17, 4095, "shared"), (64, 17, 4096, "prefill"),
+                                       (8, 17, 32767, "shared"), (8, 17, 32768, "prefill"), (32, 4096, 8192, "prefill")):
+        q, k, w = _bf16(1, heads, 128).expand(tokens, heads, 128), _bf16(1, 8, 128).expand(tokens, 8, 128), _bf16(128)
+        m = PKG.SharedPrefillAttentionMetadata(_i32(tokens), _i32(tokens), _i32(16, 1).expand(16, pages), _i32(17),
+                                               _i32(17), None, None, tokens, shared=groups)
+        if qwen:
+            PKG.qwen3_attention_core(cache, q, k, k, w, w, m, eps=1e-6, rope_theta=1e6)
+        else:
+            PKG.attention(cache, q, k, k, m)
+        assert took.pop() == name and not took, (heads, pages, tokens)
 
 
 @pytest.mark.gpu

@@ -28,7 +28,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from . import _lib
+from . import _lib, shared_prefix
 from .kernels._common import (bf16_round, inv_sqrt_head_dim_bf16, pool_pointers, require_bf16, require_device,
                               stream_handle)
 from .kernels.decode_paged_attention import decode_paged_attention, decode_pool
@@ -81,7 +81,8 @@ class SharedDecodeAttentionMetadata(DecodeAttentionMetadata):
 
 @dataclass
 class SharedPrefillAttentionMetadata(PrefillAttentionMetadata):
-    """The same for a prefill step (new tokens behind shared, cached ones)."""
+    """The same for a prefill step (new tokens behind shared, cached ones: drafts, questions).  Where the
+    plain prefill is faster it is a step without ``shared`` (``shared_prefix_pays``)."""
     shared: Optional[SharedPrefixes] = None
 
 
@@ -322,8 +323,7 @@ def _attend(kv_cache: torch.Tensor, q: torch.Tensor, metadata: AttentionMetadata
     # half goes in as page views
     pool = isinstance(kv_cache, torch.Tensor) and kv_cache.dim() == 5 and kv_cache.shape[0] >= 2
     if getattr(metadata, "shared", None) is not None:
-        # as many groups as sequences: no two share, and the plain kernels need no partials
-        if 0 < metadata.shared.shared_lens.numel() < metadata.block_tables.shape[0]:
+        if _sharing_pays(kv_cache, q, metadata):
             return _attention_shared(kv_cache, q, metadata)
         check_groups(metadata.shared, q)
     if isinstance(metadata, MixedAttentionMetadata) or not pool:
@@ -351,6 +351,16 @@ def _attend(kv_cache: torch.Tensor, q: torch.Tensor, metadata: AttentionMetadata
             outputs = decode_paged_attention(q, k_pages, v_pages, metadata.block_tables, metadata.context_lens,
                                              scale=scale)
     return outputs
+
+
+def _sharing_pays(kv_cache: torch.Tensor, q: torch.Tensor, metadata) -> bool:
+    """Whether a step with groups takes their kernels; those of one new token each decide by themselves."""
+    groups, (batch, pages) = metadata.shared.shared_lens.numel(), metadata.block_tables.shape
+    if isinstance(metadata, DecodeAttentionMetadata):
+        return 0 < groups < batch
+    bs, hkv = kv_cache.shape[2:4]
+    return 0 < groups < batch and shared_prefix.shared_prefix_pays(batch, groups, hkv, pages * bs,
+                                                                   q.shape[0] * (q.shape[1] // hkv) // batch)
 
 
 def _attention_shared(kv_cache: torch.Tensor, q: torch.Tensor, metadata) -> torch.Tensor:

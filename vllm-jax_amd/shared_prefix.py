@@ -46,10 +46,11 @@ class SharedPrefixes:
                    torch.as_tensor(list(shared_lens), dtype=torch.int32, device=device))
 
 
-def shared_prefix_pays(batch: int, num_groups: int, num_kv_heads: int, span: int) -> bool:
-    """Whether a decode step of ``batch`` sequences in ``num_groups`` groups, over
-    block tables of ``span`` tokens, is cut at the shared prefixes; else the plain
-    decode reads shared pages again and again, most of them from the caches.
+def shared_prefix_pays(batch: int, num_groups: int, num_kv_heads: int, span: int, rows: int = 1) -> bool:
+    """Whether a step of ``batch`` sequences in ``num_groups`` groups, over block
+    tables of ``span`` tokens, is cut at the shared prefixes; else the plain kernels
+    read shared pages again and again, most of them from the caches.  ``rows``: the new
+    tokens of a sequence, on average, times the q heads of a kv head.
 
     It takes more sequences than groups, and tables of 256 MB of K and V in all.
     Whole calls, 32 / 8 heads, one group: 16 sequences of 4096 shared tokens (289 MB)
@@ -57,13 +58,22 @@ def shared_prefix_pays(batch: int, num_groups: int, num_kv_heads: int, span: int
     16384 (273 MB) 39.2 and 35.4; 2 of 32768 (271 MB) 50.4 and 49.3; 16 of 2048
     (155 MB) 25.7 and 28.7.
 
+    Of several new tokens 400 ragged steps were measured (16 to 64 q heads, 4 to 64
+    sequences, 512 to 131 072 shared tokens).  With narrower tables the plain prefill was
+    faster in all but one (16 by 35 behind 1024, 80 MB: 30.5 us plain, 43.9 shared; 64 by
+    66 behind 512, 192 MB: 80 and 127).  With 2048 rows or more its 256-row tiles are
+    full enough, and it writes no partials: never slower, 1.18 times as fast on average
+    (64 by 760 behind 2048: 1.76 and 2.33 ms).  Between them it depends on the lengths: 64
+    by 4 behind 2048 77 us plain and 44 shared; by 60 behind 32 768 2.12 and 1.69 ms, by
+    60 behind 2048 147 and 182 us.
+
     Lengths and shared lengths are on the device and are not looked at, so tables far
     wider than the lengths, or groups that share little, are cut for nothing (device
     times in a graph): 16 chats of 556 tokens, 256 of them shared, in tables of 32k
     18.4 us plain and 24.2 so; 64 of them 31.1 and 35.0; 256 sequences of 4k of which
     two share 256 tokens 731 and 783.  A caller that knows as much leaves the groups
     out of the step's metadata."""
-    return batch > num_groups > 0 and batch * span * num_kv_heads * 512 >= 256 << 20
+    return batch > num_groups > 0 and rows < 2048 and batch * span * num_kv_heads * 512 >= 256 << 20
 
 
 def check_shared(q: torch.Tensor, kv_cache: torch.Tensor, prefixes: SharedPrefixes) -> None:
@@ -126,8 +136,8 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     bf16 for the matrix cores, and q is not rounded again.  How the parts are cut
     follows the whole batch, and with it a row's last bits.  One new token a sequence is computed by the plain decode
     where sharing does not pay (:func:`shared_prefix_pays`).  With ``cu_seqlens_q``
-    every row goes through 32-bit partials in the workspace, also where nothing is
-    shared; ``attention()`` takes the plain prefill there.  The workspace
+    every row goes through 32-bit partials in the workspace, also where the plain
+    prefill is faster; ``attention()`` takes that there.  The workspace
     (``shared_prefix_workspace_bytes``; the plain decode's is smaller) is made here if
     none is given, or one that is too small, not contiguous or not 256-byte aligned.
     """
